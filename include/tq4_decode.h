@@ -253,6 +253,24 @@ int tq4_store_preset(const void *key, const void *value, int dtype, const int32_
                      int64_t cache_block_stride, int layout, int norm_correction, int key_bits,
                      int value_bits, tq4_stream_t stream);
 
+/*
+ * Decode step of a layer with a sliding window: the query, the sequence's last token, attends to
+ * tokens t with t < first_tokens or t >= seq_lens[b] - window (window >= 1 counts the last token
+ * itself; first_tokens >= 0).  Only the KV blocks of visible tokens are read; the block-table
+ * entries of the others may hold anything.  key_bits / value_bits 4/4, 3/4, 3/3, or 8/4 for FP8
+ * keys (the query is used unrotated; rot_t and centroids may be NULL).  q_rot_ws, mid_o, outputs,
+ * sinks and the query as in tq4_full_decode; a sequence without tokens gets NaN rows and LSE -inf.
+ * Where the 16x16x32 kernel does not apply (block_size not a power of two >= 16, block stride not
+ * a multiple of 16) the call is rejected with TQ4_E_UNSUPPORTED.
+ * No counterpart in the reference (its decode adapters take no window).
+ */
+int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, const float *centroids,
+                      const uint8_t *kv_cache, const int32_t *block_table, const int32_t *seq_lens,
+                      float *q_rot_ws, float *mid_o, void *out, int out_dtype, float *lse, int B, int Hq,
+                      int Hk, int D, int block_size, int max_blocks_per_seq, int64_t cache_block_stride,
+                      int num_kv_splits, int layout, float attn_scale, const float *sinks, int key_bits,
+                      int value_bits, int window, int first_tokens, tq4_stream_t stream);
+
 /* Message of the last failed call on this thread ("" when none).
  * Replaces: the TORCH_CHECK messages of cuda/tq4_cuda_v1.cu:468-499. */
 const char *tq4_last_error(void);

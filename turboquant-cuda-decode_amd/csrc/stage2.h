@@ -306,12 +306,4 @@ __global__ __launch_bounds__(kWave *kRotWaves) void rotate_mfma_kernel(const InT
     }
 }
 
-__global__ void pair_lut_kernel(const float *__restrict__ cents, float *__restrict__ lut, int n) {
-    const int t = blockIdx.x * blockDim.x + threadIdx.x;
-    if (t < n * n) {
-        lut[2 * t] = cents[t / n];
-        lut[2 * t + 1] = cents[t % n];
-    }
-}
-
 }  // namespace tq4

@@ -34,6 +34,35 @@ namespace xdl {
 
 constexpr int kQRowFloats = kHeadDim + 4;  // LDS row of a rotated query (rows 16 bytes apart in bank)
 
+// Tokens of a sequence that a step leaves out (HID): a run [lo, hi) behind which the sequence goes on.
+//   window > 0: all but the first `first` and the last `window` tokens (a sliding window with first
+//               tokens that stay visible; the query is the last token, inside its window);
+//   window 0:   the first `prefix` tokens of sequences that have as many (their share of the softmax is
+//               worked out elsewhere); shorter sequences keep all of theirs.
+// The list (step_cut.h) then holds the tiles with a visible token: `head` ones, and behind them those
+// from tile head + skip on.  At least one token of each is visible.
+struct Hidden {
+    int first, window, prefix;
+    struct Span {
+        int lo, hi;      // hidden tokens (lo = hi: none)
+        int head, skip;  // list tile t is the sequence's tile t (t < head) or t + skip
+    };
+    __device__ __forceinline__ Span span(int len) const {
+        len = max(len, 0);
+        Span s{0, 0, 0, 0};
+        if (window > 0) {
+            s.lo = min(first, len);
+            s.hi = max(len - window, s.lo);
+            s.head = (s.lo + 15) >> 4;
+        } else if (len >= prefix) {
+            s.hi = prefix;
+        }
+        s.skip = max((s.hi >> 4) - s.head, 0);
+        return s;
+    }
+    __device__ __forceinline__ int tiles(int len) const { return tiles_of(len) - span(len).skip; }
+};
+
 struct StepArgs : CutArgs {
     const void *query;         // ROT: the bf16 / fp16 query; else fp32 rows, already rotated (FP8 keys: q_dtype rows)
     const float *rot_t;        // [D, D] (ROT)
@@ -51,6 +80,7 @@ struct StepArgs : CutArgs {
     int group, n_hp;           // q-heads per kv-head, head parts per kv-head
     int vw;                    // head parts per workgroup (a power of two)
     int whole;                 // workgroup x holds sequence x and writes its output rows
+    Hidden hidden;             // (HID)
 };
 
 // LDS of a workgroup besides the K table: the waves' block-table entries; a part that holds, one after the other, the operands of
@@ -352,10 +382,10 @@ __device__ __forceinline__ void join_rows(const StepArgs &a, const RowSink &s, c
 }
 
 // The kernel.  ROT: it rotates the (bf16 / fp16) query itself.  KF8 / KB3 / V3: the presets, as
-// in stage1_xdl_kernel.  Head parts are numbered
+// in stage1_xdl_kernel.  HID: sequences leave a run of tokens out (Hidden).  Head parts are numbered
 // kv-head by kv-head (part vh: kv-head vh / parts, heads G (vh % parts) .. of its group), so
 // the heads of consecutive parts are consecutive.
-template <int LAYOUT, int G, bool ROT, bool KF8 = false, bool KB3 = false, bool V3 = false>
+template <int LAYOUT, int G, bool ROT, bool KF8 = false, bool KB3 = false, bool V3 = false, bool HID = false>
 __global__ __launch_bounds__(kWave *kStepWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void decode_step_kernel(const StepArgs a) {
     static_assert(!ROT || !KF8, "FP8 keys take the query unrotated");
@@ -363,6 +393,12 @@ void decode_step_kernel(const StepArgs a) {
     constexpr int RING = 4;
     constexpr int FIRST_SLOTS = 2;  // ring slots issued before the table and the q operands (see stage1_xdl_kernel)
     constexpr bool STG = KB3 && LAYOUT == 0, STG8 = KF8 && LAYOUT == 0;
+    const auto seen = [&] {
+        if constexpr (HID)
+            return a.hidden;
+        else
+            return AllTiles{};
+    }();
     constexpr int kRec = record_bytes<LAYOUT, KF8, KB3, V3>();
     constexpr int kStage = stage_bytes<LAYOUT, KF8, KB3, V3>();
     using RK = std::conditional_t<STG8, RawRec3, std::conditional_t<KF8, RawK8, std::conditional_t<STG, RawRec, std::conditional_t<KB3, RawK3, RawK<LAYOUT>>>>>;
@@ -436,7 +472,7 @@ void decode_step_kernel(const StepArgs a) {
     if (a.whole) {
         cut.b = x;
         cut.len = a.seq_lens[x];
-        cut.tiles = tiles_of(cut.len);
+        cut.tiles = seen.tiles(cut.len);
         cut.run = Run{0, cut.tiles};
         cut.p = 0;
         cut.n_parts = 1;
@@ -450,7 +486,7 @@ void decode_step_kernel(const StepArgs a) {
             }
             return;
         }
-    } else if (!first_segment(cut, a, nx, x, lane, len_lane, single)) {
+    } else if (!first_segment(cut, a, nx, x, lane, len_lane, single, seen)) {
         return;
     }
 
@@ -481,6 +517,11 @@ void decode_step_kernel(const StepArgs a) {
         const int run_start = 16 * t_lo, run_end = n_run > 0 ? min(16 * (t_lo + n_run), cut.len) : run_start;
         const int total = max((n_run + RING - 1) & ~(RING - 1), RING);
         const int b = cut.b;
+        // list tile -> tile of the sequence
+        Hidden::Span hid{0, 0, 0, 0};
+        if constexpr (HID)
+            hid = a.hidden.span(cut.len);
+        auto tile_of = [&](int t) { return HID && t >= hid.head ? t + hid.skip : t; };
         // opaque, or the compiler hoists the operand conversions out of the segment loop and holds
         // them in registers (spilling) through the stream
         int rn = lane & 15, rg = lane >> 4, tid = threadIdx.x;
@@ -542,7 +583,7 @@ void decode_step_kernel(const StepArgs a) {
         };
         // Stream position p lives in lane p mod 64: its tile, mask and address.  p: the lane's
         // position, blk: the block of its tile (past the run: of the last one).
-        auto tile_at = [&](int p) { return t_lo + min(p, max(n_run, 1) - 1); };
+        auto tile_at = [&](int p) { return tile_of(t_lo + min(p, max(n_run, 1) - 1)); };
         auto set_position = [&](int p, int blk, bool here) {
             const int tile = tile_at(p);
             const int toff = (16 * tile) & (block_size - 1);
@@ -557,7 +598,7 @@ void decode_step_kernel(const StepArgs a) {
         };
         // the block of tile t_lo + min(p, n_run - 1), from the table or, for the first 64, the guess
         auto block_at = [&](int p, bool may_guess) {
-            if (may_guess && b == guess_b && t_lo == guess_tile)
+            if (!HID && may_guess && b == guess_b && t_lo == guess_tile)
                 return __shfl(bt_guess, tile_at(p) - t_lo, kWave);
             return bt[tile_at(p) >> tl];
         };
@@ -591,13 +632,19 @@ void decode_step_kernel(const StepArgs a) {
             __builtin_amdgcn_sched_barrier(0);
             const TileV t = decode_v<LAYOUT, TPL>(vcur, off);
             const int t0 = 16 * __builtin_amdgcn_readlane(mask_lane, j & 63);
-            const bool boundary = !(t0 >= run_start && t0 + 16 <= run_end);
+            const bool boundary = HID ? !(t0 >= 0 && t0 + 16 <= cut.len && (t0 + 16 <= hid.lo || t0 >= hid.hi))
+                                      : !(t0 >= run_start && t0 + 16 <= run_end);
             float dot[TPL], nf[TPL];
             bool valid[TPL];
             lane_dots<G>(sc, lc, dot);
 #pragma unroll
             for (int q = 0; q < TPL; ++q) {
-                valid[q] = (uint32_t)(t0 + tok0 + q - run_start) < (uint32_t)(run_end - run_start);
+                if constexpr (HID) {  // (padding: a negative token)
+                    const int tok = t0 + tok0 + q;
+                    valid[q] = (uint32_t)tok < (uint32_t)cut.len && (tok < hid.lo || tok >= hid.hi);
+                } else {
+                    valid[q] = (uint32_t)(t0 + tok0 + q - run_start) < (uint32_t)(run_end - run_start);
+                }
                 if constexpr (LAYOUT == 0 || KF8)
                     nf[q] = half_at(t.norm, q) * q_unscale;
                 else  // ||c[idx]||^2 of token tok0 + q: totals sit in lanes n = token (any row)
@@ -710,7 +757,7 @@ void decode_step_kernel(const StepArgs a) {
             emit_rows<G, V3>(a, rows, st, acc, lc, nh);
         else
             join_rows<G, V3>(a, rows, st, acc, lc, nh, reinterpret_cast<float *>(work), w, vi, sub, n_run == 0, lane);
-        if (a.whole || single || !next_segment(cut, a, x, true))
+        if (a.whole || single || !next_segment(cut, a, x, true, seen))
             return;
         if constexpr (ROT) {  // (here, not at the segment's start: there they would be live through the stream)
             rot_load_query(rot, static_cast<const uint16_t *>(a.query), (int64_t)cut.b * a.num_q_heads + h_first,

@@ -40,12 +40,17 @@ struct Cut {
     int p, n_parts;  // its part and the sequence's parts
 };
 __device__ __forceinline__ int tiles_of(int len) { return (max(len, 0) + 15) >> 4; }
+// Which of a sequence's tiles the list holds: all of them, or (step.h's Hidden) the visible ones.
+struct AllTiles {
+    __device__ __forceinline__ int tiles(int len) const { return tiles_of(len); }
+};
 __device__ __forceinline__ uint32_t weight_of(int tiles, int sw) {
     return tiles > 0 ? (uint32_t)(tiles + kSegmentTiles * sw) : 0u;
 }
 // Places the stretch in sequence c.b (c.len, c.start set).
-__device__ __forceinline__ void place(Cut &c, int x, int sw) {
-    c.tiles = tiles_of(c.len);
+template <class Seen>
+__device__ __forceinline__ void place(Cut &c, int x, int sw, const Seen &seen) {
+    c.tiles = seen.tiles(c.len);
     const int64_t first = (int64_t)c.start + kSegmentTiles * sw, lo = (int64_t)x * c.cell - first;
     const int t0 = (int)max(lo, (int64_t)0), t1 = (int)min(lo + (int64_t)c.cell, (int64_t)c.tiles);
     c.run = Run{t0, max(t1 - t0, 0)};
@@ -56,17 +61,18 @@ __device__ __forceinline__ void place(Cut &c, int x, int sw) {
     }
 }
 // The next sequence in the stretch with tiles for this workgroup; false when there is none.
-__device__ __forceinline__ bool next_segment(Cut &c, const CutArgs &a, int x, bool inside) {
+template <class Seen = AllTiles>
+__device__ __forceinline__ bool next_segment(Cut &c, const CutArgs &a, int x, bool inside, const Seen &seen = Seen{}) {
     const uint64_t end = (uint64_t)(x + 1) * c.cell;
     while (c.b < a.batch) {
         if (inside) {  // leave sequence b
-            c.start += weight_of(tiles_of(c.len), a.sw);
+            c.start += weight_of(seen.tiles(c.len), a.sw);
             if (++c.b >= a.batch || c.start >= end)
                 return false;
             c.len = a.seq_lens[c.b];
         }
         inside = true;
-        place(c, x, a.sw);
+        place(c, x, a.sw, seen);
         if (c.run.count > 0)
             return true;
     }
@@ -74,14 +80,15 @@ __device__ __forceinline__ bool next_segment(Cut &c, const CutArgs &a, int x, bo
 }
 // The first segment of workgroup x of nx.  `alone` (out): every sequence has workgroups of its own, so
 // this one has no further segment.  len_lane: seq_lens[lane], read by the caller.
+template <class Seen = AllTiles>
 __device__ __forceinline__ bool first_segment(Cut &c, const CutArgs &a, int nx, int x, int lane, int len_lane,
-                                              bool &alone) {
+                                              bool &alone, const Seen &seen = Seen{}) {
     const int32_t *sl = a.seq_lens;
     uint32_t total = 0, most = 0, w0 = 0, s0 = 0;  // (w0, s0: the first 64 sequences' weights and their scan)
     int l0 = 0;
     for (int c0 = 0; c0 < a.batch; c0 += kWave) {
         const int len = c0 + lane >= a.batch ? 0 : c0 == 0 ? len_lane : sl[c0 + lane];
-        const int t = tiles_of(len);
+        const int t = seen.tiles(len);
         const uint32_t w = weight_of(t, a.sw), sc = wave_scan(w);
         if (c0 == 0) {
             l0 = len;
@@ -109,7 +116,7 @@ __device__ __forceinline__ bool first_segment(Cut &c, const CutArgs &a, int nx, 
             if (c.b >= a.batch)
                 return false;
             c.len = c.b < kWave ? __builtin_amdgcn_readlane(l0, c.b) : sl[c.b];
-            c.tiles = tiles_of(c.len);
+            c.tiles = seen.tiles(c.len);
             c.p = x - c.b * k;
             c.n_parts = min(k, (int)div_pos(c.tiles + least - 1, least));
             if (c.p >= c.n_parts)
@@ -129,7 +136,7 @@ __device__ __forceinline__ bool first_segment(Cut &c, const CutArgs &a, int nx, 
         uint32_t w = w0, sc = s0;
         if (c0 > 0) {
             len = c0 + lane < a.batch ? sl[c0 + lane] : 0;
-            w = weight_of(tiles_of(len), a.sw);
+            w = weight_of(seen.tiles(len), a.sw);
             sc = wave_scan(w);
         }
         const uint32_t before = carry + sc - w;
@@ -139,7 +146,7 @@ __device__ __forceinline__ bool first_segment(Cut &c, const CutArgs &a, int nx, 
             c.b = c0 + l;
             c.len = __builtin_amdgcn_readlane(len, l);
             c.start = (uint32_t)__builtin_amdgcn_readlane((int)before, l);
-            return next_segment(c, a, x, false);
+            return next_segment(c, a, x, false, seen);
         }
         carry += (uint32_t)__builtin_amdgcn_readlane((int)sc, kWave - 1);
     }

@@ -21,142 +21,19 @@
 #include "step.h"
 #include "store.h"
 
+#include "abi.h"
+#include "step_launch.h"
+
+using namespace tq4::abi;
+
 namespace {
 
-thread_local char g_err[512] = "";
-
-// Events the next kernel launch of this thread stamps with its own start and end
-// (tq4_time_next_launch); cleared by that launch.
-thread_local hipEvent_t g_time_start = nullptr, g_time_stop = nullptr;
-
-// Every kernel launch goes through here: arguments are converted to the kernel's
-// parameter types (the event-stamping launch passes them by address).
-template <typename... KArgs, typename... Args>
-void launch_lds(void (*kernel)(KArgs...), dim3 grid, dim3 block, int lds_bytes, hipStream_t st, Args... args) {
-    static_assert(sizeof...(KArgs) == sizeof...(Args), "argument count");
-    if (g_time_start || g_time_stop) {
-        const hipEvent_t a = g_time_start, b = g_time_stop;
-        g_time_start = g_time_stop = nullptr;
-        hipExtLaunchKernelGGL(kernel, grid, block, lds_bytes, st, a, b, 0, static_cast<KArgs>(args)...);
-    } else {
-        hipLaunchKernelGGL(kernel, grid, block, lds_bytes, st, static_cast<KArgs>(args)...);
+__global__ void pair_lut_kernel(const float *__restrict__ cents, float *__restrict__ lut, int n) {
+    const int t = blockIdx.x * blockDim.x + threadIdx.x;
+    if (t < n * n) {
+        lut[2 * t] = cents[t / n];
+        lut[2 * t + 1] = cents[t % n];
     }
-}
-template <typename... KArgs, typename... Args>
-void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, hipStream_t st, Args... args) {
-    launch_lds(kernel, grid, block, 0, st, args...);
-}
-
-int fail(int code, const char *fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof g_err, fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-int ok() {
-    g_err[0] = '\0';
-    return TQ4_OK;
-}
-
-int launch_status(const char *what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess)
-        return fail((int)e, "%s launch failed: %s", what, hipGetErrorString(e));
-    return ok();
-}
-
-bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
-int log2_int(int x) {
-    int r = 0;
-    while ((1 << r) < x)
-        ++r;
-    return r;
-}
-
-struct Stage1Args {
-    const float *q_rot;
-    const uint8_t *cache;
-    const int32_t *bt;
-    const int32_t *seq_lens;
-    const float *lut;
-    float *mid_o;
-    int B, Hq, Hk, D, bs, max_blocks;
-    int64_t stride;
-    int S, layout;  // TQ4_LAYOUT_*
-    float scale;
-    const float *sinks = nullptr;  // [Hq] sink logits of split 0, or null
-    bool key_fp8 = false;  // the FP8-key preset (VALU kernel; pair LUT unused)
-    // > 0: the key_bits / value_bits preset on the VALU kernel; lut holds the 2^key_bits
-    // centroids (not the pair LUT)
-    int key_bits = 0, value_bits = 4;
-    // filled by check_stage1: kernel layout (0 SoA, 1 AoS) and the AoS slot strides
-    int kl = 0, slot_pos = 0, slot_head = 0;
-};
-
-// Kernel layout (0 SoA, 1 AoS) of an ABI layout id and the byte offsets of AoS slot (t, h)
-// inside a block, t * pos + h * head: position-major blocks [bs][Hk][slot] (TQ4_LAYOUT_AOS)
-// or head-major blocks [Hk][bs][slot] (TQ4_LAYOUT_AOS_HEAD_MAJOR, the layout the vLLM
-// backend's [blocks, Hk, bs, slot] cache presents through transpose(1, 2),
-// reference/turboquant_attn.py:536, :565).  SoA blocks are addressed by their own layout.
-struct CacheGeom {
-    int kl, pos, head;
-};
-bool layout_valid(int layout) {
-    return layout == TQ4_LAYOUT_SOA || layout == TQ4_LAYOUT_AOS || layout == TQ4_LAYOUT_AOS_HEAD_MAJOR;
-}
-CacheGeom cache_geom(int layout, int bs, int hk, int slot) {
-    if (layout == TQ4_LAYOUT_AOS_HEAD_MAJOR)
-        return {1, slot, bs * slot};
-    return {layout == TQ4_LAYOUT_AOS ? 1 : 0, hk * slot, slot};
-}
-#define TQ4_LAYOUT_MSG "layout must be 0 (SoA), 1 (AoS) or 2 (AoS, head-major blocks)"
-
-// Bytes of one AoS slot (= SoA bytes per (token, kv-head)) of a key_bits / value_bits preset.
-int preset_slot_bytes(int key_bits, int value_bits) {
-    const int raw = 16 * key_bits + 2 + 16 * value_bits + 4;
-    return raw + raw % 2;
-}
-
-bool preset_supported(int key_bits, int value_bits) {
-    return (key_bits == 4 && value_bits == 4) || (key_bits == 3 && (value_bits == 3 || value_bits == 4));
-}
-static_assert(tq4::kOutF32 == TQ4_F32 && tq4::kOutBf16 == TQ4_BF16 && tq4::kOutF16 == TQ4_F16,
-              "output type ids");
-
-int check_stage1(Stage1Args &a) {
-    if (!a.q_rot || !a.cache || !a.bt || !a.seq_lens || (!a.lut && !a.key_fp8) || !a.mid_o)
-        return fail(TQ4_E_INVALID, "tq4_stage1: null pointer argument");
-    if (a.B <= 0 || a.Hq <= 0 || a.Hk <= 0 || a.S <= 0 || a.bs <= 0 || a.max_blocks <= 0)
-        return fail(TQ4_E_INVALID, "tq4_stage1: B, Hq, Hk, num_kv_splits, block_size and "
-                                   "max_blocks_per_seq must be positive");
-    if (a.Hq % a.Hk)
-        return fail(TQ4_E_INVALID, "tq4_stage1: Hq (%d) must be a multiple of Hk (%d)", a.Hq, a.Hk);
-    if (a.S > 65536)
-        return fail(TQ4_E_UNSUPPORTED, "tq4_stage1: num_kv_splits %d above 65536", a.S);
-    if (a.B > 65535)  // a grid dimension
-        return fail(TQ4_E_UNSUPPORTED, "tq4_stage1: batch %d above 65535", a.B);
-    if (a.D != tq4::kHeadDim)
-        return fail(TQ4_E_UNSUPPORTED, "tq4_stage1: head_dim %d unsupported (kernels are built for 128)", a.D);
-    if (!layout_valid(a.layout))
-        return fail(TQ4_E_INVALID, "tq4_stage1: " TQ4_LAYOUT_MSG);
-    const int slot = a.key_fp8 ? tq4::store::kFp8Record + 4
-                               : (a.key_bits > 0 ? preset_slot_bytes(a.key_bits, a.value_bits) : tq4::kAosSlot);
-    const int64_t min_stride = (int64_t)a.bs * a.Hk * slot;
-    if (a.stride < min_stride || a.stride % 2)
-        return fail(TQ4_E_INVALID, "tq4_stage1: requires cache [blocks,%d,%d,%d]: block stride %lld < %lld",
-                    a.bs, a.Hk, slot, (long long)a.stride, (long long)min_stride);
-    if (!aligned(a.cache, 16) || !aligned(a.q_rot, 16) || !aligned(a.mid_o, 4))
-        return fail(TQ4_E_INVALID, "tq4_stage1: kv_cache and q_rot must be 16-byte aligned");
-    if (!(a.scale > 0.f) || a.scale != a.scale)
-        return fail(TQ4_E_INVALID, "tq4_stage1: attn_scale must be positive");
-    const CacheGeom geom = cache_geom(a.layout, a.bs, a.Hk, slot);
-    a.kl = geom.kl;
-    a.slot_pos = geom.pos;
-    a.slot_head = geom.head;
-    return TQ4_OK;
 }
 
 template <int LAYOUT, int G> void launch_simple(const Stage1Args &a, hipStream_t st) {
@@ -175,13 +52,6 @@ template <int LAYOUT, int G> void launch_simple(const Stage1Args &a, hipStream_t
                        a.max_blocks, a.stride, a.slot_pos, a.slot_head, a.S, a.scale * tq4::kLog2e);
 }
 
-// q-heads per wave of the 16x16x32 kernel (4 for GQA groups up to 4, else 8) and the waves
-// (parts) each kv-head's group takes.
-int xdl_heads(const Stage1Args &a) { return a.Hq / a.Hk <= 4 ? 4 : 8; }
-int xdl_parts(const Stage1Args &a) {
-    const int g = a.Hq / a.Hk, h = xdl_heads(a);
-    return (g + h - 1) / h;
-}
 
 // Waves per (sequence, kv-head part) for the 16x16x32 kernel; wave x takes splits
 // [x * S / W, (x + 1) * S / W).  Consecutive splits in one wave share one load
@@ -261,14 +131,6 @@ template <int LAYOUT> int dispatch_simple(const Stage1Args &a, hipStream_t st) {
     return launch_status("stage1_simple");
 }
 
-// Every GQA group: groups up to 4 on 4-head waves (1, 2 and 3 with padding heads: each KV
-// tile is still read and looked up once per wave, so MHA and GQA-2 take about the headline's
-// time, 1.4-1.5x faster than the VALU kernel), larger ones in parts of 8 heads (6: one part
-// with two padding heads; 16: two parts).
-bool mfma_applies(const Stage1Args &a) {
-    const bool pow2 = a.bs >= 16 && (a.bs & (a.bs - 1)) == 0;
-    return pow2 && a.stride % 16 == 0;
-}
 
 template <int LAYOUT> int dispatch_xdl(const Stage1Args &a, hipStream_t st) {
     if (!mfma_applies(a))
@@ -305,8 +167,10 @@ int run_stage1(Stage1Args a, int kernel, hipStream_t st) {
     return fail(TQ4_E_INVALID, "tq4_stage1_ex: unknown kernel id %d", kernel);
 }
 
-int rotate_query(const void *query, int query_dtype, const float *rot_t, float *q_rot, int rows,
-                 int D, const float *centroids, float *pair_lut, hipStream_t st) {
+}  // namespace
+
+int tq4::abi::rotate_query(const void *query, int query_dtype, const float *rot_t, float *q_rot, int rows,
+                           int D, const float *centroids, float *pair_lut, hipStream_t st) {
     if (!query || !rot_t || !q_rot)
         return fail(TQ4_E_INVALID, "tq4_rotate_query: null pointer argument");
     if (rows <= 0)
@@ -335,59 +199,8 @@ int rotate_query(const void *query, int query_dtype, const float *rot_t, float *
     return launch_status("rotate_query");
 }
 
-// ---- The full decode step on the 16x16x32 kernel (decode_step_kernel, step.h) ------------
-struct StepIo {
-    const void *query;
-    int query_dtype;
-    const float *rot_t;    // null with FP8 keys
-    float *q_rot_ws;
-    const float *centroids;
-    void *out;
-    int out_dtype;
-    float *lse;
-};
+namespace {
 
-// Waves the device holds at once: every kernel of the step is built for two per SIMD.
-int step_waves_held() {
-    static std::atomic<int> held{0};
-    int h = held.load(std::memory_order_relaxed);
-    if (!h) {
-        int dev = 0, cus = 0;
-        if (hipGetDevice(&dev) != hipSuccess ||
-            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
-            cus = 256;
-        h = cus * tq4::xdl::kStepWaves;
-        held.store(h, std::memory_order_relaxed);
-    }
-    return h;
-}
-
-using tq4::xdl::StepPlan;
-StepPlan step_plan(const Stage1Args &a, bool have_parts) {
-    const bool whole_lines = a.kl == 0 && !a.key_fp8 && a.key_bits == 0;
-    return tq4::xdl::step_plan(
-        {step_waves_held(), a.Hk * xdl_parts(a), a.B, a.max_blocks, a.bs, a.S, whole_lines}, have_parts);
-}
-
-template <int LAYOUT, int G, bool ROT, bool KF8 = false, bool KB3 = false, bool V3 = false>
-void launch_step(const tq4::xdl::StepArgs &s, const StepPlan &p, int nvh, hipStream_t st) {
-    launch_lds(&tq4::xdl::decode_step_kernel<LAYOUT, G, ROT, KF8, KB3, V3>, dim3(nvh / p.vw, p.nx),
-               dim3(tq4::kWave * p.vw * p.sw), tq4::xdl::step_lds<LAYOUT, G, ROT, KF8, KB3, V3>(p.vw, p.sw), st, s);
-}
-template <int LAYOUT, int G>
-void launch_step_format(const Stage1Args &a, const tq4::xdl::StepArgs &s, const StepPlan &p, int nvh, hipStream_t st) {
-    const bool rot = s.rot_t != nullptr, v3 = a.value_bits == 3;
-    if (a.key_fp8)
-        launch_step<LAYOUT, G, false, true>(s, p, nvh, st);
-    else if (a.key_bits == 3 && v3)
-        rot ? launch_step<LAYOUT, G, true, false, true, true>(s, p, nvh, st)
-            : launch_step<LAYOUT, G, false, false, true, true>(s, p, nvh, st);
-    else if (a.key_bits == 3)
-        rot ? launch_step<LAYOUT, G, true, false, true>(s, p, nvh, st)
-            : launch_step<LAYOUT, G, false, false, true>(s, p, nvh, st);
-    else
-        rot ? launch_step<LAYOUT, G, true>(s, p, nvh, st) : launch_step<LAYOUT, G, false>(s, p, nvh, st);
-}
 
 // merge_parts_kernel reads a sequence's rows CHUNK at a time, the first chunk ahead of the part
 // count: the smallest that holds the parts a sequence has when the lengths are equal (24 sequences
@@ -397,62 +210,15 @@ template <typename T> auto merge_kernel(int64_t parts) {
                       : parts <= 16 ? &tq4::merge_parts_kernel<T, 16> : &tq4::merge_parts_kernel<T, 32>;
 }
 
-// The step from checked arguments (check_stage1; mfma_applies).  have_parts: a.mid_o has room
-// for the part rows (else one workgroup per sequence, whatever the batch).
-int run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t st) {
-    const StepPlan plan = step_plan(a, have_parts && a.S > 1);
-    const int nvh = a.Hk * xdl_parts(a);
-    tq4::xdl::StepArgs s{};
-    s.query = io.query;
-    s.q_dtype = io.query_dtype;
-    if (!a.key_fp8) {
-        if (io.query_dtype == TQ4_F32 || !plan.rotates) {  // the in-kernel rotation takes 16-bit queries
-            const int rc = rotate_query(io.query, io.query_dtype, io.rot_t, io.q_rot_ws, a.B * a.Hq, a.D, nullptr,
-                                        nullptr, st);
-            if (rc)
-                return rc;
-            s.query = io.q_rot_ws;
-        } else {
-            s.rot_t = io.rot_t;
-        }
-    }
-    s.centroids = io.centroids;
-    s.cache = a.cache;
-    s.block_table = a.bt;
-    s.seq_lens = a.seq_lens;
-    s.sinks = a.sinks;
-    s.parts = a.mid_o;
-    s.out = io.out;
-    s.lse = io.lse;
-    s.block_stride = a.stride;
-    s.score_scale_log2 = a.scale * tq4::kLog2e;
-    s.out_dtype = io.out_dtype;
-    s.batch = a.B;
-    s.num_q_heads = a.Hq;
-    s.num_kv_heads = a.Hk;
-    s.block_size_log2 = log2_int(a.bs);
-    s.max_blocks = a.max_blocks;
-    s.slot_pos = a.slot_pos;
-    s.slot_head = a.slot_head;
-    s.num_splits = a.S;
-    s.group = a.Hq / a.Hk;
-    s.n_hp = xdl_parts(a);
-    s.vw = plan.vw;
-    s.sw = plan.sw;
-    s.per_seq = plan.per_seq;
-    s.whole = plan.whole;
-    if (xdl_heads(a) == 4)
-        a.kl == 0 ? launch_step_format<0, 4>(a, s, plan, nvh, st) : launch_step_format<1, 4>(a, s, plan, nvh, st);
-    else
-        a.kl == 0 ? launch_step_format<0, 8>(a, s, plan, nvh, st) : launch_step_format<1, 8>(a, s, plan, nvh, st);
-    int rc = launch_status("decode_step");
-    if (rc || plan.whole)
-        return rc;
-    const int64_t parts = (plan.nx + a.B - 1) / a.B;
-    const dim3 grid(a.Hq, a.B), block(tq4::kWave);
+}  // namespace
+
+// out / lse from the part rows of a step; `parts`: the parts of a sequence when the lengths are equal.
+int tq4::abi::merge_parts(const float *rows, const int32_t *seq_lens, void *out, int out_dtype, float *lse, int B,
+                          int Hq, int num_splits, int64_t parts, hipStream_t st) {
+    const dim3 grid(Hq, B), block(tq4::kWave);
 #define TQ4_MERGE_LAUNCH(T) \
-    launch(merge_kernel<T>(parts), grid, block, st, a.mid_o, a.seq_lens, static_cast<T *>(io.out), io.lse, a.Hq, a.S)
-    switch (io.out_dtype) {
+    launch(merge_kernel<T>(parts), grid, block, st, rows, seq_lens, static_cast<T *>(out), lse, Hq, num_splits)
+    switch (out_dtype) {
     case TQ4_F32: TQ4_MERGE_LAUNCH(float); break;
     case TQ4_BF16: TQ4_MERGE_LAUNCH(__bf16); break;
     default: TQ4_MERGE_LAUNCH(_Float16); break;
@@ -461,15 +227,16 @@ int run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t
     return launch_status("merge_parts");
 }
 
-// Checks of a full step's own arguments (the rest is check_stage1's).
-int check_step(const char *what, const void *query, int query_dtype, int out_dtype) {
-    if (query_dtype != TQ4_F32 && query_dtype != TQ4_BF16 && query_dtype != TQ4_F16)
-        return fail(TQ4_E_INVALID, "%s: query_dtype must be 0, 1 or 2", what);
-    if (out_dtype != TQ4_F32 && out_dtype != TQ4_BF16 && out_dtype != TQ4_F16)
-        return fail(TQ4_E_INVALID, "%s: out_dtype must be 0 (f32), 1 (bf16) or 2 (f16)", what);
-    if (!aligned(query, 16))
-        return fail(TQ4_E_INVALID, "%s: query must be 16-byte aligned", what);
-    return TQ4_OK;
+namespace {
+
+// The step from checked arguments (check_stage1; mfma_applies).  have_parts: a.mid_o has room
+// for the part rows (else one workgroup per sequence, whatever the batch).
+int run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t st) {
+    const StepPlan plan = step_plan(a, a.max_blocks, have_parts && a.S > 1);
+    const int rc = launch_step_by<false>(a, io, plan, {}, st);
+    if (rc || plan.whole)
+        return rc;
+    return merge_parts(a.mid_o, a.seq_lens, io.out, io.out_dtype, io.lse, a.B, a.Hq, a.S, (plan.nx + a.B - 1) / a.B, st);
 }
 
 // The writer for KB-bit K indices / VB-bit V codes over `rows` (token, kv-head) rows.
@@ -674,7 +441,7 @@ int tq4_build_pair_lut(const float *centroids, float *pair_lut, int n_centroids,
     if (n_centroids != 16)
         return fail(TQ4_E_UNSUPPORTED, "tq4_build_pair_lut: 16 centroids (4-bit keys) expected, got %d",
                     n_centroids);
-    launch(&tq4::pair_lut_kernel, dim3(1), dim3(256), reinterpret_cast<hipStream_t>(stream), centroids,
+    launch(&pair_lut_kernel, dim3(1), dim3(256), reinterpret_cast<hipStream_t>(stream), centroids,
            pair_lut, n_centroids);
     return launch_status("pair_lut");
 }

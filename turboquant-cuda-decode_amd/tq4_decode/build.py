@@ -10,18 +10,19 @@ import os
 import pathlib
 import shutil
 import subprocess
+import tempfile
 
 PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 LIB = PKG / "libtq4_decode.so"
+SOURCES = ("tq4_decode.hip", "span_decode.hip")
 ARCH = os.environ.get("TQ4_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",
     "-std=c++17",
-    "-shared",
     "-fPIC",
     # keep hipcc from emitting packed-fp32 VALU ops
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -39,14 +40,23 @@ def hipcc() -> str:
 
 
 def build(verbose: bool = False) -> pathlib.Path:
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, "-o", str(tmp), str(CSRC / "tq4_decode.hip")]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + res.stderr[-4000:])
-    if verbose and res.stderr:
-        print(res.stderr)
-    os.replace(tmp, LIB)
+    """Every source to an object of its own, at once, then the link."""
+    with tempfile.TemporaryDirectory(dir=PKG, prefix="_build_") as tmp:
+        objs = [pathlib.Path(tmp) / (pathlib.Path(src).stem + ".o") for src in SOURCES]
+        cmds = [[hipcc(), *HIPCC_FLAGS, "-c", "-o", str(o), str(CSRC / src)] for src, o in zip(SOURCES, objs)]
+        procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+        said = [p.communicate()[0] for p in procs]
+        for cmd, p, text in zip(cmds, procs, said):
+            if p.returncode != 0:
+                raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + text[-4000:])
+            if verbose and text:
+                print(text)
+        out = LIB.with_suffix(".so.tmp")
+        cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-o", str(out), *map(str, objs)]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + res.stderr[-4000:])
+    os.replace(out, LIB)
     return LIB
 
 

@@ -21,6 +21,7 @@ Reference call shapes kept here:
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -467,6 +468,85 @@ def _full_decode_preset(query, rotation_t, kv_cache, block_table, seq_lens, cent
         key_bits, value_bits, _stream(query.device))
     _lib.check(rc, "tq4_full_decode_preset")
     return ws.out
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(dev):
+    """The tensors' device made current, where it is not (launches go to the current device)."""
+    if dev.index is None or torch.cuda.current_device() == dev.index:
+        return _NO_GUARD
+    return torch.cuda.device(dev)
+
+
+def _int_arg(value, name, least):
+    if isinstance(value, bool) or not isinstance(value, int) or not least <= value <= 0x7FFFFFFF:
+        raise RuntimeError(f"{name} must be an int from {least} to {0x7FFFFFFF}")
+    return value
+
+
+def _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits, value_bits,
+               layout, out_dtype, attn_scale, sinks):
+    """Checks of a decode step with hidden tokens; returns the C arguments' common runs."""
+    fp8 = key_bits == 8
+    if (key_bits, value_bits) not in PRESETS + ((8, 4),):
+        raise RuntimeError(f"key/value bits must be one of {PRESETS + ((8, 4),)}")
+    _require(query.is_cuda and query.dim() == 3 and query.is_contiguous() and query.dtype in DTYPES, "invalid query")
+    B, Hq, D = query.shape
+    _require(D == HEAD_DIM, _QUERY_SHAPE)
+    _check_tensor(block_table, "block_table", torch.int32)
+    _check_tensor(seq_lens, "seq_lens", torch.int32)
+    slot = slot_bytes_fp8(D) if fp8 else slot_bytes_preset(D, key_bits, value_bits)
+    bs, Hk, stride, lid = _cache_geometry(kv_cache, slot, layout, " (FP8 keys)" if fp8 else "")
+    _require(Hq % Hk == 0, "Hq must be a multiple of Hk")
+    _require(block_table.dim() == 2 and block_table.size(0) == B, "block_table batch mismatch")
+    _require(seq_lens.dim() == 1 and seq_lens.size(0) == B, "seq_lens batch mismatch")
+    _require(ws.out.dtype == out_dtype and ws.out.shape == query.shape and ws.mid_o.shape[:3] == (B, Hq, num_kv_splits),
+             "workspace does not match this call")
+    tensors = [query, kv_cache, block_table, seq_lens, ws.out]
+    if not fp8:
+        _check_tensor(rotation_t, "rotation_t", torch.float32)
+        _require(tuple(rotation_t.shape) == (D, D), _ROTATION_SHAPE)
+        _check_tensor(centroids, "centroids", torch.float32)
+        if centroids.numel() != 1 << key_bits:
+            raise RuntimeError(f"{key_bits}-bit keys need {1 << key_bits} centroids")
+        tensors += [rotation_t, centroids]
+    _require(_same_device(*tensors), "all tensors must be on the same device")
+    scale = 1.0 / math.sqrt(D) if attn_scale is None else float(attn_scale)
+    head = (query.data_ptr(), DTYPES[query.dtype], None if fp8 else rotation_t.data_ptr(),
+            None if fp8 else centroids.data_ptr(), kv_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr())
+    tail = (ws.out.data_ptr(), DTYPES[out_dtype], ws.lse.data_ptr(), B, Hq, Hk, D, bs, block_table.size(1), stride,
+            num_kv_splits, lid, scale, _check_sinks(sinks, Hq, query.device), key_bits, value_bits)
+    return head, tail
+
+
+def window_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, window, *,
+                  first_tokens=0, key_bits=4, value_bits=4, layout="soa", out_dtype=None, attn_scale=None,
+                  workspace=None, sinks=None):
+    """Decode step of a layer with a sliding window; returns ``(out [B, Hq, D], lse [B, Hq])``.
+
+    The query is the sequence's last token and attends to tokens ``t`` with ``t < first_tokens`` or
+    ``t >= seq_lens[b] - window`` (``window`` counts the last token itself).  Only blocks with visible
+    tokens are read: the block-table entries of the others may hold anything.  ``key_bits`` /
+    ``value_bits``: 4/4, 3/4, 3/3, or 8/4 for FP8 keys (unrotated query; ``rotation_t`` and
+    ``centroids`` may be None).  Otherwise as ``full_decode``: rotation, workspace (a
+    ``DecodeWorkspace``, whose ``out`` and ``lse`` are returned), ``sinks`` (per-head sink logits), a
+    grid from shapes alone.  A sequence without tokens gets NaN rows and LSE -inf.  KV blocks are a
+    power of two of 16 tokens or more.
+    """
+    _int_arg(window, "window", 1)
+    _int_arg(first_tokens, "first_tokens", 0)
+    out_dtype = query.dtype if out_dtype is None else out_dtype
+    _require(out_dtype in DTYPES and query.dim() == 3, _QUERY_SHAPE)
+    ws = workspace or DecodeWorkspace(query.size(0), query.size(1), num_kv_splits, query.device, out_dtype)
+    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits,
+                            value_bits, layout, out_dtype, attn_scale, sinks)
+    with _on_device(query.device):
+        rc = _lib.load().tq4_window_decode(*head, ws.q_rot.data_ptr(), ws.mid_o.data_ptr(), *tail, window, first_tokens,
+                                           _stream(query.device))
+    _lib.check(rc, "tq4_window_decode")
+    return ws.out, ws.lse
 
 
 def _buffer_view(buf, shape, dtype):
