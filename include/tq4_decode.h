@@ -271,6 +271,29 @@ int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, co
                       int num_kv_splits, int layout, float attn_scale, const float *sinks, int key_bits,
                       int value_bits, int window, int first_tokens, tq4_stream_t stream);
 
+/*
+ * Decode step of a batch whose sequences share their first prefix_len tokens: the first
+ * prefix_len / block_size entries of every row of block_table name the same blocks (those of row 0 are
+ * read).  The shared tokens are read and decoded once for the query rows of all sequences; the results
+ * are those of tq4_full_decode / tq4_full_decode_preset on the same arguments, the shared part with f16
+ * operands (each factor rounded once, half a step of f16).  prefix_len: whole blocks, 0 up to the
+ * table's width; a sequence with fewer tokens (seq_lens[b] < prefix_len, 0 included) attends to its
+ * own seq_lens[b] alone and may have other blocks.  query and out are 16-bit (TQ4_BF16, TQ4_F16).
+ * workspace: at least tq4_prefix_workspace_floats(...) floats, 16-byte aligned, contents after the call
+ * unspecified; two calls that may overlap need one each.  The grid depends on the shapes and prefix_len,
+ * never on seq_lens.  key_bits / value_bits, sinks, block sizes and errors as in tq4_window_decode.
+ * No counterpart in the reference.
+ */
+int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, const float *centroids,
+                      const uint8_t *kv_cache, const int32_t *block_table, const int32_t *seq_lens,
+                      float *workspace, int64_t workspace_floats, void *out, int out_dtype, float *lse, int B,
+                      int Hq, int Hk, int D, int block_size, int max_blocks_per_seq, int64_t cache_block_stride,
+                      int num_kv_splits, int layout, float attn_scale, const float *sinks, int key_bits,
+                      int value_bits, int prefix_len, tq4_stream_t stream);
+/* Floats of workspace that tq4_prefix_decode needs for these shapes and any prefix_len; -1 (and a
+ * message) where they are invalid. */
+int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);
+
 /* Message of the last failed call on this thread ("" when none).
  * Replaces: the TORCH_CHECK messages of cuda/tq4_cuda_v1.cu:468-499. */
 const char *tq4_last_error(void);

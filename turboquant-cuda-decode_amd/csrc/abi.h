@@ -248,6 +248,7 @@ int rotate_query(const void *query, int query_dtype, const float *rot_t, float *
                  const float *centroids, float *pair_lut, hipStream_t st);
 int merge_parts(const float *parts, const int32_t *seq_lens, void *out, int out_dtype, float *lse, int B, int Hq,
                 int num_splits, int64_t expected_parts, hipStream_t st);
+int run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t st);
 // And of span_decode.hip: launch_step_by (step_launch.h) with hidden tokens.
 int launch_hidden_step(const Stage1Args &a, const StepIo &io, const StepPlan &plan, const tq4::xdl::Hidden &hidden,
                        hipStream_t st);

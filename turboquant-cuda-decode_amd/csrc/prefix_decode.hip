@@ -1,0 +1,172 @@
+// The decode step of a batch that shares its first tokens (tq4_prefix_decode, include/tq4_decode.h).
+#include <algorithm>
+
+#include "abi.h"
+#include "prefix.h"
+
+using namespace tq4::abi;
+
+namespace {
+
+// How the prefix is spread over the device: row tiles of 32 WR rows, `splits` runs of 64-token tiles.
+struct PrefixPlan {
+    int wr, row_tiles, splits, parts;
+};
+constexpr int kMaxParts = 64;  // part rows of the prefix per (sequence, head)
+
+int most_splits(int wr, int groups, int held) {
+    return std::max(1, std::min(kMaxParts * wr / 4, 2 * held / std::max(groups, 1)));
+}
+// rows: query rows per kv-head; tiles: 64-token tiles.  Two workgroups run on a CU at once.  Of the split
+// counts the one whose rounds of workgroups end first, a workgroup's start and end counted as 3 tiles.
+PrefixPlan prefix_plan(int rows, int Hk, int tiles) {
+    PrefixPlan p{};
+    const int held = step_waves_held() / tq4::xdl::kStepWaves * 2;
+    p.wr = rows > 64 ? 4 : 2;
+    p.row_tiles = (rows + 32 * p.wr - 1) / (32 * p.wr);
+    const int64_t groups = (int64_t)p.row_tiles * Hk;
+    int64_t best = INT64_MAX;
+    const int most = std::min(most_splits(p.wr, (int)std::min<int64_t>(groups, 1 << 30), held), tiles);
+    for (int s = 1; s <= most; ++s) {
+        const int64_t cost = ((groups * s + held - 1) / held) * ((tiles + s - 1) / s + 3);
+        if (cost < best) {
+            best = cost;
+            p.splits = s;
+        }
+    }
+    p.parts = p.splits * (4 / p.wr);
+    return p;
+}
+
+int64_t part_floats(int64_t rows, int parts) { return rows * parts * (tq4::kHeadDim + 1); }
+
+struct Workspace {
+    int64_t q_rot, own, shared, total;  // offsets in floats
+};
+Workspace workspace_of(int B, int Hq, int Hk, int num_kv_splits) {
+    const int64_t rows = (int64_t)B * Hq;
+    const int wr = rows / Hk > 64 ? 4 : 2;
+    const int64_t groups = (rows / Hk + 32 * wr - 1) / (32 * wr) * Hk;
+    const int held = step_waves_held() / tq4::xdl::kStepWaves * 2;
+    const int parts = most_splits(wr, (int)std::min<int64_t>(groups, 1 << 30), held) * (4 / wr);
+    auto up = [](int64_t x) { return (x + 63) / 64 * 64; };
+    Workspace w{};
+    w.own = up(rows * tq4::kHeadDim);
+    w.shared = w.own + up(part_floats(rows, num_kv_splits));
+    w.total = w.shared + up(part_floats(rows, parts));
+    return w;
+}
+
+template <int LAYOUT, int WR> void launch_prefix(const Stage1Args &a, const tq4::prefix::Args &p, dim3 grid, hipStream_t st) {
+    const dim3 block(tq4::prefix::kThreads);
+    if (a.key_fp8)
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, true, false, false, WR>, grid, block, st, p);
+    else if (a.key_bits == 3 && a.value_bits == 3)
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, true, WR>, grid, block, st, p);
+    else if (a.key_bits == 3)
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, false, WR>, grid, block, st, p);
+    else
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, false, false, WR>, grid, block, st, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits) {
+    if (B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || num_kv_splits <= 0) {
+        fail(TQ4_E_INVALID, "tq4_prefix_workspace_floats: B, Hq, Hk and num_kv_splits must be positive, Hq a multiple of Hk");
+        return -1;
+    }
+    return workspace_of(B, Hq, Hk, num_kv_splits).total;
+}
+
+int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, const float *centroids,
+                      const uint8_t *kv_cache, const int32_t *block_table, const int32_t *seq_lens, float *workspace,
+                      int64_t workspace_floats, void *out, int out_dtype, float *lse, int B, int Hq, int Hk, int D,
+                      int block_size, int max_blocks_per_seq, int64_t cache_block_stride, int num_kv_splits, int layout,
+                      float attn_scale, const float *sinks, int key_bits, int value_bits, int prefix_len,
+                      tq4_stream_t stream) {
+    constexpr char what[] = "tq4_prefix_decode";
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    Stage1Args a{};
+    int rc = span_args(a, what, query, query_dtype, rot_t, centroids, kv_cache, block_table, seq_lens, workspace,
+                       workspace, out, out_dtype, lse, B, Hq, Hk, D, block_size, max_blocks_per_seq, cache_block_stride,
+                       num_kv_splits, layout, attn_scale, sinks, key_bits, value_bits);
+    if (rc)
+        return rc;
+    if (prefix_len < 0 || prefix_len % block_size || prefix_len / block_size > max_blocks_per_seq)
+        return fail(TQ4_E_INVALID, "%s: prefix_len %d must be whole blocks of %d, at most the table's %d", what, prefix_len,
+                    block_size, max_blocks_per_seq);
+    if (query_dtype == TQ4_F32 || out_dtype == TQ4_F32)
+        return fail(TQ4_E_UNSUPPORTED, "%s: 16-bit queries and outputs only (the shared product has f16 operands)", what);
+    const Workspace ws = workspace_of(B, Hq, Hk, num_kv_splits);
+    if (workspace_floats < ws.total || !aligned(workspace, 16))
+        return fail(TQ4_E_INVALID, "%s: workspace of %lld floats, needs %lld, 16-byte aligned", what,
+                    (long long)workspace_floats, (long long)ws.total);
+    float *q_rot = workspace, *own = workspace + ws.own, *shared = workspace + ws.shared;
+    a.q_rot = q_rot;
+    a.mid_o = own;
+    StepIo io{query, query_dtype, rot_t, q_rot, centroids, out, out_dtype, lse};
+    if (prefix_len == 0)
+        return run_step(a, io, true, st);
+    if (!a.key_fp8) {
+        rc = rotate_query(query, query_dtype, rot_t, q_rot, B * Hq, D, nullptr, nullptr, st);
+        if (rc)
+            return rc;
+        io.rotated = true;
+    }
+    // the shared tokens
+    tq4::prefix::Args p{};
+    p.query = a.key_fp8 ? query : q_rot;
+    p.q_dtype = query_dtype;
+    p.centroids = centroids;
+    p.cache = kv_cache;
+    p.pages = block_table;
+    p.parts = shared;
+    p.block_stride = cache_block_stride;
+    p.score_scale_log2 = attn_scale * tq4::kLog2e;
+    p.num_q_heads = Hq;
+    p.num_kv_heads = Hk;
+    p.group = Hq / Hk;
+    p.rows = B * p.group;
+    p.total_rows = B * Hq;
+    p.tokens = prefix_len;
+    p.tiles = (prefix_len + tq4::prefix::kTile - 1) / tq4::prefix::kTile;
+    const PrefixPlan plan = prefix_plan(p.rows, Hk, p.tiles);
+    p.row_tiles = plan.row_tiles;
+    p.splits = plan.splits;
+    p.n_parts = plan.parts;
+    p.block_size_log2 = log2_int(block_size);
+    p.slot_pos = a.slot_pos;
+    p.slot_head = a.slot_head;
+    const dim3 grid((unsigned)((Hk * plan.splits + 7) / 8 * 8 * plan.row_tiles));
+    if (plan.wr == 4)
+        a.kl == 0 ? launch_prefix<0, 4>(a, p, grid, st) : launch_prefix<1, 4>(a, p, grid, st);
+    else
+        a.kl == 0 ? launch_prefix<0, 2>(a, p, grid, st) : launch_prefix<1, 2>(a, p, grid, st);
+    rc = launch_status("prefix");
+    if (rc)
+        return rc;
+    // the sequences' own tokens; whole: the rows in the place of one part
+    const int own_blocks = std::max(1, max_blocks_per_seq - prefix_len / block_size);
+    const StepPlan step = step_plan(a, own_blocks, num_kv_splits > 1);
+    const int slots = step.whole ? 1 : num_kv_splits;
+    a.sinks = nullptr;  // (the join's)
+    io.out = own;
+    io.out_dtype = TQ4_F32;
+    io.lse = own + (int64_t)B * Hq * tq4::kHeadDim;
+    rc = launch_hidden_step(a, io, step, tq4::xdl::Hidden{0, 0, prefix_len}, st);
+    if (rc)
+        return rc;
+    const dim3 rows(Hq, B), wave(tq4::kWave);
+    if (out_dtype == TQ4_BF16)
+        launch(&tq4::prefix::join_kernel<__bf16>, rows, wave, st, shared, plan.parts, own, slots, (int)step.whole, seq_lens,
+               prefix_len, sinks, static_cast<__bf16 *>(out), lse, Hq);
+    else
+        launch(&tq4::prefix::join_kernel<_Float16>, rows, wave, st, shared, plan.parts, own, slots, (int)step.whole, seq_lens,
+               prefix_len, sinks, static_cast<_Float16 *>(out), lse, Hq);
+    return launch_status("prefix join");
+}
+
+}  // extern "C"

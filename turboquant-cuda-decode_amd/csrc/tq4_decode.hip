@@ -227,17 +227,17 @@ int tq4::abi::merge_parts(const float *rows, const int32_t *seq_lens, void *out,
     return launch_status("merge_parts");
 }
 
-namespace {
-
 // The step from checked arguments (check_stage1; mfma_applies).  have_parts: a.mid_o has room
 // for the part rows (else one workgroup per sequence, whatever the batch).
-int run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t st) {
+int tq4::abi::run_step(const Stage1Args &a, const StepIo &io, bool have_parts, hipStream_t st) {
     const StepPlan plan = step_plan(a, a.max_blocks, have_parts && a.S > 1);
     const int rc = launch_step_by<false>(a, io, plan, {}, st);
     if (rc || plan.whole)
         return rc;
     return merge_parts(a.mid_o, a.seq_lens, io.out, io.out_dtype, io.lse, a.B, a.Hq, a.S, (plan.nx + a.B - 1) / a.B, st);
 }
+
+namespace {
 
 // The writer for KB-bit K indices / VB-bit V codes over `rows` (token, kv-head) rows.
 template <int KB, int VB>

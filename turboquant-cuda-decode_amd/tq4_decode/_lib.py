@@ -33,6 +33,8 @@ EXPORTS = (
     "tq4_stage1_preset_ex",
     "tq4_store_preset",
     "tq4_window_decode",
+    "tq4_prefix_decode",
+    "tq4_prefix_workspace_floats",
     "tq4_last_error",
     "tq4_abi_version",
     "tq4_time_next_launch",
@@ -56,6 +58,9 @@ _SIGS = {
     "tq4_store": [_p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _i, _p],
     "tq4_window_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
                           _p, _i, _i, _i, _i, _p],
+    "tq4_prefix_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
+                          _p, _i, _i, _i, _p],
+    "tq4_prefix_workspace_floats": [_i, _i, _i, _i],
     "tq4_last_error": [],
     "tq4_abi_version": [],
     "tq4_time_next_launch": [_p, _p],
@@ -68,6 +73,7 @@ _SIGS = {
                              _i, _i, _p],
     "tq4_store_preset": [_p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _i, _i, _i, _p],
 }
+_RESULTS = {"tq4_last_error": ctypes.c_char_p, "tq4_prefix_workspace_floats": _i64}
 
 
 class Tq4Error(RuntimeError):
@@ -86,7 +92,7 @@ def load():
         for name, args in _SIGS.items():
             fn = getattr(lib, name)
             fn.argtypes = args
-            fn.restype = ctypes.c_char_p if name == "tq4_last_error" else ctypes.c_int
+            fn.restype = _RESULTS.get(name, ctypes.c_int)
         _handle = lib
     return _handle
 

@@ -401,6 +401,12 @@ class DecodeWorkspace:
         self.out = torch.empty(batch, num_q_heads, HEAD_DIM, dtype=out_dtype, device=device)
         self.lse = torch.empty(batch, num_q_heads, dtype=torch.float32, device=device)
 
+    def fits(self, query, num_kv_heads, num_kv_splits, out_dtype):
+        B, Hq, _ = query.shape
+        return (self.out.dtype == out_dtype and self.out.shape == query.shape and self.out.is_contiguous() and
+                self.mid_o.shape == (B, Hq, num_kv_splits, HEAD_DIM + 1) and self.mid_o.is_contiguous() and
+                self.lse.shape == (B, Hq) and self.q_rot.shape == query.shape)
+
 
 def full_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, *,
                 layout="soa", out_dtype=None, attn_scale=None, workspace=None, sinks=None):
@@ -502,8 +508,7 @@ def _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, nu
     _require(Hq % Hk == 0, "Hq must be a multiple of Hk")
     _require(block_table.dim() == 2 and block_table.size(0) == B, "block_table batch mismatch")
     _require(seq_lens.dim() == 1 and seq_lens.size(0) == B, "seq_lens batch mismatch")
-    _require(ws.out.dtype == out_dtype and ws.out.shape == query.shape and ws.mid_o.shape[:3] == (B, Hq, num_kv_splits),
-             "workspace does not match this call")
+    _require(ws.fits(query, Hk, num_kv_splits, out_dtype), "workspace does not match this call")
     tensors = [query, kv_cache, block_table, seq_lens, ws.out]
     if not fp8:
         _check_tensor(rotation_t, "rotation_t", torch.float32)
@@ -546,6 +551,51 @@ def window_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
         rc = _lib.load().tq4_window_decode(*head, ws.q_rot.data_ptr(), ws.mid_o.data_ptr(), *tail, window, first_tokens,
                                            _stream(query.device))
     _lib.check(rc, "tq4_window_decode")
+    return ws.out, ws.lse
+
+
+class PrefixWorkspace:
+    """Buffers of ``prefix_decode`` (fixed shapes, any prefix length, reusable): ``out``, ``lse`` and one
+    block of scratch.  Calls that may overlap need one each."""
+
+    def __init__(self, batch, num_q_heads, num_kv_heads, num_kv_splits, device, out_dtype=torch.bfloat16):
+        self.shape = (batch, num_q_heads, num_kv_heads, num_kv_splits)
+        floats = _lib.load().tq4_prefix_workspace_floats(*self.shape)
+        if floats < 0:
+            raise Tq4Error(_lib.load().tq4_last_error().decode())
+        self.scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        self.out = torch.empty(batch, num_q_heads, HEAD_DIM, dtype=out_dtype, device=device)
+        self.lse = torch.empty(batch, num_q_heads, dtype=torch.float32, device=device)
+
+    def fits(self, query, num_kv_heads, num_kv_splits, out_dtype):
+        return (self.shape == (query.size(0), query.size(1), num_kv_heads, num_kv_splits) and
+                self.out.dtype == out_dtype)
+
+
+def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, prefix_len, *,
+                  key_bits=4, value_bits=4, layout="soa", out_dtype=None, attn_scale=None, workspace=None,
+                  sinks=None):
+    """Decode step of a batch whose sequences share their first ``prefix_len`` tokens; returns
+    ``(out [B, Hq, D], lse [B, Hq])``.
+
+    The first ``prefix_len // block_size`` entries of every row of ``block_table`` name the same blocks
+    (row 0's are read): those tokens are read and decoded once for all sequences, the rest of each
+    sequence as in ``full_decode``.  ``prefix_len`` is whole blocks (0: nothing shared); a sequence with
+    ``seq_lens[b] < prefix_len`` attends to its own ``seq_lens[b]`` tokens alone.  ``query`` and ``out`` are bf16
+    or fp16 (the shared tokens' products have f16 operands).  ``workspace``: a ``PrefixWorkspace``.
+    ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in ``window_decode``.
+    """
+    _int_arg(prefix_len, "prefix_len", 0)
+    out_dtype = query.dtype if out_dtype is None else out_dtype
+    _require(out_dtype in DTYPES and query.dim() == 3 and kv_cache.dim() == 4, _QUERY_SHAPE)
+    ws = workspace or PrefixWorkspace(query.size(0), query.size(1), kv_cache.size(2), num_kv_splits, query.device,
+                                      out_dtype)
+    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits,
+                            value_bits, layout, out_dtype, attn_scale, sinks)
+    with _on_device(query.device):
+        rc = _lib.load().tq4_prefix_decode(*head, ws.scratch.data_ptr(), ws.scratch.numel(), *tail, prefix_len,
+                                           _stream(query.device))
+    _lib.check(rc, "tq4_prefix_decode")
     return ws.out, ws.lse
 
 
