@@ -6,7 +6,7 @@
 // rows.  Against the step, whose wave has 4 or 8 rows, a tile's decoding is spread over 128 (64) rows
 // and every operand is a plain f16 tile.
 //
-//   S^T[token][row] = sum_d K[token][d] q[row][d]       v_mfma_f32_32x32x16_f16, A = K, B = q
+//   S^T[token][row] = sum_d c[token][d] q[row][d]       v_mfma_f32_32x32x16_f16, A = c, B = q
 //   O^T[dim][row]  += sum_t V^T[dim][t] P^T[t][row]     the same, A = V^T, B = P
 //
 // With the rows in the columns a lane (c, h) = (lane % 32, lane / 32) has one row's scores (tokens 8 (i / 4) +
@@ -14,16 +14,19 @@
 // rescaled by its own factor, and P's registers are the B operand as they stand: k-slot (h, j) of a
 // 16-token product is token 8 (j / 4) + 4 h + j % 4, and V^T is laid out in LDS in that order.
 //
-// A workgroup of four waves takes WR * 32 rows (WR = 4: each wave the whole tile of 64 tokens for 32
-// rows; WR = 2, for up to 64 rows: half of the tile's tokens each, as rows of their own for the merge).
-// Per tile a thread decodes 32 elements of K (a quarter of a token) and 32 of V (8 dims of 4 tokens),
-// from registers loaded one tile ahead, into one of two LDS tiles; one barrier per tile.
+// A workgroup of WR * WT waves takes WR * 32 rows and tiles of WT * 32 tokens, each wave 32 rows x 32
+// tokens of a tile; waves with the same rows join in LDS at the end.  WR = 4, WT = 2: eight waves, one
+// workgroup per CU; WR = 2, WT = 1, for up to 64 rows: two waves, three workgroups per CU.  A thread
+// decodes 32 elements of K (a quarter of a token) and / or of V (8 dims of 4 tokens) per tile, from
+// registers loaded one tile ahead, into one of two LDS tiles; one barrier per tile.
 //
-// Roundings: K = f16(f16(c) * f16(norm)), V = f16(code * scale + zero) (one fused rounding) and q scaled
-// to f16 by a power of two of its row: each is half a step of f16, 2^-12 on average, where the step's
-// hi + lo operands keep 2^-22; scores, the softmax's statistics and the sums are fp32, P is rounded to
-// nearest f16.  On outputs in 16 bits (the only ones taken) this is below their own rounding.  V beyond
-// f16's range (65504) becomes infinite here.
+// Precision: the centroids and q (times the score scale) are f16 hi + lo, three products c_hi q_hi +
+// c_lo q_hi + c_hi q_lo, and the norm multiplies the fp32 score, so scores and the log-sum-exp keep 2^-21
+// as the step's do; FP8 keys and 16-bit queries are exact in f16, one product.  (With single f16
+// operands the log-sum-exp was off by 1 to 3e-5: a centroid's rounding is the same for every token that
+// has it.)  Two roundings to f16 remain, half a step (2^-11) each: V = code * scale + zero, and P.
+// That is an eighth of a bf16 output's own; for fp16 outputs P is hi + lo too (PLO), which leaves V's.
+// V beyond f16's range (65504) becomes infinite here.
 #pragma once
 #include "step.h"
 
@@ -38,22 +41,37 @@ typedef uint32_t u32x3a2 __attribute__((ext_vector_type(3), aligned(2)));
 typedef uint32_t u32a1 __attribute__((aligned(1)));
 typedef uint32_t u32a2 __attribute__((aligned(2)));
 
-constexpr int kThreads = 256;
-constexpr int kTile = 64;                       // tokens per LDS tile
-constexpr int kTileBytes = 2 * kTile * kHeadDim * 2;  // K and V^T
+// LDS tiles.  K (hi, and lo): token t's 128 dims at kKRow t.  V^T: dim d = 8 e + i in row 16 i + e, the row's
+// 16-byte chunk 2 T + h = tokens 16 T + 8 (j / 4) + 4 h + j % 4, j = 0 .. 7.  Rows are 16 bytes longer than their
+// contents, so that 16 consecutive ones, which are read (V: also written) together, start in the 16
+// different bank quads, and every access is a thread's one address plus a constant.
+constexpr int kKRow = 2 * kHeadDim + 16;
+template <int WR, int WT, bool KF8> struct Shape {
+    static constexpr int threads = 64 * WR * WT;
+    static constexpr int tokens = 32 * WT;          // per tile
+    static constexpr int vrow = 2 * tokens + 16;
+    static constexpr int klo = tokens * kKRow;      // bytes: K hi at 0, K lo, V^T
+    static constexpr int v = klo * (KF8 ? 1 : 2);
+    static constexpr int tile = v + kHeadDim * vrow;
+    static constexpr int bufs = WT == 2 ? 2 : 1;
+    static constexpr int join = WT == 2 ? WR * 64 * 66 * 4 : 0;  // the waves' sums at the end
+    static constexpr int bytes = bufs * tile > join ? bufs * tile : join;
+    static constexpr bool halves = threads > 4 * tokens;         // threads decode K or V, else both
+    static_assert(threads == 4 * tokens * (halves ? 2 : 1), "a unit of 32 elements per thread");
+};
 
 struct Args {
     const void *query;       // fp32 rows, already rotated; FP8 keys: q_dtype rows
     const float *centroids;  // [16], 3-bit keys [8], FP8 keys null
     const uint8_t *cache;
     const int32_t *pages;    // the prefix's blocks
-    float *parts;            // part rows (stage2.h) of n_parts per (sequence, head)
+    float *parts;            // part rows (stage2.h)
     int64_t block_stride;
     float score_scale_log2;
     int q_dtype, num_q_heads, num_kv_heads, group, rows;  // rows: batch * group, per kv-head
     int total_rows;          // batch * num_q_heads
-    int row_tiles, splits, n_parts;
-    int tokens, tiles;       // of the prefix
+    int row_tiles, splits;   // splits: part rows per (sequence, head)
+    int tokens, tiles;       // of the prefix (tiles of Shape::tokens)
     int block_size_log2, slot_pos, slot_head;
 };
 
@@ -64,123 +82,141 @@ __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_ca
 __device__ __forceinline__ uint32_t as_u32(half2v x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ half2v splat(_Float16 x) { return half2v{x, x}; }
 
-// LDS tiles, in 16-byte chunks.  K: token t's row of 16 chunks (8 dims each), chunk k at k ^ (t & 15).
-// V^T: dim d's row of 8 chunks, chunk 2 T + h = tokens 16 T + 8 (j / 4) + 4 h + j % 4, j = 0 .. 7, at
-// (2 T + h) ^ vswz(d).  The 16 lanes that read (or write) together then touch all 64 banks: K reads and
-// writes, V reads; V's 8-byte writes (16 lanes: dims 8 apart) two lanes a bank.
-__device__ __forceinline__ int k_at(int t, int chunk) { return t * 16 + (chunk ^ (t & 15)); }
-__device__ __forceinline__ int vswz(int d) { return ((d >> 1) ^ (d >> 3)) & 7; }
-
-// What a thread loads of a tile: K bytes of token tid / 4 (dims 32 (tid % 4) ..), V bytes of tokens
-// 4 (tid / 16) .. +3 (dims 8 (tid % 16) ..), and their scalars.
-template <int LAYOUT, bool KF8, bool KB3> struct Raw {
+// What a thread loads of a tile, unit u: K bytes of token u / 4 (dims 32 (u % 4) ..) and its norm; V bytes
+// of tokens 4 (u / 16) .. +3 (dims 8 (u % 16) ..), their scales and zeros.
+struct RawK {
     uint4 k, k2;           // (k2: FP8 keys)
-    uint32_t v[4];
     uint32_t norm;
+};
+struct RawV {
+    uint32_t v[4];
     uint32_t sz[4];        // SoA: four scales, four zeros; AoS: scale | zero of each token
 };
 
+// Token `t` of a kv-head in block `blk`.
+template <int LAYOUT, bool KF8, bool KB3, bool V3> struct Record {
+    static constexpr int rec = xdl::record_bytes<LAYOUT, KF8, KB3, V3>(), v0 = xdl::v_offset<LAYOUT, KF8, KB3>();
+    static constexpr int kbytes = KF8 ? kHeadDim : KB3 ? xdl::kK3Bytes : kHalfD, vbytes = V3 ? xdl::kK3Bytes : kHalfD;
+    static constexpr int nf = KF8 ? 2 : 3;
+    const uint8_t *data;
+    const uint16_t *meta;  // SoA: field f at meta[f * bs]
+    int pos, bs;
+    __device__ __forceinline__ Record(const Args &a, int kvh, int t, int blk) {
+        bs = 1 << a.block_size_log2;
+        const int hk = a.num_kv_heads, off = t & (bs - 1);
+        pos = LAYOUT == 0 ? hk * rec : a.slot_pos;
+        const uint8_t *b = a.cache + (int64_t)blk * a.block_stride;
+        data = b + (int64_t)off * pos + (int64_t)kvh * (LAYOUT == 0 ? rec : a.slot_head);
+        meta = reinterpret_cast<const uint16_t *>(b + (int64_t)bs * hk * rec) + (int64_t)kvh * nf * bs + off;
+    }
+};
+
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void load_raw(Raw<LAYOUT, KF8, KB3> &r, const Args &a, int kvh, int kt, int kblk, int vt,
-                                         int vblk, int tid) {
-    constexpr int rec = xdl::record_bytes<LAYOUT, KF8, KB3, V3>(), kv0 = xdl::v_offset<LAYOUT, KF8, KB3>();
-    constexpr int kbytes = KF8 ? kHeadDim : KB3 ? xdl::kK3Bytes : kHalfD, vbytes = V3 ? xdl::kK3Bytes : kHalfD;
-    const int mask = (1 << a.block_size_log2) - 1, hk = a.num_kv_heads, bs = mask + 1;
-    const int pos = LAYOUT == 0 ? hk * rec : a.slot_pos, head = LAYOUT == 0 ? rec : a.slot_head;
-    const uint8_t *kb = a.cache + (int64_t)kblk * a.block_stride, *vb = a.cache + (int64_t)vblk * a.block_stride;
-    const int ko = kt & mask, vo = vt & mask, j = tid & 3, dg = tid & 15;
-    const uint8_t *kp = kb + (int64_t)ko * pos + (int64_t)kvh * head + j * (kbytes / 4);
+__device__ __forceinline__ void load_k(RawK &r, const Args &a, int kvh, int t, int blk, int u) {
+    using R = Record<LAYOUT, KF8, KB3, V3>;
+    const R at(a, kvh, t, blk);
+    const uint8_t *p = at.data + (u & 3) * (R::kbytes / 4);
     if constexpr (KB3) {
-        const u32x3a2 w = *reinterpret_cast<const u32x3a2 *>(kp);
+        const u32x3a2 w = *reinterpret_cast<const u32x3a2 *>(p);
         r.k = uint4{w[0], w[1], w[2], 0u};
     } else {
-        const u32x4a2 w = *reinterpret_cast<const u32x4a2 *>(kp);
+        const u32x4a2 w = *reinterpret_cast<const u32x4a2 *>(p);
         r.k = uint4{w[0], w[1], w[2], w[3]};
         if constexpr (KF8) {
-            const u32x4a2 w2 = *reinterpret_cast<const u32x4a2 *>(kp + 16);
+            const u32x4a2 w2 = *reinterpret_cast<const u32x4a2 *>(p + 16);
             r.k2 = uint4{w2[0], w2[1], w2[2], w2[3]};
         }
     }
-    const uint8_t *vp = vb + (int64_t)vo * pos + (int64_t)kvh * head + kv0 + (V3 ? 3 : 4) * dg;
+    if constexpr (!KF8)
+        r.norm = LAYOUT == 0 ? at.meta[0] : *reinterpret_cast<const uint16_t *>(at.data + R::kbytes);
+}
+// (t: a multiple of 4, its four tokens in one block)
+template <int LAYOUT, bool KF8, bool KB3, bool V3>
+__device__ __forceinline__ void load_v(RawV &r, const Args &a, int kvh, int t, int blk, int u) {
+    using R = Record<LAYOUT, KF8, KB3, V3>;
+    const R at(a, kvh, t, blk);
+    const uint8_t *p = at.data + R::v0 + (V3 ? 3 : 4) * (u & 15);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)  // (3-bit values: the fourth byte is the next field's first)
-        r.v[t] = *reinterpret_cast<const u32a1 *>(vp + (int64_t)t * pos);
+    for (int i = 0; i < 4; ++i)  // (3-bit values: the fourth byte is the next field's first)
+        r.v[i] = *reinterpret_cast<const u32a1 *>(p + (int64_t)i * at.pos);
     if constexpr (LAYOUT == 0) {
-        constexpr int nf = KF8 ? 2 : 3;
-        const uint16_t *km = reinterpret_cast<const uint16_t *>(kb + (int64_t)bs * hk * rec) + kvh * nf * bs + ko;
-        const uint16_t *vm = reinterpret_cast<const uint16_t *>(vb + (int64_t)bs * hk * rec) + kvh * nf * bs + vo;
-        if constexpr (!KF8)
-            r.norm = km[0];
-        const uint2 s = *reinterpret_cast<const uint2 *>(vm + (nf - 2) * bs), z = *reinterpret_cast<const uint2 *>(vm + (nf - 1) * bs);
+        const uint2 s = *reinterpret_cast<const uint2 *>(at.meta + (R::nf - 2) * at.bs);
+        const uint2 z = *reinterpret_cast<const uint2 *>(at.meta + (R::nf - 1) * at.bs);
         r.sz[0] = s.x;
         r.sz[1] = s.y;
         r.sz[2] = z.x;
         r.sz[3] = z.y;
     } else {
-        if constexpr (!KF8)
-            r.norm = *reinterpret_cast<const uint16_t *>(kp - j * (kbytes / 4) + kbytes);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            r.sz[t] = *reinterpret_cast<const u32a2 *>(vp - (V3 ? 3 : 4) * dg + (int64_t)t * pos + vbytes);
+        for (int i = 0; i < 4; ++i)
+            r.sz[i] = *reinterpret_cast<const u32a2 *>(at.data + R::v0 + R::vbytes + (int64_t)i * at.pos);
     }
 }
 
-// The thread's 32 K elements into the LDS tile.  4-bit keys: a byte's pair of centroids from a 256-entry
-// table; 3-bit: six bits' from 64.
+// The unit's K elements into the LDS tile(s) and, from the token's first thread, the token's score factor.
+// 4-bit keys: a byte's pair of centroids, hi and lo parts, from a 256-entry table; 3-bit: six bits' from 64.
 template <int LAYOUT, bool KF8, bool KB3>
-__device__ __forceinline__ void store_k(const Raw<LAYOUT, KF8, KB3> &r, uint4 *ktile, const uint32_t *lut, int tid) {
-    const int t = tid >> 2, j = tid & 3;
-    uint32_t e[16];
+__device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsigned char *klo, float *norms,
+                                        const uint2 *lut, int u) {
+    const int t = u >> 2, j = u & 3, at = t * kKRow + 64 * j;
+    uint32_t e[16], lo[16];
     if constexpr (KF8) {
         const uint32_t w[8] = {r.k.x, r.k.y, r.k.z, r.k.w, r.k2.x, r.k2.y, r.k2.z, r.k2.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-            const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-            e[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo[0], lo[1]));  // (exact)
-            e[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(hi[0], hi[1]));
+            const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
+            const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+            e[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));  // (exact)
+            e[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
         }
     } else {
         const uint32_t w[4] = {r.k.x, r.k.y, r.k.z, r.k.w};
 #pragma unroll
         for (int b = 0; b < 16; ++b) {
+            uint32_t v;
             if constexpr (KB3) {
                 const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
-                uint32_t v = w[wi] >> sh;
+                v = w[wi] >> sh;
                 if (sh > 26)
                     v |= w[wi + 1] << (32 - sh);
-                e[b] = lut[v & 63u];
+                v &= 63u;
             } else {
-                e[b] = lut[(w[b >> 2] >> (8 * (b & 3))) & 0xFFu];
+                v = (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
             }
+            const uint2 c = lut[v];
+            e[b] = c.x;
+            lo[b] = c.y;
         }
         float n = half_bits_to_float(r.norm);
-        if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction
-            float csq = 0.f;
+        if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction (h.h + 2 h.l: see lookup_tile)
+            float hh = 0.f, hl = 0.f;
 #pragma unroll
             for (int b = 0; b < 16; ++b) {
                 const auto h = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), e[b]);
-                csq = __builtin_amdgcn_fdot2(h, h, csq, false);
+                const auto l = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), lo[b]);
+                hh = __builtin_amdgcn_fdot2(h, h, hh, false);
+                hl = __builtin_amdgcn_fdot2(h, l, hl, false);
             }
+            float csq = fmaf(2.f, hl, hh);
             csq += xdl::dppf<0xB1>(csq);  // quad_perm [1, 0, 3, 2]: the token's four threads
             csq += xdl::dppf<0x4E>(csq);  // quad_perm [2, 3, 0, 1]
             n *= __builtin_amdgcn_rsqf(csq + 1e-16f);
         }
-        const half2v n2 = splat((_Float16)n);
+        if (j == 0)
+            norms[t] = n;
 #pragma unroll
-        for (int b = 0; b < 16; ++b)
-            e[b] = as_u32(as_half2(e[b]) * n2);
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4 *>(klo + at + 16 * q) = uint4{lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]};
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-        ktile[k_at(t, 4 * j + q)] = uint4{e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
+        *reinterpret_cast<uint4 *>(khi + at + 16 * q) = uint4{e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
 }
 
-// The thread's V elements (8 dims of 4 tokens), transposed into the LDS tile: for dim i the f16 pairs of
+// The unit's V elements (8 dims of 4 tokens), transposed into the LDS tile: for dim i the f16 pairs of
 // tokens (0, 1) and (2, 3).  A code is put into the significand of 1024 and 1024 taken off again.
-template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void store_v(const Raw<LAYOUT, KF8, KB3> &r, uint4 *vtile, int tid) {
-    const int dg = tid & 15, quad = tid >> 4;
+template <int LAYOUT, bool V3, int VROW> __device__ __forceinline__ void store_v(const RawV &r, unsigned char *vtile, int u) {
+    const int dg = u & 15, quad = u >> 4;
     half2v s01, s23, z01, z23;
     if constexpr (LAYOUT == 0) {
         s01 = as_half2(r.sz[0]);
@@ -198,11 +234,9 @@ __device__ __forceinline__ void store_v(const Raw<LAYOUT, KF8, KB3> &r, uint4 *v
         const half2v x = as_half2(codes | 0x64006400u) - k1024;
         return as_u32(__builtin_elementwise_fma(x, s, z));
     };
-    const int T = quad >> 2, h = quad & 1, half = (quad >> 1) & 1;
-    uint2 *vt = reinterpret_cast<uint2 *>(vtile);
+    unsigned char *to = vtile + dg * VROW + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1);
     auto put = [&](int i, uint32_t c01, uint32_t c23) {
-        const int d = 8 * dg + i;
-        vt[(d * 8 + ((2 * T + h) ^ vswz(d))) * 2 + half] = uint2{value(c01, s01, z01), value(c23, s23, z23)};
+        *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{value(c01, s01, z01), value(c23, s23, z23)};
     };
     if constexpr (V3) {
 #pragma unroll
@@ -221,10 +255,12 @@ __device__ __forceinline__ void store_v(const Raw<LAYOUT, KF8, KB3> &r, uint4 *v
     }
 }
 
-// The row's q as B operands (dims 16 i + 8 h .. +7), scaled by the power of two that puts its largest
-// magnitude in [0.5, 1); returns what a product has to be multiplied by for scores in log2 units.
+// The row's q as B operands (dims 16 i + 8 h .. +7).  FP8 keys: q scaled by the power of two that puts its
+// largest magnitude in [0.5, 1), exact for 16-bit queries.  Else q times the score scale, hi + lo parts;
+// rows whose largest reaches 2^15 are scaled down into f16's range.  Returns what a product has to be
+// multiplied by for scores in log2 units.
 template <bool KF8>
-__device__ __forceinline__ float load_q(half8 (&bq)[8], const Args &a, int64_t head_row, int h) {
+__device__ __forceinline__ float load_q(half8 (&hi)[8], half8 (&lo)[8], const Args &a, int64_t head_row, int h) {
     float x[8][8];
     if (KF8 && a.q_dtype != kOutF32) {
         const uint16_t *q = static_cast<const uint16_t *>(a.query) + head_row * kHeadDim + 8 * h;
@@ -258,13 +294,27 @@ __device__ __forceinline__ float load_q(half8 (&bq)[8], const Args &a, int64_t h
     const auto both = __builtin_amdgcn_permlane32_swap(xdl::fbits(amax), xdl::fbits(amax), false, false);
     const uint32_t b0 = both[0], b1 = both[1];
     amax = fmaxf(xdl::bitsf(b0), xdl::bitsf(b1));
-    const int e = (amax > 0.f && amax < __builtin_inff()) ? -__builtin_amdgcn_frexp_expf(amax) : 0;
+    if constexpr (KF8) {
+        const int e = (amax > 0.f && amax < __builtin_inff()) ? -__builtin_amdgcn_frexp_expf(amax) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                hi[i][j] = (_Float16)__builtin_ldexpf(x[i][j], e);
+        return __builtin_ldexpf(a.score_scale_log2, -e);
+    }
+    amax *= a.score_scale_log2;
+    const int e = (amax >= 32768.f && amax < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
+    const float scale = __builtin_ldexpf(a.score_scale_log2, e);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            bq[i][j] = (_Float16)__builtin_ldexpf(x[i][j], e);
-    return __builtin_ldexpf(a.score_scale_log2, -e);
+        for (int j = 0; j < 8; ++j) {
+            const float v = x[i][j] * scale;
+            hi[i][j] = (_Float16)v;
+            lo[i][j] = (_Float16)(v - (float)hi[i][j]);
+        }
+    return __builtin_ldexpf(1.f, -e);
 }
 
 // (no NaN-quieting copies of the operands, as fmaxf makes; a NaN operand is passed over)
@@ -273,50 +323,81 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
+__device__ __forceinline__ half8 pinned(half8 x) {
+    xdl::u32x4 t = __builtin_bit_cast(xdl::u32x4, x);
+    asm volatile("" : "+v"(t));
+    return __builtin_bit_cast(half8, t);
+}
 // Rows of a lane pair (c, c + 32): max and sum over both.
 __device__ __forceinline__ float pair_max(float x) { return xdl::max_xor32(x); }
 __device__ __forceinline__ float pair_sum(float x) { return xdl::sum_xor32(x); }
 
-template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_kernel(const Args a) {
-    constexpr int WT = 4 / WR;        // waves that share the rows and halve the tokens
-    constexpr int NH = 2 / WT;        // 32-token halves of a tile per wave
-    __shared__ __align__(16) uint4 tile_mem[2][kTileBytes / 16];
-    __shared__ __align__(16) uint32_t lut[KF8 ? 4 : KB3 ? 64 : 256];
+template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR, int WT, bool PLO>
+__global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(WR == 4 ? 2 : 1, 2)))
+void prefix_kernel(const Args a) {
+    using S = Shape<WR, WT, KF8>;
+    __shared__ __align__(16) unsigned char mem[S::bytes];
+    __shared__ __align__(16) float norms[S::bufs][S::tokens];
+    __shared__ __align__(16) uint2 lut[KF8 ? 1 : KB3 ? 64 : 256];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, h = lane >> 5, wr = w % WR, wt = w / WR;
-    // Row tiles of one (kv-head, split) read the same tokens: they come one after the other on one XCD
-    // (workgroup i runs on XCD i % 8).
-    const int y = blockIdx.x >> 3, rt = y % a.row_tiles, gi = (y / a.row_tiles) * 8 + (blockIdx.x & 7);
+    // Row tiles of one (kv-head, split) read the same tokens: the list of all workgroups, row tiles
+    // first, is cut into eight runs, one per XCD (workgroup i runs on XCD i % 8).
+    const int per = gridDim.x >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int gi = item / a.row_tiles, rt = item - gi * a.row_tiles;
     if (gi >= a.num_kv_heads * a.splits)
         return;
     const int kvh = gi % a.num_kv_heads, sp = gi / a.num_kv_heads;
     const int tile0 = (int)((int64_t)a.tiles * sp / a.splits), tile1 = (int)((int64_t)a.tiles * (sp + 1) / a.splits);
 
-    // this thread's tokens of a tile, kept inside the prefix (whole blocks: a multiple of 16 tokens)
-    auto k_tok = [&](int i) { return min(kTile * i + (tid >> 2), a.tokens - 1); };
-    auto v_tok = [&](int i) { return min(kTile * i + 4 * (tid >> 4), a.tokens - 4); };
-    auto page = [&](int t) { return a.pages[t >> a.block_size_log2]; };
-    Raw<LAYOUT, KF8, KB3> raw;
-    int kblk = page(k_tok(tile0)), vblk = page(v_tok(tile0));
-    if constexpr (!KF8) {
-        if constexpr (KB3) {
-            if (tid < 64)
-                lut[tid] = as_u32(half2v{(_Float16)a.centroids[tid & 7], (_Float16)a.centroids[tid >> 3]});
-        } else {
-            lut[tid] = as_u32(half2v{(_Float16)a.centroids[tid & 15], (_Float16)a.centroids[tid >> 4]});
+    // this thread's unit of a tile; its tokens are kept inside the prefix (whole blocks: a multiple of 16)
+    const int u = tid & (4 * S::tokens - 1);
+    const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
+    auto k_tok = [&](int i) { return min(S::tokens * i + (u >> 2), a.tokens - 1); };
+    auto v_tok = [&](int i) { return min(S::tokens * i + 4 * (u >> 4), a.tokens - 4); };
+    // With one LDS tile (WT = 1) tile j + 1's K takes the place of tile j's, whose scores are done, and tile
+    // j's V is decoded when tile j - 1's is done with: a tile behind K.
+    constexpr int kBehind = 2 - S::bufs;
+    int kblk = 0, vblk = 0;
+    auto within = [&](int i) { return max(min(i, tile1 - 1), tile0); };
+    auto read_pages = [&](int i) {
+        if (does_k)
+            kblk = a.pages[k_tok(within(i)) >> a.block_size_log2];
+        if (does_v)
+            vblk = a.pages[v_tok(within(i - kBehind)) >> a.block_size_log2];
+    };
+    RawK rk;
+    RawV rv;
+    auto load = [&](int i) {
+        if (does_k)
+            load_k<LAYOUT, KF8, KB3, V3>(rk, a, kvh, k_tok(within(i)), kblk, u);
+        if (does_v)
+            load_v<LAYOUT, KF8, KB3, V3>(rv, a, kvh, v_tok(within(i - kBehind)), vblk, u);
+    };
+    // tile i's K and tile i - kBehind's V
+    auto store = [&](int i) {
+        const int buf = (i - tile0) & (S::bufs - 1);
+        unsigned char *m = mem + buf * S::tile;
+        if (does_k)
+            store_k<LAYOUT, KF8, KB3>(rk, m, m + S::klo, norms[buf], lut, u);
+        if (does_v)
+            store_v<LAYOUT, V3, S::vrow>(rv, m + S::v, u);
+    };
+    read_pages(tile0);
+    if constexpr (!KF8)
+        for (int e = tid; e < (KB3 ? 64 : 256); e += S::threads) {
+            const uint32_t x = xdl::split_f16(a.centroids[KB3 ? e & 7 : e & 15]), z = xdl::split_f16(a.centroids[KB3 ? e >> 3 : e >> 4]);
+            lut[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
         }
-    }
-    load_raw<LAYOUT, KF8, KB3, V3>(raw, a, kvh, k_tok(tile0), kblk, v_tok(tile0), vblk, tid);
-    const int next = min(tile0 + 1, tile1 - 1);
-    kblk = page(k_tok(next));
-    vblk = page(v_tok(next));
+    load(tile0);
+    read_pages(tile0 + 1);
 
     const int row = rt * 32 * WR + 32 * wr + c, row_in = min(row, a.rows - 1);
     const int b = row_in / a.group, hh = row_in - b * a.group;
     const int64_t head_row = (int64_t)b * a.num_q_heads + kvh * a.group + hh;
-    half8 bq[8];
-    const float f = load_q<KF8>(bq, a, head_row, h);
+    half8 q_hi[8], q_lo[8];
+    const float f = load_q<KF8>(q_hi, q_lo, a, head_row, h);
+    const bool scaled = __any(f != 1.f);
 
     floatx16 acc[4];
 #pragma unroll
@@ -327,110 +408,180 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     float negm = __FLT_MAX__, l = 0.f;  // -max in log2 units (+FLT_MAX: no token yet), this lane's share of the sum
 
     xdl::lds_barrier();  // the table
-    store_k<LAYOUT, KF8, KB3>(raw, tile_mem[0], lut, tid);
-    store_v<LAYOUT, KF8, KB3, V3>(raw, tile_mem[0] + kTileBytes / 32, tid);
-    load_raw<LAYOUT, KF8, KB3, V3>(raw, a, kvh, k_tok(next), kblk, v_tok(next), vblk, tid);
+    store(tile0);
+    load(tile0 + 1);
+    read_pages(tile0 + 2);
     xdl::lds_barrier();
 
-    for (int i = tile0; i < tile1; ++i) {
-        const int n2 = min(i + 2, tile1 - 1);
-        kblk = page(k_tok(n2));
-        vblk = page(v_tok(n2));
-        const half8 *kt = reinterpret_cast<const half8 *>(tile_mem[(i - tile0) & 1]);
-        const half8 *vt = kt + kTileBytes / 32;
-        floatx16 s[NH];
+    // Tile j + 1's scores are worked out while tile j's weights go into the accumulators (matrix phase), then
+    // its softmax and the decoding of the next tile (vector phase).  The two waves of a SIMD are a phase
+    // apart (WT = 2): one uses the matrix core while the other uses the vector unit.  A phase ends at a
+    // barrier; tile j + 1 takes the LDS place of tile j - 1, whose last reader is a phase behind at most.
+    const bool late = WT == 2 && w >= WR;
+    auto phase_end = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        xdl::lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    floatx16 s;
+    half8 p[2], p_lo[2];
+    const unsigned char *k_from = mem + (32 * wt + c) * kKRow + 16 * h, *v_from = mem + S::v + c * S::vrow + 16 * (4 * wt + h);
+    auto scores = [&](int i) {
+        const unsigned char *k_hi = k_from + ((i - tile0) & (S::bufs - 1)) * S::tile;
 #pragma unroll
-        for (int q = 0; q < NH; ++q) {
-            const int t = 32 * (WT == 1 ? q : wt) + c;
+        for (int k = 0; k < 16; ++k)
+            s[k] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const half8 a_hi = *reinterpret_cast<const half8 *>(k_hi + 32 * k);
+            s = mfma32(a_hi, q_hi[k], s);
+            if constexpr (!KF8) {
+                s = mfma32(*reinterpret_cast<const half8 *>(k_hi + S::klo + 32 * k), q_hi[k], s);
+                s = mfma32(a_hi, q_lo[k], s);
+            }
+        }
+    };
+    auto outputs = [&](int i) {
+        const unsigned char *vt = v_from + ((i - tile0) & (S::bufs - 1)) * S::tile;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const half8 v = *reinterpret_cast<const half8 *>(vt + 32 * d * S::vrow + 32 * t);
+                acc[d] = mfma32(v, p[t], acc[d]);
+                if constexpr (PLO)
+                    acc[d] = mfma32(v, p_lo[t], acc[d]);
+            }
+    };
+    if (late)
+        phase_end();
+    scores(tile0);
+    phase_end();
+    for (int j = tile0; j < tile1; ++j) {
+        const int buf = (j - tile0) & (S::bufs - 1);
+        float n[16];
+        if constexpr (!KF8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 v = *reinterpret_cast<const float4 *>(norms[buf] + 32 * wt + 8 * k + 4 * h);
+                n[4 * k] = v.x;
+                n[4 * k + 1] = v.y;
+                n[4 * k + 2] = v.z;
+                n[4 * k + 3] = v.w;
+            }
+            if (scaled)
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    n[k] *= f;
+        } else {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-                s[q][k] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                s[q] = mfma32(kt[k_at(t, 2 * k + h)], bq[k], s[q]);
+                n[k] = f;
         }
-        if (kTile * (i + 1) > a.tokens) {  // tokens past the prefix (the last tile's)
+        if (S::tokens * (j + 1) > a.tokens) {  // tokens past the prefix (the last tile's)
 #pragma unroll
-            for (int q = 0; q < NH; ++q)
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    if (kTile * i + 32 * (WT == 1 ? q : wt) + 8 * (k >> 2) + 4 * h + (k & 3) >= a.tokens)
-                        s[q][k] = -INFINITY;
+            for (int k = 0; k < 16; ++k)
+                if (S::tokens * j + 32 * wt + 8 * (k >> 2) + 4 * h + (k & 3) >= a.tokens) {
+                    s[k] = -INFINITY;
+                    n[k] = 1.f;
+                }
         }
-        // scores less the running maximum, in log2 units; it moves only when a score passes it by more than
-        // kRescaleLogX (p stays below 256).  (The three-way maximum reads the fma's results, never the
-        // matrix core's: its wait states are the compiler's to insert, and it does not see into asm.)
-        float x[NH][16];
+        // Scores in log2 units; the running maximum moves only when one passes it by more than kRescaleLogX (p
+        // stays below 256).  (The three-way maximum reads the multiplications' results, never the matrix
+        // core's: its wait states are the compiler's to insert, and it does not see into asm.)
         float mx = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < NH; ++q)
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                x[q][k] = fmaf(s[q][k], f, negm);
-                x[q][k + 1] = fmaf(s[q][k + 1], f, negm);
-                mx = max3(mx, x[q][k], x[q][k + 1]);
-            }
-        if (__any(mx > xdl::kRescaleLogX)) {
-            float m_row = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < NH; ++q)
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    m_row = fmaxf(m_row, s[q][k] * f);
-            m_row = pair_max(m_row);
+        for (int k = 0; k < 16; k += 2) {
+            s[k] = s[k] * n[k];
+            s[k + 1] = s[k + 1] * n[k + 1];
+            mx = max3(mx, s[k], s[k + 1]);
+        }
+        if (__any(mx + negm > xdl::kRescaleLogX)) {
+            const float m_row = pair_max(mx);
             const float negm_new = m_row + negm > xdl::kRescaleLogX ? -m_row : negm;
             const float alpha = __builtin_amdgcn_exp2f(negm_new - negm);  // 0 at the first tile
             negm = negm_new;
             l *= alpha;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[j] *= alpha;
-#pragma unroll
-            for (int q = 0; q < NH; ++q)
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    x[q][k] = fmaf(s[q][k], f, negm);
+            for (int d = 0; d < 4; ++d)
+                acc[d] *= alpha;
         }
-        half8 p[2 * NH];
 #pragma unroll
-        for (int q = 0; q < NH; ++q)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float e = __builtin_amdgcn_exp2f(x[q][k]);
-                l += e;
-                p[2 * q + (k >> 3)][k & 7] = (_Float16)e;
-            }
-#pragma unroll
-        for (int u = 0; u < 2 * NH; ++u)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const int dim = 32 * d + c, T = (WT == 1 ? 0 : 2 * wt) + u;
-                acc[d] = mfma32(vt[dim * 8 + ((2 * T + h) ^ vswz(dim))], p[u], acc[d]);
-            }
-        if (i + 1 < tile1) {
-            uint4 *to = tile_mem[(i + 1 - tile0) & 1];
-            store_k<LAYOUT, KF8, KB3>(raw, to, lut, tid);
-            store_v<LAYOUT, KF8, KB3, V3>(raw, to + kTileBytes / 32, tid);
-            load_raw<LAYOUT, KF8, KB3, V3>(raw, a, kvh, k_tok(n2), kblk, v_tok(n2), vblk, tid);
+        for (int k = 0; k < 16; ++k) {
+            const float e = __builtin_amdgcn_exp2f(s[k] + negm);
+            l += e;
+            p[k >> 3][k & 7] = (_Float16)e;
+            if constexpr (PLO)
+                p_lo[k >> 3][k & 7] = (_Float16)(e - (float)p[k >> 3][k & 7]);
         }
-        xdl::lds_barrier();
+        // (worked out here: left to itself the compiler moves this into the matrix phase, next to its use)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            p[t] = pinned(p[t]);
+            if constexpr (PLO)
+                p_lo[t] = pinned(p_lo[t]);
+        }
+        if (j + 1 < tile1 || kBehind) {
+            store(j + 1);
+            load(j + 2);
+            read_pages(j + 3);
+        }
+        phase_end();
+        __builtin_amdgcn_s_setprio(1);
+        if (j + 1 < tile1)
+            scores(j + 1);
+        outputs(j);
+        __builtin_amdgcn_s_setprio(0);
+        phase_end();
     }
+    if (WT == 2 && !late)
+        phase_end();
 
     l = pair_sum(l);
+    if constexpr (WT == 2) {
+        // waves wt = 1 leave their sums in LDS, waves wt = 0 join them with theirs
+        xdl::lds_barrier();  // the tiles are no longer read
+        float *out = reinterpret_cast<float *>(mem) + wr * 64 * 66 + lane;
+        if (wt == 1) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    out[64 * (16 * d + k)] = acc[d][k];
+            out[64 * 64] = negm;
+            out[64 * 65] = l;
+        }
+        xdl::lds_barrier();
+        if (wt == 1)
+            return;
+        const float negm1 = out[64 * 64], l1 = out[64 * 65];
+        // (a half whose tokens all lie past the prefix has l = 0 and -max = FLT_MAX, the other's weight is then 1)
+        const float both = fminf(negm, negm1);
+        const float w0 = __builtin_amdgcn_exp2f(both - negm), w1 = __builtin_amdgcn_exp2f(both - negm1);
+        negm = both;
+        l = l * w0 + l1 * w1;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                acc[d][k] = acc[d][k] * w0 + out[64 * (16 * d + k)] * w1;
+    }
     if (row >= a.rows)
         return;
-    const int part = sp * WT + wt;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // (a wave whose tokens all lie past the prefix: l = 0)
-    float *o = part_row(a.parts, head_row, a.n_parts, part);
+    const float inv = 1.f / l;
+    // accumulator d, register 4 q + i: row 32 d + 8 q + 4 h + i of V^T, dim 8 (8 (q % 2) + 4 h + i) + 2 d + q / 2
+    float *o = part_row(a.parts, head_row, a.splits, sp);
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4 *>(o + 32 * d + 8 * q + 4 * h) =
-                float4{acc[d][4 * q] * inv, acc[d][4 * q + 1] * inv, acc[d][4 * q + 2] * inv, acc[d][4 * q + 3] * inv};
+        for (int i = 0; i < 4; ++i) {
+            float4 *to = reinterpret_cast<float4 *>(o + 8 * (8 * q + 4 * h + i));
+            const int k = 4 * q + i;
+            to[0] = float4{acc[0][k] * inv, acc[0][8 + k] * inv, acc[1][k] * inv, acc[1][8 + k] * inv};
+            to[1] = float4{acc[2][k] * inv, acc[2][8 + k] * inv, acc[3][k] * inv, acc[3][8 + k] * inv};
+        }
     if (h == 0)
-        part_lse(a.parts, a.total_rows, head_row, a.n_parts)[part] =
-            l == 0.f ? -INFINITY : (__builtin_amdgcn_logf(l) - negm) * kLn2;
+        part_lse(a.parts, a.total_rows, head_row, a.splits)[sp] = (__builtin_amdgcn_logf(l) - negm) * kLn2;
 }
 
 // One wave per (q-head, sequence): the prefix's part rows, of sequences that have as many tokens, and the

@@ -8,33 +8,37 @@ using namespace tq4::abi;
 
 namespace {
 
-// How the prefix is spread over the device: row tiles of 32 WR rows, `splits` runs of 64-token tiles.
+// How the prefix is spread over the device: `wr` waves of 32 rows per workgroup (4 with two waves each, or
+// 2), row tiles of 32 wr rows, `splits` runs of tiles.
 struct PrefixPlan {
-    int wr, row_tiles, splits, parts;
+    int wr, row_tiles, tiles, splits;
 };
-constexpr int kMaxParts = 64;  // part rows of the prefix per (sequence, head)
+constexpr int kMaxSplits = 64;  // part rows of the prefix per (sequence, head)
 
-int most_splits(int wr, int groups, int held) {
-    return std::max(1, std::min(kMaxParts * wr / 4, 2 * held / std::max(groups, 1)));
+int rows_waves(int64_t rows) { return rows > 64 ? 4 : 2; }
+int tile_tokens(int wr) { return wr == 4 ? 64 : 32; }
+// workgroups the device holds at once: one of eight waves or four of two per CU
+int groups_held(int wr) { return step_waves_held() / tq4::xdl::kStepWaves * (wr == 4 ? 1 : 4); }
+int most_splits(int wr, int64_t groups) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, 2 * groups_held(wr) / std::max<int64_t>(groups, 1)));
 }
-// rows: query rows per kv-head; tiles: 64-token tiles.  Two workgroups run on a CU at once.  Of the split
-// counts the one whose rounds of workgroups end first, a workgroup's start and end counted as 3 tiles.
-PrefixPlan prefix_plan(int rows, int Hk, int tiles) {
+// rows: query rows per kv-head.  Of the split counts the one whose rounds of workgroups end first, a
+// workgroup's start and end counted as kStart tiles.
+PrefixPlan prefix_plan(int rows, int Hk, int tokens) {
+    constexpr int kStart = 3;
     PrefixPlan p{};
-    const int held = step_waves_held() / tq4::xdl::kStepWaves * 2;
-    p.wr = rows > 64 ? 4 : 2;
+    p.wr = rows_waves(rows);
     p.row_tiles = (rows + 32 * p.wr - 1) / (32 * p.wr);
-    const int64_t groups = (int64_t)p.row_tiles * Hk;
+    p.tiles = (tokens + tile_tokens(p.wr) - 1) / tile_tokens(p.wr);
+    const int64_t groups = (int64_t)p.row_tiles * Hk, held = groups_held(p.wr);
     int64_t best = INT64_MAX;
-    const int most = std::min(most_splits(p.wr, (int)std::min<int64_t>(groups, 1 << 30), held), tiles);
-    for (int s = 1; s <= most; ++s) {
-        const int64_t cost = ((groups * s + held - 1) / held) * ((tiles + s - 1) / s + 3);
+    for (int s = 1; s <= std::min(most_splits(p.wr, groups), p.tiles); ++s) {
+        const int64_t cost = ((groups * s + held - 1) / held) * ((p.tiles + s - 1) / s + kStart);
         if (cost < best) {
             best = cost;
             p.splits = s;
         }
     }
-    p.parts = p.splits * (4 / p.wr);
     return p;
 }
 
@@ -45,10 +49,8 @@ struct Workspace {
 };
 Workspace workspace_of(int B, int Hq, int Hk, int num_kv_splits) {
     const int64_t rows = (int64_t)B * Hq;
-    const int wr = rows / Hk > 64 ? 4 : 2;
-    const int64_t groups = (rows / Hk + 32 * wr - 1) / (32 * wr) * Hk;
-    const int held = step_waves_held() / tq4::xdl::kStepWaves * 2;
-    const int parts = most_splits(wr, (int)std::min<int64_t>(groups, 1 << 30), held) * (4 / wr);
+    const int wr = rows_waves(rows / Hk);
+    const int parts = most_splits(wr, (rows / Hk + 32 * wr - 1) / (32 * wr) * Hk);
     auto up = [](int64_t x) { return (x + 63) / 64 * 64; };
     Workspace w{};
     w.own = up(rows * tq4::kHeadDim);
@@ -57,16 +59,24 @@ Workspace workspace_of(int B, int Hq, int Hk, int num_kv_splits) {
     return w;
 }
 
-template <int LAYOUT, int WR> void launch_prefix(const Stage1Args &a, const tq4::prefix::Args &p, dim3 grid, hipStream_t st) {
-    const dim3 block(tq4::prefix::kThreads);
+template <int LAYOUT, int WR, int WT, bool PLO>
+void launch_prefix(const Stage1Args &a, const tq4::prefix::Args &p, dim3 grid, hipStream_t st) {
+    const dim3 block(64 * WR * WT);
     if (a.key_fp8)
-        launch(&tq4::prefix::prefix_kernel<LAYOUT, true, false, false, WR>, grid, block, st, p);
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, true, false, false, WR, WT, PLO>, grid, block, st, p);
     else if (a.key_bits == 3 && a.value_bits == 3)
-        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, true, WR>, grid, block, st, p);
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, true, WR, WT, PLO>, grid, block, st, p);
     else if (a.key_bits == 3)
-        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, false, WR>, grid, block, st, p);
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, true, false, WR, WT, PLO>, grid, block, st, p);
     else
-        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, false, false, WR>, grid, block, st, p);
+        launch(&tq4::prefix::prefix_kernel<LAYOUT, false, false, false, WR, WT, PLO>, grid, block, st, p);
+}
+template <int LAYOUT>
+void launch_prefix(const Stage1Args &a, const tq4::prefix::Args &p, int wr, bool plo, dim3 grid, hipStream_t st) {
+    if (wr == 4)
+        plo ? launch_prefix<LAYOUT, 4, 2, true>(a, p, grid, st) : launch_prefix<LAYOUT, 4, 2, false>(a, p, grid, st);
+    else
+        plo ? launch_prefix<LAYOUT, 2, 1, true>(a, p, grid, st) : launch_prefix<LAYOUT, 2, 1, false>(a, p, grid, st);
 }
 
 }  // namespace
@@ -132,19 +142,16 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
     p.rows = B * p.group;
     p.total_rows = B * Hq;
     p.tokens = prefix_len;
-    p.tiles = (prefix_len + tq4::prefix::kTile - 1) / tq4::prefix::kTile;
-    const PrefixPlan plan = prefix_plan(p.rows, Hk, p.tiles);
+    const PrefixPlan plan = prefix_plan(p.rows, Hk, prefix_len);
+    p.tiles = plan.tiles;
     p.row_tiles = plan.row_tiles;
     p.splits = plan.splits;
-    p.n_parts = plan.parts;
     p.block_size_log2 = log2_int(block_size);
     p.slot_pos = a.slot_pos;
     p.slot_head = a.slot_head;
-    const dim3 grid((unsigned)((Hk * plan.splits + 7) / 8 * 8 * plan.row_tiles));
-    if (plan.wr == 4)
-        a.kl == 0 ? launch_prefix<0, 4>(a, p, grid, st) : launch_prefix<1, 4>(a, p, grid, st);
-    else
-        a.kl == 0 ? launch_prefix<0, 2>(a, p, grid, st) : launch_prefix<1, 2>(a, p, grid, st);
+    const dim3 grid((unsigned)(((int64_t)Hk * plan.splits * plan.row_tiles + 7) / 8 * 8));
+    const bool plo = out_dtype == TQ4_F16;
+    a.kl == 0 ? launch_prefix<0>(a, p, plan.wr, plo, grid, st) : launch_prefix<1>(a, p, plan.wr, plo, grid, st);
     rc = launch_status("prefix");
     if (rc)
         return rc;
@@ -161,10 +168,10 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
         return rc;
     const dim3 rows(Hq, B), wave(tq4::kWave);
     if (out_dtype == TQ4_BF16)
-        launch(&tq4::prefix::join_kernel<__bf16>, rows, wave, st, shared, plan.parts, own, slots, (int)step.whole, seq_lens,
+        launch(&tq4::prefix::join_kernel<__bf16>, rows, wave, st, shared, plan.splits, own, slots, (int)step.whole, seq_lens,
                prefix_len, sinks, static_cast<__bf16 *>(out), lse, Hq);
     else
-        launch(&tq4::prefix::join_kernel<_Float16>, rows, wave, st, shared, plan.parts, own, slots, (int)step.whole, seq_lens,
+        launch(&tq4::prefix::join_kernel<_Float16>, rows, wave, st, shared, plan.splits, own, slots, (int)step.whole, seq_lens,
                prefix_len, sinks, static_cast<_Float16 *>(out), lse, Hq);
     return launch_status("prefix join");
 }
