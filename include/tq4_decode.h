@@ -254,6 +254,33 @@ int tq4_store_preset(const void *key, const void *value, int dtype, const int32_
                      int value_bits, tq4_stream_t stream);
 
 /*
+ * Cache writer with rotary positions: queries and keys are rotated by their token's position, the
+ * rotated keys and the values written into the cache as tq4_store (key_bits / value_bits 4/4),
+ * tq4_store_fp8 (8/4) and tq4_store_preset (3/4, 3/3) do.  query [N, Hq, D], key and value [N, Hk, D] in
+ * dtype, heads contiguous, tokens query_stride / key_stride / value_stride elements apart (whole 16-byte
+ * pieces: slices of a projection's output); query_out [N, Hq, D] contiguous, may be query itself where that is
+ * contiguous; query and query_out may both be NULL.
+ * cos_sin [table_rows, rot_dim] (TQ4_F32 or dtype): row p holds the rot_dim / 2 cosines, then sines, of
+ * position p.  The first rot_dim dims (a multiple of 16) of a head are rotated in planes f: dims
+ * (f, f + rot_dim / 2) with neox, else (2f, 2f + 1); (a, b) -> (a cos - b sin, b cos + a sin).
+ * positions [axes][N] int64, axes axis_stride elements apart; axis_of (HOST array of rot_dim / 2 ints, read
+ * before the call returns; unused for one axis): the axis whose position turns plane f.
+ * K is rotated exactly (not rounded to dtype before it is quantised), and the codes, E4M3 bytes and scalars are those
+ * of the definition in 64 bits (rows of norm below 1e-19 count as zero); query_out is fp32, rounded once.
+ * A token whose slot is negative or past num_blocks * block_size is not written; one with a position outside
+ * the table is not written either, and its query rows become NaN.  Two tokens with one slot: either's bytes.
+ * kv_cache and cache_block_stride are aligned to 16 bytes (4/4), 4 (8/4) or 2.
+ * No counterpart in the reference (its backend rotates q and k in a launch of their own).
+ */
+int tq4_rope_store(const void *query, void *query_out, const void *key, const void *value, int dtype,
+                   int64_t query_stride, int64_t key_stride, int64_t value_stride, const int64_t *positions,
+                   int64_t axis_stride, int axes, const int32_t *axis_of, const void *cos_sin,
+                   int cos_sin_dtype, int table_rows, int rot_dim, int neox, const int32_t *slot_mapping,
+                   const float *rot_t, const float *midpoints, const float *centroids, uint8_t *kv_cache,
+                   int num_blocks, int N, int Hq, int Hk, int D, int block_size, int64_t cache_block_stride,
+                   int layout, int norm_correction, int key_bits, int value_bits, tq4_stream_t stream);
+
+/*
  * Decode step of a layer with a sliding window: the query, the sequence's last token, attends to
  * tokens t with t < first_tokens or t >= seq_lens[b] - window (window >= 1 counts the last token
  * itself; first_tokens >= 0).  Only the KV blocks of visible tokens are read; the block-table

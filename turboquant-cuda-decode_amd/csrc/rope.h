@@ -1,0 +1,540 @@
+// Appending keys and values to the quantised paged cache with the rotary position applied on the way
+// (and to the queries), gfx950.
+//
+// Of a head's 128 dims the first `rot` are rotated in rot / 2 planes: plane f turns by the angle of
+// position p in frequency f, whose cosine and sine are table[p][f] and table[p][rot / 2 + f]:
+//   (a, b) -> (a cos - b sin, b cos + a sin),
+// (a, b) being dims (f, f + rot / 2), or (2 f, 2 f + 1) when planes are adjacent pairs.  With several axes
+// every frequency belongs to one, and p is the token's position on it.  K then goes through the writer of
+// store.h (norm, rotation, midpoints, norm correction; FP8 keys: the cast) and V as it is.
+//
+// Against a rotary launch before the writer, K is neither written nor read again, and is not rounded to
+// its type on the way.  The bytes are those of the definition in 64 bits: the writer's fp32-grade path
+// (f16 hi + lo products) works out every row, and what lies next to a border is worked out again in fp64
+// by the whole wave (Exact): y within kNearY of a midpoint (y is off by less: the split operands by
+// 2^-22 sum |x R| <= 2.4e-7, the sums by a few 2^-24), and a K scalar whose fp16 rounding changes within
+// 2^-19 of it (its sums of at most 32 squares are off by less than 2^-20).  Gaussian keys: one element in 15000
+// and one row in 200 (4-bit keys).  FP8 keys are rotated in fp64 throughout and rounded to fp32,
+// then to E4M3.  Rows whose squares underflow fp32 (norms below 1e-19) count as zero.  Queries: fp32, rounded once.
+//
+// Layout: the writer's lane (n, g) holds 32 dims of row n; which 32 is free for the contraction, so it
+// takes the chunks (8 dims) of planes 16 g .. 16 g + 15, both members of each: unit u = 2 g, 2 g + 1 of a row is the two
+// chunks whose dims are rotated with each other and 8 frequencies (units past rot / 16: 16 dims that are
+// not rotated).  A query thread takes one unit of one row.  The query rows' workgroups come behind the writer's
+// in one launch.
+#pragma once
+#include "store.h"
+
+namespace tq4 {
+namespace rope {
+
+using store::Chunk;
+using store::half8;
+
+constexpr float kNearY = 1e-6f;
+constexpr int kQueryRows = 32;  // rows (token, head) of 128 dims that a wave takes at a time
+constexpr int kMostAxes = 4;
+
+struct Args {
+    const void *query;            // may be null
+    void *query_out;              // [tokens, num_q_heads, 128], contiguous
+    const void *key, *value;
+    int64_t q_stride, k_stride, v_stride;  // elements from token to token
+    const int64_t *positions;     // [axes][tokens], axes axis_stride apart
+    int64_t axis_stride;
+    const void *table;            // [table_rows][rot]: cosines, sines
+    const int32_t *slots;
+    const float *pit, *midpoints, *centroids;
+    uint8_t *cache;
+    int64_t block_stride, num_slots;
+    uint64_t axis_bit[2];         // bits 0 and 1 of frequency f's axis at bit f
+    int axes, table_rows, table_f32, rot, neox;
+    int tokens, num_q_heads, num_kv_heads, block_size, slot_pos, slot_head, norm_correction;
+    int store_groups;             // workgroups of the writer; the rest rotate queries
+};
+
+// ---- Planes -----------------------------------------------------------------------------
+// Chunk (of 8 dims) of member m of unit u.
+__device__ __forceinline__ int unit_chunk(const Args &a, int u, int m) {
+    const int r = a.rot >> 4;  // rotated units
+    return u < r ? (a.neox ? u + (m ? r : 0) : 2 * u + m) : 2 * u + m;
+}
+// (Rotated units first: u >= r is chunks 2 r + 2 (u - r) + m = 2 u + m.)
+
+// The token's position on axis x; a token with one outside the table has none (`ok` false).
+__device__ __forceinline__ int position(const Args &a, int tok, int x, bool &ok) {
+    const int64_t p = a.positions[(int64_t)x * a.axis_stride + tok];
+    ok = ok && p >= 0 && p < a.table_rows;
+    return p >= 0 && p < a.table_rows ? (int)p : 0;
+}
+template <class T> __device__ __forceinline__ float table_at(const Args &a, int row, int col) {
+    const int64_t i = (int64_t)row * a.rot + col;
+    return a.table_f32 ? static_cast<const float *>(a.table)[i] : (float)static_cast<const T *>(a.table)[i];
+}
+// Eight consecutive entries (col a multiple of 8).
+template <class T> __device__ __forceinline__ void table_row8(const Args &a, int row, int col, float (&v)[8]) {
+    const int64_t i = (int64_t)row * a.rot + col;
+    if (sizeof(T) == 4 || a.table_f32) {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.table) + i);
+        const float4 x = p[0], y = p[1];
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        const t8 x = *reinterpret_cast<const t8 *>(static_cast<const T *>(a.table) + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = (float)x[j];
+    }
+}
+// Cosines and sines of frequencies 8 u .. 8 u + 7 for a token (u < rot / 16).  pos: its positions.
+template <class T>
+__device__ __forceinline__ void unit_angles(const Args &a, const int (&pos)[kMostAxes], int u, float (&c)[8], float (&s)[8]) {
+    if (a.axes == 1) {
+        table_row8<T>(a, pos[0], 8 * u, c);
+        table_row8<T>(a, pos[0], a.rot / 2 + 8 * u, s);
+        return;
+    }
+    const uint32_t b0 = (uint32_t)(a.axis_bit[0] >> (8 * u)) & 0xFFu, b1 = (uint32_t)(a.axis_bit[1] >> (8 * u)) & 0xFFu;
+#pragma unroll
+    for (int x = 0; x < kMostAxes; ++x) {
+        const uint32_t mine = (x & 1 ? b0 : ~b0) & (x & 2 ? b1 : ~b1) & 0xFFu;
+        if (x >= a.axes || mine == 0)
+            continue;
+        float cx[8], sx[8];
+        table_row8<T>(a, pos[x], 8 * u, cx);
+        table_row8<T>(a, pos[x], a.rot / 2 + 8 * u, sx);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            c[j] = (mine >> j) & 1 ? cx[j] : c[j];
+            s[j] = (mine >> j) & 1 ? sx[j] : s[j];
+        }
+    }
+}
+// A unit's two chunks x0, x1 rotated in place.
+template <class F>
+__device__ __forceinline__ void turn(float (&x0)[8], float (&x1)[8], const float (&c)[8], const float (&s)[8], bool neox, F plane) {
+    if (neox) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            plane(x0[j], x1[j], c[j], s[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            plane(x0[2 * j], x0[2 * j + 1], c[j], s[j]);
+            plane(x1[2 * j], x1[2 * j + 1], c[4 + j], s[4 + j]);
+        }
+    }
+}
+__device__ __forceinline__ void plane32(float &a, float &b, float c, float s) {
+    const float x = fmaf(a, c, -(b * s)), y = fmaf(b, c, a * s);
+    a = x;
+    b = y;
+}
+// (a and b cos and sin have at most 48 bits: exact products, one rounding of each sum, one to fp32)
+__device__ __forceinline__ void plane64(float &a, float &b, float c, float s) {
+    const double x = (double)a * c - (double)b * s, y = (double)b * c + (double)a * s;
+    a = (float)x;
+    b = (float)y;
+}
+
+// 8 elements.
+template <class T> struct Eight {
+    uint4 u[sizeof(T) / 2];
+};
+template <class T> __device__ __forceinline__ Eight<T> load8(const T *p) {
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        r.u[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
+}
+template <class T> __device__ __forceinline__ void floats8(float (&x)[8], const Eight<T> &r) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint32_t w[4] = {r.u[i].x, r.u[i].y, r.u[i].z, r.u[i].w};
+#pragma unroll
+        for (int e = 0; e < 16 / (int)sizeof(T); ++e) {
+            if constexpr (sizeof(T) == 4)
+                x[4 * i + e] = __builtin_bit_cast(float, w[e]);
+            else
+                x[e] = (float)__builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e % 2))));
+        }
+    }
+}
+template <class T> __device__ __forceinline__ void put8(T *p, const float (&x)[8]) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        v[j] = (T)x[j];
+    *reinterpret_cast<t8 *>(p) = v;
+}
+
+// ---- Queries ----------------------------------------------------------------------------
+// Waves `wave` of `waves` take kQueryRows rows at a time, 8 lanes (one unit each) a row.  A query row
+// whose token has a position outside the table becomes NaN.
+template <class T> __device__ __forceinline__ void rotate_queries(const Args &a, int wave, int waves, int lane) {
+    const int rows = a.tokens * a.num_q_heads, u = lane & 7, r8 = a.rot >> 4;
+    const T *query = static_cast<const T *>(a.query);
+    T *out = static_cast<T *>(a.query_out);
+    const int c0 = 8 * unit_chunk(a, u, 0), c1 = 8 * unit_chunk(a, u, 1);
+    constexpr int kSteps = kQueryRows / 8;
+    for (int64_t r0 = (int64_t)wave * kQueryRows; r0 < rows; r0 += (int64_t)waves * kQueryRows) {
+        Eight<T> x0[kSteps], x1[kSteps];
+        int tok[kSteps], row[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            row[i] = (int)min(r0 + 8 * i + (lane >> 3), (int64_t)rows - 1);  // (past the end: the last one again)
+            tok[i] = row[i] / a.num_q_heads;
+            const T *q = query + tok[i] * a.q_stride + (int64_t)(row[i] - tok[i] * a.num_q_heads) * kHeadDim;
+            x0[i] = load8(q + c0);
+            x1[i] = load8(q + c1);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            int pos[kMostAxes] = {0, 0, 0, 0};
+            bool ok = true;
+#pragma unroll
+            for (int x = 0; x < kMostAxes; ++x)
+                if (x < a.axes)
+                    pos[x] = position(a, tok[i], x, ok);
+            float y0[8], y1[8];
+            floats8(y0, x0[i]);
+            floats8(y1, x1[i]);
+            if (u < r8) {
+                float c[8], s[8];
+                unit_angles<T>(a, pos, u, c, s);
+                turn(y0, y1, c, s, a.neox != 0, plane32);
+            }
+            if (!ok)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    y0[j] = y1[j] = __builtin_nanf("");
+            // (rows past the end are not written, so that out may be query itself)
+            if (r0 + 8 * i + (lane >> 3) < rows) {
+                T *o = out + (int64_t)row[i] * kHeadDim;
+                put8(o + c0, y0);
+                put8(o + c1, y1);
+            }
+        }
+    }
+}
+
+// ---- Keys and values --------------------------------------------------------------------
+template <class T> struct RawKey {
+    Eight<T> c[4];  // member m of unit 2 g + i at c[2 i + m]
+};
+template <class T> struct Row {
+    const T *key, *value;
+    int tok, head;
+};
+template <class T> __device__ __forceinline__ Row<T> row_at(const Args &a, int row, bool in_range) {
+    Row<T> r;
+    r.tok = in_range ? row / a.num_kv_heads : 0;
+    r.head = in_range ? row - r.tok * a.num_kv_heads : 0;
+    r.key = static_cast<const T *>(a.key) + r.tok * a.k_stride + r.head * kHeadDim;
+    r.value = static_cast<const T *>(a.value) + r.tok * a.v_stride + r.head * kHeadDim;
+    return r;
+}
+// (rows past the end read the first one and are not stored)
+template <class T> __device__ __forceinline__ void load_key(RawKey<T> &k, const T *key, const int (&chunk)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        k.c[i] = load8(key + 8 * chunk[i]);
+}
+// The rotated K of the lane's 32 dims (chunk i at x[8 i ..]); ok: the token's positions are in the table.
+template <class T, class F>
+__device__ __forceinline__ void turned_key(float (&x)[32], const RawKey<T> &k, const Args &a, int tok, int g, bool &ok, F plane) {
+    int pos[kMostAxes] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kMostAxes; ++i)
+        if (i < a.axes)
+            pos[i] = position(a, tok, i, ok);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x0[8], x1[8];
+        floats8(x0, k.c[2 * i]);
+        floats8(x1, k.c[2 * i + 1]);
+        if (2 * g + i < a.rot >> 4) {
+            float c[8], s[8];
+            unit_angles<T>(a, pos, 2 * g + i, c, s);
+            turn(x0, x1, c, s, a.neox != 0, plane);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[16 * i + j] = x0[j];
+            x[16 * i + 8 + j] = x1[j];
+        }
+    }
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1)
+        v += __shfl_xor(v, m, kWave);
+    return v;
+}
+// A row in fp64, worked out by the wave: lane f < rot / 2 has plane f, the others two dims each that are
+// not rotated.
+template <class T> struct Exact {
+    double x0, x1, norm;
+    int d0, d1;
+    __device__ __forceinline__ Exact(const Args &a, int row, int lane) {
+        const Row<T> r = row_at<T>(a, row, true);
+        const int half = a.rot / 2;
+        const bool turned = lane < half;
+        d0 = turned && a.neox ? lane : 2 * lane;  // (not rotated: rot + 2 (lane - half) = 2 lane)
+        d1 = turned && a.neox ? lane + half : 2 * lane + 1;
+        const double p = (double)(float)r.key[d0], q = (double)(float)r.key[d1];
+        x0 = p;
+        x1 = q;
+        if (turned) {
+            const int axis = a.axes == 1 ? 0 : (int)(a.axis_bit[0] >> lane & 1) + 2 * (int)(a.axis_bit[1] >> lane & 1);
+            bool ok = true;
+            const int pos = position(a, r.tok, axis, ok);
+            const double c = table_at<T>(a, pos, lane), s = table_at<T>(a, pos, half + lane);
+            x0 = p * c - q * s;
+            x1 = q * c + p * s;
+        }
+        norm = sqrt(wave_sum64(x0 * x0 + x1 * x1));
+    }
+    __device__ __forceinline__ double y(const float *pit, int dim) const {
+        return wave_sum64(x0 * pit[d0 * kHeadDim + dim] + x1 * pit[d1 * kHeadDim + dim]) / (norm + 1e-8);
+    }
+};
+
+// Code j of packed words.
+template <int KB> __device__ __forceinline__ uint32_t code_at(const uint32_t (&w)[KB], int j) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+        const int sh = KB * j - 32 * i;
+        if (sh > -KB && sh < 32)
+            v |= sh >= 0 ? w[i] >> sh : w[i] << -sh;
+    }
+    return v & ((1u << KB) - 1);
+}
+template <int KB> __device__ __forceinline__ void flip_code(uint32_t (&w)[KB], int j, uint32_t d) {
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+        const int sh = KB * j - 32 * i;
+        if (sh > -KB && sh < 32)
+            w[i] ^= sh >= 0 ? d << sh : d >> -sh;
+    }
+}
+
+// The writer's tile loop.  W: waves per workgroup (see store_kernel).
+template <int LAYOUT, class T, int KB, int VB, int W>
+__device__ __forceinline__ void store_rows(const Args &a, int group, int groups) {
+    using namespace store;
+    __shared__ __align__(16) _Float16 pt_hi[kHeadDim * kHeadDim];
+    __shared__ __align__(16) _Float16 pt_lo[kHeadDim * kHeadDim];
+    __shared__ float c2tab[16];
+    __shared__ __align__(16) float2 btab[kCells];
+    constexpr int kMids = (1 << KB) - 1;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int n = lane & 15, g = lane >> 4;
+    const int rows = a.tokens * a.num_kv_heads, tiles = (rows + kRows - 1) / kRows, stride = groups * W;
+    int tile = group * W + wave;
+    Book<KB> book;
+    load_book<KB>(book, a.midpoints, a.centroids, a.norm_correction);
+    PitLoads<W> pw;
+    load_pit<W>(pw, a.pit);
+    __builtin_amdgcn_sched_barrier(0);
+    int chunk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        chunk[i] = unit_chunk(a, 2 * g + (i >> 1), i & 1);
+    RawKey<T> kr;
+    Chunk<T> vr;
+    Row<T> at = row_at<T>(a, tile * kRows + n, tile < tiles && tile * kRows + n < rows);
+    constexpr bool kEarlyV = sizeof(T) < 4;
+    load_key<T>(kr, at.key, chunk);
+    if constexpr (kEarlyV)
+        load_raw(vr, at.value + 32 * g, true);
+    __builtin_amdgcn_sched_barrier(0);
+    store_pit<W>(pw, pt_hi, pt_lo);
+    const Cells cells = build_cells<KB>(book, a.norm_correction, c2tab, btab);
+
+    for (; tile < tiles; tile += stride) {
+        const int row = tile * kRows + n;
+        const bool in_range = row < rows;
+        const int tok = at.tok, head = at.head;
+        bool ok = in_range;
+        float x[32];
+        turned_key<T>(x, kr, a, tok, g, ok, plane32);
+        // (four sums: an error of 8 roundings each)
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            s4[i & 3] = fmaf(x[i], x[i], s4[i & 3]);
+        const float norm = sqrtf(row_sum((s4[0] + s4[1]) + (s4[2] + s4[3])));
+        const float rn = 16.f / (norm + 1e-8f);
+        half8 b_hi[4], b_lo[4];
+        split_x(x, rn, b_hi, b_lo);
+        floatx4 acc[8];
+        rotate_tile(acc, b_hi, b_lo, pt_hi, pt_lo, n, [&](int kb) { return chunk[kb]; });
+        uint32_t kw[KB];
+        float csq, nearest = __builtin_inff();
+        code_keys<KB, true>(acc, cells, book, btab, c2tab, kw, csq, nearest);
+        const int slot = ok ? a.slots[tok] : -1;
+        const bool live = slot >= 0 && slot < a.num_slots;
+        // elements next to a midpoint (a zero row has y = 0 exactly)
+        constexpr float kNear = 256.f * kNearY;
+        bool near = live && norm > 0.f && nearest < kNear;
+        if (__builtin_expect(__any(near), 0)) {
+            uint32_t which = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float v = acc[j / 4][j % 4];
+                float d = __builtin_inff();
+                if (cells.use)
+                    d = fminf(d, fabsf(v - cell_of(v, cells, btab).x));
+                else
+#pragma unroll
+                    for (int i = 0; i < kMids; ++i)
+                        d = fminf(d, fabsf(v - 256.f * book.mid[i]));
+                which |= d < 2.f * kNear ? 1u << j : 0u;  // (the other path's roundings of the same distance)
+            }
+            for (uint64_t todo = __ballot(near); todo; todo &= todo - 1) {
+                const int l = __builtin_ctzll(todo);
+                const Exact<T> r(a, tile * kRows + (l & 15), lane);
+                for (uint32_t bits = (uint32_t)__builtin_amdgcn_readlane((int)which, l); bits; bits &= bits - 1) {
+                    const int j = __builtin_ctz(bits);
+                    const double y = r.y(a.pit, 32 * (l >> 4) + j);
+                    uint32_t idx = 0;
+#pragma unroll
+                    for (int i = 0; i < kMids; ++i)
+                        idx += (double)book.mid[i] <= y ? 1u : 0u;
+                    const uint32_t old = code_at<KB>(kw, j);
+                    if (lane == l && idx != old) {
+                        flip_code<KB>(kw, j, idx ^ old);
+                        csq += c2tab[idx] - c2tab[old];
+                    }
+                }
+            }
+        }
+        const float csum = row_sum(csq);
+        float kscalar = a.norm_correction ? norm * (1.0f / sqrtf(csum + 1e-16f)) : norm;
+        const bool torn = live && half_bits(kscalar * (1.f - 0x1p-19f)) != half_bits(kscalar * (1.f + 0x1p-19f));
+        if (__builtin_expect(__any(torn), 0)) {
+            for (uint32_t todo = (uint32_t)__ballot(torn) & 0xFFFFu; todo; todo &= todo - 1) {
+                const int m = __builtin_ctz(todo);
+                const Exact<T> r(a, tile * kRows + m, lane);
+                double c2 = 0.0;
+                if (a.norm_correction) {
+                    if (n == m)
+                        for (int j = 0; j < 32; ++j) {
+                            const double c = a.centroids[code_at<KB>(kw, j)];
+                            c2 += c * c;
+                        }
+                    c2 = wave_sum64(c2);
+                }
+                const double k = a.norm_correction ? r.norm / sqrt(c2 + 1e-16) : r.norm;
+                kscalar = n == m ? (float)k : kscalar;
+            }
+        }
+        if constexpr (!kEarlyV)
+            load_raw(vr, at.value + 32 * g, true);
+        to_floats(x, vr);
+        float scale, vmin;
+        uint32_t vw[VB];
+        quantize_v<VB>(x, vw, scale, vmin);
+        if (live)
+            put_record<LAYOUT, KB, VB>(a.cache, slot, head, g, kw, vw, kscalar, scale, vmin, a.num_kv_heads, a.block_size,
+                                       a.block_stride, a.slot_pos, a.slot_head);
+        // the next tile of this wave
+        const int nrow = (tile + stride) * kRows + n;
+        at = row_at<T>(a, nrow, tile + stride < tiles && nrow < rows);
+        load_key<T>(kr, at.key, chunk);
+        if constexpr (kEarlyV)
+            load_raw(vr, at.value + 32 * g, true);
+    }
+}
+
+// W = kWaves: large launches, two workgroups per CU; kSmallWaves: few rows (see store_kernel).
+template <int LAYOUT, class T, int KB, int VB, int W>
+__global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == store::kWaves ? 4 : 1)))
+void append_kernel(const Args a) {
+    if ((int)blockIdx.x < a.store_groups)
+        store_rows<LAYOUT, T, KB, VB, W>(a, blockIdx.x, a.store_groups);
+    else
+        rotate_queries<T>(a, (blockIdx.x - a.store_groups) * W + threadIdx.x / kWave, (gridDim.x - a.store_groups) * W,
+                          threadIdx.x % kWave);
+}
+
+// FP8 keys (see store_fp8_kernel).
+template <int LAYOUT, class T>
+__global__ __launch_bounds__(kWave *store::kFp8Waves) void append_fp8_kernel(const Args a) {
+    using namespace store;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if ((int)blockIdx.x >= a.store_groups) {
+        rotate_queries<T>(a, (blockIdx.x - a.store_groups) * kFp8Waves + wave, (gridDim.x - a.store_groups) * kFp8Waves, lane);
+        return;
+    }
+    const int n = lane & 15, g = lane >> 4;
+    const int rows = a.tokens * a.num_kv_heads, tiles = (rows + kRows - 1) / kRows;
+    int chunk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        chunk[i] = unit_chunk(a, 2 * g + (i >> 1), i & 1);
+    for (int tile = blockIdx.x * kFp8Waves + wave; tile < tiles; tile += a.store_groups * kFp8Waves) {
+        const int row = tile * kRows + n;
+        bool ok = row < rows;
+        const Row<T> at = row_at<T>(a, row, ok);
+        RawKey<T> kr;
+        Chunk<T> vr;
+        load_key<T>(kr, at.key, chunk);
+        load_raw(vr, at.value + 32 * g, true);
+        float x[32];
+        turned_key<T>(x, kr, a, at.tok, g, ok, plane64);
+        uint2 kw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float *v = x + 8 * i + 4 * h;
+                int p = __builtin_amdgcn_cvt_pk_fp8_f32(sat_e4m3(v[0]), sat_e4m3(v[1]), 0, false);
+                w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(sat_e4m3(v[2]), sat_e4m3(v[3]), p, true);
+            }
+            kw[i] = uint2{w[0], w[1]};
+        }
+        to_floats(x, vr);
+        float scale, vmin;
+        uint32_t vw[4];
+        quantize_v<4>(x, vw, scale, vmin);
+        const int slot = ok ? a.slots[at.tok] : -1;
+        if (slot < 0 || slot >= a.num_slots)
+            continue;
+        const int64_t blk = slot / a.block_size, off = slot % a.block_size;
+        uint8_t *base = a.cache + blk * a.block_stride;
+        uint32_t *r = reinterpret_cast<uint32_t *>(
+            base + (LAYOUT == 0 ? (off * a.num_kv_heads + at.head) * kFp8Record : off * a.slot_pos + (int64_t)at.head * a.slot_head));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            r[2 * chunk[i]] = kw[i].x;
+            r[2 * chunk[i] + 1] = kw[i].y;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[kHeadDim / 4 + 4 * g + i] = vw[i];
+        if (g == 0) {
+            uint16_t *f;
+            int fstride;
+            if constexpr (LAYOUT == 0) {
+                f = reinterpret_cast<uint16_t *>(base + (int64_t)a.block_size * a.num_kv_heads * kFp8Record) +
+                    (int64_t)at.head * 2 * a.block_size + off;
+                fstride = a.block_size;
+            } else {
+                f = reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(r) + kFp8Record);
+                fstride = 1;
+            }
+            f[0] = half_bits(scale);
+            f[fstride] = half_bits(vmin);
+        }
+    }
+}
+
+}  // namespace rope
+}  // namespace tq4

@@ -220,101 +220,85 @@ __device__ __forceinline__ void quantize_v(const float (&x)[32], uint32_t (&vw)[
     }
 }
 
-// KB / VB: bits per K index / V code -- 4 / 4 is the turboquant_4bit_nc layout above;
-// 3 / 4 (turboquant_k3v4_nc) and 3 / 3 (turboquant_3bit_nc) pack 8 codes in 3 bytes
-// (reference/soa_store.py:319-337, :47-83): SoA record 16 KB + 16 VB bytes, AoS slot
-// K | norm | V | scale | zero padded to even, written with 2-byte stores.
-// W: waves per workgroup.  8 for large launches (two workgroups per CU share the CU's LDS,
-// 4 waves per SIMD); 4 for launches of at most kSmallTiles tiles (a decode step's few
-// rows), so that the waves spread over twice the CUs at one wave per SIMD: a wave's tile
-// arithmetic then has its SIMD to itself, at the price of staging twice the PiT share.
-template <int LAYOUT, class T, int KB = 4, int VB = 4, int W = kWaves>
-__global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == kWaves ? 4 : 1))) void store_kernel(
-    const T *__restrict__ key, const T *__restrict__ value, const int32_t *__restrict__ slot_mapping,
-    const float *__restrict__ pit, const float *__restrict__ midpoints, const float *__restrict__ centroids,
-    uint8_t *__restrict__ cache, int rows, int num_kv_heads, int block_size, int64_t block_stride,
-    int slot_pos, int slot_head, int norm_correction) {
-    __shared__ __align__(16) _Float16 pt_hi[kHeadDim * kHeadDim];
-    __shared__ __align__(16) _Float16 pt_lo[kHeadDim * kHeadDim];
-    constexpr int kMids = (1 << KB) - 1;  // Lloyd-Max midpoints
-    __shared__ float c2tab[16];
-    __shared__ __align__(16) float2 btab[kCells];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int n = lane & 15, g = lane >> 4;
-    const int tiles = (rows + kRows - 1) / kRows;
-    const int stride = gridDim.x * W;
-    int tile = blockIdx.x * W + wave;
-
-    // Every workgroup reads PiT, the midpoints and the centroids (L2 hits after the first
-    // workgroup): their loads go out ahead of the first tile's K and V.  Those reads, across
-    // the grid, keep HBM busy for microseconds, and a staging load queued behind them would
-    // hold the workgroup's staging, and with it every wave's first tile, until they drain.
-    // (centroids may be null without norm correction: read only with it)
-    constexpr int kCents = 1 << KB;
+// The codebook of a workgroup: midpoints and centroids in registers (centroids may be null without norm
+// correction: read only with it).
+template <int KB> struct Book {
+    static constexpr int kMids = (1 << KB) - 1, kCents = 1 << KB;
     float mid[kMids], cent[kCents];
+};
+template <int KB>
+__device__ __forceinline__ void load_book(Book<KB> &b, const float *midpoints, const float *centroids, int norm_correction) {
 #pragma unroll
-    for (int i = 0; i < kMids; ++i)
-        mid[i] = midpoints[i];
+    for (int i = 0; i < b.kMids; ++i)
+        b.mid[i] = midpoints[i];
 #pragma unroll
-    for (int i = 0; i < kCents; ++i)
-        cent[i] = 0.f;
+    for (int i = 0; i < b.kCents; ++i)
+        b.cent[i] = 0.f;
     if (norm_correction) {
 #pragma unroll
-        for (int i = 0; i < kCents; ++i)
-            cent[i] = centroids[i];
+        for (int i = 0; i < b.kCents; ++i)
+            b.cent[i] = centroids[i];
     }
-    // thread (c, k8): 16 * PiT[8k8 .. 8k8+7][c] (coalesced over c) -> one 16-byte LDS write
-    // into each part
-    constexpr int kStage = kHeadDim * (kHeadDim / 8) / (kWave * W);
-    float pw[kStage][8];
+}
+
+// PiT staged by W waves.  Thread (c, k8): 16 * PiT[8k8 .. 8k8+7][c] (coalesced over c) -> one 16-byte
+// LDS write into each part.
+template <int W> struct PitLoads {
+    static constexpr int kStage = kHeadDim * (kHeadDim / 8) / (kWave * W);
+    float w[kStage][8];
+};
+template <int W> __device__ __forceinline__ void load_pit(PitLoads<W> &p, const float *__restrict__ pit) {
 #pragma unroll
-    for (int it = 0; it < kStage; ++it) {
+    for (int it = 0; it < p.kStage; ++it) {
         const int i = threadIdx.x + it * kWave * W;
         const int c = i % kHeadDim, k8 = i / kHeadDim;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            pw[it][j] = pit[(8 * k8 + j) * kHeadDim + c];
+            p.w[it][j] = pit[(8 * k8 + j) * kHeadDim + c];
     }
-    __builtin_amdgcn_sched_barrier(0);
-    constexpr bool kEarlyV = sizeof(T) < 4;
-    Chunk<T> kr, vr;
-    {
-        const int64_t row = (int64_t)tile * kRows + n;
-        load_raw(kr, key + row * kHeadDim + 32 * g, row < rows);
-        if constexpr (kEarlyV)
-            load_raw(vr, value + row * kHeadDim + 32 * g, row < rows);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-
+}
+template <int W> __device__ __forceinline__ void store_pit(const PitLoads<W> &p, _Float16 *pt_hi, _Float16 *pt_lo) {
 #pragma unroll
-    for (int it = 0; it < kStage; ++it) {
+    for (int it = 0; it < p.kStage; ++it) {
         const int i = threadIdx.x + it * kWave * W;
         const int c = i % kHeadDim, k8 = i / kHeadDim;
         half8 h, l;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float w = 16.f * pw[it][j];
+            const float w = 16.f * p.w[it][j];
             h[j] = (_Float16)w;
             l[j] = (_Float16)(w - (float)h[j]);
         }
         *reinterpret_cast<half8 *>(pt_hi + pt_off(c, k8)) = h;
         *reinterpret_cast<half8 *>(pt_lo + pt_off(c, k8)) = l;
     }
+}
+
+// The bucketize tables in LDS (c2tab: c^2 of an index, 0 without norm correction; btab: the cells) and what
+// a lookup needs; ends with the workgroup's barrier.
+struct Cells {
+    bool use;           // else the 15 (7) midpoints are counted
+    float inv_w, c0;    // biased cell coordinate y / w - K + 1.5 * 2^23 of y = acc / 256
+};
+constexpr float kCellBias = 12582912.f;  // 1.5 * 2^23: the sum's low mantissa bits hold the rounded value
+template <int KB>
+__device__ __forceinline__ Cells build_cells(const Book<KB> &book, int norm_correction, float *c2tab, float2 *btab) {
+    constexpr int kMids = Book<KB>::kMids, kCents = Book<KB>::kCents;
     // c[idx]^2 (0 without norm correction) of a lane's index, selected from the registers
     auto c2_at = [&](int idx) {
         float r = 0.f;
 #pragma unroll
         for (int i = 0; i < kCents; ++i)
-            r = idx == i ? cent[i] * cent[i] : r;
+            r = idx == i ? book.cent[i] * book.cent[i] : r;
         return norm_correction ? r : 0.f;
     };
     if (threadIdx.x <= kMids)
         c2tab[threadIdx.x] = c2_at(threadIdx.x);
-    float mmin = mid[0], mmax = mid[0];
+    float mmin = book.mid[0], mmax = book.mid[0];
 #pragma unroll
     for (int i = 1; i < kMids; ++i) {
-        mmin = fminf(mmin, mid[i]);
-        mmax = fmaxf(mmax, mid[i]);
+        mmin = fminf(mmin, book.mid[i]);
+        mmax = fmaxf(mmax, book.mid[i]);
     }
     const float w = (mmax - mmin) / (float)(kCells - 4);
     // cells centred on y0 + kw, y0 = K w with K an integer: the cell coordinate y / w - K
@@ -332,20 +316,224 @@ __global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == k
         float m_in = __builtin_nanf("");  // compares false with every y
 #pragma unroll
         for (int i = 0; i < kMids; ++i) {
-            base += mid[i] < lo ? 1 : 0;
-            if (mid[i] >= lo && mid[i] <= hi) {
+            base += book.mid[i] < lo ? 1 : 0;
+            if (book.mid[i] >= lo && book.mid[i] <= hi) {
                 ++inside;
-                m_in = mid[i];
+                m_in = book.mid[i];
             }
         }
         cell_ok = cell_ok && inside <= 1 && w > 0.f && w < __builtin_inff();
         // the midpoint is stored x 256, the scale of the rotation's results
         btab[k] = float2{256.f * m_in, __builtin_bit_cast(float, base)};
     }
-    const bool use_cells = __syncthreads_and(cell_ok) != 0;
-    // biased cell coordinate y / w - K + 1.5 * 2^23 of y = acc / 256
-    constexpr float kBias = 12582912.f;  // 1.5 * 2^23: the sum's low mantissa bits hold the rounded value
-    const float inv_w = (1.f / w) * (1.f / 256.f), c0 = kBias - kcell;
+    Cells r;
+    r.use = __syncthreads_and(cell_ok) != 0;
+    r.inv_w = (1.f / w) * (1.f / 256.f);
+    r.c0 = kCellBias - kcell;
+    return r;
+}
+__device__ __forceinline__ float2 cell_of(float a, const Cells &cells, const float2 *btab) {
+    const float t = fminf(fmaxf(fmaf(a, cells.inv_w, cells.c0), kCellBias), kCellBias + (float)(kCells - 1));
+    return btab[__builtin_bit_cast(int, t) - __builtin_bit_cast(int, kCellBias)];
+}
+
+// x (the lane's 32 dims of a row) times rn, as f16 hi and lo operands.
+__device__ __forceinline__ void split_x(const float (&x)[32], float rn, half8 (&b_hi)[4], half8 (&b_lo)[4]) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            float v0 = x[8 * kb + j] * rn, v1 = x[8 * kb + j + 1] * rn, l0, l1;
+            // The fp32 products stand in registers before the split (folded into one of the f16
+            // casts and not the other, hi + lo would be off by an f16 ulp on the products that are
+            // f16 ties), and the split is a packed cast and two mixed-precision fmas, v - hi
+            // exactly: 64 VALU fewer per tile than casting each hi twice and subtracting.
+            uint32_t h;
+            asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(h) : "v"(v0), "v"(v1));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(h), "v"(v0));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(h), "v"(v1));
+            const auto hp = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(2))), h);
+            b_hi[kb][j] = hp[0];
+            b_hi[kb][j + 1] = hp[1];
+            b_lo[kb][j] = (_Float16)l0;
+            b_lo[kb][j + 1] = (_Float16)l1;
+        }
+}
+
+// y^T = PiT^T x_hat^T of a tile: step kb contracts the 8 dims of chunk(kb) of every lane.
+template <typename Chunk8>
+__device__ __forceinline__ void rotate_tile(floatx4 (&acc)[8], const half8 (&b_hi)[4], const half8 (&b_lo)[4],
+                                            const _Float16 *pt_hi, const _Float16 *pt_lo, int n, Chunk8 chunk) {
+    // column block cb: MFMA row r <-> dim 32(r/4) + 4cb + r%4 (lane (n, g) feeds row n).
+    // The operand reads are the same for every tile; an opaque base keeps them in the loop
+    // (hoisted, they would hold 256 VGPRs).
+    int ldsb = 0;
+    asm volatile("" : "+v"(ldsb));
+#pragma unroll
+    for (int cb = 0; cb < 8; ++cb) {
+        acc[cb] = floatx4{0.f, 0.f, 0.f, 0.f};
+        const int c = 32 * (n >> 2) + 4 * cb + (n & 3);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const int off = ldsb + pt_off(c, chunk(kb));
+            const half8 a_hi = *reinterpret_cast<const half8 *>(pt_hi + off);
+            const half8 a_lo = *reinterpret_cast<const half8 *>(pt_lo + off);
+            acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_hi, b_hi[kb], acc[cb], 0, 0, 0);
+            acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_lo, b_hi[kb], acc[cb], 0, 0, 0);
+            acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_hi, b_lo[kb], acc[cb], 0, 0, 0);
+        }
+    }
+}
+
+// K indices at KB bits of the lane's 32 dims (4 bits: element j at bits 4(j % 8) of word j / 8) from 256 y,
+// and the lane's sum of c[idx]^2.  NEAR: nearest (in) takes the smallest |256 (y - midpoint)|.
+template <int KB, bool NEAR>
+__device__ __forceinline__ void code_keys(const floatx4 (&acc)[8], const Cells &cells, const Book<KB> &book,
+                                          const float2 *btab, const float *c2tab, uint32_t (&kw)[KB], float &csq,
+                                          float &nearest) {
+#pragma unroll
+    for (int q = 0; q < KB; ++q)
+        kw[q] = 0u;
+    csq = 0.f;
+    if (cells.use) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            int idx[8];
+#pragma unroll
+            for (int j = 8 * q; j < 8 * q + 8; ++j) {
+                const float a = acc[j / 4][j % 4];
+                const float2 e = cell_of(a, cells, btab);
+                idx[j % 8] = __builtin_bit_cast(int, e.y) + (a >= e.x ? 1 : 0);
+                if constexpr (NEAR)
+                    nearest = fminf(nearest, fabsf(a - e.x));  // (no midpoint: NaN, passed over)
+                put_code<KB>(kw, j, (uint32_t)idx[j % 8]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                csq += c2tab[idx[j]];
+            // at most 8 table reads in flight
+            asm volatile("" ::: "memory");
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float y = acc[j / 4][j % 4] * (1.f / 256.f);
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < book.kMids; ++i) {
+                c += y >= book.mid[i] ? 1 : 0;
+                if constexpr (NEAR)
+                    nearest = fminf(nearest, fabsf(256.f * (y - book.mid[i])));
+            }
+            put_code<KB>(kw, j, (uint32_t)c);
+            csq += c2tab[c];
+        }
+    }
+}
+
+// The row's codes and scalars into cache slot `slot` (not negative); lane group g holds dims 32g ..
+template <int LAYOUT, int KB, int VB>
+__device__ __forceinline__ void put_record(uint8_t *__restrict__ cache, int slot, int head, int g, const uint32_t (&kw)[KB],
+                                           const uint32_t (&vw)[VB], float kscalar, float scale, float vmin,
+                                           int num_kv_heads, int block_size, int64_t block_stride, int slot_pos,
+                                           int slot_head) {
+    const int64_t blk = slot / block_size, off = slot % block_size;
+    uint8_t *base = cache + blk * block_stride;
+    if constexpr (KB != 4 || VB != 4) {
+        constexpr int kK = 16 * KB, kV = 16 * VB;
+        if constexpr (LAYOUT == 0) {
+            uint8_t *rec = base + (off * num_kv_heads + head) * (kK + kV);
+            store_words_a2(rec + 4 * KB * g, kw);
+            store_words_a2(rec + kK + 4 * VB * g, vw);
+            if (g == 0) {
+                uint16_t *meta = reinterpret_cast<uint16_t *>(base + (int64_t)block_size * num_kv_heads * (kK + kV)) +
+                                 (int64_t)head * 3 * block_size + off;
+                meta[0] = half_bits(kscalar);
+                meta[block_size] = half_bits(scale);
+                meta[2 * block_size] = half_bits(vmin);
+            }
+        } else {
+            uint8_t *sl = base + off * slot_pos + (int64_t)head * slot_head;
+            store_words_a2(sl + 4 * KB * g, kw);
+            store_words_a2(sl + kK + 2 + 4 * VB * g, vw);
+            if (g == 0) {
+                reinterpret_cast<uint16_t *>(sl + kK)[0] = half_bits(kscalar);
+                reinterpret_cast<uint16_t *>(sl + kK + 2 + kV)[0] = half_bits(scale);
+                reinterpret_cast<uint16_t *>(sl + kK + 4 + kV)[0] = half_bits(vmin);
+            }
+        }
+    } else {
+        const uint4 kb = uint4{kw[0], kw[KB > 1 ? 1 : 0], kw[KB > 2 ? 2 : 0], kw[KB > 3 ? 3 : 0]},
+                    vb = uint4{vw[0], vw[VB > 1 ? 1 : 0], vw[VB > 2 ? 2 : 0], vw[VB > 3 ? 3 : 0]};
+        if constexpr (LAYOUT == 0) {
+            uint8_t *rec = base + (off * num_kv_heads + head) * kSoaRecord;
+            *reinterpret_cast<uint4 *>(rec + 16 * g) = kb;
+            *reinterpret_cast<uint4 *>(rec + kHalfD + 16 * g) = vb;
+            if (g == 0) {
+                uint16_t *meta = reinterpret_cast<uint16_t *>(base + (int64_t)block_size * num_kv_heads * kSoaRecord) +
+                                 (int64_t)head * 3 * block_size + off;
+                meta[0] = half_bits(kscalar);
+                meta[block_size] = half_bits(scale);
+                meta[2 * block_size] = half_bits(vmin);
+            }
+        } else {
+            uint8_t *sl = base + off * slot_pos + (int64_t)head * slot_head;
+            store16_a2(sl + 16 * g, kb);
+            store16_a2(sl + kHalfD + 2 + 16 * g, vb);
+            if (g == 0) {
+                reinterpret_cast<uint16_t *>(sl + kHalfD)[0] = half_bits(kscalar);
+                reinterpret_cast<uint16_t *>(sl + kHeadDim + 2)[0] = half_bits(scale);
+                reinterpret_cast<uint16_t *>(sl + kHeadDim + 4)[0] = half_bits(vmin);
+            }
+        }
+    }
+}
+
+// KB / VB: bits per K index / V code -- 4 / 4 is the turboquant_4bit_nc layout above;
+// 3 / 4 (turboquant_k3v4_nc) and 3 / 3 (turboquant_3bit_nc) pack 8 codes in 3 bytes
+// (reference/soa_store.py:319-337, :47-83): SoA record 16 KB + 16 VB bytes, AoS slot
+// K | norm | V | scale | zero padded to even, written with 2-byte stores.
+// W: waves per workgroup.  8 for large launches (two workgroups per CU share the CU's LDS,
+// 4 waves per SIMD); 4 for launches of at most kSmallTiles tiles (a decode step's few
+// rows), so that the waves spread over twice the CUs at one wave per SIMD: a wave's tile
+// arithmetic then has its SIMD to itself, at the price of staging twice the PiT share.
+template <int LAYOUT, class T, int KB = 4, int VB = 4, int W = kWaves>
+__global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == kWaves ? 4 : 1))) void store_kernel(
+    const T *__restrict__ key, const T *__restrict__ value, const int32_t *__restrict__ slot_mapping,
+    const float *__restrict__ pit, const float *__restrict__ midpoints, const float *__restrict__ centroids,
+    uint8_t *__restrict__ cache, int rows, int num_kv_heads, int block_size, int64_t block_stride,
+    int slot_pos, int slot_head, int norm_correction) {
+    __shared__ __align__(16) _Float16 pt_hi[kHeadDim * kHeadDim];
+    __shared__ __align__(16) _Float16 pt_lo[kHeadDim * kHeadDim];
+    __shared__ float c2tab[16];
+    __shared__ __align__(16) float2 btab[kCells];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int n = lane & 15, g = lane >> 4;
+    const int tiles = (rows + kRows - 1) / kRows;
+    const int stride = gridDim.x * W;
+    int tile = blockIdx.x * W + wave;
+
+    // Every workgroup reads PiT, the midpoints and the centroids (L2 hits after the first
+    // workgroup): their loads go out ahead of the first tile's K and V.  Those reads, across
+    // the grid, keep HBM busy for microseconds, and a staging load queued behind them would
+    // hold the workgroup's staging, and with it every wave's first tile, until they drain.
+    Book<KB> book;
+    load_book<KB>(book, midpoints, centroids, norm_correction);
+    PitLoads<W> pw;
+    load_pit<W>(pw, pit);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr bool kEarlyV = sizeof(T) < 4;
+    Chunk<T> kr, vr;
+    {
+        const int64_t row = (int64_t)tile * kRows + n;
+        load_raw(kr, key + row * kHeadDim + 32 * g, row < rows);
+        if constexpr (kEarlyV)
+            load_raw(vr, value + row * kHeadDim + 32 * g, row < rows);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    store_pit<W>(pw, pt_hi, pt_lo);
+    const Cells cells = build_cells<KB>(book, norm_correction, c2tab, btab);
 
     for (; tile < tiles; tile += stride) {
         const int row = tile * kRows + n;
@@ -365,82 +553,13 @@ __global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == k
         // x_hat * 16 (16 is an exact power-of-two scale)
         const float rn = 16.f / (norm + 1e-8f);
         half8 b_hi[4], b_lo[4];
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float v0 = x[8 * kb + j] * rn, v1 = x[8 * kb + j + 1] * rn, l0, l1;
-                // The fp32 products stand in registers before the split (folded into one of the f16
-                // casts and not the other, hi + lo would be off by an f16 ulp on the products that are
-                // f16 ties), and the split is a packed cast and two mixed-precision fmas, v - hi
-                // exactly: 64 VALU fewer per tile than casting each hi twice and subtracting.
-                uint32_t h;
-                asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(h) : "v"(v0), "v"(v1));
-                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(h), "v"(v0));
-                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(h), "v"(v1));
-                const auto hp = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(2))), h);
-                b_hi[kb][j] = hp[0];
-                b_hi[kb][j + 1] = hp[1];
-                b_lo[kb][j] = (_Float16)l0;
-                b_lo[kb][j + 1] = (_Float16)l1;
-            }
-        // column block cb: MFMA row r <-> dim 32(r/4) + 4cb + r%4 (lane (n, g) feeds row n).
-        // The operand reads are the same for every tile; an opaque base keeps them in the loop
-        // (hoisted, they would hold 256 VGPRs).
-        int ldsb = 0;
-        asm volatile("" : "+v"(ldsb));
+        split_x(x, rn, b_hi, b_lo);
         floatx4 acc[8];
-#pragma unroll
-        for (int cb = 0; cb < 8; ++cb) {
-            acc[cb] = floatx4{0.f, 0.f, 0.f, 0.f};
-            const int c = 32 * (n >> 2) + 4 * cb + (n & 3);
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-                const int off = ldsb + pt_off(c, 4 * g + kb);
-                const half8 a_hi = *reinterpret_cast<const half8 *>(pt_hi + off);
-                const half8 a_lo = *reinterpret_cast<const half8 *>(pt_lo + off);
-                acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_hi, b_hi[kb], acc[cb], 0, 0, 0);
-                acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_lo, b_hi[kb], acc[cb], 0, 0, 0);
-                acc[cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a_hi, b_lo[kb], acc[cb], 0, 0, 0);
-            }
-        }
+        rotate_tile(acc, b_hi, b_lo, pt_hi, pt_lo, n, [&](int kb) { return 4 * g + kb; });
         // lane (n, g): acc[j / 4][j % 4] = 256 * y[row n][32g + j]
-        // K indices at KB bits (4 bits: element j at bits 4(j % 8) of word j / 8)
         uint32_t kw[KB];
-#pragma unroll
-        for (int q = 0; q < KB; ++q)
-            kw[q] = 0u;
-        float csq = 0.f;
-        if (use_cells) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                int idx[8];
-#pragma unroll
-                for (int j = 8 * q; j < 8 * q + 8; ++j) {
-                    const float a = acc[j / 4][j % 4];
-                    const float t = fminf(fmaxf(fmaf(a, inv_w, c0), kBias), kBias + (float)(kCells - 1));
-                    const float2 e = btab[__builtin_bit_cast(int, t) - __builtin_bit_cast(int, kBias)];
-                    idx[j % 8] = __builtin_bit_cast(int, e.y) + (a >= e.x ? 1 : 0);
-                    put_code<KB>(kw, j, (uint32_t)idx[j % 8]);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    csq += c2tab[idx[j]];
-                // at most 8 table reads in flight
-                asm volatile("" ::: "memory");
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float y = acc[j / 4][j % 4] * (1.f / 256.f);
-                int c = 0;
-#pragma unroll
-                for (int i = 0; i < kMids; ++i)
-                    c += y >= mid[i] ? 1 : 0;
-                put_code<KB>(kw, j, (uint32_t)c);
-                csq += c2tab[c];
-            }
-        }
+        float csq, unused = 0.f;
+        code_keys<KB, false>(acc, cells, book, btab, c2tab, kw, csq, unused);
         const float csum = row_sum(csq);
         const float kscalar = norm_correction ? norm * (1.0f / sqrtf(csum + 1e-16f)) : norm;
 
@@ -452,60 +571,9 @@ __global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == k
         uint32_t vw[VB];
         quantize_v<VB>(x, vw, scale, vmin);
         const int slot = in_range ? slot_mapping[tok] : -1;
-        if (KB != 4 || VB != 4) {
-            if (slot >= 0) {
-                const int64_t blk = slot / block_size, off = slot % block_size;
-                uint8_t *base = cache + blk * block_stride;
-                constexpr int kK = 16 * KB, kV = 16 * VB;
-                if constexpr (LAYOUT == 0) {
-                    uint8_t *rec = base + (off * num_kv_heads + head) * (kK + kV);
-                    store_words_a2(rec + 4 * KB * g, kw);
-                    store_words_a2(rec + kK + 4 * VB * g, vw);
-                    if (g == 0) {
-                        uint16_t *meta = reinterpret_cast<uint16_t *>(base + (int64_t)block_size * num_kv_heads * (kK + kV)) +
-                                         (int64_t)head * 3 * block_size + off;
-                        meta[0] = half_bits(kscalar);
-                        meta[block_size] = half_bits(scale);
-                        meta[2 * block_size] = half_bits(vmin);
-                    }
-                } else {
-                    uint8_t *sl = base + off * slot_pos + (int64_t)head * slot_head;
-                    store_words_a2(sl + 4 * KB * g, kw);
-                    store_words_a2(sl + kK + 2 + 4 * VB * g, vw);
-                    if (g == 0) {
-                        reinterpret_cast<uint16_t *>(sl + kK)[0] = half_bits(kscalar);
-                        reinterpret_cast<uint16_t *>(sl + kK + 2 + kV)[0] = half_bits(scale);
-                        reinterpret_cast<uint16_t *>(sl + kK + 4 + kV)[0] = half_bits(vmin);
-                    }
-                }
-            }
-        } else if (slot >= 0) {
-            const int64_t blk = slot / block_size, off = slot % block_size;
-            uint8_t *base = cache + blk * block_stride;
-            const uint4 kb = uint4{kw[0], kw[KB > 1 ? 1 : 0], kw[KB > 2 ? 2 : 0], kw[KB > 3 ? 3 : 0]},
-                        vb = uint4{vw[0], vw[VB > 1 ? 1 : 0], vw[VB > 2 ? 2 : 0], vw[VB > 3 ? 3 : 0]};
-            if constexpr (LAYOUT == 0) {
-                uint8_t *rec = base + (off * num_kv_heads + head) * kSoaRecord;
-                *reinterpret_cast<uint4 *>(rec + 16 * g) = kb;
-                *reinterpret_cast<uint4 *>(rec + kHalfD + 16 * g) = vb;
-                if (g == 0) {
-                    uint16_t *meta = reinterpret_cast<uint16_t *>(base + (int64_t)block_size * num_kv_heads * kSoaRecord) +
-                                     (int64_t)head * 3 * block_size + off;
-                    meta[0] = half_bits(kscalar);
-                    meta[block_size] = half_bits(scale);
-                    meta[2 * block_size] = half_bits(vmin);
-                }
-            } else {
-                uint8_t *sl = base + off * slot_pos + (int64_t)head * slot_head;
-                store16_a2(sl + 16 * g, kb);
-                store16_a2(sl + kHalfD + 2 + 16 * g, vb);
-                if (g == 0) {
-                    reinterpret_cast<uint16_t *>(sl + kHalfD)[0] = half_bits(kscalar);
-                    reinterpret_cast<uint16_t *>(sl + kHeadDim + 2)[0] = half_bits(scale);
-                    reinterpret_cast<uint16_t *>(sl + kHeadDim + 4)[0] = half_bits(vmin);
-                }
-            }
-        }
+        if (slot >= 0)
+            put_record<LAYOUT, KB, VB>(cache, slot, head, g, kw, vw, kscalar, scale, vmin, num_kv_heads, block_size,
+                                       block_stride, slot_pos, slot_head);
         // the next tile of this wave
         load_raw(kr, key + nrow * kHeadDim + 32 * g, nrow < rows);
         if constexpr (kEarlyV)

@@ -12,7 +12,7 @@ __all__ = [
     "launch_aos_v1_stage1", "launch_stage2", "ext", "DecodeWorkspace", "Tq4Error", "store",
     "triton_turboquant_store", "aos_triton_turboquant_store", "turboquant_decode_attention",
     "stage1_fp8", "store_fp8", "stage1_preset", "store_preset", "window_decode", "prefix_decode",
-    "PrefixWorkspace",
+    "PrefixWorkspace", "rope_store",
 ]
 
 

@@ -32,6 +32,7 @@ EXPORTS = (
     "tq4_stage1_preset",
     "tq4_stage1_preset_ex",
     "tq4_store_preset",
+    "tq4_rope_store",
     "tq4_window_decode",
     "tq4_prefix_decode",
     "tq4_prefix_workspace_floats",
@@ -56,6 +57,8 @@ _SIGS = {
     "tq4_full_decode_preset": [_p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i,
                                _i64, _i, _i, _f, _p, _i, _i, _p],
     "tq4_store": [_p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _i, _p],
+    "tq4_rope_store": [_p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p,
+                       _i, _i, _i, _i, _i, _i, _i64, _i, _i, _i, _i, _p],
     "tq4_window_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
                           _p, _i, _i, _i, _i, _p],
     "tq4_prefix_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,

@@ -16,7 +16,7 @@ PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 LIB = PKG / "libtq4_decode.so"
-SOURCES = ("tq4_decode.hip", "span_decode.hip", "prefix_decode.hip")
+SOURCES = ("tq4_decode.hip", "span_decode.hip", "prefix_decode.hip", "rope_store.hip")
 ARCH = os.environ.get("TQ4_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -22,6 +22,8 @@ Reference call shapes kept here:
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import functools
 import math
 
 import torch
@@ -390,6 +392,136 @@ def store_preset(key, value, kv_cache, slot_mapping, rotation_t, midpoints, cent
     return kv_cache
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(dev):
+    """The tensors' device made current, where it is not (launches go to the current device)."""
+    if dev.index is None or torch.cuda.current_device() == dev.index:
+        return _NO_GUARD
+    return torch.cuda.device(dev)
+
+
+@functools.lru_cache(maxsize=64)
+def _axis_of(sections, in_turn, half):
+    """The axis of each of ``half`` frequencies, as a C array."""
+    if any(isinstance(n, bool) or not isinstance(n, int) or n < 0 for n in sections) or sum(sections) != half:
+        raise RuntimeError(f"sections must be counts of frequencies that sum to rot_dim / 2 = {half}")
+    if not 2 <= len(sections) <= 4:
+        raise RuntimeError("sections must name 2 to 4 axes")
+    n = len(sections)
+    if in_turn:
+        if any(n * s > half for s in sections[1:]):
+            raise RuntimeError("sections in turn: an axis behind the first has at most its share of the frequencies")
+        axes = [j % n if j % n and j < n * sections[j % n] else 0 for j in range(half)]
+    else:
+        axes = [a for a, s in enumerate(sections) for _ in range(s)]
+    return (ctypes.c_int32 * half)(*axes)
+
+
+def _token_rows(t, name, like, heads=None):
+    """Checks ``t`` [N, H, D]: heads contiguous, tokens any whole 16-byte pieces apart; returns its token stride."""
+    _require(t.is_cuda and t.dtype == like.dtype, f"{name} must be CUDA and of the keys' type")
+    _require(t.dim() == 3 and t.size(2) == HEAD_DIM and t.size(0) == like.size(0), f"{name} must be [N, H, {HEAD_DIM}]")
+    _require(heads is None or t.size(1) == heads, f"{name} must have the keys' heads")
+    if t.size(0) and not (t.stride(2) == 1 and (t.stride(1) == HEAD_DIM or t.size(1) == 1)):
+        raise RuntimeError(f"{name}: the heads of a token must be contiguous")
+    return t.stride(0) if t.size(0) > 1 else t.size(1) * HEAD_DIM
+
+
+def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, rotation_t=None, midpoints=None,
+               centroids=None, *, key_bits=4, value_bits=4, layout="soa", norm_correction=True, neox=True, sections=None,
+               in_turn=False, query_out=None):
+    """Rotary positions applied to ``query`` [N, Hq, D] and ``key`` [N, Hk, D], and the rotated keys and ``value``
+    written into cache slots ``slot_mapping`` [N]; returns the rotated queries (None when ``query`` is None).
+
+    ``cos_sin`` [P, rot_dim] (fp32 or the keys' type): row ``p`` holds the ``rot_dim / 2`` cosines, then sines, of
+    position ``p``.  The first ``rot_dim`` dims (a multiple of 16) of each head are rotated in planes ``f``: dims
+    ``(f, f + rot_dim / 2)`` with ``neox``, else ``(2f, 2f + 1)``.  ``positions`` int64 ``[N]``, or ``[axes, N]`` with
+    ``sections``, the number of frequencies of each axis (time, height, width), in blocks, or with ``in_turn`` dealt
+    round the axes (frequency ``j`` to axis ``j mod axes`` as long as that has any left, else to the first).
+    ``query``, ``key`` and ``value`` may be slices of one projection's output: tokens any whole 16-byte pieces apart.
+    ``query_out`` (contiguous, may be ``query`` itself) takes the queries.
+
+    Presets, layouts, ``norm_correction`` and the cache as ``store`` (4/4), ``store_preset`` (3/4, 3/3) and
+    ``store_fp8`` (``key_bits`` 8: no rotation matrix, no codebook).  K is not rounded to its type between the
+    rotation and the quantiser, and the stored bytes are those of the definition in 64 bits.  Tokens with a
+    negative slot, a slot past the cache, or a position outside the table are not written; the queries of the
+    last become NaN.  Slots must be distinct (two tokens with one slot leave either's bytes).
+    """
+    fp8 = key_bits == 8
+    if (key_bits, value_bits) not in PRESETS + ((8, 4),):
+        raise RuntimeError(f"key/value bits must be one of {PRESETS + ((8, 4),)}")
+    _require(key.is_cuda and key.dtype in DTYPES and key.dim() == 3, _KEY_SHAPE)
+    N, Hk, D = key.shape
+    k_stride = _token_rows(key, "key", key)
+    v_stride = _token_rows(value, "value", key, Hk)
+    tensors = [key, value, positions, cos_sin, kv_cache, slot_mapping]
+    q_stride = Hq = 0
+    if query is None:
+        _require(query_out is None, "query_out needs query")
+    else:
+        q_stride, Hq = _token_rows(query, "query", key), query.size(1)
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        _require(query_out.dtype == query.dtype and query_out.shape == query.shape and query_out.is_contiguous(),
+                 "query_out must match query (shape, dtype) and be contiguous")
+        tensors += [query, query_out]
+    _check_tensor(slot_mapping, "slot_mapping", torch.int32)
+    _require(slot_mapping.numel() == N, "slot_mapping must have one entry per token")
+    _require(cos_sin.is_cuda and cos_sin.dim() == 2 and cos_sin.is_contiguous() and
+             cos_sin.dtype in (torch.float32, key.dtype), "cos_sin must be [positions, rot_dim], fp32 or the keys' type")
+    rot = cos_sin.size(1)
+    _require(0 < rot <= D and rot % 16 == 0, "rot_dim must be a multiple of 16 up to the head's")
+    _require(cos_sin.size(0) > 0, "cos_sin has no rows")
+    if sections is None:
+        _require(not in_turn, "in_turn needs sections")
+        axes, axis_of, shape = 1, None, (N,)
+    else:
+        sections = tuple(sections)
+        axes, axis_of = len(sections), _axis_of(sections, bool(in_turn), rot // 2)
+        shape = (axes, N)
+    _require(positions.is_cuda and positions.dtype is torch.int64, "positions must be CUDA int64")
+    if tuple(positions.shape) != shape or (N > 1 and positions.stride(-1) != 1):
+        raise RuntimeError(f"positions must be {list(shape)}, each axis contiguous")
+    axis_stride = positions.stride(0) if axes > 1 else 0
+    if fp8:
+        norm_correction, rot_ptr, mid_ptr, cent_ptr = False, None, None, None
+    else:
+        _check_tensor(rotation_t, "rotation_t", torch.float32)
+        _check_tensor(midpoints, "midpoints", torch.float32)
+        _require(tuple(rotation_t.shape) == (D, D), _ROTATION_SHAPE)
+        n_mid = (1 << key_bits) - 1
+        if midpoints.numel() != n_mid:
+            raise RuntimeError(f"{key_bits}-bit keys need {n_mid} midpoints")
+        if norm_correction:
+            _require(centroids is not None, "norm_correction=True requires centroids")
+        cent_ptr = None
+        if centroids is not None:
+            _check_tensor(centroids, "centroids", torch.float32)
+            if centroids.numel() != n_mid + 1:
+                raise RuntimeError(f"{key_bits}-bit keys need {n_mid + 1} centroids")
+            cent_ptr = centroids.data_ptr()
+            tensors.append(centroids)
+        tensors += [rotation_t, midpoints]
+        rot_ptr, mid_ptr = rotation_t.data_ptr(), midpoints.data_ptr()
+    slot = slot_bytes_fp8(D) if fp8 else slot_bytes_preset(D, key_bits, value_bits)
+    bs, hk, stride, lid = _cache_geometry(kv_cache, slot, layout, " (FP8 keys)" if fp8 else "")
+    _require(hk == Hk, "kv_cache must be [blocks, block_size, Hk, slot]")
+    _require(_same_device(*tensors), "all tensors must be on the same device")
+    if N == 0:
+        return query_out
+    with _on_device(key.device):
+        rc = _lib.load().tq4_rope_store(
+            None if query is None else query.data_ptr(), None if query is None else query_out.data_ptr(),
+            key.data_ptr(), value.data_ptr(), DTYPES[key.dtype], q_stride, k_stride, v_stride, positions.data_ptr(),
+            axis_stride, axes, axis_of, cos_sin.data_ptr(), DTYPES[cos_sin.dtype], cos_sin.size(0), rot, int(bool(neox)),
+            slot_mapping.data_ptr(), rot_ptr, mid_ptr, cent_ptr, kv_cache.data_ptr(), kv_cache.size(0), N, Hq, Hk, D, bs,
+            stride, lid, int(bool(norm_correction)), key_bits, value_bits, _stream(key.device))
+    _lib.check(rc, "tq4_rope_store")
+    return query_out
+
+
 class DecodeWorkspace:
     """Preallocated buffers of one full decode step (fixed shapes, reusable)."""
 
@@ -474,16 +606,6 @@ def _full_decode_preset(query, rotation_t, kv_cache, block_table, seq_lens, cent
         key_bits, value_bits, _stream(query.device))
     _lib.check(rc, "tq4_full_decode_preset")
     return ws.out
-
-
-_NO_GUARD = contextlib.nullcontext()
-
-
-def _on_device(dev):
-    """The tensors' device made current, where it is not (launches go to the current device)."""
-    if dev.index is None or torch.cuda.current_device() == dev.index:
-        return _NO_GUARD
-    return torch.cuda.device(dev)
 
 
 def _int_arg(value, name, least):
