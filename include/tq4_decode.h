@@ -268,7 +268,7 @@ int tq4_store_preset(const void *key, const void *value, int dtype, const int32_
  * K is rotated exactly (not rounded to dtype before it is quantised), and the codes, E4M3 bytes and scalars are those
  * of the definition in 64 bits (rows of norm below 1e-19 count as zero); query_out is fp32, rounded once.
  * A token whose slot is negative or past num_blocks * block_size is not written; one with a position outside
- * the table is not written either, and its query rows become NaN.  Two tokens with one slot: either's bytes.
+ * the table is not written either, and its query rows become NaN.  Slots must be distinct: what two tokens leave in one is unspecified.
  * kv_cache and cache_block_stride are aligned to 16 bytes (4/4), 4 (8/4) or 2.
  * No counterpart in the reference (its backend rotates q and k in a launch of their own).
  */
@@ -300,12 +300,13 @@ int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, co
 
 /*
  * Decode step of a batch whose sequences share their first prefix_len tokens: the first
- * prefix_len / block_size entries of every row of block_table name the same blocks (those of row 0 are
- * read).  The shared tokens are read and decoded once for the query rows of all sequences; the results
- * are those of tq4_full_decode / tq4_full_decode_preset on the same arguments, the shared part with f16
- * operands (each factor rounded once, half a step of f16).  prefix_len: whole blocks, 0 up to the
- * table's width; a sequence with fewer tokens (seq_lens[b] < prefix_len, 0 included) attends to its
- * own seq_lens[b] alone and may have other blocks.  query and out are 16-bit (TQ4_BF16, TQ4_F16).
+ * prefix_len / block_size entries of block_table name the same blocks in the row of every sequence that
+ * has as many tokens.  The shared tokens are read and decoded once for the query rows of all
+ * sequences; the results are those of tq4_full_decode / tq4_full_decode_preset on the same arguments, the
+ * shared part with f16 pairs as operands and the weights of its values rounded to f16 (pairs for f16
+ * outputs).  prefix_len: whole blocks, 0 up to the table's width; a sequence with fewer tokens
+ * (seq_lens[b] < prefix_len, 0 included) attends to its own seq_lens[b] alone: its entries behind those
+ * may hold anything.  query and out are 16-bit (TQ4_BF16, TQ4_F16).
  * workspace: at least tq4_prefix_workspace_floats(...) floats, 16-byte aligned, contents after the call
  * unspecified; two calls that may overlap need one each.  The grid depends on the shapes and prefix_len,
  * never on seq_lens.  key_bits / value_bits, sinks, block sizes and errors as in tq4_window_decode.

@@ -42,9 +42,6 @@ def build(seed, lens, prefix, hk, group, bs=16, preset="4bit", layout="soa", dty
             start = shared
         table[b, start:start + own[b]] = ids[at:at + own[b]]
         at += own[b]
-    if lens[0] < prefix:  # row 0 names the shared pages, whatever its length
-        assert lens[0] == 0, "the first sequence has the prefix, or no tokens"
-        table[0, :shared] = ids[:shared]
     hq = hk * group
     query = rng.standard_normal((len(lens), hq, D)).astype(np.float32)
     if query_scale is not None:
@@ -149,6 +146,9 @@ FORMS = {
     "stretches over tails": ([128 + 29 * i for i in range(70)], 128, 2, 4, 32),
     "one row": ([3001, 2500], 1600, 2, 4, 1),
     "nobody has the prefix": ([0, 10, 100, 4], 128, 2, 4, 8),
+    "the first to have it is the second": ([100, 128, 300, 0], 128, 2, 4, 8),
+    "the first to have it is the last": ([i % 128 for i in range(69)] + [1000], 128, 2, 4, 8),
+    "the first to have it opens the second 64": ([0] * 64 + [500, 128, 20], 128, 1, 2, 8),
     "batch past the device": ([64 + i % 9 for i in range(300)], 64, 2, 2, 4),
     "group of 16, three kv-heads": ([500, 333, 999], 320, 3, 16, 8),
 }

@@ -162,6 +162,11 @@ def test_rotated_dims(dev, rot, neox, preset):
     check(dev, build(2, 70, 4, 2, preset, rot=rot, neox=neox, table="same" if rot == 64 else "fp32"))
 
 
+def test_one_axis_in_turn(dev):
+    """Frequencies dealt round a single axis: the plain positions."""
+    check(dev, build(3, 90, 4, 2, "4bit", in_turn=True))
+
+
 @pytest.mark.parametrize("sections,in_turn", [((16, 24, 24), False), ((24, 20, 20), True), ((64, 0, 0), False), ((0, 33, 31), False),
                                               ((50, 14), False), ((10, 20, 30, 4), False), ((61, 1, 2), True), ((32, 32), True),
                                               ((22, 10, 16, 16), True)])
@@ -310,7 +315,7 @@ def test_the_writers_bytes_without_rotation(dev):
 
 REFUSED = [
     (dict(key_bits=5), "key/value bits"), (dict(sections=(10, 20)), "sections"), (dict(sections=(64,)), "sections"),
-    (dict(sections=(0, 40, 24), in_turn=True), "sections in turn"), (dict(in_turn=True), "in_turn"), (dict(layout="x"), "layout"),
+    (dict(sections=(0, 40, 24), in_turn=True), "sections in turn"), (dict(layout="x"), "layout"),
     (dict(query_out="short"), "query_out"), (dict(cents=False), "centroids"), (dict(table=72), "rot_dim"),
     (dict(table=144), "rot_dim"), (dict(stride=4), "16-byte"), (dict(positions=torch.int32), "int64"),
     (dict(heads=3), "heads"),

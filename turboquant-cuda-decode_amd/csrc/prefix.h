@@ -64,12 +64,13 @@ struct Args {
     const void *query;       // fp32 rows, already rotated; FP8 keys: q_dtype rows
     const float *centroids;  // [16], 3-bit keys [8], FP8 keys null
     const uint8_t *cache;
-    const int32_t *pages;    // the prefix's blocks
+    const int32_t *pages;    // block table [batch, table_width]
+    const int32_t *seq_lens;
     float *parts;            // part rows (stage2.h)
     int64_t block_stride;
     float score_scale_log2;
     int q_dtype, num_q_heads, num_kv_heads, group, rows;  // rows: batch * group, per kv-head
-    int total_rows;          // batch * num_q_heads
+    int total_rows, batch, table_width;  // total_rows: batch * num_q_heads
     int row_tiles, splits;   // splits: part rows per (sequence, head)
     int tokens, tiles;       // of the prefix (tiles of Shape::tokens)
     int block_size_log2, slot_pos, slot_head;
@@ -328,6 +329,15 @@ __device__ __forceinline__ half8 pinned(half8 x) {
     asm volatile("" : "+v"(t));
     return __builtin_bit_cast(half8, t);
 }
+// The first sequence of at least `tokens` tokens, -1: none.  (Wave-uniform.)
+__device__ __forceinline__ int first_as_long(const int32_t *seq_lens, int batch, int tokens, int lane) {
+    for (int b0 = 0; b0 < batch; b0 += 64) {
+        const uint64_t has = __ballot(b0 + lane < batch && seq_lens[min(b0 + lane, batch - 1)] >= tokens);
+        if (has)
+            return b0 + __builtin_ctzll(has);
+    }
+    return -1;
+}
 // Rows of a lane pair (c, c + 32): max and sum over both.
 __device__ __forceinline__ float pair_max(float x) { return xdl::max_xor32(x); }
 __device__ __forceinline__ float pair_sum(float x) { return xdl::sum_xor32(x); }
@@ -358,13 +368,14 @@ void prefix_kernel(const Args a) {
     // With one LDS tile (WT = 1) tile j + 1's K takes the place of tile j's, whose scores are done, and tile
     // j's V is decoded when tile j - 1's is done with: a tile behind K.
     constexpr int kBehind = 2 - S::bufs;
+    const int32_t *pages = a.pages;
     int kblk = 0, vblk = 0;
     auto within = [&](int i) { return max(min(i, tile1 - 1), tile0); };
     auto read_pages = [&](int i) {
         if (does_k)
-            kblk = a.pages[k_tok(within(i)) >> a.block_size_log2];
+            kblk = pages[k_tok(within(i)) >> a.block_size_log2];
         if (does_v)
-            vblk = a.pages[v_tok(within(i - kBehind)) >> a.block_size_log2];
+            vblk = pages[v_tok(within(i - kBehind)) >> a.block_size_log2];
     };
     RawK rk;
     RawV rv;
@@ -389,6 +400,15 @@ void prefix_kernel(const Args a) {
             const uint32_t x = xdl::split_f16(a.centroids[KB3 ? e & 7 : e & 15]), z = xdl::split_f16(a.centroids[KB3 ? e >> 3 : e >> 4]);
             lut[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
         }
+    // The shared blocks are named by every sequence that has the prefix, mostly by the first one, whose entries
+    // are on their way (in the table whatever they hold); if nobody has it the join reads no row of this kernel.
+    if (a.seq_lens[0] < a.tokens) {
+        const int b = first_as_long(a.seq_lens, a.batch, a.tokens, lane);
+        if (b < 0)
+            return;
+        pages += (int64_t)b * a.table_width;
+        read_pages(tile0);
+    }
     load(tile0);
     read_pages(tile0 + 1);
 

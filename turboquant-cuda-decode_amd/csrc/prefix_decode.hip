@@ -133,6 +133,9 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
     p.centroids = centroids;
     p.cache = kv_cache;
     p.pages = block_table;
+    p.seq_lens = seq_lens;
+    p.batch = B;
+    p.table_width = max_blocks_per_seq;
     p.parts = shared;
     p.block_stride = cache_block_stride;
     p.score_scale_log2 = attn_scale * tq4::kLog2e;

@@ -439,7 +439,7 @@ def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, ro
     position ``p``.  The first ``rot_dim`` dims (a multiple of 16) of each head are rotated in planes ``f``: dims
     ``(f, f + rot_dim / 2)`` with ``neox``, else ``(2f, 2f + 1)``.  ``positions`` int64 ``[N]``, or ``[axes, N]`` with
     ``sections``, the number of frequencies of each axis (time, height, width), in blocks, or with ``in_turn`` dealt
-    round the axes (frequency ``j`` to axis ``j mod axes`` as long as that has any left, else to the first).
+    round the axes (frequency ``j`` to axis ``j mod axes`` as long as that has any left, else to the first; without ``sections`` there is one axis to deal to).
     ``query``, ``key`` and ``value`` may be slices of one projection's output: tokens any whole 16-byte pieces apart.
     ``query_out`` (contiguous, may be ``query`` itself) takes the queries.
 
@@ -447,7 +447,7 @@ def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, ro
     ``store_fp8`` (``key_bits`` 8: no rotation matrix, no codebook).  K is not rounded to its type between the
     rotation and the quantiser, and the stored bytes are those of the definition in 64 bits.  Tokens with a
     negative slot, a slot past the cache, or a position outside the table are not written; the queries of the
-    last become NaN.  Slots must be distinct (two tokens with one slot leave either's bytes).
+    last become NaN.  Slots must be distinct (what two tokens leave in one slot is unspecified).
     """
     fp8 = key_bits == 8
     if (key_bits, value_bits) not in PRESETS + ((8, 4),):
@@ -475,7 +475,6 @@ def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, ro
     _require(0 < rot <= D and rot % 16 == 0, "rot_dim must be a multiple of 16 up to the head's")
     _require(cos_sin.size(0) > 0, "cos_sin has no rows")
     if sections is None:
-        _require(not in_turn, "in_turn needs sections")
         axes, axis_of, shape = 1, None, (N,)
     else:
         sections = tuple(sections)
@@ -614,8 +613,8 @@ def _int_arg(value, name, least):
     return value
 
 
-def _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits, value_bits,
-               layout, out_dtype, attn_scale, sinks):
+def _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, kind, key_bits,
+               value_bits, layout, out_dtype, attn_scale, sinks):
     """Checks of a decode step with hidden tokens; returns the C arguments' common runs."""
     fp8 = key_bits == 8
     if (key_bits, value_bits) not in PRESETS + ((8, 4),):
@@ -630,7 +629,7 @@ def _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, nu
     _require(Hq % Hk == 0, "Hq must be a multiple of Hk")
     _require(block_table.dim() == 2 and block_table.size(0) == B, "block_table batch mismatch")
     _require(seq_lens.dim() == 1 and seq_lens.size(0) == B, "seq_lens batch mismatch")
-    _require(ws.fits(query, Hk, num_kv_splits, out_dtype), "workspace does not match this call")
+    _require(isinstance(ws, kind) and ws.fits(query, Hk, num_kv_splits, out_dtype), "workspace does not match this call")
     tensors = [query, kv_cache, block_table, seq_lens, ws.out]
     if not fp8:
         _check_tensor(rotation_t, "rotation_t", torch.float32)
@@ -667,8 +666,8 @@ def window_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     out_dtype = query.dtype if out_dtype is None else out_dtype
     _require(out_dtype in DTYPES and query.dim() == 3, _QUERY_SHAPE)
     ws = workspace or DecodeWorkspace(query.size(0), query.size(1), num_kv_splits, query.device, out_dtype)
-    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits,
-                            value_bits, layout, out_dtype, attn_scale, sinks)
+    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws,
+                            DecodeWorkspace, key_bits, value_bits, layout, out_dtype, attn_scale, sinks)
     with _on_device(query.device):
         rc = _lib.load().tq4_window_decode(*head, ws.q_rot.data_ptr(), ws.mid_o.data_ptr(), *tail, window, first_tokens,
                                            _stream(query.device))
@@ -700,11 +699,12 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     """Decode step of a batch whose sequences share their first ``prefix_len`` tokens; returns
     ``(out [B, Hq, D], lse [B, Hq])``.
 
-    The first ``prefix_len // block_size`` entries of every row of ``block_table`` name the same blocks
-    (row 0's are read): those tokens are read and decoded once for all sequences, the rest of each
+    The first ``prefix_len // block_size`` entries of ``block_table`` name the same blocks in the row of every
+    sequence that has as many tokens: those are read and decoded once for all of them, the rest of each
     sequence as in ``full_decode``.  ``prefix_len`` is whole blocks (0: nothing shared); a sequence with
-    ``seq_lens[b] < prefix_len`` attends to its own ``seq_lens[b]`` tokens alone.  ``query`` and ``out`` are bf16
-    or fp16 (the shared tokens' products have f16 operands).  ``workspace``: a ``PrefixWorkspace``.
+    ``seq_lens[b] < prefix_len`` attends to its own ``seq_lens[b]`` tokens alone (its entries behind those may
+    hold anything).  ``query`` and ``out`` are bf16 or fp16 (the shared tokens' products have f16 operands, in
+    pairs where one would show in the result).  ``workspace``: a ``PrefixWorkspace``.
     ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in ``window_decode``.
     """
     _int_arg(prefix_len, "prefix_len", 0)
@@ -712,8 +712,8 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     _require(out_dtype in DTYPES and query.dim() == 3 and kv_cache.dim() == 4, _QUERY_SHAPE)
     ws = workspace or PrefixWorkspace(query.size(0), query.size(1), kv_cache.size(2), num_kv_splits, query.device,
                                       out_dtype)
-    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws, key_bits,
-                            value_bits, layout, out_dtype, attn_scale, sinks)
+    head, tail = _span_call(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, ws,
+                            PrefixWorkspace, key_bits, value_bits, layout, out_dtype, attn_scale, sinks)
     with _on_device(query.device):
         rc = _lib.load().tq4_prefix_decode(*head, ws.scratch.data_ptr(), ws.scratch.numel(), *tail, prefix_len,
                                            _stream(query.device))
