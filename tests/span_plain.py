@@ -120,3 +120,19 @@ def close(got, want, step, what, atol=1e-4, rtol=0.0):
     assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)]), f"{what}: infinities differ"
     err = np.abs(got[fine] - want[fine]) - (rtol + step) * np.abs(want[fine])
     assert err.size == 0 or err.max() <= atol, f"{what}: off by {err.max():.3e} over the step, allowed {atol:.1e}"
+
+
+def spoil(cache, tokens, preset, layout):
+    """Every byte of the given (block, offset) tokens set: NaN scalars, the highest codes (E4M3: NaN)."""
+    kb, vb = PRESETS[preset]
+    n, bs, hk, slot = cache.shape
+    nf = 2 if kb == 8 else 3
+    rec = 16 * (kb + vb)
+    for block, off in tokens:
+        if layout != "soa":
+            cache[block, off] = 0xFF
+            continue
+        flat = cache[block].view(-1)
+        flat[off * hk * rec:(off + 1) * hk * rec] = 0xFF
+        meta = flat[bs * hk * rec:].view(hk, nf, bs, 2)
+        meta[:, :, off] = 0xFF
