@@ -20,8 +20,16 @@
 // Layout: the writer's lane (n, g) holds 32 dims of row n; which 32 is free for the contraction, so it
 // takes the chunks (8 dims) of planes 16 g .. 16 g + 15, both members of each: unit u = 2 g, 2 g + 1 of a row is the two
 // chunks whose dims are rotated with each other and 8 frequencies (units past rot / 16: 16 dims that are
-// not rotated).  A query thread takes one unit of one row.  The query rows' workgroups come behind the writer's
-// in one launch.
+// not rotated).  A query thread takes one unit of one row.
+//
+// What bounds it, and what it measured (32 / 8 heads, bf16, 4-bit keys).  32768 tokens: the queries' rows are
+// copied through in 99 us (537 MB, 5.4 TB/s: the card's copy rate), the writer takes 92-109 us for 170 MB: a
+// chain per tile (positions, then angles and keys, 96 matrix products, codes, V), four waves of a SIMD in turn,
+// 16 tiles per SIMD.  4097 tokens on three axes 36 us.  64 tokens 14.5 us: one workgroup's chain, the rotation
+// matrix staged and split in LDS (8.6 us in the plain writer), positions and angles before it.  Registers bind the
+// large form (128 at four waves per SIMD): V asked for behind the products instead of ahead of the tile took
+// 34 spilled registers to 14, a unit's angles one unit at a time 50 to 12 (139 us to 104), one axis known to
+// the compiler 104 to 97; two waves per SIMD without spills 139.
 #pragma once
 #include "store.h"
 
@@ -33,6 +41,7 @@ using store::half8;
 
 constexpr float kNearY = 1e-6f;
 constexpr int kQueryRows = 32;  // rows (token, head) of 128 dims that a wave takes at a time
+constexpr int kQueryWaves = 4;  // per workgroup of query_kernel
 constexpr int kMostAxes = 4;
 
 struct Args {
@@ -61,11 +70,34 @@ __device__ __forceinline__ int unit_chunk(const Args &a, int u, int m) {
 }
 // (Rotated units first: u >= r is chunks 2 r + 2 (u - r) + m = 2 u + m.)
 
-// The token's position on axis x; a token with one outside the table has none (`ok` false).
-__device__ __forceinline__ int position(const Args &a, int tok, int x, bool &ok) {
-    const int64_t p = a.positions[(int64_t)x * a.axis_stride + tok];
-    ok = ok && p >= 0 && p < a.table_rows;
-    return p >= 0 && p < a.table_rows ? (int)p : 0;
+// A token's positions as they lie in memory (axes past the last: the last one's again, or 0), and checked:
+// ok if all are in the table.
+struct RawPositions {
+    int64_t at[kMostAxes];
+};
+struct Positions {
+    int at[kMostAxes];
+    bool ok;
+};
+template <bool ONE = false> __device__ __forceinline__ void load_positions(RawPositions &p, const Args &a, int tok) {
+    p.at[0] = a.positions[tok];
+#pragma unroll
+    for (int x = 1; x < kMostAxes; ++x)
+        p.at[x] = 0;
+    if (!ONE && a.axes > 1)
+#pragma unroll
+        for (int x = 1; x < kMostAxes; ++x)
+            p.at[x] = a.positions[min(x, a.axes - 1) * a.axis_stride + tok];
+}
+__device__ __forceinline__ Positions checked(const RawPositions &p, const Args &a, bool ok) {
+    Positions r{{}, ok};
+#pragma unroll
+    for (int x = 0; x < kMostAxes; ++x) {
+        const bool in = (uint64_t)p.at[x] < (uint64_t)(uint32_t)a.table_rows;
+        r.at[x] = in ? (int)p.at[x] : 0;
+        r.ok = r.ok && in;
+    }
+    return r;
 }
 template <class T> __device__ __forceinline__ float table_at(const Args &a, int row, int col) {
     const int64_t i = (int64_t)row * a.rot + col;
@@ -87,9 +119,10 @@ template <class T> __device__ __forceinline__ void table_row8(const Args &a, int
     }
 }
 // Cosines and sines of frequencies 8 u .. 8 u + 7 for a token (u < rot / 16).  pos: its positions.
-template <class T>
+// ONE: there is one axis.
+template <class T, bool ONE = false>
 __device__ __forceinline__ void unit_angles(const Args &a, const int (&pos)[kMostAxes], int u, float (&c)[8], float (&s)[8]) {
-    if (a.axes == 1) {
+    if (ONE || a.axes == 1) {
         table_row8<T>(a, pos[0], 8 * u, c);
         table_row8<T>(a, pos[0], a.rot / 2 + 8 * u, s);
         return;
@@ -181,32 +214,29 @@ template <class T> __device__ __forceinline__ void rotate_queries(const Args &a,
     constexpr int kSteps = kQueryRows / 8;
     for (int64_t r0 = (int64_t)wave * kQueryRows; r0 < rows; r0 += (int64_t)waves * kQueryRows) {
         Eight<T> x0[kSteps], x1[kSteps];
+        RawPositions raw[kSteps];
         int tok[kSteps], row[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             row[i] = (int)min(r0 + 8 * i + (lane >> 3), (int64_t)rows - 1);  // (past the end: the last one again)
             tok[i] = row[i] / a.num_q_heads;
+            load_positions(raw[i], a, tok[i]);
             const T *q = query + tok[i] * a.q_stride + (int64_t)(row[i] - tok[i] * a.num_q_heads) * kHeadDim;
             x0[i] = load8(q + c0);
             x1[i] = load8(q + c1);
         }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            int pos[kMostAxes] = {0, 0, 0, 0};
-            bool ok = true;
-#pragma unroll
-            for (int x = 0; x < kMostAxes; ++x)
-                if (x < a.axes)
-                    pos[x] = position(a, tok[i], x, ok);
+            const Positions pos = checked(raw[i], a, true);
             float y0[8], y1[8];
             floats8(y0, x0[i]);
             floats8(y1, x1[i]);
             if (u < r8) {
                 float c[8], s[8];
-                unit_angles<T>(a, pos, u, c, s);
+                unit_angles<T>(a, pos.at, u, c, s);
                 turn(y0, y1, c, s, a.neox != 0, plane32);
             }
-            if (!ok)
+            if (!pos.ok)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     y0[j] = y1[j] = __builtin_nanf("");
@@ -242,14 +272,9 @@ template <class T> __device__ __forceinline__ void load_key(RawKey<T> &k, const 
     for (int i = 0; i < 4; ++i)
         k.c[i] = load8(key + 8 * chunk[i]);
 }
-// The rotated K of the lane's 32 dims (chunk i at x[8 i ..]); ok: the token's positions are in the table.
-template <class T, class F>
-__device__ __forceinline__ void turned_key(float (&x)[32], const RawKey<T> &k, const Args &a, int tok, int g, bool &ok, F plane) {
-    int pos[kMostAxes] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < kMostAxes; ++i)
-        if (i < a.axes)
-            pos[i] = position(a, tok, i, ok);
+// The rotated K of the lane's 32 dims (chunk i at x[8 i ..]).
+template <class T, bool ONE, class F>
+__device__ __forceinline__ void turned_key(float (&x)[32], const RawKey<T> &k, const Positions &pos, const Args &a, int g, F plane) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float x0[8], x1[8];
@@ -257,7 +282,7 @@ __device__ __forceinline__ void turned_key(float (&x)[32], const RawKey<T> &k, c
         floats8(x1, k.c[2 * i + 1]);
         if (2 * g + i < a.rot >> 4) {
             float c[8], s[8];
-            unit_angles<T>(a, pos, 2 * g + i, c, s);
+            unit_angles<T, ONE>(a, pos.at, 2 * g + i, c, s);
             turn(x0, x1, c, s, a.neox != 0, plane);
         }
 #pragma unroll
@@ -290,8 +315,10 @@ template <class T> struct Exact {
         x1 = q;
         if (turned) {
             const int axis = a.axes == 1 ? 0 : (int)(a.axis_bit[0] >> lane & 1) + 2 * (int)(a.axis_bit[1] >> lane & 1);
-            bool ok = true;
-            const int pos = position(a, r.tok, axis, ok);
+            RawPositions raw;
+            load_positions(raw, a, r.tok);
+            const Positions p4 = checked(raw, a, true);
+            const int pos = axis == 0 ? p4.at[0] : axis == 1 ? p4.at[1] : axis == 2 ? p4.at[2] : p4.at[3];
             const double c = table_at<T>(a, pos, lane), s = table_at<T>(a, pos, half + lane);
             x0 = p * c - q * s;
             x1 = q * c + p * s;
@@ -324,7 +351,7 @@ template <int KB> __device__ __forceinline__ void flip_code(uint32_t (&w)[KB], i
 }
 
 // The writer's tile loop.  W: waves per workgroup (see store_kernel).
-template <int LAYOUT, class T, int KB, int VB, int W>
+template <int LAYOUT, class T, int KB, int VB, int W, bool ONE>
 __device__ __forceinline__ void store_rows(const Args &a, int group, int groups) {
     using namespace store;
     __shared__ __align__(16) _Float16 pt_hi[kHeadDim * kHeadDim];
@@ -345,24 +372,28 @@ __device__ __forceinline__ void store_rows(const Args &a, int group, int groups)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         chunk[i] = unit_chunk(a, 2 * g + (i >> 1), i & 1);
+    // (a tile's positions and slot are requested with its keys)
     RawKey<T> kr;
     Chunk<T> vr;
-    Row<T> at = row_at<T>(a, tile * kRows + n, tile < tiles && tile * kRows + n < rows);
-    constexpr bool kEarlyV = sizeof(T) < 4;
-    load_key<T>(kr, at.key, chunk);
-    if constexpr (kEarlyV)
-        load_raw(vr, at.value + 32 * g, true);
+    Row<T> at;
+    RawPositions raw;
+    int slot;
+    auto start = [&](int t) {
+        at = row_at<T>(a, t * kRows + n, t < tiles && t * kRows + n < rows);
+        load_positions<ONE>(raw, a, at.tok);
+        slot = a.slots[at.tok];
+        load_key<T>(kr, at.key, chunk);
+    };
+    start(tile);
     __builtin_amdgcn_sched_barrier(0);
     store_pit<W>(pw, pt_hi, pt_lo);
     const Cells cells = build_cells<KB>(book, a.norm_correction, c2tab, btab);
 
     for (; tile < tiles; tile += stride) {
-        const int row = tile * kRows + n;
-        const bool in_range = row < rows;
-        const int tok = at.tok, head = at.head;
-        bool ok = in_range;
+        const Positions pos = checked(raw, a, tile * kRows + n < rows);
+        const bool live = pos.ok && slot >= 0 && slot < a.num_slots;
         float x[32];
-        turned_key<T>(x, kr, a, tok, g, ok, plane32);
+        turned_key<T, ONE>(x, kr, pos, a, g, plane32);
         // (four sums: an error of 8 roundings each)
         float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -374,11 +405,15 @@ __device__ __forceinline__ void store_rows(const Args &a, int group, int groups)
         split_x(x, rn, b_hi, b_lo);
         floatx4 acc[8];
         rotate_tile(acc, b_hi, b_lo, pt_hi, pt_lo, n, [&](int kb) { return chunk[kb]; });
+        // (V here: earlier, or 32 registers of it, they spill at four waves per SIMD)
+        constexpr bool kEarlyV = sizeof(T) < 4;
+        if constexpr (kEarlyV) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_raw(vr, at.value + 32 * g, true);
+        }
         uint32_t kw[KB];
         float csq, nearest = __builtin_inff();
         code_keys<KB, true>(acc, cells, book, btab, c2tab, kw, csq, nearest);
-        const int slot = ok ? a.slots[tok] : -1;
-        const bool live = slot >= 0 && slot < a.num_slots;
         // elements next to a midpoint (a zero row has y = 0 exactly)
         constexpr float kNear = 256.f * kNearY;
         bool near = live && norm > 0.f && nearest < kNear;
@@ -441,26 +476,26 @@ __device__ __forceinline__ void store_rows(const Args &a, int group, int groups)
         uint32_t vw[VB];
         quantize_v<VB>(x, vw, scale, vmin);
         if (live)
-            put_record<LAYOUT, KB, VB>(a.cache, slot, head, g, kw, vw, kscalar, scale, vmin, a.num_kv_heads, a.block_size,
+            put_record<LAYOUT, KB, VB>(a.cache, slot, at.head, g, kw, vw, kscalar, scale, vmin, a.num_kv_heads, a.block_size,
                                        a.block_stride, a.slot_pos, a.slot_head);
-        // the next tile of this wave
-        const int nrow = (tile + stride) * kRows + n;
-        at = row_at<T>(a, nrow, tile + stride < tiles && nrow < rows);
-        load_key<T>(kr, at.key, chunk);
-        if constexpr (kEarlyV)
-            load_raw(vr, at.value + 32 * g, true);
+        start(tile + stride);
     }
 }
 
-// W = kWaves: large launches, two workgroups per CU; kSmallWaves: few rows (see store_kernel).
-template <int LAYOUT, class T, int KB, int VB, int W>
+// W = kWaves: large launches, two workgroups per CU, the queries in a launch of their own; kSmallWaves: few
+// rows (see store_kernel), the query rows' workgroups behind the writer's in one launch.  ONE: one axis.
+template <int LAYOUT, class T, int KB, int VB, int W, bool ONE>
 __global__ __launch_bounds__(kWave *W) __attribute__((amdgpu_waves_per_eu(W == store::kWaves ? 4 : 1)))
 void append_kernel(const Args a) {
-    if ((int)blockIdx.x < a.store_groups)
-        store_rows<LAYOUT, T, KB, VB, W>(a, blockIdx.x, a.store_groups);
+    if (W == store::kWaves || (int)blockIdx.x < a.store_groups)
+        store_rows<LAYOUT, T, KB, VB, W, ONE>(a, blockIdx.x, a.store_groups);
     else
         rotate_queries<T>(a, (blockIdx.x - a.store_groups) * W + threadIdx.x / kWave, (gridDim.x - a.store_groups) * W,
                           threadIdx.x % kWave);
+}
+
+template <class T> __global__ __launch_bounds__(kWave *kQueryWaves) void query_kernel(const Args a) {
+    rotate_queries<T>(a, blockIdx.x * kQueryWaves + threadIdx.x / kWave, gridDim.x * kQueryWaves, threadIdx.x % kWave);
 }
 
 // FP8 keys (see store_fp8_kernel).
@@ -480,14 +515,17 @@ __global__ __launch_bounds__(kWave *store::kFp8Waves) void append_fp8_kernel(con
         chunk[i] = unit_chunk(a, 2 * g + (i >> 1), i & 1);
     for (int tile = blockIdx.x * kFp8Waves + wave; tile < tiles; tile += a.store_groups * kFp8Waves) {
         const int row = tile * kRows + n;
-        bool ok = row < rows;
-        const Row<T> at = row_at<T>(a, row, ok);
+        const Row<T> at = row_at<T>(a, row, row < rows);
+        RawPositions raw;
+        load_positions(raw, a, at.tok);
+        const int slot = a.slots[at.tok];
         RawKey<T> kr;
         Chunk<T> vr;
         load_key<T>(kr, at.key, chunk);
         load_raw(vr, at.value + 32 * g, true);
+        const Positions pos = checked(raw, a, row < rows);
         float x[32];
-        turned_key<T>(x, kr, a, at.tok, g, ok, plane64);
+        turned_key<T, false>(x, kr, pos, a, g, plane64);
         uint2 kw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -504,8 +542,7 @@ __global__ __launch_bounds__(kWave *store::kFp8Waves) void append_fp8_kernel(con
         float scale, vmin;
         uint32_t vw[4];
         quantize_v<4>(x, vw, scale, vmin);
-        const int slot = ok ? a.slots[at.tok] : -1;
-        if (slot < 0 || slot >= a.num_slots)
+        if (!pos.ok || slot < 0 || slot >= a.num_slots)
             continue;
         const int64_t blk = slot / a.block_size, off = slot % a.block_size;
         uint8_t *base = a.cache + blk * a.block_stride;

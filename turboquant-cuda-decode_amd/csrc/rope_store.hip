@@ -17,17 +17,29 @@ int query_groups(const tq4::rope::Args &a, int waves) {
     return (int)std::min<int64_t>((runs + waves - 1) / waves, 2048);
 }
 
+// One launch for both roles has to hold the larger one's registers and LDS for both, two launches cost a
+// second start.  Small workgroups with both: 38.7 us at 2049 tiles (4097 tokens, 8 kv-heads) against 24.7 + 19.9
+// for two launches of large ones and 43.8 for one; at 16384 tiles 215 against 97 + 103 and 243.  Without queries
+// the plain writer's limit holds.
 template <int LAYOUT, class T, int KB, int VB> void launch_append(tq4::rope::Args &a, hipStream_t st) {
     using namespace tq4::store;
     const int64_t tiles = ((int64_t)a.tokens * a.num_kv_heads + kRows - 1) / kRows;
-    const bool small = tiles <= kSmallTiles;
+    const bool small = tiles <= (a.query ? 4 * kSmallTiles : kSmallTiles);
     const int waves = small ? kSmallWaves : kWaves;
     a.store_groups = (int)std::min<int64_t>((tiles + waves - 1) / waves, kMaxGroups);
-    const dim3 grid(a.store_groups + query_groups(a, waves)), block(tq4::kWave * waves);
-    if (small)
-        launch(&tq4::rope::append_kernel<LAYOUT, T, KB, VB, kSmallWaves>, grid, block, st, a);
+    if (small) {
+        const dim3 grid(a.store_groups + query_groups(a, waves)), block(tq4::kWave * waves);
+        launch(&tq4::rope::append_kernel<LAYOUT, T, KB, VB, kSmallWaves, false>, grid, block, st, a);
+        return;
+    }
+    const dim3 grid(a.store_groups), block(tq4::kWave * waves);
+    if (a.axes == 1)
+        launch(&tq4::rope::append_kernel<LAYOUT, T, KB, VB, kWaves, true>, grid, block, st, a);
     else
-        launch(&tq4::rope::append_kernel<LAYOUT, T, KB, VB, kWaves>, grid, block, st, a);
+        launch(&tq4::rope::append_kernel<LAYOUT, T, KB, VB, kWaves, false>, grid, block, st, a);
+    if (a.query)
+        launch(&tq4::rope::query_kernel<T>, dim3(query_groups(a, tq4::rope::kQueryWaves)), dim3(tq4::kWave * tq4::rope::kQueryWaves),
+               st, a);
 }
 template <int LAYOUT, class T> void launch_append(tq4::rope::Args &a, int key_bits, int value_bits, hipStream_t st) {
     if (key_bits == 8) {
