@@ -44,7 +44,8 @@ enum tq4_kernel {
     TQ4_KERNEL_AUTO = 0,
     TQ4_KERNEL_SIMPLE = 1,
     TQ4_KERNEL_MFMA = 2,   /* retired 4x4x4 MFMA kernel: rejected with TQ4_E_UNSUPPORTED */
-    TQ4_KERNEL_XDL = 3
+    TQ4_KERNEL_XDL = 3,
+    TQ4_KERNEL_SHARED = 4  /* tq4_prefix_decode alone */
 };
 enum tq4_status {
     TQ4_OK = 0,
@@ -306,7 +307,9 @@ int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, co
  * shared part with f16 pairs as operands and the weights of its values rounded to f16 (pairs for f16
  * outputs).  prefix_len: whole blocks, 0 up to the table's width; a sequence with fewer tokens
  * (seq_lens[b] < prefix_len, 0 included) attends to its own seq_lens[b] alone: its entries behind those
- * may hold anything.  query and out are 16-bit (TQ4_BF16, TQ4_F16).
+ * may hold anything.  query and out are 16-bit (TQ4_BF16, TQ4_F16).  kernel: TQ4_KERNEL_AUTO leaves the
+ * sharing (four launches) where the sequences' own steps are faster, by the shapes and prefix_len;
+ * TQ4_KERNEL_SHARED shares always.
  * workspace: at least tq4_prefix_workspace_floats(...) floats, 16-byte aligned, contents after the call
  * unspecified; two calls that may overlap need one each.  The grid depends on the shapes and prefix_len,
  * never on seq_lens.  key_bits / value_bits, sinks, block sizes and errors as in tq4_window_decode.
@@ -317,7 +320,7 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
                       float *workspace, int64_t workspace_floats, void *out, int out_dtype, float *lse, int B,
                       int Hq, int Hk, int D, int block_size, int max_blocks_per_seq, int64_t cache_block_stride,
                       int num_kv_splits, int layout, float attn_scale, const float *sinks, int key_bits,
-                      int value_bits, int prefix_len, tq4_stream_t stream);
+                      int value_bits, int prefix_len, int kernel, tq4_stream_t stream);
 /* Floats of workspace that tq4_prefix_decode needs for these shapes and any prefix_len; -1 (and a
  * message) where they are invalid. */
 int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);

@@ -89,6 +89,7 @@ def to_device(c, dev):
 
 def call(c, splits, sinks=False, prefix=None, **kw):
     kb, vb = plain.PRESETS[c["preset"]]
+    kw.setdefault("kernel", "shared")
     return ops.prefix_decode(c["query"], None if kb == 8 else c["rot"], c["cache"], c["table"], c["lens"], c["cents"],
                              splits, c["prefix"] if prefix is None else prefix, key_bits=kb, value_bits=vb,
                              layout="soa" if c["layout"] == "soa" else "aos", sinks=c["sinks"] if sinks else None, **kw)
@@ -172,6 +173,17 @@ def test_every_prefix_length_gives_the_full_step(dev):
     assert torch.equal(out, full) and torch.equal(lse, full_lse)
 
 
+@pytest.mark.parametrize("batch,prefix,hk,group,shares", [(8, 512, 2, 4, False), (2, 4096, 4, 4, False), (64, 4096, 8, 4, True),
+                                                          (24, 12288, 8, 8, True)])
+def test_auto_takes_one_of_the_two(dev, batch, prefix, hk, group, shares):
+    """The rows of the sharing kernels where those pay, the full step's where they do not, bit for bit."""
+    c = build(11, [prefix + 1 + (i * 13) % 60 for i in range(batch)], prefix, hk, group, dtype=torch.bfloat16)
+    d = to_device(c, dev)
+    out, lse = call(d, 16, kernel="auto")
+    want, want_lse = call(d, 16, prefix=None if shares else 0)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 def test_large_small_and_zero_queries(dev):
     """Scores that span a hundred, nearly equal and equal ones, heads of every size in one batch."""
     scale = np.ones((3, 8))
@@ -221,7 +233,7 @@ def test_workspace_stream_and_graph(dev):
 
 @pytest.mark.parametrize("over,text", [
     (dict(prefix=8), "whole blocks"), (dict(prefix=1024), "whole blocks"), (dict(prefix=-16), "prefix_len"),
-    (dict(prefix=True), "prefix_len"), (dict(out_dtype=torch.float32), "16-bit"), (dict(splits=5), "workspace"),
+    (dict(prefix=True), "prefix_len"), (dict(kernel="simple"), "kernel"), (dict(out_dtype=torch.float32), "16-bit"), (dict(splits=5), "workspace"),
 ])
 def test_refusals(dev, over, text):
     c = to_device(build(10, [60, 70], 32, 2, 4), dev)
@@ -239,7 +251,7 @@ def test_c_entry_refuses(dev):
     need = lib.tq4_prefix_workspace_floats(2, 8, 2, 4)
     assert need > 0 and lib.tq4_prefix_workspace_floats(2, 7, 2, 4) == -1
     args = lambda **o: [o.get("query", p), 1, p, p, p, p, p, o.get("ws", p), o.get("floats", need), p, 1, p, 2, 8, 2, 128,  # noqa: E731
-                        16, 4, 16 * 2 * 134, 4, 0, 0.1, None, o.get("kb", 4), 4, o.get("prefix", 32), None]
+                        16, 4, 16 * 2 * 134, 4, 0, 0.1, None, o.get("kb", 4), 4, o.get("prefix", 32), 4, None]
     for o, code in ((dict(query=None), 1), (dict(ws=None), 1), (dict(floats=need - 1), 1), (dict(prefix=80), 1),
                     (dict(prefix=-1), 1), (dict(prefix=33), 1), (dict(kb=5), 2)):
         assert lib.tq4_prefix_decode(*args(**o)) == code, o

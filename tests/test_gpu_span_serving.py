@@ -30,7 +30,8 @@ def codes(kb, dev):
 
 @pytest.mark.parametrize("preset,layout,dtype", [("4bit", "soa", torch.bfloat16), ("4bit", "aos", torch.float16),
                                                  ("k8v4", "aos_heads", torch.bfloat16), ("3bit", "soa", torch.float16)])
-def test_prefill_then_replayed_decode_steps(dev, preset, layout, dtype):
+@pytest.mark.parametrize("kernel", ["auto", "shared"])
+def test_prefill_then_replayed_decode_steps(dev, preset, layout, dtype, kernel):
     kb, vb = plain.PRESETS[preset]
     rng, gen = np.random.default_rng(1), torch.Generator().manual_seed(1)
     hk, group, prefix, window, first, splits = 2, 4, 64, 24, 3, 4
@@ -94,7 +95,8 @@ def test_prefill_then_replayed_decode_steps(dev, preset, layout, dtype):
 
     def step():
         write(static["qkv"], None, None, True, q_out, static["pos"], static["slots"])
-        ops.prefix_decode(q_out, rot_arg, cache, dev_table, static["lens"], cents, splits, prefix, workspace=whole, **kw)
+        ops.prefix_decode(q_out, rot_arg, cache, dev_table, static["lens"], cents, splits, prefix, workspace=whole,
+                          kernel=kernel, **kw)
         ops.window_decode(q_out, rot_arg, cache, dev_table, static["lens"], cents, splits, window, first_tokens=first,
                           workspace=local, **kw)
 
@@ -171,7 +173,7 @@ def test_nans_in_tokens_that_are_not_visible(dev, preset, layout):
     behind = {at(b, t) for b, n in enumerate(lens) for t in range(n, most * BS)}
     past = cache.clone()
     plain.spoil(past, behind, preset, layout)
-    out, lse = ops.prefix_decode(*args(past), prefix, **kw)
+    out, lse = ops.prefix_decode(*args(past), prefix, kernel="shared", **kw)
     for b, n in enumerate(lens):
         t = np.arange(n)
         kk, vv = k[table[b, t // BS], t % BS], v[table[b, t // BS], t % BS]
@@ -220,7 +222,7 @@ def test_blocks_past_4_gib(dev, preset, layout):
         args = (q[-2:].contiguous(), rot, cache, put(np.stack([rows, rows]).astype(np.int32)),
                 torch.tensor([n, n - 70], dtype=torch.int32, device=dev), cents, 4)
         got = [cache[base:].clone(), *ops.window_decode(*args, 100, first_tokens=20, **kw),
-               *ops.prefix_decode(*args, prefix, **kw)]
+               *ops.prefix_decode(*args, prefix, kernel="shared", **kw)]
         assert not cache[:base].any()
         assert all(not x.isnan().any() for x in got[1:])
         seen.append(got)

@@ -19,12 +19,12 @@ def _span(name, over):
     """A valid call's arguments up to the pointer that makes it invalid: sequences of 4 blocks of 16, 8 / 2 heads."""
     a = dict(query=P, qd=1, rot=P, cents=P, cache=P, table=P, lens=P, ws=P, mid=P, floats=1 << 30, out=P, od=1, lse=P,
              B=2, Hq=8, Hk=2, D=128, bs=16, width=4, stride=16 * 2 * 134, S=4, layout=0, scale=0.1, kb=4, vb=4,
-             window=32, first=0, prefix=32)
+             window=32, first=0, prefix=32, kernel=4)
     a.update(over)
     head = [a[n] for n in ("query", "qd", "rot", "cents", "cache", "table", "lens", "ws")]
     head += [a["mid"]] if name == "window" else [a["floats"]]
     mid = [a[n] for n in ("out", "od", "lse", "B", "Hq", "Hk", "D", "bs", "width", "stride", "S", "layout", "scale")]
-    tail = [None, a["kb"], a["vb"]] + ([a["window"], a["first"]] if name == "window" else [a["prefix"]]) + [None]
+    tail = [None, a["kb"], a["vb"]] + ([a["window"], a["first"]] if name == "window" else [a["prefix"], a["kernel"]]) + [None]
     return getattr(_lib.load(), f"tq4_{name}_decode")(*head, *mid, *tail)
 
 
@@ -57,7 +57,7 @@ def test_window_refuses(over):
 @pytest.mark.parametrize("over,code,text", [
     (dict(prefix=-16), 1, "whole blocks"), (dict(prefix=8), 1, "whole blocks"), (dict(prefix=80), 1, "whole blocks"),
     (dict(prefix=MOST - 15), 1, "whole blocks"), (dict(floats=1000), 1, "workspace"), (dict(ws=P + 4), 1, "aligned"),
-    (dict(qd=0), 2, "16-bit"), (dict(od=0), 2, "16-bit"),
+    (dict(qd=0), 2, "16-bit"), (dict(od=0), 2, "16-bit"), (dict(kernel=1), 1, "kernel"), (dict(kernel=-1), 1, "kernel"),
 ])
 def test_prefix_refuses(over, code, text):
     assert _span("prefix", over) == code

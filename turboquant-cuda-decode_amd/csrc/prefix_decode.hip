@@ -12,6 +12,7 @@ namespace {
 // 2), row tiles of 32 wr rows, `splits` runs of tiles.
 struct PrefixPlan {
     int wr, row_tiles, tiles, splits;
+    int64_t in_turn;  // tiles that the busiest place works through
 };
 constexpr int kMaxSplits = 64;  // part rows of the prefix per (sequence, head)
 
@@ -37,9 +38,25 @@ PrefixPlan prefix_plan(int rows, int Hk, int tokens) {
         if (cost < best) {
             best = cost;
             p.splits = s;
+            p.in_turn = ((groups * s + held - 1) / held) * ((p.tiles + s - 1) / s);
         }
     }
     return p;
+}
+
+// Whether reading the prefix once is worth its launches.  In microseconds: the step on its own decodes a
+// million (token, kv-head) pairs in 19 (waves of four query heads) or 23 (of eight), 3-bit keys in a fifth more, and
+// starts in 15; the shared way takes 30 for its four launches, 2.3 per tile in turn, and writes and reads a
+// part row of 516 bytes per query row and split.
+// Measured (32 / 8 heads, 4-bit keys, tails of 100): batch 8, prefix 2048 36.2 against 17.9 for the step alone,
+// 16 x 8192 49 : 36, 64 x 2048 48 : 35, 8 x 32768 63 : 53; 64 x 4096 52 : 54, 32 x 8192 52 : 54,
+// 16 x 32768 67 : 95, 64 x 8192 58 : 95.  16 / 2 heads 64 x 8192 52 : 41; 8 / 8 heads 64 x 4096 45 : 52,
+// 16 x 8192 38 : 34; 32 / 4 heads, 3-bit, 100 x 4000 56 : 60.
+bool sharing_pays(const Stage1Args &a, const PrefixPlan &p, int prefix_len) {
+    const double each = (xdl_heads(a) == 4 ? 19e-6 : 23e-6) * (a.key_bits == 3 ? 1.2 : 1.0);
+    const double alone = 15 + each * a.B * (double)prefix_len * a.Hk * xdl_parts(a);
+    const double shared = 30 + 2.3 * p.in_turn + 2.06e-4 * a.B * (double)a.Hq * p.splits;
+    return shared < alone;
 }
 
 int64_t part_floats(int64_t rows, int parts) { return rows * parts * (tq4::kHeadDim + 1); }
@@ -95,7 +112,7 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
                       const uint8_t *kv_cache, const int32_t *block_table, const int32_t *seq_lens, float *workspace,
                       int64_t workspace_floats, void *out, int out_dtype, float *lse, int B, int Hq, int Hk, int D,
                       int block_size, int max_blocks_per_seq, int64_t cache_block_stride, int num_kv_splits, int layout,
-                      float attn_scale, const float *sinks, int key_bits, int value_bits, int prefix_len,
+                      float attn_scale, const float *sinks, int key_bits, int value_bits, int prefix_len, int kernel,
                       tq4_stream_t stream) {
     constexpr char what[] = "tq4_prefix_decode";
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -110,6 +127,8 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
                     block_size, max_blocks_per_seq);
     if (query_dtype == TQ4_F32 || out_dtype == TQ4_F32)
         return fail(TQ4_E_UNSUPPORTED, "%s: 16-bit queries and outputs only (the shared product has f16 operands)", what);
+    if (kernel != TQ4_KERNEL_AUTO && kernel != TQ4_KERNEL_SHARED)
+        return fail(TQ4_E_INVALID, "%s: kernel must be %d (auto) or %d (shared)", what, TQ4_KERNEL_AUTO, TQ4_KERNEL_SHARED);
     const Workspace ws = workspace_of(B, Hq, Hk, num_kv_splits);
     if (workspace_floats < ws.total || !aligned(workspace, 16))
         return fail(TQ4_E_INVALID, "%s: workspace of %lld floats, needs %lld, 16-byte aligned", what,
@@ -118,7 +137,8 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
     a.q_rot = q_rot;
     a.mid_o = own;
     StepIo io{query, query_dtype, rot_t, q_rot, centroids, out, out_dtype, lse};
-    if (prefix_len == 0)
+    const PrefixPlan plan = prefix_plan(B * (Hq / Hk), Hk, prefix_len);
+    if (prefix_len == 0 || (kernel == TQ4_KERNEL_AUTO && !sharing_pays(a, plan, prefix_len)))
         return run_step(a, io, true, st);
     if (!a.key_fp8) {
         rc = rotate_query(query, query_dtype, rot_t, q_rot, B * Hq, D, nullptr, nullptr, st);
@@ -145,7 +165,6 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
     p.rows = B * p.group;
     p.total_rows = B * Hq;
     p.tokens = prefix_len;
-    const PrefixPlan plan = prefix_plan(p.rows, Hk, prefix_len);
     p.tiles = plan.tiles;
     p.row_tiles = plan.row_tiles;
     p.splits = plan.splits;

@@ -62,7 +62,7 @@ _SIGS = {
     "tq4_window_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
                           _p, _i, _i, _i, _i, _p],
     "tq4_prefix_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
-                          _p, _i, _i, _i, _p],
+                          _p, _i, _i, _i, _i, _p],
     "tq4_prefix_workspace_floats": [_i, _i, _i, _i],
     "tq4_last_error": [],
     "tq4_abi_version": [],

@@ -33,6 +33,7 @@ from ._lib import Tq4Error  # noqa: F401  (raised by every wrapper)
 from .layout import AOS, AOS_HEAD_MAJOR, LAYOUTS, SOA, slot_bytes, slot_bytes_fp8, slot_bytes_preset
 
 KERNELS = {"auto": 0, "simple": 1, "xdl": 3}
+PREFIX_KERNELS = {"auto": 0, "shared": 4}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 HEAD_DIM = 128
 _KEY_SHAPE = f"key must be [N, Hk, {HEAD_DIM}]"
@@ -695,7 +696,7 @@ class PrefixWorkspace:
 
 def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids, num_kv_splits, prefix_len, *,
                   key_bits=4, value_bits=4, layout="soa", out_dtype=None, attn_scale=None, workspace=None,
-                  sinks=None):
+                  sinks=None, kernel="auto"):
     """Decode step of a batch whose sequences share their first ``prefix_len`` tokens; returns
     ``(out [B, Hq, D], lse [B, Hq])``.
 
@@ -705,9 +706,13 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     ``seq_lens[b] < prefix_len`` attends to its own ``seq_lens[b]`` tokens alone (its entries behind those may
     hold anything).  ``query`` and ``out`` are bf16 or fp16 (the shared tokens' products have f16 operands, in
     pairs where one would show in the result).  ``workspace``: a ``PrefixWorkspace``.
-    ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in ``window_decode``.
+    ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in ``window_decode``.  ``kernel``: "auto" shares the
+    prefix where that is faster than every sequence's own step (by the shapes and ``prefix_len``: about two
+    million tokens times kv-heads, summed over the batch), "shared" always.
     """
     _int_arg(prefix_len, "prefix_len", 0)
+    if kernel not in PREFIX_KERNELS:
+        raise RuntimeError(f"kernel must be one of {sorted(PREFIX_KERNELS)}")
     out_dtype = query.dtype if out_dtype is None else out_dtype
     _require(out_dtype in DTYPES and query.dim() == 3 and kv_cache.dim() == 4, _QUERY_SHAPE)
     ws = workspace or PrefixWorkspace(query.size(0), query.size(1), kv_cache.size(2), num_kv_splits, query.device,
@@ -716,7 +721,7 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
                             PrefixWorkspace, key_bits, value_bits, layout, out_dtype, attn_scale, sinks)
     with _on_device(query.device):
         rc = _lib.load().tq4_prefix_decode(*head, ws.scratch.data_ptr(), ws.scratch.numel(), *tail, prefix_len,
-                                           _stream(query.device))
+                                           PREFIX_KERNELS[kernel], _stream(query.device))
     _lib.check(rc, "tq4_prefix_decode")
     return ws.out, ws.lse
 
