@@ -307,7 +307,8 @@ int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, co
  * shared part with f16 pairs as operands and the weights of its values rounded to f16 (pairs for f16
  * outputs).  prefix_len: whole blocks, 0 up to the table's width; a sequence with fewer tokens
  * (seq_lens[b] < prefix_len, 0 included) attends to its own seq_lens[b] alone: its entries behind those
- * may hold anything.  query and out are 16-bit (TQ4_BF16, TQ4_F16).  kernel: TQ4_KERNEL_AUTO leaves the
+ * may hold anything.  Shared values beyond f16's range (code * scale + zero past 65504) become infinite.
+ * query and out are 16-bit (TQ4_BF16, TQ4_F16).  kernel: TQ4_KERNEL_AUTO leaves the
  * sharing (four launches) where the sequences' own steps are faster, by the shapes and prefix_len;
  * TQ4_KERNEL_SHARED shares always.
  * workspace: at least tq4_prefix_workspace_floats(...) floats, 16-byte aligned, contents after the call

@@ -16,9 +16,19 @@
 //
 // A workgroup of WR * WT waves takes WR * 32 rows and tiles of WT * 32 tokens, each wave 32 rows x 32
 // tokens of a tile; waves with the same rows join in LDS at the end.  WR = 4, WT = 2: eight waves, one
-// workgroup per CU; WR = 2, WT = 1, for up to 64 rows: two waves, three workgroups per CU.  A thread
+// workgroup per CU; WR = 2, WT = 1, for up to 64 rows: two waves, four workgroups per CU.  A thread
 // decodes 32 elements of K (a quarter of a token) and / or of V (8 dims of 4 tokens) per tile, from
-// registers loaded one tile ahead, into one of two LDS tiles; one barrier per tile.
+// registers loaded one tile ahead, into one of two LDS tiles (WT = 1: the only one).
+//
+// What bounds it: the matrix cores at the rate that they keep up under load, and what runs beside them.
+// 64 sequences of 4 heads a kv-head, 8 kv-heads, 32768 shared tokens (AoS): 98 us.  A 64-token tile is 64
+// products per SIMD; on zeros one takes 16 ns (2.1 PFLOP/s), on random operands read from LDS with four fma
+// beside it 25 ns (1.3 PFLOP/s: the card slows down with the bits that change), so 1.6 us of the 2.5 per tile.
+// Leaving out K's decoding saves 24 us, K's scores 24, V's decoding 11, the loads 13: none of them hides
+// another.  Orders that hide latencies better change little: every wave on its own 100 us, two workgroups of
+// four waves per CU 96, all products of a tile in one stretch with the exponentials between them 88 (but 1 to 4 %
+// slower whole calls at 2048 to 8192 tokens).  Start and end cost 11 to 15 us (8192 tokens: 35 us; one tile per
+// workgroup: 13): the chain pages, K, decoding, first product, and part rows of 516 bytes (17 MB at 16 splits).
 //
 // Precision: the centroids and q (times the score scale) are f16 hi + lo, three products c_hi q_hi +
 // c_lo q_hi + c_hi q_lo, and the norm multiplies the fp32 score, so scores and the log-sum-exp keep 2^-21
@@ -606,7 +616,9 @@ void prefix_kernel(const Args a) {
 
 // One wave per (q-head, sequence): the prefix's part rows, of sequences that have as many tokens, and the
 // sequence's own (one row when `whole`, else as many as its step left), joined as merge_parts_kernel
-// does; a sink logit (fp32 [Hq], may be null) adds to the sum.  Lane: dims 2 lane, 2 lane + 1.
+// does; a sink logit (fp32 [Hq], may be null) adds to the sum.  Lane: dims 2 lane, 2 lane + 1.  Latency
+// (both kinds of rows, the lengths and the counts are asked for at once): 7 us for 256 rows of 32 parts, 8 for 2048 of 16
+// (17 MB, 2.2 TB/s).
 template <typename OutT>
 __global__ __launch_bounds__(kWave) void join_kernel(const float *__restrict__ shared, int n_shared,
                                                      const float *__restrict__ own, int num_splits, int whole,
