@@ -188,6 +188,39 @@ def test_many_tokens(dev, preset, dtype):
     check(dev, build(5, 20011, 3, 8, preset, dtype=dtype))
 
 
+@pytest.mark.parametrize("n,preset,dtype,layout", [(9001, "4bit", "bf16", "soa"), (9001, "3bit", "fp32", "aos"),
+                                                   (5000, "4bit", "fp16", "aos_heads"), (5000, "k8v4", "bf16", "soa")])
+def test_many_tokens_on_several_axes(dev, n, preset, dtype, layout):
+    """Both sides of the size from which the queries have a launch of their own; and the writer alone."""
+    c = build(15, n, 2, 8, preset, layout=layout, dtype=dtype, sections=(16, 24, 24), in_turn=False)
+    check(dev, c)
+    _, want = call(c, dev)
+    c["q"] = None
+    out, got = call(c, dev)
+    assert out is None and np.array_equal(got, want)
+
+
+def test_query_out_among_the_inputs(dev):
+    c = build(16, 20, 4, 2)
+    q, k, v = (c[n].to(dev) for n in "qkv")
+    qkv = torch.cat([x.reshape(20, -1) for x in (q, k, v)], 1)
+    parts = [x.view(20, -1, D) for x in qkv.split([4 * D, 2 * D, 2 * D], 1)]
+    put = lambda x: torch.from_numpy(x).to(dev)  # noqa: E731
+    rest = (c["positions"].to(dev), c["table"].to(dev), c["cache"].to(dev), put(c["slots"]), put(c["rot_t"]), put(c["mids"]),
+            put(c["cents"]))
+    before = qkv.clone()
+    for out in (qkv.view(-1)[:20 * 4 * D].view(20, 4, D), qkv.view(-1)[64:64 + 20 * 4 * D].view(20, 4, D)):
+        with pytest.raises(RuntimeError, match="query_out"):
+            ops.rope_store(*parts, *rest, query_out=out)
+    with pytest.raises(RuntimeError, match="query_out"):
+        ops.rope_store(q, k, v, *rest, query_out=torch.cat([k, v], 1)[:, :, :].contiguous()[:19])
+    assert torch.equal(qkv, before)
+    beside = torch.empty(2, 20, 4, D, dtype=q.dtype, device=dev)
+    beside[0].copy_(q)
+    got = ops.rope_store(beside[0], k, v, *rest, query_out=beside[1])
+    assert torch.equal(got, ops.rope_store(*parts, *rest)) and torch.equal(beside[0], q)
+
+
 @pytest.mark.parametrize("preset", ["4bit", "k3v4"])
 def test_elements_next_to_midpoints(dev, preset):
     """Keys whose rotated direction lies on midpoints up to the type's own rounding: every row has elements that

@@ -420,6 +420,15 @@ def _axis_of(sections, in_turn, half):
     return (ctypes.c_int32 * half)(*axes)
 
 
+def _overlap(a, b):
+    """Whether the address ranges of two tensors meet."""
+    def ends(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
 def _token_rows(t, name, like, heads=None):
     """Checks ``t`` [N, H, D]: heads contiguous, tokens any whole 16-byte pieces apart; returns its token stride."""
     _require(t.is_cuda and t.dtype == like.dtype, f"{name} must be CUDA and of the keys' type")
@@ -465,6 +474,9 @@ def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, ro
         q_stride, Hq = _token_rows(query, "query", key), query.size(1)
         if query_out is None:
             query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        elif query_out.data_ptr() != query.data_ptr() or not query.is_contiguous():
+            _require(not any(_overlap(query_out, t) for t in (query, key, value)),
+                     "query_out must be query itself or lie apart from the inputs")
         _require(query_out.dtype == query.dtype and query_out.shape == query.shape and query_out.is_contiguous(),
                  "query_out must match query (shape, dtype) and be contiguous")
         tensors += [query, query_out]
