@@ -23,13 +23,15 @@
 // not rotated).  A query thread takes one unit of one row.
 //
 // What bounds it, and what it measured (32 / 8 heads, bf16, 4-bit keys).  32768 tokens: the queries' rows are
-// copied through in 99 us (537 MB, 5.4 TB/s: the card's copy rate), the writer takes 92-109 us for 170 MB: a
+// copied through in 99 us (537 MB, 5.4 TB/s: the card's copy rate), the writer takes 77-89 us for 170 MB: a
 // chain per tile (positions, then angles and keys, 96 matrix products, codes, V), four waves of a SIMD in turn,
-// 16 tiles per SIMD.  4097 tokens on three axes 36 us.  64 tokens 14.5 us: one workgroup's chain, the rotation
-// matrix staged and split in LDS (8.6 us in the plain writer), positions and angles before it.  Registers bind the
+// 16 tiles per SIMD; without the fp64 rows 61, without the angles too 53.  4097 tokens on three axes 36 us.  64 tokens 14.5 us: one workgroup's chain, the rotation
+// matrix staged and split in LDS (8.6 us in the plain writer), positions and angles before it, and the fp64 rows of the
+// slowest wave (4 us).  Registers bind the
 // large form (128 at four waves per SIMD): V asked for behind the products instead of ahead of the tile took
 // 34 spilled registers to 14, a unit's angles one unit at a time 50 to 12 (139 us to 104), one axis known to
-// the compiler 104 to 97; two waves per SIMD without spills 139.
+// the compiler 104 to 97; two waves per SIMD without spills 139.  A row in fp64 without a loop over its codes'
+// centroids, its sums by register moves: 97 to 89.
 #pragma once
 #include "store.h"
 
@@ -293,11 +295,26 @@ __device__ __forceinline__ void turned_key(float (&x)[32], const RawKey<T> &k, c
     }
 }
 
+// The sum over the wave, in every lane, by register moves (a shuffle goes through LDS and waits for it).
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1)
-        v += __shfl_xor(v, m, kWave);
-    return v;
+    v += dpp64<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+    v += dpp64<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+    v += dpp64<0x141>(v);  // row_half_mirror
+    v += dpp64<0x140>(v);  // row_mirror
+    auto pairs = [](double x, auto swap) {  // x of the one half of the lanes plus x of the other
+        const uint64_t b = __builtin_bit_cast(uint64_t, x);
+        const auto lo = swap((uint32_t)b), hi = swap((uint32_t)(b >> 32));
+        const uint32_t l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+        return __builtin_bit_cast(double, (uint64_t)h0 << 32 | l0) + __builtin_bit_cast(double, (uint64_t)h1 << 32 | l1);
+    };
+    v = pairs(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    return pairs(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
 }
 // A row in fp64, worked out by the wave: lane f < rot / 2 has plane f, the others two dims each that are
 // not rotated.
@@ -453,17 +470,22 @@ __device__ __forceinline__ void store_rows(const Args &a, int group, int groups)
         float kscalar = a.norm_correction ? norm * (1.0f / sqrtf(csum + 1e-16f)) : norm;
         const bool torn = live && half_bits(kscalar * (1.f - 0x1p-19f)) != half_bits(kscalar * (1.f + 0x1p-19f));
         if (__builtin_expect(__any(torn), 0)) {
+            const float cent = a.norm_correction ? a.centroids[lane & kMids] : 0.f;
             for (uint32_t todo = (uint32_t)__ballot(torn) & 0xFFFFu; todo; todo &= todo - 1) {
                 const int m = __builtin_ctz(todo);
                 const Exact<T> r(a, tile * kRows + m, lane);
                 double c2 = 0.0;
-                if (a.norm_correction) {
-                    if (n == m)
-                        for (int j = 0; j < 32; ++j) {
-                            const double c = a.centroids[code_at<KB>(kw, j)];
-                            c2 += c * c;
-                        }
-                    c2 = wave_sum64(c2);
+                if (a.norm_correction) {  // this lane's two of the row's 128 codes
+                    uint32_t two = 0;
+                    const int bit = 2 * KB * n;
+#pragma unroll
+                    for (int i = 0; i < KB; ++i) {
+                        const uint32_t w = (uint32_t)__shfl((int)kw[i], m + 16 * g, kWave);
+                        const int sh = bit - 32 * i;
+                        two |= sh >= 0 && sh < 32 ? w >> sh : sh < 0 && sh > -2 * KB ? w << -sh : 0u;
+                    }
+                    const double c0 = __shfl(cent, (int)(two & kMids), kWave), c1 = __shfl(cent, (int)(two >> KB & kMids), kWave);
+                    c2 = wave_sum64(c0 * c0 + c1 * c1);
                 }
                 const double k = a.norm_correction ? r.norm / sqrt(c2 + 1e-16) : r.norm;
                 kscalar = n == m ? (float)k : kscalar;
