@@ -38,6 +38,7 @@
 // That is an eighth of a bf16 output's own; for fp16 outputs P is hi + lo too (PLO), which leaves V's.
 // V beyond f16's range (65504) becomes infinite here.
 #pragma once
+#include "prefix_tiles.h"
 #include "step.h"
 
 namespace tq4 {
@@ -63,7 +64,7 @@ template <int WR, int WT, bool KF8> struct Shape {
     static constexpr int klo = tokens * kKRow;      // bytes: K hi at 0, K lo, V^T
     static constexpr int v = klo * (KF8 ? 1 : 2);
     static constexpr int tile = v + kHeadDim * vrow;
-    static constexpr int bufs = WT == 2 ? 2 : 1;
+    static constexpr int bufs = Buffers<WT>::tiles;
     static constexpr int join = WT == 2 ? WR * 64 * 66 * 4 : 0;  // the waves' sums at the end
     static constexpr int bytes = bufs * tile > join ? bufs * tile : join;
     static constexpr bool halves = threads > 4 * tokens;         // threads decode K or V, else both
@@ -356,8 +357,9 @@ template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR, int WT, bool PLO>
 __global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(WR == 4 ? 2 : 1, 2)))
 void prefix_kernel(const Args a) {
     using S = Shape<WR, WT, KF8>;
+    using B = Buffers<WT>;
     __shared__ __align__(16) unsigned char mem[S::bytes];
-    __shared__ __align__(16) float norms[S::bufs][S::tokens];
+    __shared__ __align__(16) float norms[B::factors][S::tokens];
     __shared__ __align__(16) uint2 lut[KF8 ? 1 : KB3 ? 64 : 256];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, h = lane >> 5, wr = w % WR, wt = w / WR;
@@ -375,17 +377,16 @@ void prefix_kernel(const Args a) {
     const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
     auto k_tok = [&](int i) { return min(S::tokens * i + (u >> 2), a.tokens - 1); };
     auto v_tok = [&](int i) { return min(S::tokens * i + 4 * (u >> 4), a.tokens - 4); };
-    // With one LDS tile (WT = 1) tile j + 1's K takes the place of tile j's, whose scores are done, and tile
-    // j's V is decoded when tile j - 1's is done with: a tile behind K.
-    constexpr int kBehind = 2 - S::bufs;
     const int32_t *pages = a.pages;
     int kblk = 0, vblk = 0;
-    auto within = [&](int i) { return max(min(i, tile1 - 1), tile0); };
+    // tile i of this workgroup's (past either end: the next one inside)
+    const int n_tiles = tile1 - tile0;
+    auto within = [&](int i) { return tile0 + max(min(i, n_tiles - 1), 0); };
     auto read_pages = [&](int i) {
         if (does_k)
             kblk = pages[k_tok(within(i)) >> a.block_size_log2];
         if (does_v)
-            vblk = pages[v_tok(within(i - kBehind)) >> a.block_size_log2];
+            vblk = pages[v_tok(within(i - B::behind)) >> a.block_size_log2];
     };
     RawK rk;
     RawV rv;
@@ -393,18 +394,16 @@ void prefix_kernel(const Args a) {
         if (does_k)
             load_k<LAYOUT, KF8, KB3, V3>(rk, a, kvh, k_tok(within(i)), kblk, u);
         if (does_v)
-            load_v<LAYOUT, KF8, KB3, V3>(rv, a, kvh, v_tok(within(i - kBehind)), vblk, u);
+            load_v<LAYOUT, KF8, KB3, V3>(rv, a, kvh, v_tok(within(i - B::behind)), vblk, u);
     };
-    // tile i's K and tile i - kBehind's V
     auto store = [&](int i) {
-        const int buf = (i - tile0) & (S::bufs - 1);
-        unsigned char *m = mem + buf * S::tile;
+        unsigned char *m = mem + B::tile(i) * S::tile;
         if (does_k)
-            store_k<LAYOUT, KF8, KB3>(rk, m, m + S::klo, norms[buf], lut, u);
+            store_k<LAYOUT, KF8, KB3>(rk, m, m + S::klo, norms[B::factor(i)], lut, u);
         if (does_v)
             store_v<LAYOUT, V3, S::vrow>(rv, m + S::v, u);
     };
-    read_pages(tile0);
+    read_pages(0);
     if constexpr (!KF8)
         for (int e = tid; e < (KB3 ? 64 : 256); e += S::threads) {
             const uint32_t x = xdl::split_f16(a.centroids[KB3 ? e & 7 : e & 15]), z = xdl::split_f16(a.centroids[KB3 ? e >> 3 : e >> 4]);
@@ -417,10 +416,10 @@ void prefix_kernel(const Args a) {
         if (b < 0)
             return;
         pages += (int64_t)b * a.table_width;
-        read_pages(tile0);
+        read_pages(0);
     }
-    load(tile0);
-    read_pages(tile0 + 1);
+    load(0);
+    read_pages(1);
 
     const int row = rt * 32 * WR + 32 * wr + c, row_in = min(row, a.rows - 1);
     const int b = row_in / a.group, hh = row_in - b * a.group;
@@ -438,15 +437,11 @@ void prefix_kernel(const Args a) {
     float negm = __FLT_MAX__, l = 0.f;  // -max in log2 units (+FLT_MAX: no token yet), this lane's share of the sum
 
     xdl::lds_barrier();  // the table
-    store(tile0);
-    load(tile0 + 1);
-    read_pages(tile0 + 2);
-    xdl::lds_barrier();
-
-    // Tile j + 1's scores are worked out while tile j's weights go into the accumulators (matrix phase), then
-    // its softmax and the decoding of the next tile (vector phase).  The two waves of a SIMD are a phase
-    // apart (WT = 2): one uses the matrix core while the other uses the vector unit.  A phase ends at a
-    // barrier; tile j + 1 takes the LDS place of tile j - 1, whose last reader is a phase behind at most.
+    auto fill = [&](int i) {
+        store(i);
+        load(i + 1);
+        read_pages(i + 2);
+    };
     const bool late = WT == 2 && w >= WR;
     auto phase_end = [] {
         __builtin_amdgcn_sched_barrier(0);
@@ -457,7 +452,7 @@ void prefix_kernel(const Args a) {
     half8 p[2], p_lo[2];
     const unsigned char *k_from = mem + (32 * wt + c) * kKRow + 16 * h, *v_from = mem + S::v + c * S::vrow + 16 * (4 * wt + h);
     auto scores = [&](int i) {
-        const unsigned char *k_hi = k_from + ((i - tile0) & (S::bufs - 1)) * S::tile;
+        const unsigned char *k_hi = k_from + B::tile(i) * S::tile;
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             s[k] = 0.f;
@@ -472,7 +467,7 @@ void prefix_kernel(const Args a) {
         }
     };
     auto outputs = [&](int i) {
-        const unsigned char *vt = v_from + ((i - tile0) & (S::bufs - 1)) * S::tile;
+        const unsigned char *vt = v_from + B::tile(i) * S::tile;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -483,17 +478,12 @@ void prefix_kernel(const Args a) {
                     acc[d] = mfma32(v, p_lo[t], acc[d]);
             }
     };
-    if (late)
-        phase_end();
-    scores(tile0);
-    phase_end();
-    for (int j = tile0; j < tile1; ++j) {
-        const int buf = (j - tile0) & (S::bufs - 1);
+    auto softmax = [&](int j) {
         float n[16];
         if constexpr (!KF8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float4 v = *reinterpret_cast<const float4 *>(norms[buf] + 32 * wt + 8 * k + 4 * h);
+                const float4 v = *reinterpret_cast<const float4 *>(norms[B::factor(j)] + 32 * wt + 8 * k + 4 * h);
                 n[4 * k] = v.x;
                 n[4 * k + 1] = v.y;
                 n[4 * k + 2] = v.z;
@@ -508,10 +498,11 @@ void prefix_kernel(const Args a) {
             for (int k = 0; k < 16; ++k)
                 n[k] = f;
         }
-        if (S::tokens * (j + 1) > a.tokens) {  // tokens past the prefix (the last tile's)
+        const int first = S::tokens * (tile0 + j);
+        if (first + S::tokens > a.tokens) {  // tokens past the prefix (the last tile's)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-                if (S::tokens * j + 32 * wt + 8 * (k >> 2) + 4 * h + (k & 3) >= a.tokens) {
+                if (first + 32 * wt + 8 * (k >> 2) + 4 * h + (k & 3) >= a.tokens) {
                     s[k] = -INFINITY;
                     n[k] = 1.f;
                 }
@@ -551,21 +542,9 @@ void prefix_kernel(const Args a) {
             if constexpr (PLO)
                 p_lo[t] = pinned(p_lo[t]);
         }
-        if (j + 1 < tile1 || kBehind) {
-            store(j + 1);
-            load(j + 2);
-            read_pages(j + 3);
-        }
-        phase_end();
-        __builtin_amdgcn_s_setprio(1);
-        if (j + 1 < tile1)
-            scores(j + 1);
-        outputs(j);
-        __builtin_amdgcn_s_setprio(0);
-        phase_end();
-    }
-    if (WT == 2 && !late)
-        phase_end();
+    };
+    run_tiles<WT>(n_tiles, late, [] { xdl::lds_barrier(); }, phase_end, fill, scores, softmax, outputs,
+                  [](bool up) { up ? __builtin_amdgcn_s_setprio(1) : __builtin_amdgcn_s_setprio(0); });
 
     l = pair_sum(l);
     if constexpr (WT == 2) {
