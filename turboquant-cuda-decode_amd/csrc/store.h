@@ -255,6 +255,7 @@ template <int W> __device__ __forceinline__ void load_pit(PitLoads<W> &p, const 
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             p.w[it][j] = pit[(8 * k8 + j) * kHeadDim + c];
+        __builtin_amdgcn_sched_barrier(0);  // (in the order in which store_pit takes them)
     }
 }
 template <int W> __device__ __forceinline__ void store_pit(const PitLoads<W> &p, _Float16 *pt_hi, _Float16 *pt_lo) {
@@ -271,6 +272,7 @@ template <int W> __device__ __forceinline__ void store_pit(const PitLoads<W> &p,
         }
         *reinterpret_cast<half8 *>(pt_hi + pt_off(c, k8)) = h;
         *reinterpret_cast<half8 *>(pt_lo + pt_off(c, k8)) = l;
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
