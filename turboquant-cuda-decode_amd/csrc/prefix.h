@@ -322,7 +322,10 @@ __device__ __forceinline__ float load_q(half8 (&hi)[8], half8 (&lo)[8], const Ar
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float v = x[i][j] * scale;
+            // (the product stands in a register: folded into one of the two casts, and rounded once there, hi
+            // and lo would not belong together where it is next to a tie of f16)
+            float v = x[i][j] * scale;
+            asm("" : "+v"(v));
             hi[i][j] = (_Float16)v;
             lo[i][j] = (_Float16)(v - (float)hi[i][j]);
         }
