@@ -304,10 +304,10 @@ int tq4_window_decode(const void *query, int query_dtype, const float *rot_t, co
  * prefix_len / block_size entries of block_table name the same blocks in the row of every sequence that
  * has as many tokens.  The shared tokens are read and decoded once for the query rows of all
  * sequences; the results are those of tq4_full_decode / tq4_full_decode_preset on the same arguments, the
- * shared part with f16 pairs as operands and the weights of its values rounded to f16 (pairs for f16
- * outputs).  prefix_len: whole blocks, 0 up to the table's width; a sequence with fewer tokens
+ * shared part's scores from f16 pairs and its weights (softmax weight times V scale) rounded to f16 for bf16
+ * outputs, to f16 pairs for f16 outputs.  prefix_len: whole blocks, 0 up to the table's width; a sequence with fewer tokens
  * (seq_lens[b] < prefix_len, 0 included) attends to its own seq_lens[b] alone: its entries behind those
- * may hold anything.  Shared values beyond f16's range (code * scale + zero past 65504) become infinite.
+ * may hold anything.
  * query and out are 16-bit (TQ4_BF16, TQ4_F16).  kernel: TQ4_KERNEL_AUTO leaves the
  * sharing (four launches) where the sequences' own steps are faster, by the shapes and prefix_len;
  * TQ4_KERNEL_SHARED shares always.

@@ -153,3 +153,73 @@ def test_query_elements_next_to_a_tie(dev, batch, dtype):
 @pytest.mark.parametrize("batch,hk,group", [(150, 2, 8), (6, 2, 8)])
 def test_log_sum_exps(dev, preset, layout, dtype, batch, hk, group):
     check_lse(dev, build(2, batch, 160, 30, hk, group, preset=preset, layout=layout, dtype=dtype))
+
+
+FORMATS = [("4bit", "soa", torch.bfloat16), ("4bit", "aos", torch.float16), ("4bit", "soa", torch.float16), ("k3v4", "aos", torch.bfloat16),
+           ("3bit", "aos_heads", torch.float16), ("k3v4", "soa", torch.float16), ("k8v4", "soa", torch.bfloat16), ("k8v4", "aos", torch.float16)]
+
+
+def check(dev, c, splits, **kw):
+    got = call(dev, c, splits, **kw)
+    out, lse, bar_out, bar_lse = want(c)
+    for what, x, y, bar in (("lse", got[1], lse, bar_lse), ("out", got[0], out, bar_out)):
+        assert np.isfinite(x).all(), what
+        assert (np.abs(x - y) / bar).max() <= 1.0, (what, (np.abs(x - y) / bar).max())
+
+
+@pytest.mark.parametrize("preset,layout,dtype", FORMATS)
+@pytest.mark.parametrize("batch,hk,group", [(40, 2, 8), (7, 2, 4)])
+def test_outputs(dev, preset, layout, dtype, batch, hk, group):
+    """V's codes are exact, its scales and middles fp32: fp16 outputs are as near as their own rounding."""
+    check(dev, build(3, batch, 208, 40, hk, group, preset=preset, layout=layout, dtype=dtype), 8)
+
+
+def scalars_of(scales, zeros, norms=None):
+    """A hook of `build`: the cache with other scales and zeros of V (and norms)."""
+    def put(rng, cache, preset, layout):
+        kb, vb = plain.PRESETS[preset]
+        n, bs, hk, slot = cache.shape
+        assert layout != "aos_heads"
+        raw = cache.numpy()
+        kc, vc, fields = plain.split_cache(raw, kb, vb, layout)
+        new = [f.copy() for f in fields]
+        new[-2], new[-1] = scales(rng, (n, bs, hk)).astype(np.float16), zeros(rng, (n, bs, hk)).astype(np.float16)
+        if norms is not None and kb != 8:
+            new[0] = norms(rng, (n, bs, hk)).astype(np.float16)
+        rec = 16 * (kb + vb)
+        if layout == "soa":
+            meta = np.stack([f.transpose(0, 2, 1) for f in new], 2)
+            raw.reshape(n, -1)[:, bs * hk * rec:] = np.ascontiguousarray(meta).view(np.uint8).reshape(n, -1)
+        else:
+            at = 16 * kb + (0 if kb == 8 else 2) + 16 * vb
+            for i, f in enumerate(new[-2:]):
+                raw[..., at + 2 * i:at + 2 * i + 2] = np.ascontiguousarray(f[..., None]).view(np.uint8)
+            if kb != 8:
+                raw[..., 16 * kb:16 * kb + 2] = np.ascontiguousarray(new[0][..., None]).view(np.uint8)
+        return (cache, *plain.values_of(kc, vc, new, kb, layout))
+    return put
+
+
+@pytest.mark.parametrize("preset,layout", [("4bit", "soa"), ("4bit", "aos"), ("3bit", "soa"), ("k8v4", "aos")])
+@pytest.mark.parametrize("batch,prefix", [(40, 1040), (6, 528)])
+def test_values_past_f16(dev, preset, layout, batch, prefix):
+    """Scales up to f16's largest number beside small ones, values beyond it: finite, and as near as others."""
+    log = lambda rng, shape: np.exp(rng.uniform(np.log(0.01), np.log(65000.0), shape))  # noqa: E731
+    zero = lambda rng, shape: rng.uniform(-65000.0, 65000.0, shape)  # noqa: E731
+    c = build(4, batch, prefix, 40, 8, 4, preset=preset, layout=layout, dtype=torch.bfloat16, scalars=scalars_of(log, zero))
+    assert np.abs(c["v"]).max() > 3e5
+    check(dev, c, 8)
+
+
+@pytest.mark.parametrize("preset,layout,dtype", FORMATS)
+@pytest.mark.parametrize("batch,hk,group,prefix", [(36, 8, 6, 3120), (12, 8, 5, 6192)])
+def test_several_tiles_a_workgroup(dev, preset, layout, dtype, batch, hk, group, prefix):
+    """Runs of three and four tiles on 256 CUs, the last tile ending early: 49 tiles of 64 tokens cut into 13 runs
+    (216 rows, eight waves), 194 of 32 into 49 (60 rows, two waves)."""
+    check(dev, build(5, batch, prefix, 24, hk, group, preset=preset, layout=layout, dtype=dtype), 8)
+
+
+def test_sharing_by_rule_is_as_near(dev):
+    """`kernel="auto"` where it shares: 64 x 4096, five tiles a workgroup."""
+    c = build(6, 64, 4144, 30, 8, 4, dtype=torch.bfloat16)
+    check(dev, c, 16, kernel="auto")

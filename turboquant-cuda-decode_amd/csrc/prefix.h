@@ -7,7 +7,7 @@
 // and every operand is a plain f16 tile.
 //
 //   S^T[token][row] = sum_d c[token][d] q[row][d]       v_mfma_f32_32x32x16_f16, A = c, B = q
-//   O^T[dim][row]  += sum_t V^T[dim][t] P^T[t][row]     the same, A = V^T, B = P
+//   O^T[dim][row]  += sum_t V^T[dim][t] P^T[t][row]     the same, A = V's codes less the middle one, B = P x V's scale
 //
 // With the rows in the columns a lane (c, h) = (lane % 32, lane / 32) has one row's scores (tokens 8 (i / 4) +
 // 4 h + i % 4 of its 32): the running maximum and the sum are its own values, the accumulators are
@@ -34,9 +34,12 @@
 // c_lo q_hi + c_hi q_lo, and the norm multiplies the fp32 score, so scores and the log-sum-exp keep 2^-21
 // as the step's do; FP8 keys and 16-bit queries are exact in f16, one product.  (With single f16
 // operands the log-sum-exp was off by 1 to 3e-5: a centroid's rounding is the same for every token that
-// has it.)  Two roundings to f16 remain, half a step (2^-11) each: V = code * scale + zero, and P.
-// That is an eighth of a bf16 output's own; for fp16 outputs P is hi + lo too (PLO), which leaves V's.
-// V beyond f16's range (65504) becomes infinite here.
+// has it.)  V's codes are exact, p times a token's V scale is the operand, and the sum of p times V's value at the middle
+// code is the row's own in fp32.  For bf16 outputs the operand is one f16 (half a step, 2^-11, of the distance from the middle:
+// with the codes themselves it would be of twice as much), for fp16 outputs hi + lo (PLO).  Relative errors of 64 x 8192
+// tokens in bf16 1.675e-3 where rounding the output alone makes 1.662e-3 (hi + lo: a quarter more matrix products), of 100 x 4000 in
+// fp16 2.074e-4, as rounding alone.  (V itself as f16, code * scale + zero: 1.683e-3 and 2.65e-4, infinite past 65504,
+// and 0.5 to 1.5 us faster: 65.9 : 67.4 us the whole call for the first, 61.1 : 61.8 for the second.)
 #pragma once
 #include "prefix_tiles.h"
 #include "step.h"
@@ -65,10 +68,21 @@ template <int WR, int WT, bool KF8> struct Shape {
     static constexpr int v = klo * (KF8 ? 1 : 2);
     static constexpr int tile = v + kHeadDim * vrow;
     static constexpr int bufs = Buffers<WT>::tiles;
-    static constexpr int join = WT == 2 ? WR * 64 * 66 * 4 : 0;  // the waves' sums at the end
+    static constexpr int join = WT == 2 ? WR * 64 * 67 * 4 : 0;  // the waves' sums at the end
     static constexpr int bytes = bufs * tile > join ? bufs * tile : join;
     static constexpr bool halves = threads > 4 * tokens;         // threads decode K or V, else both
+    static constexpr int k_waves = halves ? WR * WT / 2 : WR * WT;  // that decode K
     static_assert(threads == 4 * tokens * (halves ? 2 : 1), "a unit of 32 elements per thread");
+};
+
+// What the softmax takes of a tile's tokens: the score factor (not with FP8 keys), V's scale and V's value at the
+// middle code; and, from each wave that decodes K, whether one of its scales is above kLargeScale.
+constexpr float kLargeScale = 128.f;
+template <bool V3> constexpr float kMiddle = V3 ? 4.f : 8.f;
+template <int TOKENS, int K_WAVES, bool KF8> struct alignas(16) Factors {
+    float norm[KF8 ? 4 : TOKENS];
+    float2 v[TOKENS];
+    uint32_t large[K_WAVES];
 };
 
 struct Args {
@@ -94,15 +108,11 @@ __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_ca
 __device__ __forceinline__ uint32_t as_u32(half2v x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ half2v splat(_Float16 x) { return half2v{x, x}; }
 
-// What a thread loads of a tile, unit u: K bytes of token u / 4 (dims 32 (u % 4) ..) and its norm; V bytes
-// of tokens 4 (u / 16) .. +3 (dims 8 (u % 16) ..), their scales and zeros.
+// What a thread loads of a tile, unit u: K bytes of token u / 4 (dims 32 (u % 4) ..) and one of its scalars (u % 4:
+// norm, V's scale, V's zero; FP8 keys: no norm); V bytes of tokens 4 (u / 16) .. +3 (dims 8 (u % 16) ..), four of each.
 struct RawK {
     uint4 k, k2;           // (k2: FP8 keys)
-    uint32_t norm;
-};
-struct RawV {
-    uint32_t v[4];
-    uint32_t sz[4];        // SoA: four scales, four zeros; AoS: scale | zero of each token
+    uint32_t scalar;
 };
 
 // Token `t` of a kv-head in block `blk`.
@@ -139,38 +149,30 @@ __device__ __forceinline__ void load_k(RawK &r, const Args &a, int kvh, int t, i
             r.k2 = uint4{w2[0], w2[1], w2[2], w2[3]};
         }
     }
-    if constexpr (!KF8)
-        r.norm = LAYOUT == 0 ? at.meta[0] : *reinterpret_cast<const uint16_t *>(at.data + R::kbytes);
+    const int f = min(u & 3, R::nf - 1), v = KF8 ? f : f - 1;  // (v: -1 norm, 0 scale, 1 zero)
+    if constexpr (LAYOUT == 0)
+        r.scalar = at.meta[f * at.bs];
+    else
+        r.scalar = *reinterpret_cast<const uint16_t *>(at.data + (v < 0 ? R::kbytes : R::v0 + R::vbytes + 2 * v));
 }
 // (t: a multiple of 4, its four tokens in one block)
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void load_v(RawV &r, const Args &a, int kvh, int t, int blk, int u) {
+__device__ __forceinline__ void load_v(uint4 &r, const Args &a, int kvh, int t, int blk, int u) {
     using R = Record<LAYOUT, KF8, KB3, V3>;
     const R at(a, kvh, t, blk);
     const uint8_t *p = at.data + R::v0 + (V3 ? 3 : 4) * (u & 15);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)  // (3-bit values: the fourth byte is the next field's first)
-        r.v[i] = *reinterpret_cast<const u32a1 *>(p + (int64_t)i * at.pos);
-    if constexpr (LAYOUT == 0) {
-        const uint2 s = *reinterpret_cast<const uint2 *>(at.meta + (R::nf - 2) * at.bs);
-        const uint2 z = *reinterpret_cast<const uint2 *>(at.meta + (R::nf - 1) * at.bs);
-        r.sz[0] = s.x;
-        r.sz[1] = s.y;
-        r.sz[2] = z.x;
-        r.sz[3] = z.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            r.sz[i] = *reinterpret_cast<const u32a2 *>(at.data + R::v0 + R::vbytes + (int64_t)i * at.pos);
-    }
+    auto token = [&](int i) { return *reinterpret_cast<const u32a1 *>(p + (int64_t)i * at.pos); };
+    r = uint4{token(0), token(1), token(2), token(3)};  // (3-bit values: the fourth byte is the next field's first)
 }
 
-// The unit's K elements into the LDS tile(s) and, from the token's first thread, the token's score factor.
+// The unit's K elements into the LDS tile(s) and, from the token's first thread, the token's factors; `wave`: the
+// wave's number among those that decode K.
 // 4-bit keys: a byte's pair of centroids, hi and lo parts, from a 256-entry table; 3-bit: six bits' from 64.
-template <int LAYOUT, bool KF8, bool KB3>
-__device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsigned char *klo, float *norms,
-                                        const uint2 *lut, int u) {
+template <int LAYOUT, bool KF8, bool KB3, bool V3, class F>
+__device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsigned char *klo, F &factors,
+                                        const uint2 *lut, int u, int wave) {
     const int t = u >> 2, j = u & 3, at = t * kKRow + 64 * j;
+    const float own = half_bits_to_float(r.scalar);
     uint32_t e[16], lo[16];
     if constexpr (KF8) {
         const uint32_t w[8] = {r.k.x, r.k.y, r.k.z, r.k.w, r.k2.x, r.k2.y, r.k2.z, r.k2.w};
@@ -199,7 +201,7 @@ __device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsig
             e[b] = c.x;
             lo[b] = c.y;
         }
-        float n = half_bits_to_float(r.norm);
+        float n = own;
         if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction (h.h + 2 h.l: see lookup_tile)
             float hh = 0.f, hl = 0.f;
 #pragma unroll
@@ -215,7 +217,7 @@ __device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsig
             n *= __builtin_amdgcn_rsqf(csq + 1e-16f);
         }
         if (j == 0)
-            norms[t] = n;
+            factors.norm[t] = n;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<uint4 *>(klo + at + 16 * q) = uint4{lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]};
@@ -223,44 +225,36 @@ __device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsig
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         *reinterpret_cast<uint4 *>(khi + at + 16 * q) = uint4{e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
+    const float scale = xdl::quad_bcast<KF8 ? 0 : 1>(own);
+    if (j == (KF8 ? 1 : 2))
+        factors.v[t] = float2{scale, fmaf(scale, kMiddle<V3>, own)};
+    const bool large = __any(fabsf(scale) > kLargeScale);
+    if ((u & 63) == 0)
+        factors.large[wave] = large;
 }
 
-// The unit's V elements (8 dims of 4 tokens), transposed into the LDS tile: for dim i the f16 pairs of
-// tokens (0, 1) and (2, 3).  A code is put into the significand of 1024 and 1024 taken off again.
-template <int LAYOUT, bool V3, int VROW> __device__ __forceinline__ void store_v(const RawV &r, unsigned char *vtile, int u) {
+// The unit's V codes (8 dims of 4 tokens) less the middle one, transposed into the LDS tile: for dim i the f16
+// pairs of tokens (0, 1) and (2, 3).  A code is put into the significand of 1024 and 1024 + the middle taken off.
+template <bool V3, int VROW> __device__ __forceinline__ void store_v(const uint4 &r, unsigned char *vtile, int u) {
     const int dg = u & 15, quad = u >> 4;
-    half2v s01, s23, z01, z23;
-    if constexpr (LAYOUT == 0) {
-        s01 = as_half2(r.sz[0]);
-        s23 = as_half2(r.sz[1]);
-        z01 = as_half2(r.sz[2]);
-        z23 = as_half2(r.sz[3]);
-    } else {
-        s01 = as_half2(__builtin_amdgcn_perm(r.sz[1], r.sz[0], 0x05040100u));
-        z01 = as_half2(__builtin_amdgcn_perm(r.sz[1], r.sz[0], 0x07060302u));
-        s23 = as_half2(__builtin_amdgcn_perm(r.sz[3], r.sz[2], 0x05040100u));
-        z23 = as_half2(__builtin_amdgcn_perm(r.sz[3], r.sz[2], 0x07060302u));
-    }
-    const half2v k1024 = splat((_Float16)1024.f);
-    auto value = [&](uint32_t codes, half2v s, half2v z) {
-        const half2v x = as_half2(codes | 0x64006400u) - k1024;
-        return as_u32(__builtin_elementwise_fma(x, s, z));
-    };
+    const uint32_t v[4] = {r.x, r.y, r.z, r.w};
+    const half2v k0 = splat((_Float16)(1024.f + kMiddle<V3>));
+    auto value = [&](uint32_t codes) { return as_u32(as_half2(codes | 0x64006400u) - k0); };
     unsigned char *to = vtile + dg * VROW + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1);
     auto put = [&](int i, uint32_t c01, uint32_t c23) {
-        *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{value(c01, s01, z01), value(c23, s23, z23)};
+        *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{value(c01), value(c23)};
     };
     if constexpr (V3) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            auto code = [&](int t) { return (r.v[t] >> (3 * i)) & 7u; };
+            auto code = [&](int t) { return (v[t] >> (3 * i)) & 7u; };
             put(i, code(0) | (code(1) << 16), code(2) | (code(3) << 16));
         }
     } else {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const uint32_t sel = (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u;
-            const uint32_t p01 = __builtin_amdgcn_perm(r.v[1], r.v[0], sel), p23 = __builtin_amdgcn_perm(r.v[3], r.v[2], sel);
+            const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel), p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
             put(2 * m, p01 & 0x000F000Fu, p23 & 0x000F000Fu);
             put(2 * m + 1, (p01 >> 4) & 0x000F000Fu, (p23 >> 4) & 0x000F000Fu);
         }
@@ -357,12 +351,12 @@ __device__ __forceinline__ float pair_max(float x) { return xdl::max_xor32(x); }
 __device__ __forceinline__ float pair_sum(float x) { return xdl::sum_xor32(x); }
 
 template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR, int WT, bool PLO>
-__global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(WR == 4 ? 2 : 1, 2)))
+__global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void prefix_kernel(const Args a) {
     using S = Shape<WR, WT, KF8>;
     using B = Buffers<WT>;
     __shared__ __align__(16) unsigned char mem[S::bytes];
-    __shared__ __align__(16) float norms[B::factors][S::tokens];
+    __shared__ __align__(16) Factors<S::tokens, S::k_waves, KF8> factors[B::factors];
     __shared__ __align__(16) uint2 lut[KF8 ? 1 : KB3 ? 64 : 256];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, h = lane >> 5, wr = w % WR, wt = w / WR;
@@ -376,35 +370,46 @@ void prefix_kernel(const Args a) {
     const int tile0 = (int)((int64_t)a.tiles * sp / a.splits), tile1 = (int)((int64_t)a.tiles * (sp + 1) / a.splits);
 
     // this thread's unit of a tile; its tokens are kept inside the prefix (whole blocks: a multiple of 16)
-    const int u = tid & (4 * S::tokens - 1);
+    // (worked out again in every tile: what depends on it alone would be kept from tile to tile, and spill)
+    auto unit = [&] {
+        int u = tid & (4 * S::tokens - 1);
+        asm volatile("" : "+v"(u));
+        return u;
+    };
     const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
-    auto k_tok = [&](int i) { return min(S::tokens * i + (u >> 2), a.tokens - 1); };
-    auto v_tok = [&](int i) { return min(S::tokens * i + 4 * (u >> 4), a.tokens - 4); };
+    auto k_tok = [&](int i, int u) { return min(S::tokens * i + (u >> 2), a.tokens - 1); };
+    auto v_tok = [&](int i, int u) { return min(S::tokens * i + 4 * (u >> 4), a.tokens - 4); };
     const int32_t *pages = a.pages;
-    int kblk = 0, vblk = 0;
+    // (a thread that decodes one of the two has the same registers for both)
+    int blks[2] = {};
+    int &kblk = blks[0], &vblk = blks[S::halves ? 0 : 1];
+    RawK rk;
+    uint4 rv_own;
+    uint4 &rv = S::halves ? rk.k : rv_own;
     // tile i of this workgroup's (past either end: the next one inside)
     const int n_tiles = tile1 - tile0;
     auto within = [&](int i) { return tile0 + max(min(i, n_tiles - 1), 0); };
     auto read_pages = [&](int i) {
+        const int u = unit();
         if (does_k)
-            kblk = pages[k_tok(within(i)) >> a.block_size_log2];
+            kblk = pages[k_tok(within(i), u) >> a.block_size_log2];
         if (does_v)
-            vblk = pages[v_tok(within(i - B::behind)) >> a.block_size_log2];
+            vblk = pages[v_tok(within(i - B::behind), u) >> a.block_size_log2];
     };
-    RawK rk;
-    RawV rv;
     auto load = [&](int i) {
+        const int u = unit();
         if (does_k)
-            load_k<LAYOUT, KF8, KB3, V3>(rk, a, kvh, k_tok(within(i)), kblk, u);
+            load_k<LAYOUT, KF8, KB3, V3>(rk, a, kvh, k_tok(within(i), u), kblk, u);
         if (does_v)
-            load_v<LAYOUT, KF8, KB3, V3>(rv, a, kvh, v_tok(within(i - B::behind)), vblk, u);
+            load_v<LAYOUT, KF8, KB3, V3>(rv, a, kvh, v_tok(within(i - B::behind), u), vblk, u);
     };
     auto store = [&](int i) {
+        const int u = unit();
         unsigned char *m = mem + B::tile(i) * S::tile;
         if (does_k)
-            store_k<LAYOUT, KF8, KB3>(rk, m, m + S::klo, norms[B::factor(i)], lut, u);
+            store_k<LAYOUT, KF8, KB3, V3>(rk, m, m + S::klo, factors[B::factor(i)], lut, u, w);
         if (does_v)
-            store_v<LAYOUT, V3, S::vrow>(rv, m + S::v, u);
+            store_v<V3, S::vrow>(rv, m + S::v, u);
     };
     read_pages(0);
     if constexpr (!KF8)
@@ -437,7 +442,8 @@ void prefix_kernel(const Args a) {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             acc[i][k] = 0.f;
-    float negm = __FLT_MAX__, l = 0.f;  // -max in log2 units (+FLT_MAX: no token yet), this lane's share of the sum
+    // -max in log2 units (+FLT_MAX: no token yet), this lane's shares of the sum and of V's middle values
+    float negm = __FLT_MAX__, l = 0.f, z = 0.f;
 
     xdl::lds_barrier();  // the table
     auto fill = [&](int i) {
@@ -482,11 +488,13 @@ void prefix_kernel(const Args a) {
             }
     };
     auto softmax = [&](int j) {
+        const auto &of = factors[B::factor(j)];
+        const int tok0 = 32 * wt + 4 * h;  // s[k]: token tok0 + 8 (k / 4) + k % 4 of the tile
         float n[16];
         if constexpr (!KF8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float4 v = *reinterpret_cast<const float4 *>(norms[B::factor(j)] + 32 * wt + 8 * k + 4 * h);
+                const float4 v = *reinterpret_cast<const float4 *>(of.norm + tok0 + 8 * k);
                 n[4 * k] = v.x;
                 n[4 * k + 1] = v.y;
                 n[4 * k + 2] = v.z;
@@ -501,17 +509,30 @@ void prefix_kernel(const Args a) {
             for (int k = 0; k < 16; ++k)
                 n[k] = f;
         }
+        uint32_t large = 0;
+#pragma unroll
+        for (int k = 0; k < S::k_waves; ++k)
+            large |= of.large[k];
+        // V's scales and middles a quarter (four tokens) ahead: there are no registers for all
+        float4 v[2][2];
+        auto read_v = [&](int q) {
+            const float4 *from = reinterpret_cast<const float4 *>(of.v + tok0 + 8 * q);
+            v[q & 1][0] = from[0];
+            v[q & 1][1] = from[1];
+        };
+        read_v(0);
         const int first = S::tokens * (tile0 + j);
         if (first + S::tokens > a.tokens) {  // tokens past the prefix (the last tile's)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-                if (first + 32 * wt + 8 * (k >> 2) + 4 * h + (k & 3) >= a.tokens) {
+                if (first + tok0 + 8 * (k >> 2) + (k & 3) >= a.tokens) {
                     s[k] = -INFINITY;
                     n[k] = 1.f;
                 }
         }
         // Scores in log2 units; the running maximum moves only when one passes it by more than kRescaleLogX (p
-        // stays below 256).  (The three-way maximum reads the multiplications' results, never the matrix
+        // stays below 256), with a large scale in the tile whenever one passes it: p times a scale, an f16
+        // operand, stays below 2^15, or 65504.  (The three-way maximum reads the multiplications' results, never the matrix
         // core's: its wait states are the compiler's to insert, and it does not see into asm.)
         float mx = -INFINITY;
 #pragma unroll
@@ -520,23 +541,37 @@ void prefix_kernel(const Args a) {
             s[k + 1] = s[k + 1] * n[k + 1];
             mx = max3(mx, s[k], s[k + 1]);
         }
-        if (__any(mx + negm > xdl::kRescaleLogX)) {
+        const float most = large ? 0.f : xdl::kRescaleLogX;
+        if (__any(mx + negm > most)) {
             const float m_row = pair_max(mx);
-            const float negm_new = m_row + negm > xdl::kRescaleLogX ? -m_row : negm;
+            const float negm_new = m_row + negm > most ? -m_row : negm;
             const float alpha = __builtin_amdgcn_exp2f(negm_new - negm);  // 0 at the first tile
             negm = negm_new;
             l *= alpha;
+            z *= alpha;
 #pragma unroll
             for (int d = 0; d < 4; ++d)
                 acc[d] *= alpha;
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float e = __builtin_amdgcn_exp2f(s[k] + negm);
-            l += e;
-            p[k >> 3][k & 7] = (_Float16)e;
-            if constexpr (PLO)
-                p_lo[k >> 3][k & 7] = (_Float16)(e - (float)p[k >> 3][k & 7]);
+        for (int q = 0; q < 4; ++q) {
+            if (q < 3)
+                read_v(q + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 4 * q + i;
+                const float4 &vv = v[q & 1][i >> 1];
+                const float e = __builtin_amdgcn_exp2f(s[k] + negm);
+                l += e;
+                z = fmaf(e, i & 1 ? vv.w : vv.y, z);
+                float x = e * (i & 1 ? vv.z : vv.x);
+                if constexpr (PLO)
+                    asm("" : "+v"(x));  // (see load_q)
+                p[k >> 3][k & 7] = (_Float16)x;
+                if constexpr (PLO)
+                    p_lo[k >> 3][k & 7] = (_Float16)(x - (float)p[k >> 3][k & 7]);
+            }
         }
         // (worked out here: left to itself the compiler moves this into the matrix phase, next to its use)
 #pragma unroll
@@ -550,10 +585,11 @@ void prefix_kernel(const Args a) {
                   [](bool up) { up ? __builtin_amdgcn_s_setprio(1) : __builtin_amdgcn_s_setprio(0); });
 
     l = pair_sum(l);
+    z = pair_sum(z);
     if constexpr (WT == 2) {
         // waves wt = 1 leave their sums in LDS, waves wt = 0 join them with theirs
         xdl::lds_barrier();  // the tiles are no longer read
-        float *out = reinterpret_cast<float *>(mem) + wr * 64 * 66 + lane;
+        float *out = reinterpret_cast<float *>(mem) + wr * 64 * 67 + lane;
         if (wt == 1) {
 #pragma unroll
             for (int d = 0; d < 4; ++d)
@@ -562,6 +598,7 @@ void prefix_kernel(const Args a) {
                     out[64 * (16 * d + k)] = acc[d][k];
             out[64 * 64] = negm;
             out[64 * 65] = l;
+            out[64 * 66] = z;
         }
         xdl::lds_barrier();
         if (wt == 1)
@@ -572,6 +609,7 @@ void prefix_kernel(const Args a) {
         const float w0 = __builtin_amdgcn_exp2f(both - negm), w1 = __builtin_amdgcn_exp2f(both - negm1);
         negm = both;
         l = l * w0 + l1 * w1;
+        z = z * w0 + out[64 * 66] * w1;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -589,8 +627,8 @@ void prefix_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) {
             float4 *to = reinterpret_cast<float4 *>(o + 8 * (8 * q + 4 * h + i));
             const int k = 4 * q + i;
-            to[0] = float4{acc[0][k] * inv, acc[0][8 + k] * inv, acc[1][k] * inv, acc[1][8 + k] * inv};
-            to[1] = float4{acc[2][k] * inv, acc[2][8 + k] * inv, acc[3][k] * inv, acc[3][8 + k] * inv};
+            to[0] = float4{(acc[0][k] + z) * inv, (acc[0][8 + k] + z) * inv, (acc[1][k] + z) * inv, (acc[1][8 + k] + z) * inv};
+            to[1] = float4{(acc[2][k] + z) * inv, (acc[2][8 + k] + z) * inv, (acc[3][k] + z) * inv, (acc[3][8 + k] + z) * inv};
         }
     if (h == 0)
         part_lse(a.parts, a.total_rows, head_row, a.splits)[sp] = (__builtin_amdgcn_logf(l) - negm) * kLn2;

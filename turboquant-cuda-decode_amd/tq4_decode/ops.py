@@ -716,8 +716,8 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     sequence that has as many tokens: those are read and decoded once for all of them, the rest of each
     sequence as in ``full_decode``.  ``prefix_len`` is whole blocks (0: nothing shared); a sequence with
     ``seq_lens[b] < prefix_len`` attends to its own ``seq_lens[b]`` tokens alone (its entries behind those may
-    hold anything).  ``query`` and ``out`` are bf16 or fp16 (the shared tokens' products have f16 operands, in
-    pairs where one would show in the result).  ``workspace``: a ``PrefixWorkspace``.
+    hold anything).  ``query`` and ``out`` are bf16 or fp16: the shared tokens' scores are products of f16 pairs, their
+    weights are rounded to f16 for bf16 outputs and to f16 pairs for fp16 outputs.  ``workspace``: a ``PrefixWorkspace``.
     ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in ``window_decode``.  ``kernel``: "auto" shares the
     prefix where that is faster than every sequence's own step (by the shapes and ``prefix_len``: about two
     million tokens times kv-heads, summed over the batch), "shared" always.
