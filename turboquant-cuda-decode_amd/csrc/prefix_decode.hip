@@ -178,8 +178,7 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
     if (rc)
         return rc;
     // the sequences' own tokens; whole: the rows in the place of one part
-    const int own_blocks = std::max(1, max_blocks_per_seq - prefix_len / block_size);
-    const StepPlan step = step_plan(a, own_blocks, num_kv_splits > 1);
+    const StepPlan step = step_plan(a, tq4::xdl::own_blocks(max_blocks_per_seq, prefix_len / block_size), num_kv_splits > 1);
     const int slots = step.whole ? 1 : num_kv_splits;
     a.sinks = nullptr;  // (the join's)
     io.out = own;
