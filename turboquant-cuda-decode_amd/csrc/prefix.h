@@ -76,8 +76,7 @@ template <int WR, int WT, bool KF8> struct Shape {
 };
 
 // What the softmax takes of a tile's tokens: the score factor (not with FP8 keys), V's scale and V's value at the
-// middle code; and, from each wave that decodes K, whether one of its scales is above kLargeScale.
-constexpr float kLargeScale = 128.f;
+// middle code; and, from each wave that decodes K, whether one of its scales is above xdl::kLargeScale.
 template <bool V3> constexpr float kMiddle = V3 ? 4.f : 8.f;
 template <int TOKENS, int K_WAVES, bool KF8> struct alignas(16) Factors {
     float norm[KF8 ? 4 : TOKENS];
@@ -228,7 +227,7 @@ __device__ __forceinline__ void store_k(const RawK &r, unsigned char *khi, unsig
     const float scale = xdl::quad_bcast<KF8 ? 0 : 1>(own);
     if (j == (KF8 ? 1 : 2))
         factors.v[t] = float2{scale, fmaf(scale, kMiddle<V3>, own)};
-    const bool large = __any(fabsf(scale) > kLargeScale);
+    const bool large = __any(fabsf(scale) > xdl::kLargeScale);
     if ((u & 63) == 0)
         factors.large[wave] = large;
 }

@@ -50,6 +50,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kRescaleLogX = 8.0f;
+constexpr float kLargeScale = 128.f;  // V scales above it let no p pass 1 (2^8 times them would pass f16's range)
 constexpr int kRor4 = 0x124, kRor8 = 0x128, kRor12 = 0x12C;  // DPP row_ror:N
 
 // DPP row_ror:N -- lane r of a 16-lane row reads lane (r - N) mod 16.
@@ -943,9 +944,10 @@ __device__ __forceinline__ void softmax_tile(const float (&dot)[G / 4], const fl
             vzero[j] = valid[j] ? vzero[j] : 0.f;
         }
     }
+    // (p times a scale, an f16 operand, stays below 2^15: a token with a large scale lets no p pass 1)
 #pragma unroll
     for (int j = 0; j < TPL; ++j)
-        need |= s2[j] > kRescaleLogX;
+        need |= s2[j] > kRescaleLogX || fabsf(vscale[j]) > kLargeScale;
     if constexpr (SECOND)
         need |= st.pend != 1.f;
     if (__builtin_expect(__any(need), 0)) {
@@ -960,7 +962,12 @@ __device__ __forceinline__ void softmax_tile(const float (&dot)[G / 4], const fl
             mx = max_score(mx, sn[j]);
         }
         mx = head_max<G>(mx);
-        const float negm_new = (mx + st.negm > kRescaleLogX) ? -mx : st.negm;
+        float large = 0.f;
+#pragma unroll
+        for (int j = 0; j < TPL; ++j)
+            large = s2[j] > 0.f && fabsf(vscale[j]) > kLargeScale ? 1.f : large;
+        const bool moved = mx + st.negm > kRescaleLogX || head_max<G>(large) > 0.f;
+        const float negm_new = moved ? -mx : st.negm;
         // exp2(m_old - m_new): 1 for heads that keep their max, 0 after a split start
         const float alpha = __builtin_amdgcn_exp2f(negm_new - st.negm);
         st.l *= alpha;
