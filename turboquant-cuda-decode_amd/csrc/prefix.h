@@ -617,7 +617,8 @@ void prefix_kernel(const Args a) {
     }
     if (row >= a.rows)
         return;
-    const float inv = 1.f / l;
+    // (no weight at all where every score of the run is -inf: zeros that the join leaves out, as their lse is -inf)
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     // accumulator d, register 4 q + i: row 32 d + 8 q + 4 h + i of V^T, dim 8 (8 (q % 2) + 4 h + i) + 2 d + q / 2
     float *o = part_row(a.parts, head_row, a.splits, sp);
 #pragma unroll
