@@ -412,7 +412,7 @@ def _axis_of(sections, in_turn, half):
         raise RuntimeError("sections must name 2 to 4 axes")
     n = len(sections)
     if in_turn:
-        if any(n * s > half for s in sections[1:]):
+        if any(s > (half - x + n - 1) // n for x, s in enumerate(sections) if x):  # (frequencies j = x mod n)
             raise RuntimeError("sections in turn: an axis behind the first has at most its share of the frequencies")
         axes = [j % n if j % n and j < n * sections[j % n] else 0 for j in range(half)]
     else:
