@@ -474,8 +474,9 @@ def rope_store(query, key, value, positions, cos_sin, kv_cache, slot_mapping, ro
         q_stride, Hq = _token_rows(query, "query", key), query.size(1)
         if query_out is None:
             query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        elif query_out.data_ptr() != query.data_ptr() or not query.is_contiguous():
-            _require(not any(_overlap(query_out, t) for t in (query, key, value)),
+        else:  # (in place: keys or values in the queries' memory would be turned while they are read)
+            in_place = query_out.data_ptr() == query.data_ptr() and query.is_contiguous()
+            _require(not any(_overlap(query_out, t) for t in ((key, value) if in_place else (query, key, value))),
                      "query_out must be query itself or lie apart from the inputs")
         _require(query_out.dtype == query.dtype and query_out.shape == query.shape and query_out.is_contiguous(),
                  "query_out must match query (shape, dtype) and be contiguous")
