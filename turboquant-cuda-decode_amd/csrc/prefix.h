@@ -646,6 +646,9 @@ __global__ __launch_bounds__(kWave) void join_kernel(const float *__restrict__ s
                                                      const float *__restrict__ sinks, OutT *__restrict__ out,
                                                      float *__restrict__ lse, int num_q_heads) {
     constexpr int CHUNK = 16;
+    // Own rows asked for ahead: tails have few of the num_splits there are places for (16 ahead: 200 sequences of up to 100
+    // tokens behind 4096 82.5 us the whole call, 78.2 with four).
+    constexpr int kFewParts = 4;
     const int b = blockIdx.y, lane = threadIdx.x;
     const int64_t row = (int64_t)b * num_q_heads + blockIdx.x;
     const int64_t total_rows = (int64_t)gridDim.y * num_q_heads;
@@ -664,7 +667,7 @@ __global__ __launch_bounds__(kWave) void join_kernel(const float *__restrict__ s
     // the first rows of both go out before the length and the count arrive (all in bounds)
     Chunk ks, ko;
     load(ks, shared, n_shared, 0, min(CHUNK, n_shared));
-    load(ko, own, num_splits, 0, min(CHUNK, num_splits));
+    load(ko, own, num_splits, 0, min(kFewParts, num_splits));
     const uint32_t mark = __builtin_bit_cast(uint32_t, part_lse(const_cast<float *>(own), total_rows, row, num_splits)[num_splits - 1]);
     const int len = seq_lens[b];
     const bool has_shared = len >= prefix;
@@ -696,8 +699,8 @@ __global__ __launch_bounds__(kWave) void join_kernel(const float *__restrict__ s
                 load(ks, shared, n_shared, s0, n);
             add(ks, n);
         }
-    for (int s0 = 0; s0 < n_own; s0 += CHUNK) {
-        const int n = min(CHUNK, n_own - s0);
+    for (int s0 = 0, n; s0 < n_own; s0 += n) {
+        n = min(s0 == 0 ? kFewParts : CHUNK, n_own - s0);
         if (s0 > 0)
             load(ko, own, num_splits, s0, n);
         add(ko, n);

@@ -45,8 +45,9 @@ inline int floor_pow2(int64_t x, int most) {
 
 // Blocks of the longest sequence that a step behind a shared prefix may have to read: a sequence shorter than the
 // prefix keeps all its tokens in it.  (Planned for the tails alone, one of 29000 tokens among 64 tails of 100 behind 32768
-// was one workgroup's: 380 us the whole call, 144 now; four of 8000 behind 8192 134 / 70, half the batch of
-// 4000 93 / 78.  Tails alone, planned so: 64 of 1 to 1100 the same, 64 of 600 behind 32768 117.8 / 119.4, 200 of 100 78.9 / 82.1.)
+// was one workgroup's: 380 us the whole call, 142 now; four of 8000 behind 8192 134 / 69, half the batch of
+// 4000 93 / 77.  Tails alone, planned so: within 1 % (64 of 90 to 1100 67.2 / 67.9, 64 of 40 to 600 behind 32768 116.8 /
+// 117.8, 200 of 10 to 100 79.0 / 78.2).)
 inline int own_blocks(int max_blocks, int prefix_blocks) { return std::max(prefix_blocks, max_blocks - prefix_blocks); }
 
 // What the plan depends on.
