@@ -21,7 +21,7 @@
 // registers loaded one tile ahead, into one of two LDS tiles (WT = 1: the only one).
 //
 // What bounds it: the matrix cores at the rate that they keep up under load, and what runs beside them.
-// 64 sequences of 4 heads a kv-head, 8 kv-heads, 32768 shared tokens (AoS): 98 us.  A 64-token tile is 64
+// 64 sequences of 4 heads a kv-head, 8 kv-heads, 32768 shared tokens (AoS): 96 to 100 us.  A 64-token tile is 64
 // products per SIMD; on zeros one takes 16 ns (2.1 PFLOP/s), on random operands read from LDS with four fma
 // beside it 25 ns (1.3 PFLOP/s: the card slows down with the bits that change), so 1.6 us of the 2.5 per tile.
 // Leaving out K's decoding saves 24 us, K's scores 24, V's decoding 11, the loads 13: none of them hides

@@ -9,7 +9,7 @@ using namespace tq4::abi;
 namespace {
 
 // How the prefix is spread over the device: `wr` waves of 32 rows per workgroup (4 with two waves each, or
-// 2), row tiles of 32 wr rows, `splits` runs of tiles.
+// 2 up to 64 rows, which four would leave half empty), row tiles of 32 wr rows, `splits` runs of tiles.
 struct PrefixPlan {
     int wr, row_tiles, tiles, splits;
     int64_t in_turn;  // tiles that the busiest place works through
@@ -48,10 +48,11 @@ PrefixPlan prefix_plan(int rows, int Hk, int tokens) {
 // million (token, kv-head) pairs in 19 (waves of four query heads) or 23 (of eight), 3-bit keys in a fifth more, and
 // starts in 15; the shared way takes 30 for its four launches, 2.3 per tile in turn, and writes and reads a
 // part row of 516 bytes per query row and split.
-// Measured (32 / 8 heads, 4-bit keys, tails of 100): batch 8, prefix 2048 36.2 against 17.9 for the step alone,
-// 16 x 8192 49 : 36, 64 x 2048 48 : 35, 8 x 32768 63 : 53; 64 x 4096 52 : 54, 32 x 8192 52 : 54,
-// 16 x 32768 67 : 95, 64 x 8192 58 : 95.  16 / 2 heads 64 x 8192 52 : 41; 8 / 8 heads 64 x 4096 45 : 52,
-// 16 x 8192 38 : 34; 32 / 4 heads, 3-bit, 100 x 4000 56 : 60.
+// Measured (32 / 8 heads, 4-bit keys, tails of 100): batch 8, prefix 2048 36.8 against 17.8 for the step alone,
+// 16 x 8192 49 : 36, 64 x 2048 48 : 37, 8 x 32768 66 : 54; 64 x 4096 52 : 56, 32 x 8192 51 : 55,
+// 16 x 32768 69 : 94, 64 x 8192 59 : 94.  16 / 2 heads 64 x 8192 49 : 43; 8 / 8 heads 64 x 4096 45 : 56,
+// 16 x 8192 39 : 35; 32 / 32 heads 64 x 2048 60 : 97; 32 / 4 heads, 3-bit, 100 x 4000 56 : 58.
+// (40 / 8 heads, FP8 keys, 12 x 16384 46 : 49, where it takes the steps.)
 bool sharing_pays(const Stage1Args &a, const PrefixPlan &p, int prefix_len) {
     const double each = (xdl_heads(a) == 4 ? 19e-6 : 23e-6) * (a.key_bits == 3 ? 1.2 : 1.0);
     const double alone = 15 + each * a.B * (double)prefix_len * a.Hk * xdl_parts(a);

@@ -23,10 +23,11 @@
 // not rotated).  A query thread takes one unit of one row.
 //
 // What bounds it, and what it measured (32 / 8 heads, bf16, 4-bit keys).  32768 tokens: the queries' rows are
-// copied through in 99 us (537 MB, 5.4 TB/s: the card's copy rate), the writer takes 77-89 us for 170 MB: a
+// copied through in 99 to 104 us (537 MB, 5.4 TB/s: the card's copy rate), the writer takes 78 to 87 us for 170 MB: a
 // chain per tile (positions, then angles and keys, 96 matrix products, codes, V), four waves of a SIMD in turn,
-// 16 tiles per SIMD; without the fp64 rows 61, without the angles too 53.  4097 tokens on three axes 36 us.  64 tokens 14.5 us: one workgroup's chain, the rotation
-// matrix staged and split in LDS (8.6 us in the plain writer), positions and angles before it, and the fp64 rows of the
+// 16 tiles per SIMD; without the fp64 rows 61, without the angles too 53.  4097 tokens on three axes 36 us: one tile for all
+// but one of the 2048 waves, and at most two workgroups of either role on a CU, for the writer's LDS.  64 tokens
+// 14.5 us: one workgroup's chain, the rotation matrix staged and split in LDS (8.6 us in the plain writer), positions and angles before it, and the fp64 rows of the
 // slowest wave (4 us).  Registers bind the
 // large form (128 at four waves per SIMD): V asked for behind the products instead of ahead of the tile took
 // 34 spilled registers to 14, a unit's angles one unit at a time 50 to 12 (139 us to 104), one axis known to

@@ -8,8 +8,8 @@ using namespace tq4::abi;
 
 namespace {
 
-// Workgroups of `waves` waves for the query rows: enough that a wave takes one run of rows, at most as many
-// as two per CU hold.
+// Workgroups of `waves` waves for the query rows: enough that a wave takes one run of rows, at most 2048 (eight per
+// CU; behind the writer's in one launch they hold its LDS too, 67 KB, and two run on a CU at a time).
 int query_groups(const tq4::rope::Args &a, int waves) {
     if (!a.query)
         return 0;
