@@ -326,6 +326,34 @@ int tq4_prefix_decode(const void *query, int query_dtype, const float *rot_t, co
  * message) where they are invalid. */
 int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);
 
+/*
+ * Attention of several new tokens per sequence over the cache: chunks of prompts, drafted tokens.  Sequence b
+ * has the new tokens query_starts[b] .. query_starts[b + 1] - 1 of query [tokens, Hq, D] (query_starts [B + 1],
+ * not decreasing; rows of no sequence are not written) and seq_lens[b] tokens in the cache.  causal: its new tokens
+ * are the last of those, and each sees itself and what lies before it; with window > 0 only the last `window` of
+ * these (itself included) and the first `first_tokens`.  Not causal (window 0): every new token sees all seq_lens[b]
+ * tokens, as the context of a chunk whose own tokens are attended to elsewhere (tq4_merge_states joins the two).
+ * A new token that sees nothing gets zeros and LSE -inf.  What starts and lengths name outside of query and
+ * the table counts as not there; only the blocks of visible tokens are read.
+ * query: heads contiguous, tokens query_stride elements apart (whole 16-byte pieces); query and out are 16-bit
+ * (TQ4_BF16, TQ4_F16), out [tokens, Hq, D] contiguous and 16-byte aligned.  lse [tokens, Hq] fp32 may be NULL: with it, and
+ * for TQ4_F16 outputs, scores are products of f16 pairs and V's codes exact (weights times V's scale are rounded to f16);
+ * else key codes, rotated queries, values and weights are rounded to f16 each, and outputs to bf16.
+ * workspace: at least tq4_chunk_workspace_floats(...) floats, 16-byte aligned, contents after the call unspecified;
+ * two calls that may overlap need one each.  The grid depends on the shapes alone.  Cache, rot_t, centroids, sinks,
+ * key_bits / value_bits, block sizes and errors as in tq4_window_decode.
+ * No counterpart in the reference (its backend expands the cache for chunks).
+ */
+int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride, const float *rot_t,
+                        const float *centroids, const uint8_t *kv_cache, const int32_t *block_table,
+                        const int32_t *seq_lens, const int32_t *query_starts, float *workspace, int64_t workspace_floats,
+                        void *out, int out_dtype, float *lse, int tokens, int B, int Hq, int Hk, int D, int block_size,
+                        int max_blocks_per_seq, int64_t cache_block_stride, int layout, float attn_scale,
+                        const float *sinks, int key_bits, int value_bits, int causal, int window, int first_tokens,
+                        tq4_stream_t stream);
+/* Floats of workspace that tq4_chunk_attention needs for these shapes; -1 (and a message) where they are invalid. */
+int64_t tq4_chunk_workspace_floats(int tokens, int B, int Hq, int Hk);
+
 /* Message of the last failed call on this thread ("" when none).
  * Replaces: the TORCH_CHECK messages of cuda/tq4_cuda_v1.cu:468-499. */
 const char *tq4_last_error(void);

@@ -1,0 +1,951 @@
+// Attention of several new tokens per sequence over the paged quantised cache: chunks of prompts, drafted tokens.
+//
+// For a kv-head a sequence has M = new tokens * group query rows (new tokens first), so scores are a matrix product with
+// M rows.  As in the shared prefix (prefix.h) the rows stand in the columns:
+//
+//   S^T[token][row] = sum_d c[token][d] q[row][d]       v_mfma_f32_32x32x16_f16, A = the keys' codes, B = q
+//   O^T[dim][row]  += sum_t V^T[dim][t] P^T[t][row]     the same, A = V, B = the weights
+//
+// so a lane (c, h) = (lane % 32, lane / 32) has one row's scores (tokens 8 (i / 4) + 4 h + i % 4 of 32): the running
+// maximum and sum are its own values, and the weights' registers are the B operand as they stand.
+//
+// Three launches.  chunk_start_kernel turns the queries into the keys' basis and rounds them to the products' operands;
+// one workgroup of it cuts the work (chunk_plan.h).  chunk_kernel: a workgroup of WR * WT waves takes its stretch of
+// the list of row tiles of 32 WR rows; each wave has 32 rows and 1 / WT of the tokens of a tile of KT, which the
+// workgroup decodes once into LDS.  A row tile that one workgroup had whole is written as the result, the parts of one
+// that was cut go to the workspace, where chunk_merge_kernel joins them.
+//
+// Precision.  FINE (fp16 results, or a log-sum-exp): keys' codes and queries are f16 hi + lo, three products, V's codes
+// are exact and its scale is part of the weight, one f16.  Otherwise (bf16 results): codes, queries, V and weights
+// are one f16 each, a sixteenth of the result's own rounding.
+#pragma once
+#include "chunk_plan.h"
+#include "prefix.h"
+
+namespace tq4 {
+namespace chunk {
+
+using prefix::floatx16;
+using prefix::half2v;
+using xdl::half8;
+typedef uint32_t u32x2a8 __attribute__((ext_vector_type(2), aligned(8)));
+
+struct Args {
+    const void *query;       // [tokens, heads, 128] of q_dtype
+    const float *rot_t;      // null: FP8 keys
+    const float *centroids;
+    const uint8_t *cache;
+    const int32_t *pages;    // block table [batch, table_width]
+    const int32_t *seq_lens, *starts;
+    const float *sinks;
+    void *out;
+    float *lse;              // may be null
+    // workspace
+    _Float16 *q_hi, *q_lo;   // [tokens * heads, 128]
+    float *q_factor;         // [tokens * heads]
+    double *work;            // [batch + 1]
+    Cut *cuts;               // [groups + 1]
+    float *parts;            // [2 groups][rows][128], then [2 groups][rows] log-sum-exps in log2 units
+    int64_t block_stride, query_stride;
+    float score_scale_log2;
+    int q_dtype, out_dtype, num_q_heads, num_kv_heads;
+    int tokens, batch, table_width, groups;  // groups: workgroups of the grid
+    int block_size_log2, slot_pos, slot_head;
+    Shape shape;
+    int longest;             // table_width blocks
+};
+
+// ---- Queries and cuts ------------------------------------------------------------------------
+
+constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 16 * kStartWaves;
+// The least work that a workgroup is given, in token tiles.
+constexpr double kLeast = 4.0;
+constexpr int kSnap = 2;
+
+// One workgroup: the work before each sequence, and from it every workgroup's place in the list.
+__device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
+    const int tid = threadIdx.x, per = (a.batch + kStartThreads - 1) / kStartThreads;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    auto seq = [&](int b) { return seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest); };
+    double own = 0;
+    for (int b = b0; b < b1; ++b)
+        own += work_of(a.shape, seq(b));
+    sums[tid] = own;
+    __syncthreads();
+    for (int d = 1; d < kStartThreads; d <<= 1) {
+        const double before = tid >= d ? sums[tid - d] : 0.0;
+        __syncthreads();
+        sums[tid] += before;
+        __syncthreads();
+    }
+    double at = tid > 0 ? sums[tid - 1] : 0.0;
+    for (int b = b0; b < b1; ++b) {
+        a.work[b] = at;
+        at += work_of(a.shape, seq(b));
+    }
+    const double total = sums[kStartThreads - 1];
+    __syncthreads();
+    const int used = max(1, (int)fmin((double)a.groups, total / kLeast));
+    for (int w = tid; w <= a.groups; w += kStartThreads) {
+        Cut c{a.batch, 0, 0, 0};
+        if (w < used && total > 0) {
+            const double target = total * w / used;
+            int lo = 0, hi = a.batch - 1;  // the last sequence with as little before it
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (a.work[mid] <= target)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            Seq q = seq(lo);
+            c = Cut{lo, 0, 0, 0};
+            if (q.n > 0 && w > 0)
+                c = cut_in(a.shape, q, lo, target - a.work[lo], kSnap);
+            if (c.at == 0 && c.r == 0 && c.h == 0)
+                while (c.b < a.batch && seq(c.b).n == 0)
+                    ++c.b;
+        }
+        a.cuts[w] = c;
+    }
+}
+
+// Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two
+// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range are scaled down and q_factor
+// undoes it.  FP8 keys: the row itself, scaled by the power of two that puts its largest magnitude in [0.5, 1): exact.
+template <typename InT, bool KF8, bool LO>
+__global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
+    constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
+    __shared__ __align__(16) _Float16 pt_hi[PT], pt_lo[PT];
+    if (blockIdx.x == gridDim.x - 1) {
+        __shared__ double sums[kStartThreads];
+        plan_cuts(a, sums);
+        return;
+    }
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, n = lane & 15, g = lane >> 4;
+    const int64_t rows = (int64_t)a.tokens * a.num_q_heads, r0 = (int64_t)blockIdx.x * kStartRows + 16 * wave;
+    const int64_t ra = min(r0 + n, rows - 1);
+    const int64_t token = ra / a.num_q_heads;
+    const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (ra - token * a.num_q_heads) * kHeadDim;
+    typedef InT in8 __attribute__((ext_vector_type(8)));
+    in8 qv[4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+        qv[kb] = *reinterpret_cast<const in8 *>(from + 32 * kb + 8 * g);
+    float amax = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            amax = fmaxf(amax, fabsf(to_float<InT>(qv[kb][j])));
+    amax = rot_row_max(amax);
+    const bool finite = amax > 0.f && amax < __builtin_inff();
+    if constexpr (KF8) {
+        const int e = finite ? -__builtin_amdgcn_frexp_expf(amax) : 0;
+        if (r0 + n >= rows)
+            return;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            half8 y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
+            *reinterpret_cast<half8 *>(a.q_hi + ra * kHeadDim + 32 * kb + 8 * g) = y;
+        }
+        if (g == 0)
+            a.q_factor[ra] = __builtin_ldexpf(a.score_scale_log2, -e);
+        return;
+    } else {
+        constexpr int kIters = kHeadDim * (kHeadDim / 8) / kStartThreads;
+#pragma unroll
+        for (int it = 0; it < kIters; ++it) {
+            const int i = threadIdx.x + it * kStartThreads, c = i % kHeadDim, kg = i / kHeadDim;
+            half8 h, l;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float w = a.rot_t[(8 * kg + j) * kHeadDim + c];
+                h[j] = (_Float16)w;
+                l[j] = (_Float16)(w - (float)h[j]);
+            }
+            *reinterpret_cast<half8 *>(pt_hi + c * kRotPt + 8 * kg) = h;
+            *reinterpret_cast<half8 *>(pt_lo + c * kRotPt + 8 * kg) = l;
+        }
+        __syncthreads();
+        if (r0 >= rows)
+            return;
+        const int e = finite ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
+        half8 q[4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                q[kb][j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
+        // D: lane (n, g) has dims 16 cb + 4 g .. +3 of row n
+        floatx4 y[8];
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) {
+            y[cb] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                const int off = (16 * cb + n) * kRotPt + 32 * kb + 8 * g;
+                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_hi + off), q[kb], y[cb]);
+                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + off), q[kb], y[cb]);
+            }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                y[cb][i] = __builtin_ldexpf(y[cb][i], -e) * a.score_scale_log2;
+                top = fmaxf(top, fabsf(y[cb][i]));
+            }
+        top = rot_row_max(top);
+        const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        if (r0 + n >= rows)
+            return;
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) {
+            half4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = __builtin_ldexpf(y[cb][i], f);
+                asm("" : "+v"(v));  // (rounded once: hi and lo belong together)
+                hi[i] = (_Float16)v;
+                lo[i] = (_Float16)(v - (float)hi[i]);
+            }
+            *reinterpret_cast<half4 *>(a.q_hi + ra * kHeadDim + 16 * cb + 4 * g) = hi;
+            if constexpr (LO)
+                *reinterpret_cast<half4 *>(a.q_lo + ra * kHeadDim + 16 * cb + 4 * g) = lo;
+        }
+        if (g == 0)
+            a.q_factor[ra] = __builtin_ldexpf(1.f, -f);
+    }
+}
+
+// ---- Token tiles -----------------------------------------------------------------------------
+
+// LDS tiles as prefix.h's: K (hi, and lo) in rows of a token, V^T in rows of a dim.
+constexpr int kKRow = prefix::kKRow;
+template <int WR, int WT, int KT, int BUFS, bool KF8, bool FINE> struct Lds {
+    static constexpr int threads = 64 * WR * WT;
+    static constexpr int vrow = 2 * KT + 16;
+    static constexpr int klo = KT * kKRow;  // bytes: K hi at 0, K lo, V^T
+    static constexpr int v = klo * (!KF8 && FINE ? 2 : 1);
+    static constexpr int tile = v + kHeadDim * vrow;
+    static constexpr int join = (WT - 1) * WR * 64 * 67 * 4;
+    static constexpr int bytes = BUFS * tile > join ? BUFS * tile : join;
+    static constexpr bool halves = threads == 8 * KT;  // threads decode K or V, else both
+    static constexpr int units = halves ? 1 : 4 * KT / threads;  // of either that a thread decodes
+    static constexpr int v_waves = halves ? WR * WT / 2 : WR * WT;
+    static constexpr int sub = KT / (32 * WT);         // products of 32 tokens per wave and tile
+    static_assert(halves || (4 * KT) % threads == 0, "whole units");
+};
+// What the softmax takes of a tile's tokens.  v: V's scale and its value at the middle code (FINE); special: per wave
+// that decodes V, whether a token's `fix` is not 1: the weight's factor where V is stored smaller, NaN where V is not finite.
+template <int KT, int V_WAVES, bool KF8, bool FINE> struct alignas(16) Factors {
+    float norm[KF8 ? 4 : KT];
+    float2 v[FINE ? KT : 1];
+    float fix[KT];
+    uint32_t special[V_WAVES];
+};
+template <bool V3> constexpr float kMiddle = prefix::kMiddle<V3>;
+constexpr float kShrink = 1.f / 32.f;   // 15 codes of the largest f16 scale and the largest zero are below 2^20
+constexpr float kMostV = 60000.f;
+
+struct Raw {
+    uint4 a, b;
+};
+// Unit u of K: token u / 4, dims 32 (u % 4) .. +31; b: the norm (FP8 keys: the second half of the bytes).
+template <int LAYOUT, bool KF8, bool KB3, bool V3>
+__device__ __forceinline__ void load_k(Raw &r, const prefix::Args &a, int kvh, int t, int blk, int u) {
+    using R = prefix::Record<LAYOUT, KF8, KB3, V3>;
+    const R at(a, kvh, t, blk);
+    const uint8_t *p = at.data + (u & 3) * (R::kbytes / 4);
+    if constexpr (KB3) {
+        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(p);
+        r.a = uint4{w[0], w[1], w[2], 0u};
+    } else {
+        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(p);
+        r.a = uint4{w[0], w[1], w[2], w[3]};
+    }
+    if constexpr (KF8) {
+        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(p + 16);
+        r.b = uint4{w[0], w[1], w[2], w[3]};
+    } else {
+        r.b.x = LAYOUT == 0 ? at.meta[0] : *reinterpret_cast<const uint16_t *>(at.data + R::kbytes);
+    }
+}
+// Unit u of V: tokens t = 4 (u / 16) .. +3 (one block), dims 8 (u % 16) .. +7; b: their scales and zeros.
+template <int LAYOUT, bool KF8, bool KB3, bool V3>
+__device__ __forceinline__ void load_v(Raw &r, const prefix::Args &a, int kvh, int t, int blk, int u) {
+    using R = prefix::Record<LAYOUT, KF8, KB3, V3>;
+    const R at(a, kvh, t, blk);
+    const uint8_t *p = at.data + R::v0 + (V3 ? 3 : 4) * (u & 15);
+    auto token = [&](int i) { return *reinterpret_cast<const prefix::u32a1 *>(p + (int64_t)i * at.pos); };
+    r.a = uint4{token(0), token(1), token(2), token(3)};
+    if constexpr (LAYOUT == 0) {
+        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(at.meta + (R::nf - 2) * at.bs);
+        const u32x2a8 z = *reinterpret_cast<const u32x2a8 *>(at.meta + (R::nf - 1) * at.bs);
+        r.b = uint4{s[0], s[1], z[0], z[1]};
+    } else {
+        auto both = [&](int i) {
+            return *reinterpret_cast<const prefix::u32a2 *>(at.data + (int64_t)i * at.pos + R::v0 + R::vbytes);
+        };
+        r.b = uint4{both(0), both(1), both(2), both(3)};
+    }
+}
+
+template <int LAYOUT, bool KF8, bool KB3, bool FINE, class L, class F>
+__device__ __forceinline__ void store_k(const Raw &r, unsigned char *khi, unsigned char *klo, F &factors, const uint2 *lut2,
+                                        const uint32_t *lut, int u) {
+    const int t = u >> 2, j = u & 3, at = t * kKRow + 64 * j;
+    uint32_t e[16], lo[16];
+    if constexpr (KF8) {
+        const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
+            const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+            e[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));  // (exact)
+            e[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
+        }
+    } else {
+        const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+        float sq = 0.f;
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+            uint32_t v;
+            if constexpr (KB3) {
+                const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
+                v = w[wi] >> sh;
+                if (sh > 26)
+                    v |= w[wi + 1] << (32 - sh);
+                v &= 63u;
+            } else {
+                v = (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
+            }
+            if constexpr (FINE || LAYOUT == 1) {
+                const uint2 c = lut2[v];
+                e[b] = c.x;
+                lo[b] = c.y;
+            } else {
+                e[b] = lut[v];
+            }
+        }
+        float n = half_bits_to_float(r.b.x);
+        if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction (h.h + 2 h.l)
+            float hl = 0.f;
+#pragma unroll
+            for (int b = 0; b < 16; ++b) {
+                const auto h = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), e[b]);
+                const auto l = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), lo[b]);
+                sq = __builtin_amdgcn_fdot2(h, h, sq, false);
+                hl = __builtin_amdgcn_fdot2(h, l, hl, false);
+            }
+            sq = fmaf(2.f, hl, sq);
+            sq += xdl::dppf<0xB1>(sq);  // quad_perm [1, 0, 3, 2]: the token's four threads
+            sq += xdl::dppf<0x4E>(sq);  // quad_perm [2, 3, 0, 1]
+            n *= __builtin_amdgcn_rsqf(sq + 1e-16f);
+        }
+        if (j == 0)
+            factors.norm[t] = n;
+        if constexpr (FINE)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4 *>(klo + at + 16 * q) = uint4{lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]};
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4 *>(khi + at + 16 * q) = uint4{e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
+}
+
+// Returns whether a token's `fix` is not 1.  `valid`: tokens of the unit that the sequence has (4, or fewer at its end:
+// the others' bytes may hold anything, and count as zeros).
+template <int LAYOUT, bool V3, bool FINE, int VROW, class F>
+__device__ __forceinline__ bool store_v(const Raw &r, unsigned char *vtile, F &factors, int u, int valid) {
+    const int dg = u & 15, quad = u >> 4;
+    const uint32_t v[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    // (scale | zero << 16) of each token
+    uint32_t sz[4];
+    if constexpr (LAYOUT == 0) {
+        sz[0] = __builtin_amdgcn_perm(r.b.z, r.b.x, 0x05040100u);
+        sz[1] = __builtin_amdgcn_perm(r.b.z, r.b.x, 0x07060302u);
+        sz[2] = __builtin_amdgcn_perm(r.b.w, r.b.y, 0x05040100u);
+        sz[3] = __builtin_amdgcn_perm(r.b.w, r.b.y, 0x07060302u);
+    } else {
+        sz[0] = r.b.x;
+        sz[1] = r.b.y;
+        sz[2] = r.b.z;
+        sz[3] = r.b.w;
+    }
+    float scale[4], zero[4], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sz[i] = i < valid ? sz[i] : 0u;
+        scale[i] = half_bits_to_float(sz[i]);
+        zero[i] = half_bits_to_float(sz[i] >> 16);
+        // (a NaN is passed over by no comparison below: !(x <= most))
+        const float top = fmaf(15.f, fabsf(scale[i]), fabsf(zero[i]));
+        most = top <= most ? most : top;
+    }
+    const bool special = !(most <= (FINE ? 128.f * 15.f : kMostV));
+    float fix[4] = {1.f, 1.f, 1.f, 1.f};
+    if (special)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float top = fmaf(15.f, fabsf(scale[i]), fabsf(zero[i]));
+            if (!(top < __builtin_inff())) {
+                fix[i] = __builtin_nanf("");
+                scale[i] = zero[i] = 0.f;
+            } else if (!FINE && top > kMostV) {
+                fix[i] = 1.f / kShrink;
+                scale[i] *= kShrink;
+                zero[i] *= kShrink;
+            }
+        }
+    const int t0 = 4 * quad;
+    if (dg == 0) {
+        *reinterpret_cast<float4 *>(factors.fix + t0) = float4{fix[0], fix[1], fix[2], fix[3]};
+        if constexpr (FINE)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                factors.v[t0 + i] = float2{scale[i], fmaf(scale[i], kMiddle<V3>, zero[i])};
+    }
+    // codes to f16: into the significand of 1024, then less 1024 (FINE: less 1024 and the middle code)
+    const half2v k0 = prefix::splat((_Float16)(1024.f + (FINE ? kMiddle<V3> : 0.f)));
+    half2v s01, s23, z01, z23;
+    if constexpr (!FINE) {
+        s01 = half2v{(_Float16)scale[0], (_Float16)scale[1]};
+        s23 = half2v{(_Float16)scale[2], (_Float16)scale[3]};
+        z01 = half2v{(_Float16)zero[0], (_Float16)zero[1]};
+        z23 = half2v{(_Float16)zero[2], (_Float16)zero[3]};
+    }
+    unsigned char *to = vtile + dg * VROW + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1);
+    auto put = [&](int i, uint32_t c01, uint32_t c23) {
+        half2v x = prefix::as_half2(c01 | 0x64006400u) - k0, y = prefix::as_half2(c23 | 0x64006400u) - k0;
+        if constexpr (!FINE) {
+            x = __builtin_elementwise_fma(x, s01, z01);
+            y = __builtin_elementwise_fma(y, s23, z23);
+        }
+        *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{prefix::as_u32(x), prefix::as_u32(y)};
+    };
+    if constexpr (V3) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            auto code = [&](int t) { return (v[t] >> (3 * i)) & 7u; };
+            put(i, code(0) | (code(1) << 16), code(2) | (code(3) << 16));
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const uint32_t sel = (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u;
+            const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel), p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
+            put(2 * m, p01 & 0x000F000Fu, p23 & 0x000F000Fu);
+            put(2 * m + 1, (p01 >> 4) & 0x000F000Fu, (p23 >> 4) & 0x000F000Fu);
+        }
+    }
+    return special;
+}
+
+// ---- The product -----------------------------------------------------------------------------
+
+__device__ __forceinline__ float *part_rows(const Args &a, int slot) { return a.parts + (int64_t)slot * a.shape.rows * kHeadDim; }
+__device__ __forceinline__ float *part_sums(const Args &a, int slot) {
+    return a.parts + (int64_t)2 * a.groups * a.shape.rows * kHeadDim + (int64_t)slot * a.shape.rows;
+}
+template <typename T> __device__ __forceinline__ void put8(void *out, int64_t at, const float (&v)[8]) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = (T)v[i];
+    *reinterpret_cast<t8 *>(static_cast<T *>(out) + at) = x;
+}
+
+template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR, int WT, int KT, int BUFS, bool FINE>
+__global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void chunk_kernel(const Args a) {
+    using S = Lds<WR, WT, KT, BUFS, KF8, FINE>;
+    using F = Factors<KT, S::v_waves, KF8, FINE>;
+    constexpr bool LUT2 = !KF8 && (FINE || LAYOUT == 1);
+    constexpr int kEntries = KB3 ? 64 : 256;
+    __shared__ __align__(16) unsigned char mem[S::bytes];
+    __shared__ __align__(16) F factors[BUFS];
+    __shared__ __align__(16) uint2 lut2[LUT2 ? kEntries : 1];
+    __shared__ __align__(16) uint32_t lut[KF8 || LUT2 ? 4 : kEntries];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, h = lane >> 5, wr = w % WR, wt = w / WR;
+    // neighbours in the list read the same tokens: eight runs of it, one per XCD (workgroup i runs on XCD i % 8)
+    const int per = gridDim.x >> 3, group_id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (group_id >= a.groups)
+        return;
+    Cut at = a.cuts[group_id];
+    const Cut end = a.cuts[group_id + 1];
+    if (at.b >= a.batch || (same_tile(at, end) && at.at == end.at))
+        return;
+    if constexpr (!KF8)
+        for (int e = tid; e < kEntries; e += S::threads) {
+            const uint32_t x = xdl::split_f16(a.centroids[KB3 ? e & 7 : e & 15]), z = xdl::split_f16(a.centroids[KB3 ? e >> 3 : e >> 4]);
+            if constexpr (LUT2)
+                lut2[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
+            else {
+                const half2v both{(_Float16)a.centroids[KB3 ? e & 7 : e & 15], (_Float16)a.centroids[KB3 ? e >> 3 : e >> 4]};
+                lut[e] = prefix::as_u32(both);
+            }
+        }
+    prefix::Args rec{};  // what the records' addresses need
+    rec.cache = a.cache;
+    rec.block_stride = a.block_stride;
+    rec.num_kv_heads = a.num_kv_heads;
+    rec.block_size_log2 = a.block_size_log2;
+    rec.slot_pos = a.slot_pos;
+    rec.slot_head = a.slot_head;
+
+    const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
+    const int group = a.shape.group;
+    xdl::lds_barrier();  // the table
+    while (at.b < a.batch) {
+        const Seq seq = seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest);
+        const int rows = seq.n * group, kvh = at.h;
+        const Visits vis = visits_of(a.shape, seq, at.r);
+        const bool last = same_tile(at, end);
+        const int tile0 = at.at, tile1 = last ? end.at : vis.count;
+        if (last && tile0 >= tile1)
+            break;
+        const int n_tiles = tile1 - tile0;
+        const int32_t *pages = a.pages + (int64_t)at.b * a.table_width;
+
+        auto unit = [&](int k) {
+            int u = S::halves ? tid & (4 * KT - 1) : tid + k * S::threads;
+            asm volatile("" : "+v"(u));
+            return u;
+        };
+        auto first_of = [&](int i) {  // the first token of tile i of this stretch (past its end: of the last one)
+            const int p = tile0 + min(i, n_tiles - 1);
+            return KT * (p < vis.head ? p : p + vis.skip);
+        };
+        auto k_tok = [&](int t0, int u) { return min(t0 + (u >> 2), seq.len - 1); };
+        auto v_tok = [&](int t0, int u) { return min(t0 + 4 * (u >> 4), (seq.len - 1) & ~3); };
+        constexpr int U = S::units;
+        int kblk[U], vblk[U];
+        Raw rk[U], rv_own[U];
+        Raw(&rv)[U] = S::halves ? rk : rv_own;
+        int(&vb)[U] = S::halves ? kblk : vblk;
+        auto read_pages = [&](int i) {
+            const int t0 = first_of(i);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int u = unit(k);
+                if (does_k)
+                    kblk[k] = pages[k_tok(t0, u) >> a.block_size_log2];
+                if (does_v)
+                    vb[k] = pages[v_tok(t0, u) >> a.block_size_log2];
+            }
+        };
+        auto load = [&](int i) {
+            const int t0 = first_of(i);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int u = unit(k);
+                if (does_k)
+                    load_k<LAYOUT, KF8, KB3, V3>(rk[k], rec, kvh, k_tok(t0, u), kblk[k], u);
+                if (does_v)
+                    load_v<LAYOUT, KF8, KB3, V3>(rv[k], rec, kvh, v_tok(t0, u), vb[k], u);
+            }
+        };
+        auto store = [&](int i) {
+            const int t0 = first_of(i);
+            unsigned char *m = mem + (i % BUFS) * S::tile;
+            F &f = factors[i % BUFS];
+            bool special = false;
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int u = unit(k);
+                if (does_k)
+                    store_k<LAYOUT, KF8, KB3, FINE, S>(rk[k], m, m + S::klo, f, lut2, lut, u);
+                if (does_v)
+                    special |= store_v<LAYOUT, V3, FINE, S::vrow>(rv[k], m + S::v, f, u, seq.len - (t0 + 4 * (u >> 4)));
+            }
+            if (does_v) {
+                const bool any = __any(special);
+                if (lane == 0)
+                    f.special[S::halves ? w - WR * WT / 2 : w] = any;
+            }
+        };
+        if (n_tiles > 0) {
+            read_pages(0);
+            load(0);
+            read_pages(1);
+        }
+
+        // this lane's row and its query
+        const int wave_row = at.r * a.shape.rows + 32 * wr, row = wave_row + c, row_in = min(row, rows - 1);
+        const int token = row_in / group, head = kvh * group + (row_in - token * group);
+        const int64_t q_row = (int64_t)(seq.row0 + token) * a.num_q_heads + head;
+        half8 q_hi[8], q_lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            q_hi[k] = *reinterpret_cast<const half8 *>(a.q_hi + q_row * kHeadDim + 16 * k + 8 * h);
+            if constexpr (FINE && !KF8)
+                q_lo[k] = *reinterpret_cast<const half8 *>(a.q_lo + q_row * kHeadDim + 16 * k + 8 * h);
+        }
+        const float fac = a.q_factor[q_row];
+        const bool scaled = KF8 || __any(fac != 1.f);
+        const int limit = limit_of(a.shape, seq, row_in), from = a.shape.window ? limit - a.shape.window : 0;
+        const int limit_lo = __builtin_amdgcn_readfirstlane(limit_of(a.shape, seq, min(wave_row, rows - 1)));
+        const int limit_hi = __builtin_amdgcn_readfirstlane(limit_of(a.shape, seq, min(wave_row + 31, rows - 1)));
+
+        floatx16 acc[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                acc[d][k] = 0.f;
+        float negm = __FLT_MAX__, l = 0.f, z = 0.f;  // -max in log2 units, this lane's shares of the sum and of V's middle values
+
+        auto tile = [&](int i) {
+            const unsigned char *m = mem + (i % BUFS) * S::tile;
+            const F &f = factors[i % BUFS];
+            const int t0 = first_of(i) + 32 * S::sub * wt;  // this wave's first token
+            // no row of the wave sees a token of it
+            if (t0 >= limit_hi || (a.shape.window && t0 >= a.shape.first && t0 + 32 * S::sub <= limit_lo - a.shape.window))
+                return;
+            floatx16 s[S::sub];
+#pragma unroll
+            for (int b = 0; b < S::sub; ++b) {
+                const unsigned char *k_from = m + (32 * (S::sub * wt + b) + c) * kKRow + 16 * h;
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    s[b][k] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const half8 hi = *reinterpret_cast<const half8 *>(k_from + 32 * k);
+                    s[b] = prefix::mfma32(hi, q_hi[k], s[b]);
+                    if constexpr (FINE && !KF8) {
+                        s[b] = prefix::mfma32(*reinterpret_cast<const half8 *>(k_from + S::klo + 32 * k), q_hi[k], s[b]);
+                        s[b] = prefix::mfma32(hi, q_lo[k], s[b]);
+                    }
+                }
+            }
+            uint32_t special = 0;
+#pragma unroll
+            for (int k = 0; k < S::v_waves; ++k)
+                special |= f.special[k];
+            special = __builtin_amdgcn_readfirstlane(special);
+            const int tok0 = 32 * S::sub * wt + 4 * h;  // s[b][k]: token tok0 + 32 b + 8 (k / 4) + k % 4 of the tile
+            const bool masked = t0 + 32 * S::sub > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
+            float n[S::sub][16];
+#pragma unroll
+            for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (KF8) {
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4)
+                            n[b][4 * k + i4] = fac;
+                    } else {
+                        const float4 v = *reinterpret_cast<const float4 *>(f.norm + tok0 + 32 * b + 8 * k);
+                        n[b][4 * k] = v.x;
+                        n[b][4 * k + 1] = v.y;
+                        n[b][4 * k + 2] = v.z;
+                        n[b][4 * k + 3] = v.w;
+                    }
+                }
+            if (!KF8 && scaled)
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        n[b][k] *= fac;
+            if (masked) {
+                const int first = first_of(i) + tok0;
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int t = first + 32 * b + 8 * (k >> 2) + (k & 3);
+                        if (t >= limit || (t < from && t >= a.shape.first)) {
+                            s[b][k] = -INFINITY;
+                            n[b][k] = 1.f;
+                        }
+                    }
+            }
+            // The scores less the running maximum, in log2 units; the maximum moves only when one passes it by more than
+            // kRescaleLogX (weights stay below 2^8).
+            float x[S::sub][16], mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    x[b][k] = fmaf(s[b][k], n[b][k], negm);
+                    x[b][k + 1] = fmaf(s[b][k + 1], n[b][k + 1], negm);
+                    mx = prefix::max3(mx, x[b][k], x[b][k + 1]);
+                }
+            const float most = FINE && special ? 0.f : xdl::kRescaleLogX;
+            if (__any(mx > most)) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        x[b][k] = s[b][k] * n[b][k];
+                        x[b][k + 1] = s[b][k + 1] * n[b][k + 1];
+                        top = prefix::max3(top, x[b][k], x[b][k + 1]);
+                    }
+                top = prefix::pair_max(top);
+                const float negm_new = top + negm > most ? -top : negm;
+                const float alpha = __builtin_amdgcn_exp2f(negm_new - negm);
+                negm = negm_new;
+                l *= alpha;
+                z *= alpha;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    acc[d] *= alpha;
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        x[b][k] += negm;
+            }
+            half8 p[S::sub][2];
+            if (special) {
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int t = tok0 + 32 * b + 8 * (k >> 2) + (k & 3);
+                        const float e = __builtin_amdgcn_exp2f(x[b][k]);
+                        l += e;
+                        // (a hidden token's V is nothing, whatever it holds)
+                        const float fix = x[b][k] == -INFINITY ? 0.f : f.fix[t];
+                        float y = e * fix;
+                        if constexpr (FINE) {
+                            const float2 v = f.v[t];
+                            z = fmaf(y, v.y, z);
+                            y *= v.x;
+                        }
+                        p[b][k >> 3][k & 7] = (_Float16)y;
+                    }
+            } else {
+#pragma unroll
+                for (int b = 0; b < S::sub; ++b) {
+                    if constexpr (FINE) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            const float4 v = *reinterpret_cast<const float4 *>(f.v + tok0 + 32 * b + 8 * (k >> 2) + (k & 3));
+                            const float e0 = __builtin_amdgcn_exp2f(x[b][k]), e1 = __builtin_amdgcn_exp2f(x[b][k + 1]);
+                            l += e0;
+                            l += e1;
+                            z = fmaf(e0, v.y, z);
+                            z = fmaf(e1, v.w, z);
+                            p[b][k >> 3][k & 7] = (_Float16)(e0 * v.x);
+                            p[b][k >> 3][(k & 7) + 1] = (_Float16)(e1 * v.z);
+                        }
+                    } else {
+                        // (the sum is of the rounded weights, so that their roundings' common part cancels)
+                        typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
+                        uint32_t pk[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const fp16x2 two = __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_exp2f(x[b][2 * k]),
+                                                                          __builtin_amdgcn_exp2f(x[b][2 * k + 1]));
+                            l = __builtin_amdgcn_fdot2(two, fp16x2{(__fp16)1.f, (__fp16)1.f}, l, false);
+                            pk[k] = __builtin_bit_cast(uint32_t, two);
+                        }
+                        p[b][0] = xdl::as_half8(pk[0], pk[1], pk[2], pk[3]);
+                        p[b][1] = xdl::as_half8(pk[4], pk[5], pk[6], pk[7]);
+                    }
+                }
+            }
+            const unsigned char *v_from = m + S::v + c * S::vrow + 16 * (4 * S::sub * wt + h);
+#pragma unroll
+            for (int b = 0; b < S::sub; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        acc[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(v_from + 32 * d * S::vrow + 32 * (2 * b + t)),
+                                                p[b][t], acc[d]);
+        };
+
+        if constexpr (BUFS == 2) {
+            if (n_tiles > 0) {
+                store(0);
+                load(1);
+                read_pages(2);
+            }
+            xdl::lds_barrier();
+            for (int i = 0; i < n_tiles; ++i) {
+                if (i + 1 < n_tiles) {
+                    store(i + 1);
+                    load(i + 2);
+                    read_pages(i + 3);
+                }
+                tile(i);
+                xdl::lds_barrier();
+            }
+        } else {
+            for (int i = 0; i < n_tiles; ++i) {
+                store(i);
+                load(i + 1);
+                read_pages(i + 2);
+                xdl::lds_barrier();
+                tile(i);
+                xdl::lds_barrier();
+            }
+        }
+
+        l = prefix::pair_sum(l);
+        z = prefix::pair_sum(z);
+        if constexpr (WT > 1) {
+            // waves wt > 0 leave their sums in LDS, waves wt = 0 join them with theirs
+            constexpr int kWords = 64 * 67;
+            float *mine = reinterpret_cast<float *>(mem) + lane;
+            if (wt > 0) {
+                float *to = mine + ((wt - 1) * WR + wr) * kWords;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        to[64 * (16 * d + k)] = acc[d][k];
+                to[64 * 64] = negm;
+                to[64 * 65] = l;
+                to[64 * 66] = z;
+            }
+            xdl::lds_barrier();
+            if (wt == 0)
+                for (int o = 0; o < WT - 1; ++o) {
+                    const float *of = mine + (o * WR + wr) * kWords;
+                    const float negm1 = of[64 * 64], both = fminf(negm, negm1);
+                    const float w0 = __builtin_amdgcn_exp2f(both - negm), w1 = __builtin_amdgcn_exp2f(both - negm1);
+                    negm = both;
+                    l = l * w0 + of[64 * 65] * w1;
+                    z = z * w0 + of[64 * 66] * w1;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            acc[d][k] = acc[d][k] * w0 + of[64 * (16 * d + k)] * w1;
+                }
+        }
+        const bool whole = tile0 == 0 && tile1 == vis.count;
+        if (wt == 0 && row < rows) {
+            if (whole && a.sinks) {
+                const float sink = a.sinks[head] * kLog2e, negm_new = fminf(negm, -sink);
+                const float w0 = __builtin_amdgcn_exp2f(negm_new - negm);
+                negm = negm_new;
+                l = l * w0 + __builtin_amdgcn_exp2f(sink + negm);
+                z *= w0;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    acc[d] *= w0;
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int slot = 2 * group_id + (tile0 == 0 ? 1 : 0), place = 32 * wr + c;
+            float *part = part_rows(a, slot) + (int64_t)place * kHeadDim;
+            const int64_t o = q_row * kHeadDim;
+            // accumulator d, register 4 q + i: row 32 d + 8 q + 4 h + i of V^T, dim 8 (8 (q % 2) + 4 h + i) + 2 d + q / 2
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 4 * q + i, dim = 8 * (8 * q + 4 * h + i);
+                    const float v[8] = {(acc[0][k] + z) * inv, (acc[0][8 + k] + z) * inv, (acc[1][k] + z) * inv, (acc[1][8 + k] + z) * inv,
+                                        (acc[2][k] + z) * inv, (acc[2][8 + k] + z) * inv, (acc[3][k] + z) * inv, (acc[3][8 + k] + z) * inv};
+                    if (!whole) {
+                        *reinterpret_cast<float4 *>(part + dim) = float4{v[0], v[1], v[2], v[3]};
+                        *reinterpret_cast<float4 *>(part + dim + 4) = float4{v[4], v[5], v[6], v[7]};
+                    } else if (a.out_dtype == kOutBf16) {
+                        put8<__bf16>(a.out, o + dim, v);
+                    } else {
+                        put8<_Float16>(a.out, o + dim, v);
+                    }
+                }
+            const float lse2 = __builtin_amdgcn_logf(l) - negm;
+            if (h == 0 && !whole)
+                part_sums(a, slot)[place] = lse2;
+            else if (h == 0 && a.lse)
+                a.lse[q_row] = l == 0.f ? -INFINITY : lse2 * kLn2;
+        }
+        if (last)
+            break;
+        if constexpr (WT > 1)
+            xdl::lds_barrier();  // the sums are read
+        // the next row tile
+        at.at = 0;
+        if (++at.r == row_tiles(a.shape, seq.n)) {
+            at.r = 0;
+            if (++at.h == a.num_kv_heads) {
+                at.h = 0;
+                do
+                    ++at.b;
+                while (at.b < a.batch && seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest).n == 0);
+            }
+        }
+    }
+}
+
+// Joins the parts of a row tile that was cut: workgroup (w, i) the rows 4 i .. +3 of the one that workgroup w of
+// chunk_kernel began and did not end, a row per wave.  Lane: dims 2 lane, 2 lane + 1.
+constexpr int kMergeRows = 4;
+template <typename OutT> __global__ __launch_bounds__(kWave *kMergeRows) void chunk_merge_kernel(const Args a) {
+    const int w = blockIdx.x, lane = threadIdx.x & 63;
+    const Cut from = a.cuts[w], cut = a.cuts[w + 1];
+    if (cut.b >= a.batch || cut.at == 0 || (same_tile(from, cut) && from.at > 0))
+        return;
+    const Seq seq = seq_of(a.starts, a.seq_lens, cut.b, a.tokens, a.longest);
+    const int place = blockIdx.y * kMergeRows + (threadIdx.x >> 6), row = cut.r * a.shape.rows + place;
+    if (row >= seq.n * a.shape.group)
+        return;
+    int parts = 1;  // part i: of workgroup w + i
+    while (same_tile(a.cuts[w + parts], cut))
+        ++parts;
+    // (workgroup w + parts - 1 has the end: the first whose own stretch ends in another row tile)
+    float mx = -INFINITY, a0 = 0.f, a1 = 0.f, sum = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += kWave) {
+        const int i = i0 + lane;
+        auto slot = [&](int j) { return 2 * (w + j) + (j == 0 ? 1 : 0); };
+        float s = -INFINITY;
+        if (i < parts) {
+            const Cut x = a.cuts[w + i], y = a.cuts[w + i + 1];
+            if (i == 0 || !same_tile(x, y) || x.at < y.at)  // (a workgroup without tiles wrote nothing)
+                s = part_sums(a, slot(i))[place];
+        }
+        const float m_new = fmaxf(mx, wave_max(s));
+        const float scale = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m_new);
+        const float wt = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
+        sum = sum * scale + wave_sum(wt);
+        a0 *= scale;
+        a1 *= scale;
+        const int n = min(kWave, parts - i0);
+        for (int j = 0; j < n; ++j) {
+            const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), j));
+            if (wj == 0.f)
+                continue;
+            const float2 v = *reinterpret_cast<const float2 *>(part_rows(a, slot(i0 + j)) + (int64_t)place * kHeadDim + 2 * lane);
+            a0 = fmaf(wj, v.x, a0);
+            a1 = fmaf(wj, v.y, a1);
+        }
+        mx = m_new;
+    }
+    const int token = row / a.shape.group, head = cut.h * a.shape.group + row - token * a.shape.group;
+    if (a.sinks) {
+        const float sink = a.sinks[head] * kLog2e, m_new = fmaxf(mx, sink);
+        const float scale = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m_new);
+        a0 *= scale;
+        a1 *= scale;
+        sum = sum * scale + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m_new));
+        mx = m_new;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t q_row = (int64_t)(seq.row0 + token) * a.num_q_heads + head;
+    typedef OutT out2 __attribute__((ext_vector_type(2)));
+    *reinterpret_cast<out2 *>(static_cast<OutT *>(a.out) + q_row * kHeadDim + 2 * lane) = out2{(OutT)(a0 * inv), (OutT)(a1 * inv)};
+    if (lane == 0 && a.lse)
+        a.lse[q_row] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+}  // namespace chunk
+}  // namespace tq4

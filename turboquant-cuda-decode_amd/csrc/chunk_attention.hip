@@ -1,0 +1,183 @@
+// Attention of several new tokens per sequence (tq4_chunk_attention, include/tq4_decode.h).
+#include <algorithm>
+
+#include "abi.h"
+#include "chunk.h"
+
+using namespace tq4::abi;
+
+namespace {
+
+// How a call is spread over the device: workgroups of `wr` * `wt` waves on row tiles of 32 wr rows, `held` of them at once.
+struct ChunkPlan {
+    int wr, groups;
+};
+int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
+ChunkPlan chunk_plan(int tokens, int batch, int group) {
+    const int64_t rows = (int64_t)tokens * group / batch;  // of a sequence, on average
+    if (rows > 64)
+        return {8, cus()};
+    if (rows > 32)
+        return {2, 2 * cus()};
+    return {1, 4 * cus()};
+}
+
+struct Workspace {
+    int64_t q_lo, factor, work, cuts, parts, total;  // offsets in floats
+};
+Workspace workspace_of(int tokens, int batch, int Hq, int Hk) {
+    const int64_t rows = (int64_t)tokens * Hq;
+    const ChunkPlan p = chunk_plan(tokens, batch, Hq / Hk);
+    auto up = [](int64_t x) { return (x + 63) / 64 * 64; };
+    Workspace w{};
+    w.q_lo = up(rows * tq4::kHeadDim / 2);
+    w.factor = w.q_lo + up(rows * tq4::kHeadDim / 2);
+    w.work = w.factor + up(rows);
+    w.cuts = w.work + up(2 * ((int64_t)batch + 1));
+    w.parts = w.cuts + up(4 * ((int64_t)p.groups + 1));
+    w.total = w.parts + up((int64_t)2 * p.groups * 32 * p.wr * (tq4::kHeadDim + 1));
+    return w;
+}
+const char *shape_error(int tokens, int B, int Hq, int Hk) {
+    if (tokens <= 0 || B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk)
+        return "tokens, B, Hq and Hk must be positive, Hq a multiple of Hk";
+    if ((int64_t)tokens * Hq > 1 << 30)
+        return "more than 2^30 query rows";
+    return nullptr;
+}
+
+template <int LAYOUT, int WR, int WT, int KT, int BUFS, bool FINE>
+void launch_chunk(const Stage1Args &a, const tq4::chunk::Args &p, hipStream_t st) {
+    const dim3 block(64 * WR * WT), grid((p.groups + 7) / 8 * 8);
+    using namespace tq4::chunk;
+    if (a.key_fp8)
+        launch(&chunk_kernel<LAYOUT, true, false, false, WR, WT, KT, BUFS, FINE>, grid, block, st, p);
+    else if (a.key_bits == 3 && a.value_bits == 3)
+        launch(&chunk_kernel<LAYOUT, false, true, true, WR, WT, KT, BUFS, FINE>, grid, block, st, p);
+    else if (a.key_bits == 3)
+        launch(&chunk_kernel<LAYOUT, false, true, false, WR, WT, KT, BUFS, FINE>, grid, block, st, p);
+    else
+        launch(&chunk_kernel<LAYOUT, false, false, false, WR, WT, KT, BUFS, FINE>, grid, block, st, p);
+}
+template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq4::chunk::Args &p, int wr, hipStream_t st) {
+    if (wr == 8)
+        launch_chunk<LAYOUT, 8, 1, 64, 2, FINE>(a, p, st);
+    else if (wr == 2)
+        launch_chunk<LAYOUT, 2, 2, 64, 1, FINE>(a, p, st);
+    else
+        launch_chunk<LAYOUT, 1, 2, 64, 1, FINE>(a, p, st);
+}
+template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStream_t st) {
+    using namespace tq4::chunk;
+    const int64_t rows = (int64_t)p.tokens * p.num_q_heads;
+    const dim3 grid((unsigned)((rows + kStartRows - 1) / kStartRows + 1)), block(kStartThreads);
+    if (p.q_dtype == TQ4_BF16)
+        launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p);
+    else
+        launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tq4_chunk_workspace_floats(int tokens, int B, int Hq, int Hk) {
+    if (const char *why = shape_error(tokens, B, Hq, Hk)) {
+        fail(TQ4_E_INVALID, "tq4_chunk_workspace_floats: %s", why);
+        return -1;
+    }
+    return workspace_of(tokens, B, Hq, Hk).total;
+}
+
+int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride, const float *rot_t,
+                        const float *centroids, const uint8_t *kv_cache, const int32_t *block_table,
+                        const int32_t *seq_lens, const int32_t *query_starts, float *workspace, int64_t workspace_floats,
+                        void *out, int out_dtype, float *lse, int tokens, int B, int Hq, int Hk, int D, int block_size,
+                        int max_blocks_per_seq, int64_t cache_block_stride, int layout, float attn_scale,
+                        const float *sinks, int key_bits, int value_bits, int causal, int window, int first_tokens,
+                        tq4_stream_t stream) {
+    constexpr char what[] = "tq4_chunk_attention";
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    Stage1Args a{};
+    // (the log-sum-exp may be left out: another pointer stands in for it in the common checks)
+    int rc = span_args(a, what, query, query_dtype, rot_t, centroids, kv_cache, block_table, seq_lens, workspace, workspace,
+                       out, out_dtype, workspace, B, Hq, Hk, D, block_size, max_blocks_per_seq, cache_block_stride, 1,
+                       layout, attn_scale, sinks, key_bits, value_bits);
+    if (rc)
+        return rc;
+    if (const char *why = shape_error(tokens, B, Hq, Hk))
+        return fail(TQ4_E_INVALID, "%s: %s", what, why);
+    if (!query_starts)
+        return fail(TQ4_E_INVALID, "%s: null pointer argument", what);
+    if (query_dtype == TQ4_F32 || out_dtype == TQ4_F32)
+        return fail(TQ4_E_UNSUPPORTED, "%s: 16-bit queries and outputs only (the products have f16 operands)", what);
+    if (query_stride < (int64_t)Hq * D || query_stride % 8)
+        return fail(TQ4_E_INVALID, "%s: query_stride %lld must be whole 16-byte pieces, at least Hq * D", what,
+                    (long long)query_stride);
+    if (!aligned(out, 16))
+        return fail(TQ4_E_INVALID, "%s: out must be 16-byte aligned", what);
+    if (window < 0 || first_tokens < 0 || (window > 0 && !causal))
+        return fail(TQ4_E_INVALID, "%s: window (%d) and first_tokens (%d) must be at least 0, a window only with causal", what,
+                    window, first_tokens);
+    const Workspace ws = workspace_of(tokens, B, Hq, Hk);
+    if (workspace_floats < ws.total || !aligned(workspace, 16))
+        return fail(TQ4_E_INVALID, "%s: workspace of %lld floats, needs %lld, 16-byte aligned", what,
+                    (long long)workspace_floats, (long long)ws.total);
+    const ChunkPlan plan = chunk_plan(tokens, B, Hq / Hk);
+    tq4::chunk::Args p{};
+    p.query = query;
+    p.rot_t = rot_t;
+    p.centroids = centroids;
+    p.cache = kv_cache;
+    p.pages = block_table;
+    p.seq_lens = seq_lens;
+    p.starts = query_starts;
+    p.sinks = sinks;
+    p.out = out;
+    p.lse = lse;
+    p.q_hi = reinterpret_cast<_Float16 *>(workspace);
+    p.q_lo = reinterpret_cast<_Float16 *>(workspace + ws.q_lo);
+    p.q_factor = workspace + ws.factor;
+    p.work = reinterpret_cast<double *>(workspace + ws.work);
+    p.cuts = reinterpret_cast<tq4::chunk::Cut *>(workspace + ws.cuts);
+    p.parts = workspace + ws.parts;
+    p.block_stride = cache_block_stride;
+    p.query_stride = query_stride;
+    p.score_scale_log2 = attn_scale * tq4::kLog2e;
+    p.q_dtype = query_dtype;
+    p.out_dtype = out_dtype;
+    p.num_q_heads = Hq;
+    p.num_kv_heads = Hk;
+    p.tokens = tokens;
+    p.batch = B;
+    p.table_width = max_blocks_per_seq;
+    p.groups = plan.groups;
+    p.block_size_log2 = log2_int(block_size);
+    p.slot_pos = a.slot_pos;
+    p.slot_head = a.slot_head;
+    p.shape = tq4::chunk::Shape{32 * plan.wr, 64, Hq / Hk, Hk, causal != 0, std::min(window, 1 << 30), std::min(first_tokens, 1 << 30)};
+    p.longest = (int)std::min<int64_t>((int64_t)max_blocks_per_seq * block_size, (1 << 30));
+    const bool fine = lse || out_dtype == TQ4_F16;
+    if (a.key_fp8)
+        launch_start<true, false>(p, st);
+    else
+        fine ? launch_start<false, true>(p, st) : launch_start<false, false>(p, st);
+    rc = launch_status("chunk start");
+    if (rc)
+        return rc;
+    if (a.kl == 0)
+        fine ? launch_chunk<0, true>(a, p, plan.wr, st) : launch_chunk<0, false>(a, p, plan.wr, st);
+    else
+        fine ? launch_chunk<1, true>(a, p, plan.wr, st) : launch_chunk<1, false>(a, p, plan.wr, st);
+    rc = launch_status("chunk");
+    if (rc)
+        return rc;
+    const dim3 grid(plan.groups, 32 * plan.wr / tq4::chunk::kMergeRows), block(tq4::kWave * tq4::chunk::kMergeRows);
+    if (out_dtype == TQ4_BF16)
+        launch(&tq4::chunk::chunk_merge_kernel<__bf16>, grid, block, st, p);
+    else
+        launch(&tq4::chunk::chunk_merge_kernel<_Float16>, grid, block, st, p);
+    return launch_status("chunk merge");
+}
+
+}  // extern "C"

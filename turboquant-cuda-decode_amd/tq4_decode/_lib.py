@@ -36,6 +36,8 @@ EXPORTS = (
     "tq4_window_decode",
     "tq4_prefix_decode",
     "tq4_prefix_workspace_floats",
+    "tq4_chunk_attention",
+    "tq4_chunk_workspace_floats",
     "tq4_last_error",
     "tq4_abi_version",
     "tq4_time_next_launch",
@@ -64,6 +66,9 @@ _SIGS = {
     "tq4_prefix_decode": [_p, _i, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _f,
                           _p, _i, _i, _i, _i, _p],
     "tq4_prefix_workspace_floats": [_i, _i, _i, _i],
+    "tq4_chunk_attention": [_p, _i, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i64,
+                            _i, _f, _p, _i, _i, _i, _i, _i, _p],
+    "tq4_chunk_workspace_floats": [_i, _i, _i, _i],
     "tq4_last_error": [],
     "tq4_abi_version": [],
     "tq4_time_next_launch": [_p, _p],
@@ -76,7 +81,8 @@ _SIGS = {
                              _i, _i, _p],
     "tq4_store_preset": [_p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _i, _i, _i, _p],
 }
-_RESULTS = {"tq4_last_error": ctypes.c_char_p, "tq4_prefix_workspace_floats": _i64}
+_RESULTS = {"tq4_last_error": ctypes.c_char_p, "tq4_prefix_workspace_floats": _i64,
+            "tq4_chunk_workspace_floats": _i64}
 
 
 class Tq4Error(RuntimeError):

@@ -739,6 +739,89 @@ def prefix_decode(query, rotation_t, kv_cache, block_table, seq_lens, centroids,
     return ws.out, ws.lse
 
 
+class ChunkWorkspace:
+    """Buffers of ``chunk_attention`` (fixed shapes, any lengths, reusable): ``out``, ``lse`` and one block of
+    scratch.  Calls that may overlap need one each."""
+
+    def __init__(self, tokens, batch, num_q_heads, num_kv_heads, device, out_dtype=torch.bfloat16):
+        self.shape = (tokens, batch, num_q_heads, num_kv_heads)
+        floats = _lib.load().tq4_chunk_workspace_floats(*self.shape)
+        if floats < 0:
+            raise Tq4Error(_lib.load().tq4_last_error().decode())
+        self.scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        self.out = torch.empty(tokens, num_q_heads, HEAD_DIM, dtype=out_dtype, device=device)
+        self.lse = torch.empty(tokens, num_q_heads, dtype=torch.float32, device=device)
+
+
+def chunk_attention(query, rotation_t, kv_cache, block_table, seq_lens, query_starts, centroids, *, causal=True, window=0,
+                    first_tokens=0, key_bits=4, value_bits=4, layout="soa", out_dtype=None, attn_scale=None,
+                    return_lse=False, workspace=None, sinks=None):
+    """Attention of several new tokens per sequence over the cache: chunks of prompts, drafted tokens.  Returns
+    ``out [T, Hq, D]``, with ``return_lse`` also ``lse [T, Hq]``.
+
+    Sequence ``b`` has the rows ``query_starts[b]`` to ``query_starts[b + 1] - 1`` of ``query [T, Hq, D]``
+    (``query_starts`` int32 ``[B + 1]`` on the device, not decreasing; rows of no sequence keep what ``out`` held) and
+    ``seq_lens[b]`` tokens in the cache.  ``causal``: its new tokens are the last of those (``rope_store`` and the other writers
+    put them there) and each sees itself and what lies before it; with ``window`` only the last ``window`` tokens
+    (itself included) and the ``first_tokens`` first ones.  ``causal=False``: every new token sees all ``seq_lens[b]``
+    tokens, as a context whose result ``merge_states`` joins with that of the chunk's own tokens.  A new token that sees
+    nothing gets zeros and LSE -inf.
+
+    ``query`` and the outputs are bf16 or fp16; heads are contiguous, tokens may be strided (a slice of a projection's
+    output).  fp16 outputs and calls with ``return_lse`` take scores from f16 pairs and V's codes as they are, others
+    round keys, rotated queries, values and weights to f16.  ``workspace``: a ``ChunkWorkspace``, whose ``out`` and ``lse``
+    are returned.  Launches depend on shapes alone.  ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in
+    ``window_decode``.
+    """
+    _int_arg(window, "window", 0)
+    _int_arg(first_tokens, "first_tokens", 0)
+    _require(window == 0 or causal, "a window needs causal=True")
+    fp8 = key_bits == 8
+    if (key_bits, value_bits) not in PRESETS + ((8, 4),):
+        raise RuntimeError(f"key/value bits must be one of {PRESETS + ((8, 4),)}")
+    _require(query.is_cuda and query.dim() == 3 and query.dtype in DTYPES, "invalid query")
+    T, Hq, D = query.shape
+    _require(D == HEAD_DIM, _QUERY_SHAPE)
+    s0, s1, s2 = query.stride()
+    _require(s2 == 1 and (s1 == D or Hq == 1), "query: heads must be contiguous")
+    stride = max(s0, Hq * D) if T <= 1 else s0
+    out_dtype = query.dtype if out_dtype is None else out_dtype
+    _check_tensor(block_table, "block_table", torch.int32)
+    _check_tensor(seq_lens, "seq_lens", torch.int32)
+    _check_tensor(query_starts, "query_starts", torch.int32)
+    slot = slot_bytes_fp8(D) if fp8 else slot_bytes_preset(D, key_bits, value_bits)
+    bs, Hk, block_stride, lid = _cache_geometry(kv_cache, slot, layout, " (FP8 keys)" if fp8 else "")
+    _require(T > 0 and Hq % Hk == 0, "query must have tokens, Hq must be a multiple of Hk")
+    _require(seq_lens.dim() == 1, "seq_lens must be [B]")
+    B = seq_lens.size(0)
+    _require(block_table.dim() == 2 and block_table.size(0) == B, "block_table batch mismatch")
+    _require(query_starts.dim() == 1 and query_starts.size(0) == B + 1, "query_starts must be [B + 1]")
+    _require(out_dtype in DTYPES, "invalid out_dtype")
+    ws = workspace or ChunkWorkspace(T, B, Hq, Hk, query.device, out_dtype)
+    _require(isinstance(ws, ChunkWorkspace) and ws.shape == (T, B, Hq, Hk) and ws.out.dtype == out_dtype,
+             "workspace does not match this call")
+    tensors = [query, kv_cache, block_table, seq_lens, query_starts, ws.out]
+    if not fp8:
+        _check_tensor(rotation_t, "rotation_t", torch.float32)
+        _require(tuple(rotation_t.shape) == (D, D), _ROTATION_SHAPE)
+        _check_tensor(centroids, "centroids", torch.float32)
+        if centroids.numel() != 1 << key_bits:
+            raise RuntimeError(f"{key_bits}-bit keys need {1 << key_bits} centroids")
+        tensors += [rotation_t, centroids]
+    _require(_same_device(*tensors), "all tensors must be on the same device")
+    scale = 1.0 / math.sqrt(D) if attn_scale is None else float(attn_scale)
+    with _on_device(query.device):
+        rc = _lib.load().tq4_chunk_attention(
+            query.data_ptr(), DTYPES[query.dtype], stride, None if fp8 else rotation_t.data_ptr(),
+            None if fp8 else centroids.data_ptr(), kv_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            query_starts.data_ptr(), ws.scratch.data_ptr(), ws.scratch.numel(), ws.out.data_ptr(), DTYPES[out_dtype],
+            ws.lse.data_ptr() if return_lse else None, T, B, Hq, Hk, D, bs, block_table.size(1), block_stride, lid, scale,
+            _check_sinks(sinks, Hq, query.device), key_bits, value_bits, int(causal), window, first_tokens,
+            _stream(query.device))
+    _lib.check(rc, "tq4_chunk_attention")
+    return (ws.out, ws.lse) if return_lse else ws.out
+
+
 def _buffer_view(buf, shape, dtype):
     """``buf`` cut to ``shape`` (leading sub-block) when it fits and stays contiguous."""
     if buf is None or buf.dtype != dtype or buf.dim() != len(shape):
