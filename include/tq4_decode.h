@@ -354,6 +354,29 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
 /* Floats of workspace that tq4_chunk_attention needs for these shapes; -1 (and a message) where they are invalid. */
 int64_t tq4_chunk_workspace_floats(int tokens, int B, int Hq, int Hk);
 
+/*
+ * Reads keys and values back from their slots: the way back of tq4_store, tq4_store_fp8 and tq4_store_preset.
+ * Row i of key and value [N, Hk, D] (contiguous, 16-byte aligned, of dtype) is token slot_mapping[i]'s: value
+ * = code * scale + zero; key = norm * (centroids[codes] @ rot_t^T) with the rot_t that it was written with (orthogonal),
+ * norm * centroids[codes] with rot_t NULL, the E4M3 values for FP8 keys (rot_t and centroids unused).  A slot that is negative or
+ * past num_blocks * block_size gives zeros; slots may repeat.  For bf16 keys the turn's factors are rounded to f16,
+ * else to pairs of f16.  Layouts, presets and block sizes as the writers'; key, value and the cache must not overlap.
+ * Replaces: _tq_full_dequant_kv reference/soa_decode_v1.py:322-454 (keys rotated, fp16, one sequence's blocks).
+ */
+int tq4_cache_load(const uint8_t *kv_cache, const int32_t *slot_mapping, const float *rot_t, const float *centroids,
+                   void *key, void *value, int dtype, int num_blocks, int N, int Hk, int D, int block_size,
+                   int64_t cache_block_stride, int layout, int key_bits, int value_bits, tq4_stream_t stream);
+
+/*
+ * Joins two attention results of the same rows over different tokens: lse = log(exp(lse_a) + exp(lse_b)), out =
+ * exp(lse_a - lse) out_a + exp(lse_b - lse) out_b.  Rows [rows, D] of dtype, contiguous and 16-byte aligned, lse fp32
+ * [rows].  A result of weight zero counts as nothing, whatever it holds (LSE -inf: one over no tokens); two of them
+ * give zeros and -inf.  out may be out_a or out_b and lse lse_a or lse_b; other overlaps are refused.
+ * No counterpart in the reference.
+ */
+int tq4_merge_states(const void *out_a, const float *lse_a, const void *out_b, const float *lse_b, void *out, int dtype,
+                     float *lse, int64_t rows, int D, tq4_stream_t stream);
+
 /* Message of the last failed call on this thread ("" when none).
  * Replaces: the TORCH_CHECK messages of cuda/tq4_cuda_v1.cu:468-499. */
 const char *tq4_last_error(void);

@@ -1,0 +1,349 @@
+// Keys and values read back from their slots of the quantised cache, and two attention results joined.
+//
+// A row is one (token, kv-head): v = code * scale + zero, k = norm * sum_j c[code_j] rot_t[d][j] (the keys' rotation is
+// orthogonal, so its transpose turns them back).  The turn is a matrix product with the rows in the columns,
+//
+//   K^T[dim][row] = sum_j rot_t[dim][j] c[row][j]       v_mfma_f32_16x16x32_f16, A = rot_t, B = the codes' centroids
+//
+// in which lane (n, g) = (lane % 16, lane / 16) holds dims 32 g .. +31 of row n as they lie in the cache (one load), and gets
+// eight dims in a row of it per two products: with the contraction in the order k-slot (kb, g, j) = dim 32 g + 8 kb + j,
+// and the products' rows in the order row 4 g + i of block cb = dim 32 (cb / 2) + 8 g + 4 (cb % 2) + i.  Both factors are
+// scaled by 16 (out of f16's denormals) and rounded to f16 for bf16 keys (an eighth of their own rounding, together), to
+// pairs of f16 for others.
+//
+// Bound by the bytes: a wave asks for its next 16 rows, and their slots after them, before it works on these.
+#pragma once
+#include "stage1_xdl.h"
+
+namespace tq4 {
+namespace load {
+
+using xdl::half8;
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x3a2 __attribute__((ext_vector_type(3), aligned(2)));
+typedef uint32_t u32a1 __attribute__((aligned(1)));
+typedef float floatx4a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+struct Args {
+    const uint8_t *cache;
+    const int32_t *slots;
+    const float *rot_t;      // null: keys as they are stored
+    const float *centroids;  // null: FP8 keys
+    void *key, *value;
+    int64_t block_stride;
+    int64_t num_slots;       // of the cache
+    int rows;                // tokens * kv-heads
+    int num_kv_heads, block_size, slot_pos, slot_head;
+};
+
+constexpr int kWaves = 4, kThreads = kWave * kWaves, kRows = 16;  // rows of a wave's tile
+constexpr int kPitch = kHeadDim + 8;
+
+// Eight values in a row.
+template <typename T> __device__ __forceinline__ void put8(void *out, int64_t at, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
+        to[0] = float4{v[0], v[1], v[2], v[3]};
+        to[1] = float4{v[4], v[5], v[6], v[7]};
+    } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        t8 x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = (T)v[i];
+        *reinterpret_cast<t8 *>(static_cast<T *>(out) + at) = x;
+    }
+}
+
+template <int LAYOUT, bool KF8, bool KB3, bool V3, typename OutT, bool TURN>
+__global__ __launch_bounds__(kThreads) void load_kernel(const Args a) {
+    constexpr bool PAIRS = !std::is_same<OutT, __bf16>::value;
+    constexpr int rec = xdl::record_bytes<LAYOUT, KF8, KB3, V3>(), v0 = xdl::v_offset<LAYOUT, KF8, KB3>();
+    constexpr int kbytes = KF8 ? kHeadDim : KB3 ? xdl::kK3Bytes : kHalfD, vbytes = V3 ? xdl::kK3Bytes : kHalfD, nf = KF8 ? 2 : 3;
+    constexpr int kEntries = KF8 ? 1 : KB3 ? 64 : 256;
+    __shared__ __align__(16) _Float16 pt_hi[TURN ? kHeadDim * kPitch : 8], pt_lo[TURN && PAIRS ? kHeadDim * kPitch : 8];
+    __shared__ __align__(16) uint2 lut[KF8 || !TURN ? 1 : kEntries];  // pairs of centroids times 16, f16 hi and lo
+    __shared__ __align__(16) float2 lut32[KF8 || TURN ? 1 : kEntries];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int waves = gridDim.x * kWaves, wave = blockIdx.x * kWaves + (tid >> 6);
+    const int tiles = (a.rows + kRows - 1) / kRows;
+
+    // A row's place: its block, and in it the bytes to its record and the index of its first scalar (SoA).
+    struct Place {
+        int block, data, meta;  // block < 0: no slot of the cache
+    };
+    struct Where {
+        const uint8_t *data;
+        const uint16_t *meta;
+    };
+    auto row_of = [&](int tile, int r) { return min((int64_t)tile * kRows + r, (int64_t)a.rows - 1); };
+    auto slot_of = [&](int tile, int r) { return a.slots[(int)row_of(tile, r) / a.num_kv_heads]; };
+    auto place_of = [&](int tile, int r, int slot) {
+        const int head = (int)row_of(tile, r) % a.num_kv_heads;
+        const bool there = slot >= 0 && slot < a.num_slots;
+        const int s = there ? slot : 0, blk = s / a.block_size, off = s - blk * a.block_size;
+        if constexpr (LAYOUT == 0)
+            return Place{there ? blk : -1, (off * a.num_kv_heads + head) * rec, head * nf * a.block_size + off};
+        else
+            return Place{there ? blk : -1, off * a.slot_pos + head * a.slot_head, 0};
+    };
+    auto where = [&](const Place &p) {
+        const uint8_t *b = a.cache + (int64_t)max(p.block, 0) * a.block_stride;
+        return Where{b + p.data, reinterpret_cast<const uint16_t *>(b + a.block_size * a.num_kv_heads * rec) + p.meta};
+    };
+    struct Raw {
+        uint4 k, k2;
+        uint32_t norm, v[4], scale[4], zero[4];
+        bool k_there, v_there[4];
+    };
+    // lane (n, g): a quarter of row n's key, and a sixteenth of the values of rows 4 i + g, whose places lanes 4 i + g have
+    auto fetch = [&](Raw &r, int tile, int slot) {
+        const Place own = place_of(tile, n, slot);
+        const Where w = where(own);
+        r.k_there = own.block >= 0;
+        const uint8_t *p = w.data + g * (kbytes / 4);
+        if constexpr (KB3) {
+            const u32x3a2 x = *reinterpret_cast<const u32x3a2 *>(p);
+            r.k = uint4{x[0], x[1], x[2], 0u};
+        } else {
+            const u32x4a2 x = *reinterpret_cast<const u32x4a2 *>(p);
+            r.k = uint4{x[0], x[1], x[2], x[3]};
+        }
+        if constexpr (KF8) {
+            const u32x4a2 x = *reinterpret_cast<const u32x4a2 *>(p + 16);
+            r.k2 = uint4{x[0], x[1], x[2], x[3]};
+        } else {
+            r.norm = LAYOUT == 0 ? w.meta[0] : *reinterpret_cast<const uint16_t *>(w.data + kbytes);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int vr = 4 * i + g;
+            const Place at{__shfl(own.block, vr, kWave), __shfl(own.data, vr, kWave), LAYOUT == 0 ? __shfl(own.meta, vr, kWave) : 0};
+            const Where x = where(at);
+            r.v_there[i] = at.block >= 0;
+            r.v[i] = *reinterpret_cast<const u32a1 *>(x.data + v0 + (V3 ? 3 : 4) * n);
+            if constexpr (LAYOUT == 0) {
+                r.scale[i] = x.meta[(nf - 2) * a.block_size];
+                r.zero[i] = x.meta[(nf - 1) * a.block_size];
+            } else {
+                r.scale[i] = *reinterpret_cast<const uint16_t *>(x.data + v0 + vbytes);
+                r.zero[i] = *reinterpret_cast<const uint16_t *>(x.data + v0 + vbytes + 2);
+            }
+        }
+    };
+
+    Raw raw;
+    int slot = wave < tiles ? slot_of(wave, n) : 0;
+    if (wave < tiles)
+        fetch(raw, wave, slot);
+    slot = slot_of(min(wave + waves, tiles - 1), n);
+    if constexpr (TURN) {
+#pragma unroll
+        for (int it = 0; it < kHeadDim * 16 / kThreads; ++it) {
+            const int i = tid + it * kThreads, r = i >> 4, kb = (i >> 2) & 3, kg = i & 3;  // (row, k-slots 32 kb + 8 kg ..)
+            const int cb = r >> 4, dim = 32 * (cb >> 1) + 8 * ((r >> 2) & 3) + 4 * (cb & 1) + (r & 3);
+            const float *from = a.rot_t + dim * kHeadDim + 32 * kg + 8 * kb;
+            const floatx4a4 x = *reinterpret_cast<const floatx4a4 *>(from), y = *reinterpret_cast<const floatx4a4 *>(from + 4);
+            half8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float w = 16.f * (j < 4 ? x[j & 3] : y[j & 3]);
+                asm("" : "+v"(w));
+                hi[j] = (_Float16)w;
+                lo[j] = (_Float16)(w - (float)hi[j]);
+            }
+            *reinterpret_cast<half8 *>(pt_hi + r * kPitch + 32 * kb + 8 * kg) = hi;
+            if constexpr (PAIRS)
+                *reinterpret_cast<half8 *>(pt_lo + r * kPitch + 32 * kb + 8 * kg) = lo;
+        }
+    }
+    if constexpr (!KF8)
+        for (int e = tid; e < kEntries; e += kThreads) {
+            const float c0 = a.centroids[KB3 ? e & 7 : e & 15], c1 = a.centroids[KB3 ? e >> 3 : e >> 4];
+            if constexpr (TURN) {
+                float x = 16.f * c0, y = 16.f * c1;
+                asm("" : "+v"(x), "+v"(y));
+                const _Float16 h0 = (_Float16)x, h1 = (_Float16)y;
+                const _Float16 l0 = (_Float16)(x - (float)h0), l1 = (_Float16)(y - (float)h1);
+                auto pack = [](_Float16 p, _Float16 q) {
+                    return (uint32_t)__builtin_bit_cast(unsigned short, p) | ((uint32_t)__builtin_bit_cast(unsigned short, q) << 16);
+                };
+                lut[e] = uint2{pack(h0, h1), pack(l0, l1)};
+            } else {
+                lut32[e] = float2{c0, c1};
+            }
+        }
+    if constexpr (TURN || !KF8)
+        __syncthreads();
+
+    for (int tile = wave; tile < tiles; tile += waves) {
+        const Raw r = raw;
+        if (tile + waves < tiles) {
+            fetch(raw, tile + waves, slot);
+            slot = slot_of(min(tile + 2 * waves, tiles - 1), n);
+        }
+        // values
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t row = (int64_t)tile * kRows + 4 * i + g;
+            const float scale = half_bits_to_float(r.scale[i]), zero = half_bits_to_float(r.zero[i]);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t code = V3 ? (r.v[i] >> (3 * j)) & 7u : (r.v[i] >> (4 * j)) & 15u;
+                v[j] = r.v_there[i] ? fmaf((float)code, scale, zero) : 0.f;
+            }
+            if (row < a.rows)
+                put8<OutT>(a.value, row * kHeadDim + 8 * n, v);
+        }
+        // keys
+        const int64_t row = (int64_t)tile * kRows + n;
+        float norm = 0.f;
+        if constexpr (!KF8)
+            norm = half_bits_to_float(r.norm);
+        const uint32_t w[4] = {r.k.x, r.k.y, r.k.z, r.k.w};
+        auto code_pair = [&](int b) {  // codes 2 b, 2 b + 1 of the lane's 32
+            if constexpr (KB3) {
+                const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
+                uint32_t v = w[wi] >> sh;
+                if (sh > 26)
+                    v |= w[wi + 1] << (32 - sh);
+                return v & 63u;
+            } else {
+                return (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
+            }
+        };
+        if constexpr (TURN) {
+            typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
+            half8 c_hi[4], c_lo[4];
+            float hh = 0.f, hl = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                uint32_t e[4], f[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const uint2 c = lut[code_pair(4 * kb + b)];
+                    e[b] = c.x;
+                    f[b] = c.y;
+                    if constexpr (LAYOUT == 1) {
+                        const auto h = __builtin_bit_cast(fp16x2, e[b]), l = __builtin_bit_cast(fp16x2, f[b]);
+                        hh = __builtin_amdgcn_fdot2(h, h, hh, false);
+                        hl = __builtin_amdgcn_fdot2(h, l, hl, false);
+                    }
+                }
+                c_hi[kb] = xdl::as_half8(e[0], e[1], e[2], e[3]);
+                c_lo[kb] = xdl::as_half8(f[0], f[1], f[2], f[3]);
+            }
+            if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction
+                const float sq = xdl::sum_xor32(xdl::sum_xor16(fmaf(2.f, hl, hh))) * (1.f / 256.f);
+                norm /= __builtin_amdgcn_sqrtf(sq + 1e-16f);
+            }
+            norm = r.k_there ? norm * (1.f / 256.f) : 0.f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                float v[8];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    floatx4 y{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb) {
+                        const int at = (16 * (2 * p + half) + n) * kPitch + 32 * kb + 8 * g;
+                        const half8 hi = *reinterpret_cast<const half8 *>(pt_hi + at);
+                        y = xdl::mfma(hi, c_hi[kb], y);
+                        if constexpr (PAIRS) {
+                            y = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + at), c_hi[kb], y);
+                            y = xdl::mfma(hi, c_lo[kb], y);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[4 * half + i] = r.k_there ? y[i] * norm : 0.f;
+                }
+                if (row < a.rows)
+                    put8<OutT>(a.key, row * kHeadDim + 32 * p + 8 * g, v);
+            }
+        } else {
+            float k[32], sq = 0.f;
+            if constexpr (KF8) {
+                const uint32_t w8[8] = {w[0], w[1], w[2], w[3], r.k2.x, r.k2.y, r.k2.z, r.k2.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w8[i], false);
+                    const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w8[i], true);
+                    k[4 * i] = x[0];
+                    k[4 * i + 1] = x[1];
+                    k[4 * i + 2] = y[0];
+                    k[4 * i + 3] = y[1];
+                }
+                norm = 1.f;
+            } else {
+#pragma unroll
+                for (int b = 0; b < 16; ++b) {
+                    const float2 c = lut32[code_pair(b)];
+                    k[2 * b] = c.x;
+                    k[2 * b + 1] = c.y;
+                    sq = fmaf(c.x, c.x, fmaf(c.y, c.y, sq));
+                }
+                if constexpr (LAYOUT == 1) {
+                    sq = xdl::sum_xor32(xdl::sum_xor16(sq));
+                    norm /= __builtin_amdgcn_sqrtf(sq + 1e-16f);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[j] = r.k_there ? (KF8 ? k[8 * p + j] : k[8 * p + j] * norm) : 0.f;
+                if (row < a.rows)
+                    put8<OutT>(a.key, row * kHeadDim + 32 * g + 8 * p, v);
+            }
+        }
+    }
+}
+
+// ---- Two results joined ----------------------------------------------------------------------
+
+// lse = log(exp(lse_a) + exp(lse_b)), out = exp(lse_a - lse) a + exp(lse_b - lse) b; a result of weight zero counts as
+// nothing, whatever it holds, and two of them give zeros and -inf.  A row is 16 lanes' (8 values each), kJoinRows of
+// them a thread's: bound by the bytes.
+constexpr int kJoinRows = 4;
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_states_kernel(const T *a, const float *lse_a, const T *b, const float *lse_b,
+                                                               T *out, float *lse, int64_t rows) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const int j = threadIdx.x & 15;
+    const int64_t r0 = (int64_t)blockIdx.x * (kThreads / 16 * kJoinRows) + (threadIdx.x >> 4);
+    t8 x[kJoinRows], y[kJoinRows];
+    float la[kJoinRows], lb[kJoinRows];
+#pragma unroll
+    for (int i = 0; i < kJoinRows; ++i) {
+        const int64_t r = min(r0 + i * (kThreads / 16), rows - 1);
+        la[i] = lse_a[r];
+        lb[i] = lse_b[r];
+        x[i] = *reinterpret_cast<const t8 *>(a + r * kHeadDim + 8 * j);
+        y[i] = *reinterpret_cast<const t8 *>(b + r * kHeadDim + 8 * j);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoinRows; ++i) {
+        const int64_t r = r0 + i * (kThreads / 16);
+        if (r >= rows)
+            return;
+        const float top = fmaxf(la[i], lb[i]);
+        const bool none = la[i] == -INFINITY && lb[i] == -INFINITY;
+        const float wa = none ? 0.f : expf(la[i] - top), wb = none ? 0.f : expf(lb[i] - top), sum = wa + wb;
+        const float inv = none ? 0.f : 1.f / sum, sa = wa * inv, sb = wb * inv;
+        t8 z;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float u = sa == 0.f ? 0.f : sa * (float)x[i][k], v = sb == 0.f ? 0.f : sb * (float)y[i][k];
+            z[k] = (T)(u + v);
+        }
+        *reinterpret_cast<t8 *>(out + r * kHeadDim + 8 * j) = z;
+        if (j == 0)
+            lse[r] = none ? -INFINITY : top + logf(sum);
+    }
+}
+
+}  // namespace load
+}  // namespace tq4

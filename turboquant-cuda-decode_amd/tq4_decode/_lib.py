@@ -38,6 +38,8 @@ EXPORTS = (
     "tq4_prefix_workspace_floats",
     "tq4_chunk_attention",
     "tq4_chunk_workspace_floats",
+    "tq4_cache_load",
+    "tq4_merge_states",
     "tq4_last_error",
     "tq4_abi_version",
     "tq4_time_next_launch",
@@ -69,6 +71,8 @@ _SIGS = {
     "tq4_chunk_attention": [_p, _i, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i64,
                             _i, _f, _p, _i, _i, _i, _i, _i, _p],
     "tq4_chunk_workspace_floats": [_i, _i, _i, _i],
+    "tq4_cache_load": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _i, _p],
+    "tq4_merge_states": [_p, _p, _p, _p, _p, _i, _p, _i64, _i, _p],
     "tq4_last_error": [],
     "tq4_abi_version": [],
     "tq4_time_next_launch": [_p, _p],

@@ -16,7 +16,8 @@ PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 LIB = PKG / "libtq4_decode.so"
-SOURCES = ("tq4_decode.hip", "span_decode.hip", "prefix_decode.hip", "rope_store.hip", "chunk_attention.hip")
+SOURCES = ("tq4_decode.hip", "span_decode.hip", "prefix_decode.hip", "rope_store.hip", "chunk_attention.hip",
+           "cache_load.hip")
 ARCH = os.environ.get("TQ4_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

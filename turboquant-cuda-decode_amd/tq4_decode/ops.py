@@ -822,6 +822,82 @@ def chunk_attention(query, rotation_t, kv_cache, block_table, seq_lens, query_st
     return (ws.out, ws.lse) if return_lse else ws.out
 
 
+def cache_load(kv_cache, slot_mapping, rotation_t, centroids, *, key_bits=4, value_bits=4, layout="soa",
+               dtype=torch.bfloat16, key=None, value=None):
+    """Keys and values ``[N, Hk, D]`` read back from the slots ``slot_mapping [N]`` (int32) of the cache, as the values
+    that their codes stand for; returns ``(key, value)``, new tensors of ``dtype`` where none are given.
+
+    ``rotation_t`` is the writer's ``PiT``: keys come back in the basis that they were given in; None leaves them
+    rotated (``q @ PiT`` attends to those).  ``centroids``: the 2^``key_bits`` of the codebook.  FP8 keys (``key_bits=8``) take neither.
+    A negative slot, or one past the cache, gives zeros.  Presets, layouts and block sizes as the writers'
+    (``store``, ``store_preset``, ``store_fp8``, ``rope_store``).
+    """
+    fp8 = key_bits == 8
+    if (key_bits, value_bits) not in PRESETS + ((8, 4),):
+        raise RuntimeError(f"key/value bits must be one of {PRESETS + ((8, 4),)}")
+    slot = slot_bytes_fp8(HEAD_DIM) if fp8 else slot_bytes_preset(HEAD_DIM, key_bits, value_bits)
+    bs, Hk, stride, lid = _cache_geometry(kv_cache, slot, layout, " (FP8 keys)" if fp8 else "")
+    _check_tensor(slot_mapping, "slot_mapping", torch.int32)
+    _require(slot_mapping.dim() == 1 and slot_mapping.size(0) > 0, "slot_mapping must be [N], N > 0")
+    _require(dtype in DTYPES, "dtype must be float32, bfloat16 or float16")
+    N = slot_mapping.size(0)
+    shape = (N, Hk, HEAD_DIM)
+    key = torch.empty(shape, dtype=dtype, device=kv_cache.device) if key is None else key
+    value = torch.empty(shape, dtype=key.dtype, device=kv_cache.device) if value is None else value
+    _require(key.dtype in DTYPES and key.dtype == value.dtype, "key and value must have one floating type")
+    for t, name in ((key, "key"), (value, "value")):
+        _check_tensor(t, name, key.dtype)
+        if tuple(t.shape) != shape:
+            raise RuntimeError(f"{name} must be {list(shape)}")
+    tensors = [kv_cache, slot_mapping, key, value]
+    if not fp8:
+        _check_tensor(centroids, "centroids", torch.float32)
+        if centroids.numel() != 1 << key_bits:
+            raise RuntimeError(f"{key_bits}-bit keys need {1 << key_bits} centroids")
+        tensors.append(centroids)
+        if rotation_t is not None:
+            _check_tensor(rotation_t, "rotation_t", torch.float32)
+            _require(tuple(rotation_t.shape) == (HEAD_DIM, HEAD_DIM), _ROTATION_SHAPE)
+            tensors.append(rotation_t)
+    _require(_same_device(*tensors), "all tensors must be on the same device")
+    with _on_device(kv_cache.device):
+        rc = _lib.load().tq4_cache_load(
+            kv_cache.data_ptr(), slot_mapping.data_ptr(), None if fp8 or rotation_t is None else rotation_t.data_ptr(),
+            None if fp8 else centroids.data_ptr(), key.data_ptr(), value.data_ptr(), DTYPES[key.dtype], kv_cache.size(0), N,
+            Hk, HEAD_DIM, bs, stride, lid, key_bits, value_bits, _stream(kv_cache.device))
+    _lib.check(rc, "tq4_cache_load")
+    return key, value
+
+
+def merge_states(out_a, lse_a, out_b, lse_b, *, out=None, lse=None):
+    """Two attention results of the same rows over different tokens made one; returns ``(out, lse)``.
+
+    ``out_a`` and ``out_b`` ``[..., D]`` (one of fp32, bf16, fp16), ``lse_a`` and ``lse_b`` fp32 ``[...]``, all contiguous:
+    ``lse = log(exp(lse_a) + exp(lse_b))``, ``out`` their mean with weights ``exp(lse_a - lse)`` and ``exp(lse_b - lse)``.
+    A result over no tokens (LSE -inf) counts as nothing, whatever its rows hold; two of them give zeros and -inf.
+    ``out`` and ``lse`` are new tensors where none are given, and may be an input.
+    """
+    _require(out_a.is_cuda and out_a.dtype in DTYPES and out_a.dim() >= 1 and out_a.size(-1) == HEAD_DIM,
+             f"out_a must be [..., {HEAD_DIM}]")
+    out = torch.empty_like(out_a, memory_format=torch.contiguous_format) if out is None else out
+    lse = torch.empty_like(lse_a, memory_format=torch.contiguous_format) if lse is None else lse
+    for t, name in ((out_a, "out_a"), (out_b, "out_b"), (out, "out")):
+        _check_tensor(t, name, out_a.dtype)
+        _require(t.shape == out_a.shape, "out_a, out_b and out must have one shape")
+    for t, name in ((lse_a, "lse_a"), (lse_b, "lse_b"), (lse, "lse")):
+        _check_tensor(t, name, torch.float32)
+        _require(t.shape == out_a.shape[:-1], "lse_a, lse_b and lse must be [...] of out_a [..., D]")
+    _require(_same_device(out_a, out_b, out, lse_a, lse_b, lse), "all tensors must be on the same device")
+    if lse.numel() == 0:
+        return out, lse
+    with _on_device(out_a.device):
+        rc = _lib.load().tq4_merge_states(out_a.data_ptr(), lse_a.data_ptr(), out_b.data_ptr(), lse_b.data_ptr(),
+                                          out.data_ptr(), DTYPES[out_a.dtype], lse.data_ptr(), lse.numel(), HEAD_DIM,
+                                          _stream(out_a.device))
+    _lib.check(rc, "tq4_merge_states")
+    return out, lse
+
+
 def _buffer_view(buf, shape, dtype):
     """``buf`` cut to ``shape`` (leading sub-block) when it fits and stays contiguous."""
     if buf is None or buf.dtype != dtype or buf.dim() != len(shape):
