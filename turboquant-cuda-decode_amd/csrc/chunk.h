@@ -228,7 +228,11 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
 
 // LDS tiles as prefix.h's: K (hi, and lo) in rows of a token, V^T in rows of a dim.
 constexpr int kKRow = prefix::kKRow;
-template <int WR, int WT, int KT, int BUFS, bool KF8, bool FINE> struct Lds {
+template <bool V3> constexpr float kMiddle = prefix::kMiddle<V3>;
+constexpr float kShrink = 1.f / 32.f;   // 15 codes of the largest f16 scale and the largest zero are below 2^20
+constexpr int kAhead = 4;               // operands that are read ahead of their products
+
+template <int WR, int WT, int KT, int BUFS, bool KF8, bool FINE> struct Form {
     static constexpr int threads = 64 * WR * WT;
     static constexpr int vrow = 2 * KT + 16;
     static constexpr int klo = KT * kKRow;  // bytes: K hi at 0, K lo, V^T
@@ -238,216 +242,266 @@ template <int WR, int WT, int KT, int BUFS, bool KF8, bool FINE> struct Lds {
     static constexpr int bytes = BUFS * tile > join ? BUFS * tile : join;
     static constexpr bool halves = threads == 8 * KT;  // threads decode K or V, else both
     static constexpr int units = halves ? 1 : 4 * KT / threads;  // of either that a thread decodes
-    static constexpr int v_waves = halves ? WR * WT / 2 : WR * WT;
     static constexpr int sub = KT / (32 * WT);         // products of 32 tokens per wave and tile
     static_assert(halves || (4 * KT) % threads == 0, "whole units");
 };
-// What the softmax takes of a tile's tokens.  v: V's scale and its value at the middle code (FINE); special: per wave
-// that decodes V, whether a token's `fix` is not 1: the weight's factor where V is stored smaller, NaN where V is not finite.
-template <int KT, int V_WAVES, bool KF8, bool FINE> struct alignas(16) Factors {
+// What the softmax takes of a tile's tokens.  v: V's scale and its value at the middle code (FINE).  special: of each 16
+// tokens (those that one wave decodes at a time), whether their `fix` may differ from 1: the weight's factor where V is
+// stored smaller, NaN where V is not finite.
+template <int KT, bool KF8, bool FINE> struct alignas(16) Factors {
     float norm[KF8 ? 4 : KT];
-    float2 v[FINE ? KT : 1];
+    float2 v[FINE ? KT : 2];
     float fix[KT];
-    uint32_t special[V_WAVES];
+    uint32_t special[KT / 16];
 };
-template <bool V3> constexpr float kMiddle = prefix::kMiddle<V3>;
-constexpr float kShrink = 1.f / 32.f;   // 15 codes of the largest f16 scale and the largest zero are below 2^20
-constexpr float kMostV = 60000.f;
+// The codes' table: pairs of centroids as f16, with their low parts (FINE), or with the sum of their squares (AoS slots,
+// which hold the raw norm).  It has LDS address 0, so that a lookup's address is the byte of codes, shifted.
+template <bool KF8, bool KB3, bool WIDE> struct Table {
+    using Entry = std::conditional_t<WIDE, uint2, uint32_t>;
+    static constexpr int entries = KF8 ? 4 : KB3 ? 64 : 256;
+};
 
-struct Raw {
-    uint4 a, b;
+// Unit u of K: token u / 4 of the tile, dims 32 (u % 4) .. +31; of V: tokens 4 (u / 16) .. +3, dims 8 (u % 16) .. +7.  The 64
+// units that a wave decodes at a time are those of 16 tokens, which lie in one block: where they begin is the wave's, a
+// lane's place in them the same in every tile, and a load takes one address of each.
+template <int LAYOUT, bool KF8, bool KB3, bool V3> struct Codes {
+    static constexpr int rec = xdl::record_bytes<LAYOUT, KF8, KB3, V3>(), v0 = xdl::v_offset<LAYOUT, KF8, KB3>();
+    static constexpr int kbytes = KF8 ? kHeadDim : KB3 ? xdl::kK3Bytes : kHalfD, vbytes = V3 ? xdl::kK3Bytes : kHalfD;
+    static constexpr int nf = KF8 ? 2 : 3;
 };
-// Unit u of K: token u / 4, dims 32 (u % 4) .. +31; b: the norm (FP8 keys: the second half of the bytes).
+struct Raw {
+    uint4 a, b;  // codes; K: norm (FP8 keys: the codes' second half), V: scales and zeros
+};
+// The wave's 16 tokens: their records of the kv-head, and (SoA) its scalars.
+struct Place {
+    const uint8_t *data, *meta;
+};
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void load_k(Raw &r, const prefix::Args &a, int kvh, int t, int blk, int u) {
-    using R = prefix::Record<LAYOUT, KF8, KB3, V3>;
-    const R at(a, kvh, t, blk);
-    const uint8_t *p = at.data + (u & 3) * (R::kbytes / 4);
+__device__ __forceinline__ Place place_of(const Args &a, int kvh, int blk, int within) {
+    using C = Codes<LAYOUT, KF8, KB3, V3>;
+    const uint8_t *b = a.cache + (uint64_t)(uint32_t)blk * (uint32_t)a.block_stride;
+    const int bs = 1 << a.block_size_log2;
+    return Place{b + (uint32_t)(within * a.slot_pos + kvh * a.slot_head),
+                 LAYOUT == 0 ? b + (uint32_t)(bs * a.num_kv_heads * C::rec + 2 * (kvh * C::nf * bs + within)) : nullptr};
+}
+template <int LAYOUT, bool KF8, bool KB3, bool V3>
+__device__ __forceinline__ void load_k(Raw &r, const Args &a, const Place &at, int lane) {
+    using C = Codes<LAYOUT, KF8, KB3, V3>;
+    const uint32_t token = (uint32_t)(lane >> 2) * (uint32_t)a.slot_pos, part = token + (lane & 3) * (C::kbytes / 4);
     if constexpr (KB3) {
-        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(p);
+        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(at.data + part);
         r.a = uint4{w[0], w[1], w[2], 0u};
     } else {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(p);
+        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part);
         r.a = uint4{w[0], w[1], w[2], w[3]};
     }
     if constexpr (KF8) {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(p + 16);
+        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part + 16);
         r.b = uint4{w[0], w[1], w[2], w[3]};
+    } else if constexpr (LAYOUT == 0) {
+        r.b.x = *reinterpret_cast<const uint16_t *>(at.meta + 2u * (lane >> 2));
     } else {
-        r.b.x = LAYOUT == 0 ? at.meta[0] : *reinterpret_cast<const uint16_t *>(at.data + R::kbytes);
+        r.b.x = *reinterpret_cast<const uint16_t *>(at.data + token + C::kbytes);
     }
 }
-// Unit u of V: tokens t = 4 (u / 16) .. +3 (one block), dims 8 (u % 16) .. +7; b: their scales and zeros.
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void load_v(Raw &r, const prefix::Args &a, int kvh, int t, int blk, int u) {
-    using R = prefix::Record<LAYOUT, KF8, KB3, V3>;
-    const R at(a, kvh, t, blk);
-    const uint8_t *p = at.data + R::v0 + (V3 ? 3 : 4) * (u & 15);
-    auto token = [&](int i) { return *reinterpret_cast<const prefix::u32a1 *>(p + (int64_t)i * at.pos); };
+__device__ __forceinline__ void load_v(Raw &r, const Args &a, const Place &at, int lane) {
+    using C = Codes<LAYOUT, KF8, KB3, V3>;
+    const uint32_t quad = (uint32_t)(lane >> 4) * (uint32_t)(4 * a.slot_pos), part = quad + C::v0 + (V3 ? 3 : 4) * (lane & 15);
+    auto token = [&](int i) { return *reinterpret_cast<const prefix::u32a1 *>(at.data + (uint32_t)(i * a.slot_pos) + part); };
     r.a = uint4{token(0), token(1), token(2), token(3)};
     if constexpr (LAYOUT == 0) {
-        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(at.meta + (R::nf - 2) * at.bs);
-        const u32x2a8 z = *reinterpret_cast<const u32x2a8 *>(at.meta + (R::nf - 1) * at.bs);
+        const uint8_t *m = at.meta + (uint32_t)((C::nf - 2) * 2 << a.block_size_log2);
+        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(m + 8u * (lane >> 4));
+        const u32x2a8 z = *reinterpret_cast<const u32x2a8 *>(m + (2u << a.block_size_log2) + 8u * (lane >> 4));
         r.b = uint4{s[0], s[1], z[0], z[1]};
     } else {
         auto both = [&](int i) {
-            return *reinterpret_cast<const prefix::u32a2 *>(at.data + (int64_t)i * at.pos + R::v0 + R::vbytes);
+            return *reinterpret_cast<const prefix::u32a2 *>(at.data + (uint32_t)(i * a.slot_pos + C::v0 + C::vbytes) + quad);
         };
         r.b = uint4{both(0), both(1), both(2), both(3)};
     }
 }
 
-template <int LAYOUT, bool KF8, bool KB3, bool FINE, class L, class F>
-__device__ __forceinline__ void store_k(const Raw &r, unsigned char *khi, unsigned char *klo, F &factors, const uint2 *lut2,
-                                        const uint32_t *lut, int u) {
-    const int t = u >> 2, j = u & 3, at = t * kKRow + 64 * j;
-    uint32_t e[16], lo[16];
-    if constexpr (KF8) {
-        const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+// A unit of K into LDS, in four steps (a quarter of its codes looked up, the quarter before written); the fifth
+// writes the last.
+template <int LAYOUT, bool KF8, bool KB3, bool FINE> struct KUnit {
+    static constexpr bool WIDE = FINE || LAYOUT == 1;
+    uint32_t hi[2][4], lo[2][4];
+    float sq = 0.f, hl = 0.f;
+    __device__ __forceinline__ void look_up(const Raw &r, const typename Table<KF8, KB3, WIDE>::Entry *table, int q) {
+        if constexpr (KF8) {
+            const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-            const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-            e[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));  // (exact)
-            e[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
-        }
-    } else {
-        const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-        float sq = 0.f;
-#pragma unroll
-        for (int b = 0; b < 16; ++b) {
-            uint32_t v;
-            if constexpr (KB3) {
-                const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
-                v = w[wi] >> sh;
-                if (sh > 26)
-                    v |= w[wi + 1] << (32 - sh);
-                v &= 63u;
-            } else {
-                v = (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
+            for (int i = 0; i < 2; ++i) {
+                const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * q + i], false);
+                const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * q + i], true);
+                hi[q & 1][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));  // (exact)
+                hi[q & 1][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
             }
-            if constexpr (FINE || LAYOUT == 1) {
-                const uint2 c = lut2[v];
-                e[b] = c.x;
-                lo[b] = c.y;
-            } else {
-                e[b] = lut[v];
+        } else {
+            const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = 4 * q + i;
+                uint32_t v;
+                if constexpr (KB3) {
+                    const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
+                    v = w[wi] >> sh;
+                    if (sh > 26)
+                        v |= w[wi + 1] << (32 - sh);
+                    v &= 63u;
+                } else {
+                    v = (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
+                }
+                if constexpr (WIDE) {
+                    const uint2 c = table[v];
+                    hi[q & 1][i] = c.x;
+                    lo[q & 1][i] = c.y;
+                } else {
+                    hi[q & 1][i] = table[v];
+                }
             }
         }
-        float n = half_bits_to_float(r.b.x);
-        if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction (h.h + 2 h.l)
-            float hl = 0.f;
-#pragma unroll
-            for (int b = 0; b < 16; ++b) {
-                const auto h = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), e[b]);
-                const auto l = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), lo[b]);
-                sq = __builtin_amdgcn_fdot2(h, h, sq, false);
-                hl = __builtin_amdgcn_fdot2(h, l, hl, false);
-            }
-            sq = fmaf(2.f, hl, sq);
-            sq += xdl::dppf<0xB1>(sq);  // quad_perm [1, 0, 3, 2]: the token's four threads
-            sq += xdl::dppf<0x4E>(sq);  // quad_perm [2, 3, 0, 1]
-            n *= __builtin_amdgcn_rsqf(sq + 1e-16f);
-        }
-        if (j == 0)
-            factors.norm[t] = n;
-        if constexpr (FINE)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<uint4 *>(klo + at + 16 * q) = uint4{lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]};
     }
+    // `at`: the unit's place among K's rows
+    __device__ __forceinline__ void write(unsigned char *khi, unsigned char *klo, int at, int q) {
+        const uint32_t(&e)[4] = hi[q & 1], (&f)[4] = lo[q & 1];
+        *reinterpret_cast<uint4 *>(khi + at + 16 * q) = uint4{e[0], e[1], e[2], e[3]};
+        if constexpr (FINE && !KF8)
+            *reinterpret_cast<uint4 *>(klo + at + 16 * q) = uint4{f[0], f[1], f[2], f[3]};
+        if constexpr (LAYOUT == 1 && !KF8)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4 *>(khi + at + 16 * q) = uint4{e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
-}
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (FINE) {  // h.h + 2 h.l
+                    const auto h = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), e[i]);
+                    const auto l = __builtin_bit_cast(__fp16 __attribute__((ext_vector_type(2))), f[i]);
+                    sq = __builtin_amdgcn_fdot2(h, h, sq, false);
+                    hl = __builtin_amdgcn_fdot2(h, l, hl, false);
+                } else {
+                    sq += xdl::bitsf(f[i]);
+                }
+            }
+    }
+    // (every thread of a token writes its norm: the same one)
+    template <class F> __device__ __forceinline__ void write_norm(const Raw &r, F &factors, int u) {
+        if constexpr (!KF8) {
+            float n = half_bits_to_float(r.b.x);
+            if constexpr (LAYOUT == 1) {  // the raw norm over the norm of the decoded direction
+                sq = fmaf(2.f, hl, sq);
+                sq += xdl::dppf<0xB1>(sq);  // quad_perm [1, 0, 3, 2]: the token's four threads
+                sq += xdl::dppf<0x4E>(sq);  // quad_perm [2, 3, 0, 1]
+                n *= __builtin_amdgcn_rsqf(sq + 1e-16f);
+            }
+            factors.norm[u >> 2] = n;
+        }
+    }
+};
 
-// Returns whether a token's `fix` is not 1.  `valid`: tokens of the unit that the sequence has (4, or fewer at its end:
-// the others' bytes may hold anything, and count as zeros).
-template <int LAYOUT, bool V3, bool FINE, int VROW, class F>
-__device__ __forceinline__ bool store_v(const Raw &r, unsigned char *vtile, F &factors, int u, int valid) {
-    const int dg = u & 15, quad = u >> 4;
-    const uint32_t v[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-    // (scale | zero << 16) of each token
-    uint32_t sz[4];
-    if constexpr (LAYOUT == 0) {
-        sz[0] = __builtin_amdgcn_perm(r.b.z, r.b.x, 0x05040100u);
-        sz[1] = __builtin_amdgcn_perm(r.b.z, r.b.x, 0x07060302u);
-        sz[2] = __builtin_amdgcn_perm(r.b.w, r.b.y, 0x05040100u);
-        sz[3] = __builtin_amdgcn_perm(r.b.w, r.b.y, 0x07060302u);
-    } else {
-        sz[0] = r.b.x;
-        sz[1] = r.b.y;
-        sz[2] = r.b.z;
-        sz[3] = r.b.w;
-    }
-    float scale[4], zero[4], most = 0.f;
+// A unit of V into LDS: begin() takes its scalars, write(m) dims 2 m and 2 m + 1 of it.
+template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
+    half2v s01, s23, z01, z23;
+    // `valid`: tokens of the unit that the sequence has (4 or more: all; the others' bytes may hold anything, and count as
+    // zeros).  (Of a wave, together.)
+    template <class F> __device__ __forceinline__ void begin(const Raw &r, F &factors, int u, bool cut, int valid) {
+        uint32_t s[2], z[2];  // scales and zeros of tokens (0, 1) and (2, 3)
+        if constexpr (LAYOUT == 0) {
+            s[0] = r.b.x;
+            s[1] = r.b.y;
+            z[0] = r.b.z;
+            z[1] = r.b.w;
+        } else {
+            s[0] = __builtin_amdgcn_perm(r.b.y, r.b.x, 0x05040100u);
+            s[1] = __builtin_amdgcn_perm(r.b.w, r.b.z, 0x05040100u);
+            z[0] = __builtin_amdgcn_perm(r.b.y, r.b.x, 0x07060302u);
+            z[1] = __builtin_amdgcn_perm(r.b.w, r.b.z, 0x07060302u);
+        }
+        if (cut) {
+            const uint32_t m0 = valid <= 0 ? 0u : valid == 1 ? 0xFFFFu : 0xFFFFFFFFu, m1 = valid <= 2 ? 0u : valid == 3 ? 0xFFFFu : 0xFFFFFFFFu;
+            s[0] &= m0;
+            s[1] &= m1;
+            z[0] &= m0;
+            z[1] &= m1;
+        }
+        // magnitudes as whole numbers: scales of 2048 or zeros of 16384 and more might pass f16's range together
+        // (FINE: scales of 128 and more times weights); NaN and infinities are above those
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7FFF7FFFu); };
+        const u16x2 ms = __builtin_elementwise_max(mag(s[0]), mag(s[1])), mz = __builtin_elementwise_max(mag(z[0]), mag(z[1]));
+        const uint32_t top_s = ms[0] > ms[1] ? ms[0] : ms[1], top_z = mz[0] > mz[1] ? mz[0] : mz[1];
+        const bool special = __any(top_s >= (FINE ? 0x5800u : 0x6800u) || top_z >= (FINE ? 0x7C00u : 0x7400u));
+        float scale[4], zero[4];
+        if (FINE || special)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        sz[i] = i < valid ? sz[i] : 0u;
-        scale[i] = half_bits_to_float(sz[i]);
-        zero[i] = half_bits_to_float(sz[i] >> 16);
-        // (a NaN is passed over by no comparison below: !(x <= most))
-        const float top = fmaf(15.f, fabsf(scale[i]), fabsf(zero[i]));
-        most = top <= most ? most : top;
-    }
-    const bool special = !(most <= (FINE ? 128.f * 15.f : kMostV));
-    float fix[4] = {1.f, 1.f, 1.f, 1.f};
-    if (special)
+            for (int i = 0; i < 4; ++i) {
+                scale[i] = half_bits_to_float(s[i >> 1] >> (16 * (i & 1)));
+                zero[i] = half_bits_to_float(z[i >> 1] >> (16 * (i & 1)));
+            }
+        if (special) {
+            float fix[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float top = fmaf(15.f, fabsf(scale[i]), fabsf(zero[i]));
-            if (!(top < __builtin_inff())) {
-                fix[i] = __builtin_nanf("");
-                scale[i] = zero[i] = 0.f;
-            } else if (!FINE && top > kMostV) {
-                fix[i] = 1.f / kShrink;
-                scale[i] *= kShrink;
-                zero[i] *= kShrink;
+            for (int i = 0; i < 4; ++i) {
+                const float top = fmaf(15.f, fabsf(scale[i]), fabsf(zero[i]));
+                fix[i] = 1.f;
+                if (!(top < __builtin_inff())) {
+                    fix[i] = __builtin_nanf("");
+                    scale[i] = zero[i] = 0.f;
+                } else if (!FINE && top > 60000.f) {
+                    fix[i] = 1.f / kShrink;
+                    scale[i] *= kShrink;
+                    zero[i] *= kShrink;
+                }
+            }
+            *reinterpret_cast<float4 *>(factors.fix + 4 * (u >> 4)) = float4{fix[0], fix[1], fix[2], fix[3]};
+            if constexpr (!FINE) {
+                auto pair = [](float x, float y) { return prefix::as_u32(half2v{(_Float16)x, (_Float16)y}); };
+                s[0] = pair(scale[0], scale[1]);
+                s[1] = pair(scale[2], scale[3]);
+                z[0] = pair(zero[0], zero[1]);
+                z[1] = pair(zero[2], zero[3]);
             }
         }
-    const int t0 = 4 * quad;
-    if (dg == 0) {
-        *reinterpret_cast<float4 *>(factors.fix + t0) = float4{fix[0], fix[1], fix[2], fix[3]};
-        if constexpr (FINE)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                factors.v[t0 + i] = float2{scale[i], fmaf(scale[i], kMiddle<V3>, zero[i])};
+        factors.special[u >> 6] = special;
+        if constexpr (FINE) {
+            float4 *to = reinterpret_cast<float4 *>(factors.v + 4 * (u >> 4));
+            auto mid = [&](int i) { return fmaf(scale[i], kMiddle<V3>, zero[i]); };
+            to[0] = float4{scale[0], mid(0), scale[1], mid(1)};
+            to[1] = float4{scale[2], mid(2), scale[3], mid(3)};
+        } else {
+            s01 = prefix::as_half2(s[0]);
+            s23 = prefix::as_half2(s[1]);
+            z01 = prefix::as_half2(z[0]);
+            z23 = prefix::as_half2(z[1]);
+        }
     }
     // codes to f16: into the significand of 1024, then less 1024 (FINE: less 1024 and the middle code)
-    const half2v k0 = prefix::splat((_Float16)(1024.f + (FINE ? kMiddle<V3> : 0.f)));
-    half2v s01, s23, z01, z23;
-    if constexpr (!FINE) {
-        s01 = half2v{(_Float16)scale[0], (_Float16)scale[1]};
-        s23 = half2v{(_Float16)scale[2], (_Float16)scale[3]};
-        z01 = half2v{(_Float16)zero[0], (_Float16)zero[1]};
-        z23 = half2v{(_Float16)zero[2], (_Float16)zero[3]};
-    }
-    unsigned char *to = vtile + dg * VROW + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1);
-    auto put = [&](int i, uint32_t c01, uint32_t c23) {
-        half2v x = prefix::as_half2(c01 | 0x64006400u) - k0, y = prefix::as_half2(c23 | 0x64006400u) - k0;
-        if constexpr (!FINE) {
-            x = __builtin_elementwise_fma(x, s01, z01);
-            y = __builtin_elementwise_fma(y, s23, z23);
-        }
-        *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{prefix::as_u32(x), prefix::as_u32(y)};
-    };
-    if constexpr (V3) {
+    __device__ __forceinline__ void write(const Raw &r, unsigned char *to, int m) {
+        const half2v k0 = prefix::splat((_Float16)(1024.f + (FINE ? kMiddle<V3> : 0.f)));
+        uint32_t magic = 0x64006400u;
+        asm("" : "+v"(magic));
+        auto put = [&](int i, uint32_t c01, uint32_t c23, uint32_t mask) {
+            half2v x = prefix::as_half2((c01 & mask) | magic) - k0, y = prefix::as_half2((c23 & mask) | magic) - k0;
+            if constexpr (!FINE) {
+                x = __builtin_elementwise_fma(x, s01, z01);
+                y = __builtin_elementwise_fma(y, s23, z23);
+            }
+            *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{prefix::as_u32(x), prefix::as_u32(y)};
+        };
+        const uint32_t v[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+        if constexpr (V3) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            auto code = [&](int t) { return (v[t] >> (3 * i)) & 7u; };
-            put(i, code(0) | (code(1) << 16), code(2) | (code(3) << 16));
-        }
-    } else {
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
+            for (int i = 2 * m; i < 2 * m + 2; ++i) {
+                auto pair = [&](int t) { return ((v[t] >> (3 * i)) & 7u) | (((v[t + 1] >> (3 * i)) & 7u) << 16); };
+                put(i, pair(0), pair(2), 0xFFFFFFFFu);
+            }
+        } else {
             const uint32_t sel = (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u;
             const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel), p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
-            put(2 * m, p01 & 0x000F000Fu, p23 & 0x000F000Fu);
-            put(2 * m + 1, (p01 >> 4) & 0x000F000Fu, (p23 >> 4) & 0x000F000Fu);
+            put(2 * m, p01, p23, 0x000F000Fu);
+            put(2 * m + 1, p01 >> 4, p23 >> 4, 0x000F000Fu);
         }
     }
-    return special;
-}
+};
 
 // ---- The product -----------------------------------------------------------------------------
 
@@ -467,14 +521,18 @@ template <typename T> __device__ __forceinline__ void put8(void *out, int64_t at
 template <int LAYOUT, bool KF8, bool KB3, bool V3, int WR, int WT, int KT, int BUFS, bool FINE>
 __global__ __launch_bounds__(64 * WR * WT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void chunk_kernel(const Args a) {
-    using S = Lds<WR, WT, KT, BUFS, KF8, FINE>;
-    using F = Factors<KT, S::v_waves, KF8, FINE>;
-    constexpr bool LUT2 = !KF8 && (FINE || LAYOUT == 1);
-    constexpr int kEntries = KB3 ? 64 : 256;
-    __shared__ __align__(16) unsigned char mem[S::bytes];
-    __shared__ __align__(16) F factors[BUFS];
-    __shared__ __align__(16) uint2 lut2[LUT2 ? kEntries : 1];
-    __shared__ __align__(16) uint32_t lut[KF8 || LUT2 ? 4 : kEntries];
+    using S = Form<WR, WT, KT, BUFS, KF8, FINE>;
+    using F = Factors<KT, KF8, FINE>;
+    using K = KUnit<LAYOUT, KF8, KB3, FINE>;
+    using V = VUnit<LAYOUT, V3, FINE, S::vrow>;
+    using T = Table<KF8, KB3, K::WIDE>;
+    __shared__ struct alignas(16) {
+        typename T::Entry table[T::entries];
+        F factors[BUFS];
+        alignas(16) unsigned char mem[S::bytes];
+    } lds;
+    auto &factors = lds.factors;
+    unsigned char *mem = lds.mem;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, h = lane >> 5, wr = w % WR, wt = w / WR;
     // neighbours in the list read the same tokens: eight runs of it, one per XCD (workgroup i runs on XCD i % 8)
@@ -486,23 +544,19 @@ void chunk_kernel(const Args a) {
     if (at.b >= a.batch || (same_tile(at, end) && at.at == end.at))
         return;
     if constexpr (!KF8)
-        for (int e = tid; e < kEntries; e += S::threads) {
-            const uint32_t x = xdl::split_f16(a.centroids[KB3 ? e & 7 : e & 15]), z = xdl::split_f16(a.centroids[KB3 ? e >> 3 : e >> 4]);
-            if constexpr (LUT2)
-                lut2[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
-            else {
-                const half2v both{(_Float16)a.centroids[KB3 ? e & 7 : e & 15], (_Float16)a.centroids[KB3 ? e >> 3 : e >> 4]};
-                lut[e] = prefix::as_u32(both);
+        for (int e = tid; e < T::entries; e += S::threads) {
+            const float c0 = a.centroids[KB3 ? e & 7 : e & 15], c1 = a.centroids[KB3 ? e >> 3 : e >> 4];
+            if constexpr (FINE) {
+                const uint32_t x = xdl::split_f16(c0), z = xdl::split_f16(c1);
+                lds.table[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
+            } else {
+                const uint32_t both = prefix::as_u32(half2v{(_Float16)c0, (_Float16)c1});
+                if constexpr (LAYOUT == 1)
+                    lds.table[e] = uint2{both, xdl::fbits(fmaf(c0, c0, c1 * c1))};
+                else
+                    lds.table[e] = both;
             }
         }
-    prefix::Args rec{};  // what the records' addresses need
-    rec.cache = a.cache;
-    rec.block_stride = a.block_stride;
-    rec.num_kv_heads = a.num_kv_heads;
-    rec.block_size_log2 = a.block_size_log2;
-    rec.slot_pos = a.slot_pos;
-    rec.slot_head = a.slot_head;
-
     const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
     const int group = a.shape.group;
     xdl::lds_barrier();  // the table
@@ -517,66 +571,66 @@ void chunk_kernel(const Args a) {
         const int n_tiles = tile1 - tile0;
         const int32_t *pages = a.pages + (int64_t)at.b * a.table_width;
 
-        auto unit = [&](int k) {
-            int u = S::halves ? tid & (4 * KT - 1) : tid + k * S::threads;
-            asm volatile("" : "+v"(u));
-            return u;
-        };
-        auto first_of = [&](int i) {  // the first token of tile i of this stretch (past its end: of the last one)
+        auto first_of = [&](int i) __attribute__((always_inline)) {  // the first token of tile i of this stretch (past its end: of the last one)
             const int p = tile0 + min(i, n_tiles - 1);
             return KT * (p < vis.head ? p : p + vis.skip);
         };
-        auto k_tok = [&](int t0, int u) { return min(t0 + (u >> 2), seq.len - 1); };
-        auto v_tok = [&](int t0, int u) { return min(t0 + 4 * (u >> 4), (seq.len - 1) & ~3); };
         constexpr int U = S::units;
-        int kblk[U], vblk[U];
+        auto unit = [&](int k) __attribute__((always_inline)) { return S::halves ? tid & (4 * KT - 1) : tid + k * S::threads; };
         Raw rk[U], rv_own[U];
         Raw(&rv)[U] = S::halves ? rk : rv_own;
-        int(&vb)[U] = S::halves ? kblk : vblk;
-        auto read_pages = [&](int i) {
-            const int t0 = first_of(i);
+        int blk[U];
+        // the first of the 16 tokens of the wave's units, in the tile
+        auto group_of = [&](int k) __attribute__((always_inline)) { return 16 * (S::halves ? w % (WR * WT / 2) : w + k * WR * WT); };
+        // (no block past the sequence's last one is asked for; in that, any token is in bounds.  A vector load, though
+        // every lane's is the same: a scalar one in flight makes every wait for LDS a wait for it)
+        auto read_pages = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const int u = unit(k);
-                if (does_k)
-                    kblk[k] = pages[k_tok(t0, u) >> a.block_size_log2];
-                if (does_v)
-                    vb[k] = pages[v_tok(t0, u) >> a.block_size_log2];
+                uint32_t at = (uint32_t)min(first_of(i) + group_of(k), seq.len - 1) >> a.block_size_log2;
+                asm("" : "+v"(at));
+                blk[k] = pages[at];
             }
         };
-        auto load = [&](int i) {
-            const int t0 = first_of(i);
+        auto load = [&](int i, bool does_k, bool does_v) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const int u = unit(k);
+                const Place at = place_of<LAYOUT, KF8, KB3, V3>(a, kvh, __builtin_amdgcn_readfirstlane(blk[k]), (first_of(i) + group_of(k)) & ((1 << a.block_size_log2) - 1));
                 if (does_k)
-                    load_k<LAYOUT, KF8, KB3, V3>(rk[k], rec, kvh, k_tok(t0, u), kblk[k], u);
+                    load_k<LAYOUT, KF8, KB3, V3>(rk[k], a, at, lane);
                 if (does_v)
-                    load_v<LAYOUT, KF8, KB3, V3>(rv[k], rec, kvh, v_tok(t0, u), vb[k], u);
+                    load_v<LAYOUT, KF8, KB3, V3>(rv[k], a, at, lane);
             }
         };
-        auto store = [&](int i) {
-            const int t0 = first_of(i);
+        // A tile's decoding, in steps 0 .. kSteps - 1; `k`, `v`: of which.
+        constexpr int kSteps = 5 * U;
+        K kdec[U];
+        V vdec[U];
+        auto decode = [&](int i, int step, auto k_too, auto v_too) __attribute__((always_inline)) {
             unsigned char *m = mem + (i % BUFS) * S::tile;
-            F &f = factors[i % BUFS];
-            bool special = false;
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const int u = unit(k);
-                if (does_k)
-                    store_k<LAYOUT, KF8, KB3, FINE, S>(rk[k], m, m + S::klo, f, lut2, lut, u);
-                if (does_v)
-                    special |= store_v<LAYOUT, V3, FINE, S::vrow>(rv[k], m + S::v, f, u, seq.len - (t0 + 4 * (u >> 4)));
+            const int x = step / 5, q = step % 5, u = unit(x);
+            if constexpr (k_too) {
+                const int at = (u >> 2) * kKRow + 64 * (u & 3);
+                if (q < 4)
+                    kdec[x].look_up(rk[x], lds.table, q);
+                if (q > 0)
+                    kdec[x].write(m, m + S::klo, at, q - 1);
+                if (q == 4)
+                    kdec[x].write_norm(rk[x], factors[i % BUFS], u);
+                if (q == 4)
+                    kdec[x].sq = kdec[x].hl = 0.f;
             }
-            if (does_v) {
-                const bool any = __any(special);
-                if (lane == 0)
-                    f.special[S::halves ? w - WR * WT / 2 : w] = any;
+            if constexpr (v_too) {
+                const int t = first_of(i) + 4 * (u >> 4);
+                if (q == 0)
+                    vdec[x].begin(rv[x], factors[i % BUFS], u, first_of(i) + KT > seq.len, seq.len - t);
+                else
+                    vdec[x].write(rv[x], m + S::v + (u & 15) * S::vrow + 16 * (2 * (u >> 6) + ((u >> 4) & 1)) + 8 * ((u >> 5) & 1), q - 1);
             }
         };
         if (n_tiles > 0) {
             read_pages(0);
-            load(0);
+            load(0, does_k, does_v);
             read_pages(1);
         }
 
@@ -592,7 +646,14 @@ void chunk_kernel(const Args a) {
                 q_lo[k] = *reinterpret_cast<const half8 *>(a.q_lo + q_row * kHeadDim + 16 * k + 8 * h);
         }
         const float fac = a.q_factor[q_row];
-        const bool scaled = KF8 || __any(fac != 1.f);
+        // (arrived before the loop: a wait inside it would wait for the tiles' loads too)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            q_hi[k] = prefix::pinned(q_hi[k]);
+            if constexpr (FINE && !KF8)
+                q_lo[k] = prefix::pinned(q_lo[k]);
+        }
+        const bool scaled = !KF8 && __any(fac != 1.f);
         const int limit = limit_of(a.shape, seq, row_in), from = a.shape.window ? limit - a.shape.window : 0;
         const int limit_lo = __builtin_amdgcn_readfirstlane(limit_of(a.shape, seq, min(wave_row, rows - 1)));
         const int limit_hi = __builtin_amdgcn_readfirstlane(limit_of(a.shape, seq, min(wave_row + 31, rows - 1)));
@@ -605,98 +666,118 @@ void chunk_kernel(const Args a) {
                 acc[d][k] = 0.f;
         float negm = __FLT_MAX__, l = 0.f, z = 0.f;  // -max in log2 units, this lane's shares of the sum and of V's middle values
 
-        auto tile = [&](int i) {
-            const unsigned char *m = mem + (i % BUFS) * S::tile;
-            const F &f = factors[i % BUFS];
-            const int t0 = first_of(i) + 32 * S::sub * wt;  // this wave's first token
-            // no row of the wave sees a token of it
-            if (t0 >= limit_hi || (a.shape.window && t0 >= a.shape.first && t0 + 32 * S::sub <= limit_lo - a.shape.window))
-                return;
-            floatx16 s[S::sub];
+        constexpr int kAtOnce = FINE ? 1 : S::sub;  // sub-tiles of 32 tokens at once
+        constexpr int kEvery = 4;                   // products between two steps of decoding
+        const unsigned char *k_at = mem + (32 * S::sub * wt + c) * kKRow + 16 * h;
+        const unsigned char *v_at = mem + S::v + c * S::vrow + 16 * (4 * S::sub * wt + h);
+        const int tok0 = 32 * S::sub * wt + 4 * h;  // s[b][k]: token tok0 + 32 b + 8 (k / 4) + k % 4 of the tile
+        std::integral_constant<bool, true> yes;
+        std::integral_constant<bool, false> no;
+
+        // Scores of sub-tiles b0 .. b0 + kAtOnce - 1 of tile i, and between their products a share of the decoding of
+        // tile j (`decodes`), whose codes are here; with the last ones the loads of the tile after it.
+        floatx16 s[kAtOnce];
+        auto scores = [&](int i, int b0, int j, auto decodes, auto k_too, auto v_too) __attribute__((always_inline)) {
+            const unsigned char *k_from = k_at + (i % BUFS) * S::tile + 32 * b0 * kKRow;
+            constexpr int N = 8 * kAtOnce, kSlots = 8 * S::sub / kEvery;  // slots for decoding in a whole tile
+            constexpr bool LO = FINE && !KF8;
+            constexpr int AHEAD = LO ? 2 : kAhead;  // (three products from one pair of reads)
+            half8 hi[AHEAD], lo[LO ? AHEAD : 1];
+            auto read = [&](int x) __attribute__((always_inline)) {
+                const unsigned char *from = k_from + 32 * (x >> 3) * kKRow + 32 * (x & 7);
+                hi[x % AHEAD] = *reinterpret_cast<const half8 *>(from);
+                if constexpr (LO)
+                    lo[x % AHEAD] = *reinterpret_cast<const half8 *>(from + S::klo);
+            };
 #pragma unroll
-            for (int b = 0; b < S::sub; ++b) {
-                const unsigned char *k_from = m + (32 * (S::sub * wt + b) + c) * kKRow + 16 * h;
+            for (int x = 0; x < AHEAD; ++x)
+                read(x);
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b)
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                     s[b][k] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const half8 hi = *reinterpret_cast<const half8 *>(k_from + 32 * k);
-                    s[b] = prefix::mfma32(hi, q_hi[k], s[b]);
-                    if constexpr (FINE && !KF8) {
-                        s[b] = prefix::mfma32(*reinterpret_cast<const half8 *>(k_from + S::klo + 32 * k), q_hi[k], s[b]);
-                        s[b] = prefix::mfma32(hi, q_lo[k], s[b]);
-                    }
+            for (int x = 0; x < N; ++x) {
+                if (decodes && x % kEvery == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int slot = (8 * b0 + x) / kEvery;
+#pragma unroll
+                    for (int y = slot * kSteps / (kSlots + 1); y < (slot + 1) * kSteps / (kSlots + 1); ++y)
+                        decode(j, y, k_too, v_too);
                 }
+                const int b = x >> 3, k = x & 7;
+                s[b] = prefix::mfma32(hi[x % AHEAD], q_hi[k], s[b]);
+                if constexpr (LO) {
+                    s[b] = prefix::mfma32(lo[x % AHEAD], q_hi[k], s[b]);
+                    s[b] = prefix::mfma32(hi[x % AHEAD], q_lo[k], s[b]);
+                }
+                if (x + AHEAD < N)
+                    read(x + AHEAD);
             }
+            if (decodes && b0 + kAtOnce == S::sub) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = kSlots * kSteps / (kSlots + 1); y < kSteps; ++y)
+                    decode(j, y, k_too, v_too);
+                load(j + 1, k_too, v_too);
+                read_pages(j + 2);
+            }
+        };
+        auto softmax_outputs = [&](int i, int b0) __attribute__((always_inline)) {
+            const F &f = factors[i % BUFS];
+            const int t0 = first_of(i) + 32 * (S::sub * wt + b0), tok = tok0 + 32 * b0;  // the first token, this lane's in the tile
             uint32_t special = 0;
 #pragma unroll
-            for (int k = 0; k < S::v_waves; ++k)
+            for (int k = 0; k < KT / 16; ++k)
                 special |= f.special[k];
             special = __builtin_amdgcn_readfirstlane(special);
-            const int tok0 = 32 * S::sub * wt + 4 * h;  // s[b][k]: token tok0 + 32 b + 8 (k / 4) + k % 4 of the tile
-            const bool masked = t0 + 32 * S::sub > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
-            float n[S::sub][16];
+            const bool masked = t0 + 32 * kAtOnce > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
+            // The scores in log2 units, less the running maximum.  That one moves when the weights' sum passes `most`: a weight
+            // is then at most 2^13, in f16's range (FINE: times a scale of up to 128; with a larger one in the tile at most 1).
+            const float most = !FINE ? 8192.f : special ? 1.f : 256.f;
+            const bool fresh = __any(negm == __FLT_MAX__);  // rows that have seen nothing yet
+            const float less = fresh ? 0.f : negm;
 #pragma unroll
-            for (int b = 0; b < S::sub; ++b)
+            for (int b = 0; b < kAtOnce; ++b) {
+                float n[16];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if constexpr (KF8) {
-#pragma unroll
-                        for (int i4 = 0; i4 < 4; ++i4)
-                            n[b][4 * k + i4] = fac;
+                        n[4 * k] = n[4 * k + 1] = n[4 * k + 2] = n[4 * k + 3] = fac;
                     } else {
-                        const float4 v = *reinterpret_cast<const float4 *>(f.norm + tok0 + 32 * b + 8 * k);
-                        n[b][4 * k] = v.x;
-                        n[b][4 * k + 1] = v.y;
-                        n[b][4 * k + 2] = v.z;
-                        n[b][4 * k + 3] = v.w;
+                        const float4 v = *reinterpret_cast<const float4 *>(f.norm + tok + 32 * b + 8 * k);
+                        n[4 * k] = v.x;
+                        n[4 * k + 1] = v.y;
+                        n[4 * k + 2] = v.z;
+                        n[4 * k + 3] = v.w;
                     }
                 }
-            if (!KF8 && scaled)
-#pragma unroll
-                for (int b = 0; b < S::sub; ++b)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        n[b][k] *= fac;
-            if (masked) {
-                const int first = first_of(i) + tok0;
-#pragma unroll
-                for (int b = 0; b < S::sub; ++b)
+                if (masked || scaled) {
+                    const int first = t0 + 4 * h;
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const int t = first + 32 * b + 8 * (k >> 2) + (k & 3);
-                        if (t >= limit || (t < from && t >= a.shape.first)) {
-                            s[b][k] = -INFINITY;
-                            n[b][k] = 1.f;
-                        }
+                        const bool out = t >= limit || (t < from && t >= a.shape.first);
+                        s[b][k] = out ? -INFINITY : s[b][k];
+                        n[k] = out ? 1.f : KF8 ? n[k] : n[k] * fac;
                     }
-            }
-            // The scores less the running maximum, in log2 units; the maximum moves only when one passes it by more than
-            // kRescaleLogX (weights stay below 2^8).
-            float x[S::sub][16], mx = -INFINITY;
-#pragma unroll
-            for (int b = 0; b < S::sub; ++b)
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                    x[b][k] = fmaf(s[b][k], n[b][k], negm);
-                    x[b][k + 1] = fmaf(s[b][k + 1], n[b][k + 1], negm);
-                    mx = prefix::max3(mx, x[b][k], x[b][k + 1]);
                 }
-            const float most = FINE && special ? 0.f : xdl::kRescaleLogX;
-            if (__any(mx > most)) {
-                float top = -INFINITY;
 #pragma unroll
-                for (int b = 0; b < S::sub; ++b)
+                for (int k = 0; k < 16; ++k)
+                    s[b][k] = fmaf(s[b][k], n[k], less);
+            }
+            // the maximum moved by what the scores are above it (`up`: where they are; first: to the tile's own)
+            auto move = [&](bool first) __attribute__((always_inline)) {
+                float mx = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        x[b][k] = s[b][k] * n[b][k];
-                        x[b][k + 1] = s[b][k + 1] * n[b][k + 1];
-                        top = prefix::max3(top, x[b][k], x[b][k + 1]);
-                    }
-                top = prefix::pair_max(top);
-                const float negm_new = top + negm > most ? -top : negm;
-                const float alpha = __builtin_amdgcn_exp2f(negm_new - negm);
+                for (int b = 0; b < kAtOnce; ++b)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2)
+                        mx = prefix::max3(mx, s[b][k], s[b][k + 1]);
+                const float top = prefix::pair_max(mx), above = first ? top + negm : top;
+                const float negm_new = above > 0.f ? (first ? -top : negm - top) : negm;
+                const float alpha = __builtin_amdgcn_exp2f(negm_new - negm), add = first ? negm_new : negm_new - negm;
                 negm = negm_new;
                 l *= alpha;
                 z *= alpha;
@@ -704,42 +785,48 @@ void chunk_kernel(const Args a) {
                 for (int d = 0; d < 4; ++d)
                     acc[d] *= alpha;
 #pragma unroll
-                for (int b = 0; b < S::sub; ++b)
+                for (int b = 0; b < kAtOnce; ++b)
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                        x[b][k] += negm;
-            }
-            half8 p[S::sub][2];
-            if (special) {
+                        s[b][k] += add;
+            };
+            if (fresh)
+                move(true);
+            half8 p[kAtOnce][2];
+            float sum = 0.f, mid = 0.f;
+            auto weights = [&]() __attribute__((always_inline)) {
+                sum = mid = 0.f;
+                if (special) {
 #pragma unroll
-                for (int b = 0; b < S::sub; ++b)
+                    for (int b = 0; b < kAtOnce; ++b)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const int t = tok0 + 32 * b + 8 * (k >> 2) + (k & 3);
-                        const float e = __builtin_amdgcn_exp2f(x[b][k]);
-                        l += e;
-                        // (a hidden token's V is nothing, whatever it holds)
-                        const float fix = x[b][k] == -INFINITY ? 0.f : f.fix[t];
-                        float y = e * fix;
-                        if constexpr (FINE) {
-                            const float2 v = f.v[t];
-                            z = fmaf(y, v.y, z);
-                            y *= v.x;
+                        for (int k = 0; k < 16; ++k) {
+                            const int t = tok + 32 * b + 8 * (k >> 2) + (k & 3);
+                            const float e = __builtin_amdgcn_exp2f(s[b][k]);
+                            sum += e;
+                            // (a hidden token's V is nothing, whatever it holds)
+                            const float fix = s[b][k] == -INFINITY ? 0.f : f.special[t >> 4] ? f.fix[t] : 1.f;
+                            float y = e * fix;
+                            if constexpr (FINE) {
+                                const float2 vv = f.v[t];
+                                mid = fmaf(y, vv.y, mid);
+                                y *= vv.x;
+                            }
+                            p[b][k >> 3][k & 7] = (_Float16)y;
                         }
-                        p[b][k >> 3][k & 7] = (_Float16)y;
-                    }
-            } else {
+                    return;
+                }
 #pragma unroll
-                for (int b = 0; b < S::sub; ++b) {
+                for (int b = 0; b < kAtOnce; ++b) {
                     if constexpr (FINE) {
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            const float4 v = *reinterpret_cast<const float4 *>(f.v + tok0 + 32 * b + 8 * (k >> 2) + (k & 3));
-                            const float e0 = __builtin_amdgcn_exp2f(x[b][k]), e1 = __builtin_amdgcn_exp2f(x[b][k + 1]);
-                            l += e0;
-                            l += e1;
-                            z = fmaf(e0, v.y, z);
-                            z = fmaf(e1, v.w, z);
+                            const float4 v = *reinterpret_cast<const float4 *>(f.v + tok + 32 * b + 8 * (k >> 2) + (k & 3));
+                            const float e0 = __builtin_amdgcn_exp2f(s[b][k]), e1 = __builtin_amdgcn_exp2f(s[b][k + 1]);
+                            sum += e0;
+                            sum += e1;
+                            mid = fmaf(e0, v.y, mid);
+                            mid = fmaf(e1, v.w, mid);
                             p[b][k >> 3][k & 7] = (_Float16)(e0 * v.x);
                             p[b][k >> 3][(k & 7) + 1] = (_Float16)(e1 * v.z);
                         }
@@ -749,53 +836,80 @@ void chunk_kernel(const Args a) {
                         uint32_t pk[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const fp16x2 two = __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_exp2f(x[b][2 * k]),
-                                                                          __builtin_amdgcn_exp2f(x[b][2 * k + 1]));
-                            l = __builtin_amdgcn_fdot2(two, fp16x2{(__fp16)1.f, (__fp16)1.f}, l, false);
+                            const fp16x2 two = __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_exp2f(s[b][2 * k]),
+                                                                          __builtin_amdgcn_exp2f(s[b][2 * k + 1]));
+                            sum = __builtin_amdgcn_fdot2(two, fp16x2{(__fp16)1.f, (__fp16)1.f}, sum, false);
                             pk[k] = __builtin_bit_cast(uint32_t, two);
                         }
                         p[b][0] = xdl::as_half8(pk[0], pk[1], pk[2], pk[3]);
                         p[b][1] = xdl::as_half8(pk[4], pk[5], pk[6], pk[7]);
                     }
                 }
+            };
+            weights();
+            if (__any(sum > most)) {
+                move(false);
+                weights();
             }
-            const unsigned char *v_from = m + S::v + c * S::vrow + 16 * (4 * S::sub * wt + h);
+            l += sum;
+            z += mid;
+            const unsigned char *v_from = v_at + (i % BUFS) * S::tile;
+            half8 v[kAhead];
+            constexpr int N = 8 * kAtOnce;
+            auto read = [&](int x) __attribute__((always_inline)) {
+                v[x % kAhead] = *reinterpret_cast<const half8 *>(v_from + 32 * (x & 3) * S::vrow + 32 * (2 * b0 + (x >> 2)));
+            };
 #pragma unroll
-            for (int b = 0; b < S::sub; ++b)
+            for (int x = 0; x < kAhead; ++x)
+                read(x);
+            auto output = [&](int x) __attribute__((always_inline)) {
+                acc[x & 3] = prefix::mfma32(v[x % kAhead], p[x >> 3][(x >> 2) & 1], acc[x & 3]);
+                if (x + kAhead < N)
+                    read(x + kAhead);
+            };
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        acc[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(v_from + 32 * d * S::vrow + 32 * (2 * b + t)),
-                                                p[b][t], acc[d]);
+            for (int x = 0; x < N; ++x)
+                output(x);
         };
-
-        if constexpr (BUFS == 2) {
-            if (n_tiles > 0) {
-                store(0);
-                load(1);
-                read_pages(2);
-            }
-            xdl::lds_barrier();
-            for (int i = 0; i < n_tiles; ++i) {
-                if (i + 1 < n_tiles) {
-                    store(i + 1);
-                    load(i + 2);
-                    read_pages(i + 3);
-                }
-                tile(i);
-                xdl::lds_barrier();
-            }
-        } else {
-            for (int i = 0; i < n_tiles; ++i) {
-                store(i);
-                load(i + 1);
+        // (each kind of wave has a loop of its own: where the two met, the codes in flight would have to arrive)
+        auto loop = [&](auto k_too, auto v_too) __attribute__((always_inline)) {
+            auto all = [&](int i) __attribute__((always_inline)) {  // all of a tile's decoding at once
+#pragma unroll
+                for (int y = 0; y < kSteps; ++y)
+                    decode(i, y, k_too, v_too);
+                load(i + 1, k_too, v_too);
                 read_pages(i + 2);
+            };
+            if constexpr (BUFS == 2) {
+                if (n_tiles > 0)
+                    all(0);
                 xdl::lds_barrier();
-                tile(i);
-                xdl::lds_barrier();
+                // (the last tile's turn decodes it again, into the other buffer: no branch in the loop)
+                for (int i = 0; i < n_tiles; ++i) {
+#pragma unroll
+                    for (int b = 0; b < S::sub; b += kAtOnce) {
+                        scores(i, b, i + 1, yes, k_too, v_too);
+                        softmax_outputs(i, b);
+                    }
+                    xdl::lds_barrier();
+                }
+            } else {
+                for (int i = 0; i < n_tiles; ++i) {
+                    all(i);
+                    xdl::lds_barrier();
+#pragma unroll
+                    for (int b = 0; b < S::sub; b += kAtOnce) {
+                        scores(i, b, 0, no, no, no);
+                        softmax_outputs(i, b);
+                    }
+                    xdl::lds_barrier();
+                }
             }
-        }
+        };
+        if constexpr (S::halves)
+            does_k ? loop(yes, no) : loop(no, yes);
+        else
+            loop(yes, yes);
 
         l = prefix::pair_sum(l);
         z = prefix::pair_sum(z);

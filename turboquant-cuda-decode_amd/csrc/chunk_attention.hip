@@ -114,6 +114,8 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     if (query_stride < (int64_t)Hq * D || query_stride % 8)
         return fail(TQ4_E_INVALID, "%s: query_stride %lld must be whole 16-byte pieces, at least Hq * D", what,
                     (long long)query_stride);
+    if (cache_block_stride > 0x7FFFFFFF)
+        return fail(TQ4_E_UNSUPPORTED, "%s: block stride %lld above 2^31 - 1", what, (long long)cache_block_stride);
     if (!aligned(out, 16))
         return fail(TQ4_E_INVALID, "%s: out must be 16-byte aligned", what);
     if (window < 0 || first_tokens < 0 || (window > 0 && !causal))
@@ -153,8 +155,9 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     p.table_width = max_blocks_per_seq;
     p.groups = plan.groups;
     p.block_size_log2 = log2_int(block_size);
-    p.slot_pos = a.slot_pos;
-    p.slot_head = a.slot_head;
+    const int record = 16 * (key_bits + value_bits);  // SoA: bytes of codes
+    p.slot_pos = a.kl == 0 ? Hk * record : a.slot_pos;
+    p.slot_head = a.kl == 0 ? record : a.slot_head;
     p.shape = tq4::chunk::Shape{32 * plan.wr, 64, Hq / Hk, Hk, causal != 0, std::min(window, 1 << 30), std::min(first_tokens, 1 << 30)};
     p.longest = (int)std::min<int64_t>((int64_t)max_blocks_per_seq * block_size, (1 << 30));
     const bool fine = lse || out_dtype == TQ4_F16;
