@@ -261,9 +261,10 @@ template <bool KF8, bool KB3, bool WIDE> struct Table {
     static constexpr int entries = KF8 ? 4 : KB3 ? 64 : 256;
 };
 
-// Unit u of K: token u / 4 of the tile, dims 32 (u % 4) .. +31; of V: tokens 4 (u / 16) .. +3, dims 8 (u % 16) .. +7.  The 64
-// units that a wave decodes at a time are those of 16 tokens, which lie in one block: where they begin is the wave's, a
-// lane's place in them the same in every tile, and a load takes one address of each.
+// Unit u of K: token u / 4 of the tile, dims 32 (u % 4) .. +31.  Unit u of V: tokens 16 (u / 64) + 4 q .. +3, dims 8 e .. +7, where
+// u % 64 = 16 r + 4 q + j and e = 4 j + r: the lane loads 32 dims of one token (r of the four), and the four lanes with
+// the same q and j exchange what they hold.  The 64 units that a wave decodes at a time are those of 16 tokens,
+// which lie in one block: where they begin is the wave's, a lane's place in them the same in every tile.
 template <int LAYOUT, bool KF8, bool KB3, bool V3> struct Codes {
     static constexpr int rec = xdl::record_bytes<LAYOUT, KF8, KB3, V3>(), v0 = xdl::v_offset<LAYOUT, KF8, KB3>();
     static constexpr int kbytes = KF8 ? kHeadDim : KB3 ? xdl::kK3Bytes : kHalfD, vbytes = V3 ? xdl::kK3Bytes : kHalfD;
@@ -304,22 +305,73 @@ __device__ __forceinline__ void load_k(Raw &r, const Args &a, const Place &at, i
         r.b.x = *reinterpret_cast<const uint16_t *>(at.data + token + C::kbytes);
     }
 }
+// (a: the lane's token's codes, 32 dims; b.xy or b.x: scales and zeros, see exchange)
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
 __device__ __forceinline__ void load_v(Raw &r, const Args &a, const Place &at, int lane) {
     using C = Codes<LAYOUT, KF8, KB3, V3>;
-    const uint32_t quad = (uint32_t)(lane >> 4) * (uint32_t)(4 * a.slot_pos), part = quad + C::v0 + (V3 ? 3 : 4) * (lane & 15);
-    auto token = [&](int i) { return *reinterpret_cast<const prefix::u32a1 *>(at.data + (uint32_t)(i * a.slot_pos) + part); };
-    r.a = uint4{token(0), token(1), token(2), token(3)};
-    if constexpr (LAYOUT == 0) {
-        const uint8_t *m = at.meta + (uint32_t)((C::nf - 2) * 2 << a.block_size_log2);
-        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(m + 8u * (lane >> 4));
-        const u32x2a8 z = *reinterpret_cast<const u32x2a8 *>(m + (2u << a.block_size_log2) + 8u * (lane >> 4));
-        r.b = uint4{s[0], s[1], z[0], z[1]};
+    const int row = lane >> 4, quad = (lane >> 2) & 3, j = lane & 3;
+    const uint32_t token = (uint32_t)(4 * quad + row) * (uint32_t)a.slot_pos + C::v0;
+    if constexpr (V3) {
+        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(at.data + token + 12 * j);
+        r.a = uint4{w[0], w[1], w[2], 0u};
     } else {
-        auto both = [&](int i) {
-            return *reinterpret_cast<const prefix::u32a2 *>(at.data + (uint32_t)(i * a.slot_pos + C::v0 + C::vbytes) + quad);
-        };
-        r.b = uint4{both(0), both(1), both(2), both(3)};
+        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + token + 16 * j);
+        r.a = uint4{w[0], w[1], w[2], w[3]};
+    }
+    if constexpr (LAYOUT == 0) {  // even rows the four tokens' scales, odd rows their zeros
+        const uint8_t *m = at.meta + (uint32_t)((C::nf - 2) * 2 << a.block_size_log2);
+        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(m + ((uint32_t)(row & 1) << (a.block_size_log2 + 1)) + 8u * quad);
+        r.b.x = s[0];
+        r.b.y = s[1];
+    } else {  // the token's own
+        r.b.x = *reinterpret_cast<const prefix::u32a2 *>(at.data + token + C::vbytes);
+    }
+}
+// Swaps x of the odd rows of 16 lanes with y of the even rows before them; of the upper two rows with the lower two.
+__device__ __forceinline__ void swap16(uint32_t &x, uint32_t &y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    const uint32_t a = r[0], b = r[1];
+    x = a;
+    y = b;
+}
+__device__ __forceinline__ void swap32(uint32_t &x, uint32_t &y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    const uint32_t a = r[0], b = r[1];
+    x = a;
+    y = b;
+}
+// The loaded parts to units: v[t] the eight codes of token t; s, z: scales and zeros of tokens (0, 1) and (2, 3).
+template <int LAYOUT, bool V3> __device__ __forceinline__ void exchange(const Raw &r, uint32_t (&v)[4], uint32_t (&s)[2], uint32_t (&z)[2]) {
+    v[0] = r.a.x;
+    v[1] = r.a.y;
+    v[2] = r.a.z;
+    v[3] = r.a.w;
+    if constexpr (V3) {  // 24 bits each
+        const uint32_t w0 = v[0], w1 = v[1], w2 = v[2];
+        v[1] = __builtin_amdgcn_alignbit(w1, w0, 24);
+        v[2] = __builtin_amdgcn_alignbit(w2, w1, 16);
+        v[3] = w2 >> 8;
+    }
+    // row r has parts 0 .. 3 of token r: to part r of tokens 0 .. 3
+    swap32(v[0], v[2]);
+    swap32(v[1], v[3]);
+    swap16(v[0], v[1]);
+    swap16(v[2], v[3]);
+    if constexpr (LAYOUT == 0) {
+        s[0] = z[0] = r.b.x;
+        s[1] = z[1] = r.b.y;
+        swap16(s[0], z[0]);
+        swap16(s[1], z[1]);
+    } else {
+        uint32_t t[4] = {r.b.x, r.b.x, r.b.x, r.b.x};
+        swap32(t[0], t[2]);
+        swap32(t[1], t[3]);
+        swap16(t[0], t[1]);
+        swap16(t[2], t[3]);
+        s[0] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100u);
+        s[1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100u);
+        z[0] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302u);
+        z[1] = __builtin_amdgcn_perm(t[3], t[2], 0x07060302u);
     }
 }
 
@@ -401,21 +453,12 @@ template <int LAYOUT, bool KF8, bool KB3, bool FINE> struct KUnit {
 // A unit of V into LDS: begin() takes its scalars, write(m) dims 2 m and 2 m + 1 of it.
 template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
     half2v s01, s23, z01, z23;
+    uint32_t v[4];
     // `valid`: tokens of the unit that the sequence has (4 or more: all; the others' bytes may hold anything, and count as
-    // zeros).  (Of a wave, together.)
-    template <class F> __device__ __forceinline__ void begin(const Raw &r, F &factors, int u, bool cut, int valid) {
+    // zeros).  `quad`: of the tile.  (Of a wave, together.)
+    template <class F> __device__ __forceinline__ void begin(const Raw &r, F &factors, int quad, bool cut, int valid) {
         uint32_t s[2], z[2];  // scales and zeros of tokens (0, 1) and (2, 3)
-        if constexpr (LAYOUT == 0) {
-            s[0] = r.b.x;
-            s[1] = r.b.y;
-            z[0] = r.b.z;
-            z[1] = r.b.w;
-        } else {
-            s[0] = __builtin_amdgcn_perm(r.b.y, r.b.x, 0x05040100u);
-            s[1] = __builtin_amdgcn_perm(r.b.w, r.b.z, 0x05040100u);
-            z[0] = __builtin_amdgcn_perm(r.b.y, r.b.x, 0x07060302u);
-            z[1] = __builtin_amdgcn_perm(r.b.w, r.b.z, 0x07060302u);
-        }
+        exchange<LAYOUT, V3>(r, v, s, z);
         if (cut) {
             const uint32_t m0 = valid <= 0 ? 0u : valid == 1 ? 0xFFFFu : 0xFFFFFFFFu, m1 = valid <= 2 ? 0u : valid == 3 ? 0xFFFFu : 0xFFFFFFFFu;
             s[0] &= m0;
@@ -452,7 +495,7 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
                     zero[i] *= kShrink;
                 }
             }
-            *reinterpret_cast<float4 *>(factors.fix + 4 * (u >> 4)) = float4{fix[0], fix[1], fix[2], fix[3]};
+            *reinterpret_cast<float4 *>(factors.fix + 4 * quad) = float4{fix[0], fix[1], fix[2], fix[3]};
             if constexpr (!FINE) {
                 auto pair = [](float x, float y) { return prefix::as_u32(half2v{(_Float16)x, (_Float16)y}); };
                 s[0] = pair(scale[0], scale[1]);
@@ -461,9 +504,9 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
                 z[1] = pair(zero[2], zero[3]);
             }
         }
-        factors.special[u >> 6] = special;
+        factors.special[quad >> 2] = special;
         if constexpr (FINE) {
-            float4 *to = reinterpret_cast<float4 *>(factors.v + 4 * (u >> 4));
+            float4 *to = reinterpret_cast<float4 *>(factors.v + 4 * quad);
             auto mid = [&](int i) { return fmaf(scale[i], kMiddle<V3>, zero[i]); };
             to[0] = float4{scale[0], mid(0), scale[1], mid(1)};
             to[1] = float4{scale[2], mid(2), scale[3], mid(3)};
@@ -475,7 +518,7 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
         }
     }
     // codes to f16: into the significand of 1024, then less 1024 (FINE: less 1024 and the middle code)
-    __device__ __forceinline__ void write(const Raw &r, unsigned char *to, int m) {
+    __device__ __forceinline__ void write(unsigned char *to, int m) {
         const half2v k0 = prefix::splat((_Float16)(1024.f + (FINE ? kMiddle<V3> : 0.f)));
         uint32_t magic = 0x64006400u;
         asm("" : "+v"(magic));
@@ -487,7 +530,6 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
             }
             *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{prefix::as_u32(x), prefix::as_u32(y)};
         };
-        const uint32_t v[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
         if constexpr (V3) {
 #pragma unroll
             for (int i = 2 * m; i < 2 * m + 2; ++i) {
@@ -621,11 +663,11 @@ void chunk_kernel(const Args a) {
                     kdec[x].sq = kdec[x].hl = 0.f;
             }
             if constexpr (v_too) {
-                const int t = first_of(i) + 4 * (u >> 4);
+                const int quad = 4 * (u >> 6) + ((u >> 2) & 3), e = 4 * (u & 3) + ((u >> 4) & 3);
                 if (q == 0)
-                    vdec[x].begin(rv[x], factors[i % BUFS], u, first_of(i) + KT > seq.len, seq.len - t);
+                    vdec[x].begin(rv[x], factors[i % BUFS], quad, first_of(i) + KT > seq.len, seq.len - first_of(i) - 4 * quad);
                 else
-                    vdec[x].write(rv[x], m + S::v + (u & 15) * S::vrow + 16 * (2 * (u >> 6) + ((u >> 4) & 1)) + 8 * ((u >> 5) & 1), q - 1);
+                    vdec[x].write(m + S::v + e * S::vrow + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1), q - 1);
             }
         };
         if (n_tiles > 0) {
