@@ -57,7 +57,7 @@ struct Args {
 
 // ---- Queries and cuts ------------------------------------------------------------------------
 
-constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 16 * kStartWaves;
+constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 32 * kStartWaves;
 // The least work that a workgroup is given, in token tiles.
 constexpr double kLeast = 4.0;
 constexpr int kSnap = 2;
@@ -110,9 +110,13 @@ __device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
     }
 }
 
-// Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two
-// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range are scaled down and q_factor
-// undoes it.  FP8 keys: the row itself, scaled by the power of two that puts its largest magnitude in [0.5, 1): exact.
+// Query rows into operands: y = q @ rot_t, times the score scale, as f16 hi (and lo); rows that would pass f16's range are
+// scaled down and q_factor undoes it.  The rotation is a product with the rows in the columns, y^T = rot_t^T q^T, rot_t as f16
+// hi + lo and each row scaled by a power of two that puts its largest magnitude in [2^14, 2^15).  A workgroup stages
+// rot_t once and takes row tiles of 128, whose next rows are on their way; a lane has rows' dims in a row of eight (rot_t's
+// columns are dealt to the product's rows in that order).  FP8 keys: the row itself, scaled by the power of two that
+// puts its largest magnitude in [0.5, 1): exact.
+// Bound by the bytes it moves: 8192 x 32 rows 30 us (134 MB), where one tile a workgroup took 56.
 template <typename InT, bool KF8, bool LO>
 __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
@@ -122,105 +126,123 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
         plan_cuts(a, sums);
         return;
     }
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, n = lane & 15, g = lane >> 4;
-    const int64_t rows = (int64_t)a.tokens * a.num_q_heads, r0 = (int64_t)blockIdx.x * kStartRows + 16 * wave;
-    const int64_t ra = min(r0 + n, rows - 1);
-    const int64_t token = ra / a.num_q_heads;
-    const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (ra - token * a.num_q_heads) * kHeadDim;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
+    const int rows = a.tokens * a.num_q_heads, step = (gridDim.x - 1) * kStartRows;
     typedef InT in8 __attribute__((ext_vector_type(8)));
-    in8 qv[4];
+    struct Rows {
+        in8 v[8];  // dims 16 k + 8 h ..
+    };
+    auto fetch = [&](Rows &q, int r0) __attribute__((always_inline)) {
+        const int r = min(r0 + c, rows - 1), token = r / a.num_q_heads;
+        const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (int64_t)(r - token * a.num_q_heads) * kHeadDim + 8 * h;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-        qv[kb] = *reinterpret_cast<const in8 *>(from + 32 * kb + 8 * g);
-    float amax = 0.f;
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            amax = fmaxf(amax, fabsf(to_float<InT>(qv[kb][j])));
-    amax = rot_row_max(amax);
-    const bool finite = amax > 0.f && amax < __builtin_inff();
-    if constexpr (KF8) {
-        const int e = finite ? -__builtin_amdgcn_frexp_expf(amax) : 0;
-        if (r0 + n >= rows)
-            return;
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            half8 y;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                y[j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
-            *reinterpret_cast<half8 *>(a.q_hi + ra * kHeadDim + 32 * kb + 8 * g) = y;
-        }
-        if (g == 0)
-            a.q_factor[ra] = __builtin_ldexpf(a.score_scale_log2, -e);
-        return;
-    } else {
+        for (int k = 0; k < 8; ++k)
+            q.v[k] = *reinterpret_cast<const in8 *>(from + 16 * k);
+    };
+    auto row_max = [](float x) { return prefix::pair_max(x); };
+    int r0 = blockIdx.x * kStartRows + 32 * wave;
+    Rows q;
+    fetch(q, r0);
+    if constexpr (!KF8) {
         constexpr int kIters = kHeadDim * (kHeadDim / 8) / kStartThreads;
 #pragma unroll
         for (int it = 0; it < kIters; ++it) {
-            const int i = threadIdx.x + it * kStartThreads, c = i % kHeadDim, kg = i / kHeadDim;
-            half8 h, l;
+            const int i = threadIdx.x + it * kStartThreads, d = i % kHeadDim, kg = i / kHeadDim;
+            half8 hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float w = a.rot_t[(8 * kg + j) * kHeadDim + c];
-                h[j] = (_Float16)w;
-                l[j] = (_Float16)(w - (float)h[j]);
+                const float w = a.rot_t[(8 * kg + j) * kHeadDim + d];
+                hi[j] = (_Float16)w;
+                lo[j] = (_Float16)(w - (float)hi[j]);
             }
-            *reinterpret_cast<half8 *>(pt_hi + c * kRotPt + 8 * kg) = h;
-            *reinterpret_cast<half8 *>(pt_lo + c * kRotPt + 8 * kg) = l;
+            // dim 8 e + i in row 16 i + e (as V^T's)
+            const int row = 16 * (d & 7) + (d >> 3);
+            *reinterpret_cast<half8 *>(pt_hi + row * kRotPt + 8 * kg) = hi;
+            *reinterpret_cast<half8 *>(pt_lo + row * kRotPt + 8 * kg) = lo;
         }
         __syncthreads();
-        if (r0 >= rows)
-            return;
-        const int e = finite ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
-        half8 q[4];
+    }
+    for (; r0 < rows; r0 += step) {
+        const Rows now = q;
+        if (r0 + step < rows)
+            fetch(q, r0 + step);
+        const int64_t row = r0 + c;
+        float amax = 0.f;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                q[kb][j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
-        // D: lane (n, g) has dims 16 cb + 4 g .. +3 of row n
-        floatx4 y[8];
+                amax = fmaxf(amax, fabsf(to_float<InT>(now.v[k][j])));
+        amax = row_max(amax);
+        const bool finite = amax > 0.f && amax < __builtin_inff();
+        if constexpr (KF8) {
+            const int e = finite ? -__builtin_amdgcn_frexp_expf(amax) : 0;
+            if (row >= rows)
+                continue;
 #pragma unroll
-        for (int cb = 0; cb < 8; ++cb) {
-            y[cb] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < 8; ++k) {
+                half8 y;
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-                const int off = (16 * cb + n) * kRotPt + 32 * kb + 8 * g;
-                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_hi + off), q[kb], y[cb]);
-                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + off), q[kb], y[cb]);
+                for (int j = 0; j < 8; ++j)
+                    y[j] = (_Float16)__builtin_ldexpf(to_float<InT>(now.v[k][j]), e);
+                *reinterpret_cast<half8 *>(a.q_hi + row * kHeadDim + 16 * k + 8 * h) = y;
             }
+            if (h == 0)
+                a.q_factor[row] = __builtin_ldexpf(a.score_scale_log2, -e);
+        } else {
+            const int e = finite ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
+            half8 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[k][j] = (_Float16)__builtin_ldexpf(to_float<InT>(now.v[k][j]), e);
+            // accumulator d, register 4 u + i: dim 8 (8 (u % 2) + 4 h + i) + 2 d + u / 2 of row c
+            floatx16 y[4];
+            float top = 0.f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    y[d][k] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int off = (32 * d + c) * kRotPt + 16 * k + 8 * h;
+                    y[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(pt_hi + off), x[k], y[d]);
+                    y[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(pt_lo + off), x[k], y[d]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    y[d][k] = __builtin_ldexpf(y[d][k], -e) * a.score_scale_log2;
+                    top = fmaxf(top, fabsf(y[d][k]));
+                }
+            top = row_max(top);
+            const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            if (row >= rows)
+                continue;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    half8 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float v = __builtin_ldexpf(y[j >> 1][8 * (j & 1) + 4 * u + i], f);
+                        asm("" : "+v"(v));  // (rounded once: hi and lo belong together)
+                        hi[j] = (_Float16)v;
+                        lo[j] = (_Float16)(v - (float)hi[j]);
+                    }
+                    const int64_t at = row * kHeadDim + 8 * (8 * u + 4 * h + i);
+                    *reinterpret_cast<half8 *>(a.q_hi + at) = hi;
+                    if constexpr (LO)
+                        *reinterpret_cast<half8 *>(a.q_lo + at) = lo;
+                }
+            if (h == 0)
+                a.q_factor[row] = __builtin_ldexpf(1.f, -f);
         }
-        float top = 0.f;
-#pragma unroll
-        for (int cb = 0; cb < 8; ++cb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                y[cb][i] = __builtin_ldexpf(y[cb][i], -e) * a.score_scale_log2;
-                top = fmaxf(top, fabsf(y[cb][i]));
-            }
-        top = rot_row_max(top);
-        const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-        if (r0 + n >= rows)
-            return;
-        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-        for (int cb = 0; cb < 8; ++cb) {
-            half4 hi, lo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v = __builtin_ldexpf(y[cb][i], f);
-                asm("" : "+v"(v));  // (rounded once: hi and lo belong together)
-                hi[i] = (_Float16)v;
-                lo[i] = (_Float16)(v - (float)hi[i]);
-            }
-            *reinterpret_cast<half4 *>(a.q_hi + ra * kHeadDim + 16 * cb + 4 * g) = hi;
-            if constexpr (LO)
-                *reinterpret_cast<half4 *>(a.q_lo + ra * kHeadDim + 16 * cb + 4 * g) = lo;
-        }
-        if (g == 0)
-            a.q_factor[ra] = __builtin_ldexpf(1.f, -f);
     }
 }
 
@@ -1043,64 +1065,97 @@ void chunk_kernel(const Args a) {
     }
 }
 
-// Joins the parts of a row tile that was cut: workgroup (w, i) the rows 4 i .. +3 of the one that workgroup w of
-// chunk_kernel began and did not end, a row per wave.  Lane: dims 2 lane, 2 lane + 1.
-constexpr int kMergeRows = 4;
-template <typename OutT> __global__ __launch_bounds__(kWave *kMergeRows) void chunk_merge_kernel(const Args a) {
-    const int w = blockIdx.x, lane = threadIdx.x & 63;
+// Joins the parts of a row tile that was cut: workgroup (w, i) rows of the one that workgroup w of chunk_kernel began and
+// did not end, PER of them per half wave.  Lane: dims 4 x .. +3 of its half's row.
+constexpr int kMergeThreads = 256, kMergeHalves = kMergeThreads / 32;
+template <typename OutT, int PER> __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(const Args a) {
+    const int w = blockIdx.x, x = threadIdx.x & 31, half = threadIdx.x >> 5;
     const Cut from = a.cuts[w], cut = a.cuts[w + 1];
     if (cut.b >= a.batch || cut.at == 0 || (same_tile(from, cut) && from.at > 0))
         return;
     const Seq seq = seq_of(a.starts, a.seq_lens, cut.b, a.tokens, a.longest);
-    const int place = blockIdx.y * kMergeRows + (threadIdx.x >> 6), row = cut.r * a.shape.rows + place;
-    if (row >= seq.n * a.shape.group)
-        return;
-    int parts = 1;  // part i: of workgroup w + i
+    const int rows = seq.n * a.shape.group, place0 = (blockIdx.y * kMergeHalves + half) * PER;
+    int parts = 2;  // part i: of workgroup w + i; the last is of the first whose own stretch ends in another row tile
     while (same_tile(a.cuts[w + parts], cut))
         ++parts;
-    // (workgroup w + parts - 1 has the end: the first whose own stretch ends in another row tile)
-    float mx = -INFINITY, a0 = 0.f, a1 = 0.f, sum = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += kWave) {
-        const int i = i0 + lane;
-        auto slot = [&](int j) { return 2 * (w + j) + (j == 0 ? 1 : 0); };
-        float s = -INFINITY;
-        if (i < parts) {
-            const Cut x = a.cuts[w + i], y = a.cuts[w + i + 1];
-            if (i == 0 || !same_tile(x, y) || x.at < y.at)  // (a workgroup without tiles wrote nothing)
-                s = part_sums(a, slot(i))[place];
-        }
-        const float m_new = fmaxf(mx, wave_max(s));
-        const float scale = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m_new);
-        const float wt = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
-        sum = sum * scale + wave_sum(wt);
-        a0 *= scale;
-        a1 *= scale;
-        const int n = min(kWave, parts - i0);
-        for (int j = 0; j < n; ++j) {
-            const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), j));
-            if (wj == 0.f)
-                continue;
-            const float2 v = *reinterpret_cast<const float2 *>(part_rows(a, slot(i0 + j)) + (int64_t)place * kHeadDim + 2 * lane);
-            a0 = fmaf(wj, v.x, a0);
-            a1 = fmaf(wj, v.y, a1);
-        }
-        mx = m_new;
+    auto slot = [&](int j) { return 2 * (w + j) + (j == 0 ? 1 : 0); };
+    auto wrote = [&](int j) {  // (a workgroup without tiles wrote nothing)
+        const Cut p = a.cuts[w + j], q = a.cuts[w + j + 1];
+        return j == 0 || !same_tile(p, q) || p.at < q.at;
+    };
+    float mx[PER], sum[PER];
+    float4 acc[PER];
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+        mx[r] = -INFINITY;
+        sum[r] = 0.f;
+        acc[r] = float4{0.f, 0.f, 0.f, 0.f};
     }
-    const int token = row / a.shape.group, head = cut.h * a.shape.group + row - token * a.shape.group;
-    if (a.sinks) {
-        const float sink = a.sinks[head] * kLog2e, m_new = fmaxf(mx, sink);
-        const float scale = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m_new);
-        a0 *= scale;
-        a1 *= scale;
-        sum = sum * scale + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m_new));
-        mx = m_new;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        const int i = i0 + x, n = min(32, parts - i0);
+        const bool there = i < parts && wrote(i);
+        float wt[PER];
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+            const float s = there ? part_sums(a, slot(i))[min(place0 + r, a.shape.rows - 1)] : -INFINITY;
+            float top = s;
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1)
+                top = fmaxf(top, __shfl_xor(top, m, 32));
+            const float m_new = fmaxf(mx[r], top), scale = mx[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[r] - m_new);
+            wt[r] = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
+            float all = wt[r];
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1)
+                all += __shfl_xor(all, m, 32);
+            sum[r] = sum[r] * scale + all;
+            acc[r] = float4{acc[r].x * scale, acc[r].y * scale, acc[r].z * scale, acc[r].w * scale};
+            mx[r] = m_new;
+        }
+        constexpr int AT_ONCE = PER >= 4 ? 1 : 4;  // parts
+        for (int j0 = 0; j0 < n; j0 += AT_ONCE) {
+            float4 v[AT_ONCE][PER];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+                for (int r = 0; r < PER; ++r)
+                    v[j][r] = reinterpret_cast<const float4 *>(part_rows(a, slot(i0 + min(j0 + j, n - 1))) +
+                                                               (int64_t)min(place0 + r, a.shape.rows - 1) * kHeadDim)[x];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+                for (int r = 0; r < PER; ++r) {
+                    const float wj = __shfl(wt[r], j0 + j, 32);
+                    if (j0 + j < n && wj != 0.f) {  // (a part without weight may hold anything)
+                        acc[r].x = fmaf(wj, v[j][r].x, acc[r].x);
+                        acc[r].y = fmaf(wj, v[j][r].y, acc[r].y);
+                        acc[r].z = fmaf(wj, v[j][r].z, acc[r].z);
+                        acc[r].w = fmaf(wj, v[j][r].w, acc[r].w);
+                    }
+                }
+        }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t q_row = (int64_t)(seq.row0 + token) * a.num_q_heads + head;
-    typedef OutT out2 __attribute__((ext_vector_type(2)));
-    *reinterpret_cast<out2 *>(static_cast<OutT *>(a.out) + q_row * kHeadDim + 2 * lane) = out2{(OutT)(a0 * inv), (OutT)(a1 * inv)};
-    if (lane == 0 && a.lse)
-        a.lse[q_row] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+        const int row = cut.r * a.shape.rows + place0 + r;
+        if (place0 + r >= a.shape.rows || row >= rows)
+            break;
+        const int token = row / a.shape.group, head = cut.h * a.shape.group + row - token * a.shape.group;
+        float scale = 1.f;
+        if (a.sinks) {
+            const float sink = a.sinks[head] * kLog2e, m_new = fmaxf(mx[r], sink);
+            scale = mx[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[r] - m_new);
+            sum[r] = sum[r] * scale + (sink == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sink - m_new));
+            mx[r] = m_new;
+        }
+        const float inv = sum[r] == 0.f ? 0.f : scale / sum[r];
+        const int64_t q_row = (int64_t)(seq.row0 + token) * a.num_q_heads + head;
+        typedef OutT out4 __attribute__((ext_vector_type(4)));
+        reinterpret_cast<out4 *>(static_cast<OutT *>(a.out) + q_row * kHeadDim)[x] =
+            out4{(OutT)(acc[r].x * inv), (OutT)(acc[r].y * inv), (OutT)(acc[r].z * inv), (OutT)(acc[r].w * inv)};
+        if (x == 0 && a.lse)
+            a.lse[q_row] = sum[r] == 0.f ? -INFINITY : (mx[r] + __builtin_amdgcn_logf(sum[r])) * kLn2;
+    }
 }
 
 }  // namespace chunk

@@ -70,11 +70,22 @@ template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq
 template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
     const int64_t rows = (int64_t)p.tokens * p.num_q_heads;
-    const dim3 grid((unsigned)((rows + kStartRows - 1) / kStartRows + 1)), block(kStartThreads);
+    // (two workgroups' rotation matrices fit into a CU's LDS; the last workgroup makes the plan)
+    const dim3 grid((unsigned)(std::min<int64_t>((rows + kStartRows - 1) / kStartRows, 2 * cus()) + 1)), block(kStartThreads);
     if (p.q_dtype == TQ4_BF16)
         launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p);
     else
         launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p);
+}
+// Few rows: many parts; many rows: two parts, most often, and several rows' loads at once.
+template <typename OutT> void launch_merge(const tq4::chunk::Args &p, int wr, hipStream_t st) {
+    using namespace tq4::chunk;
+    const int per = wr == 8 ? 8 : 1;
+    const dim3 grid(p.groups, (32 * wr + kMergeHalves * per - 1) / (kMergeHalves * per)), block(kMergeThreads);
+    if (wr == 8)
+        launch(&chunk_merge_kernel<OutT, 8>, grid, block, st, p);
+    else
+        launch(&chunk_merge_kernel<OutT, 1>, grid, block, st, p);
 }
 
 }  // namespace
@@ -175,11 +186,10 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     rc = launch_status("chunk");
     if (rc)
         return rc;
-    const dim3 grid(plan.groups, 32 * plan.wr / tq4::chunk::kMergeRows), block(tq4::kWave * tq4::chunk::kMergeRows);
     if (out_dtype == TQ4_BF16)
-        launch(&tq4::chunk::chunk_merge_kernel<__bf16>, grid, block, st, p);
+        launch_merge<__bf16>(p, plan.wr, st);
     else
-        launch(&tq4::chunk::chunk_merge_kernel<_Float16>, grid, block, st, p);
+        launch_merge<_Float16>(p, plan.wr, st);
     return launch_status("chunk merge");
 }
 
