@@ -282,6 +282,35 @@ template <bool KF8, bool KB3, bool WIDE> struct Table {
     using Entry = std::conditional_t<WIDE, uint2, uint32_t>;
     static constexpr int entries = KF8 ? 4 : KB3 ? 64 : 256;
 };
+template <int LAYOUT, bool KF8, bool KB3, bool FINE, class Entry>
+__device__ __forceinline__ void fill_table(Entry *table, const float *centroids, int tid, int threads) {
+    if constexpr (!KF8)
+        for (int e = tid; e < (KB3 ? 64 : 256); e += threads) {
+            const float c0 = centroids[KB3 ? e & 7 : e & 15], c1 = centroids[KB3 ? e >> 3 : e >> 4];
+            if constexpr (FINE) {
+                const uint32_t x = xdl::split_f16(c0), z = xdl::split_f16(c1);
+                table[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
+            } else {
+                const uint32_t both = prefix::as_u32(half2v{(_Float16)c0, (_Float16)c1});
+                if constexpr (LAYOUT == 1)
+                    table[e] = uint2{both, xdl::fbits(fmaf(c0, c0, c1 * c1))};
+                else
+                    table[e] = both;
+            }
+        }
+}
+// Codes 2 b, 2 b + 1 of a lane's 32.
+template <bool KB3> __device__ __forceinline__ uint32_t code_pair(const uint32_t (&w)[4], int b) {
+    if constexpr (KB3) {
+        const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
+        uint32_t v = w[wi] >> sh;
+        if (sh > 26)
+            v |= w[wi + 1] << (32 - sh);
+        return v & 63u;
+    } else {
+        return (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
+    }
+}
 
 // Unit u of K: token u / 4 of the tile, dims 32 (u % 4) .. +31.  Unit u of V: tokens 16 (u / 64) + 4 q .. +3, dims 8 e .. +7, where
 // u % 64 = 16 r + 4 q + j and e = 4 j + r: the lane loads 32 dims of one token (r of the four), and the four lanes with
@@ -417,17 +446,7 @@ template <int LAYOUT, bool KF8, bool KB3, bool FINE> struct KUnit {
             const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int b = 4 * q + i;
-                uint32_t v;
-                if constexpr (KB3) {
-                    const int bit = 6 * b, wi = bit >> 5, sh = bit & 31;
-                    v = w[wi] >> sh;
-                    if (sh > 26)
-                        v |= w[wi + 1] << (32 - sh);
-                    v &= 63u;
-                } else {
-                    v = (w[b >> 2] >> (8 * (b & 3))) & 0xFFu;
-                }
+                const uint32_t v = code_pair<KB3>(w, 4 * q + i);
                 if constexpr (WIDE) {
                     const uint2 c = table[v];
                     hi[q & 1][i] = c.x;
@@ -607,20 +626,7 @@ void chunk_kernel(const Args a) {
     const Cut end = a.cuts[group_id + 1];
     if (at.b >= a.batch || (same_tile(at, end) && at.at == end.at))
         return;
-    if constexpr (!KF8)
-        for (int e = tid; e < T::entries; e += S::threads) {
-            const float c0 = a.centroids[KB3 ? e & 7 : e & 15], c1 = a.centroids[KB3 ? e >> 3 : e >> 4];
-            if constexpr (FINE) {
-                const uint32_t x = xdl::split_f16(c0), z = xdl::split_f16(c1);
-                lds.table[e] = uint2{(x & 0xFFFFu) | (z << 16), (x >> 16) | (z & 0xFFFF0000u)};
-            } else {
-                const uint32_t both = prefix::as_u32(half2v{(_Float16)c0, (_Float16)c1});
-                if constexpr (LAYOUT == 1)
-                    lds.table[e] = uint2{both, xdl::fbits(fmaf(c0, c0, c1 * c1))};
-                else
-                    lds.table[e] = both;
-            }
-        }
+    fill_table<LAYOUT, KF8, KB3, FINE>(lds.table, a.centroids, tid, S::threads);
     const bool does_k = !S::halves || w < WR * WT / 2, does_v = !S::halves || w >= WR * WT / 2;
     const int group = a.shape.group;
     xdl::lds_barrier();  // the table

@@ -2,24 +2,27 @@
 #include <algorithm>
 
 #include "abi.h"
-#include "chunk.h"
+#include "chunk_few.h"
 
 using namespace tq4::abi;
 
 namespace {
 
-// How a call is spread over the device: workgroups of `wr` * `wt` waves on row tiles of 32 wr rows, `held` of them at once.
+// How a call is spread over the device, by a sequence's query rows per kv-head (on average): workgroups on row tiles of
+// `rows` rows and token tiles of `tile`, `groups` of them at once.
+enum class Form { kMany, kSome, kFew };
 struct ChunkPlan {
-    int wr, groups;
+    Form form;
+    int rows, tile, groups;
 };
 int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
 ChunkPlan chunk_plan(int tokens, int batch, int group) {
-    const int64_t rows = (int64_t)tokens * group / batch;  // of a sequence, on average
+    const int64_t rows = (int64_t)tokens * group / batch;
     if (rows > 64)
-        return {8, cus()};
+        return {Form::kMany, 256, 64, cus()};
     if (rows > 32)
-        return {2, 2 * cus()};
-    return {1, 4 * cus()};
+        return {Form::kSome, 64, 64, 2 * cus()};
+    return {Form::kFew, tq4::chunk::kFewRows, tq4::chunk::kFewTile, 2 * cus()};
 }
 
 struct Workspace {
@@ -35,7 +38,7 @@ Workspace workspace_of(int tokens, int batch, int Hq, int Hk) {
     w.work = w.factor + up(rows);
     w.cuts = w.work + up(2 * ((int64_t)batch + 1));
     w.parts = w.cuts + up(4 * ((int64_t)p.groups + 1));
-    w.total = w.parts + up((int64_t)2 * p.groups * 32 * p.wr * (tq4::kHeadDim + 1));
+    w.total = w.parts + up((int64_t)2 * p.groups * p.rows * (tq4::kHeadDim + 1));
     return w;
 }
 const char *shape_error(int tokens, int B, int Hq, int Hk) {
@@ -59,30 +62,42 @@ void launch_chunk(const Stage1Args &a, const tq4::chunk::Args &p, hipStream_t st
     else
         launch(&chunk_kernel<LAYOUT, false, false, false, WR, WT, KT, BUFS, FINE>, grid, block, st, p);
 }
-template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq4::chunk::Args &p, int wr, hipStream_t st) {
-    if (wr == 8)
+template <int LAYOUT, bool FINE> void launch_few(const Stage1Args &a, const tq4::chunk::Args &p, hipStream_t st) {
+    using namespace tq4::chunk;
+    const dim3 block(tq4::kWave * kFewWaves), grid((p.groups + 7) / 8 * 8);
+    if (a.key_fp8)
+        launch(&chunk_few_kernel<LAYOUT, true, false, false, FINE>, grid, block, st, p);
+    else if (a.key_bits == 3 && a.value_bits == 3)
+        launch(&chunk_few_kernel<LAYOUT, false, true, true, FINE>, grid, block, st, p);
+    else if (a.key_bits == 3)
+        launch(&chunk_few_kernel<LAYOUT, false, true, false, FINE>, grid, block, st, p);
+    else
+        launch(&chunk_few_kernel<LAYOUT, false, false, false, FINE>, grid, block, st, p);
+}
+template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq4::chunk::Args &p, Form form, hipStream_t st) {
+    if (form == Form::kMany)
         launch_chunk<LAYOUT, 8, 1, 64, 2, FINE>(a, p, st);
-    else if (wr == 2)
+    else if (form == Form::kSome)
         launch_chunk<LAYOUT, 2, 2, 64, 1, FINE>(a, p, st);
     else
-        launch_chunk<LAYOUT, 1, 2, 64, 1, FINE>(a, p, st);
+        launch_few<LAYOUT, FINE>(a, p, st);
 }
 template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
     const int64_t rows = (int64_t)p.tokens * p.num_q_heads;
     // (two workgroups' rotation matrices fit into a CU's LDS; the last workgroup makes the plan)
-    const dim3 grid((unsigned)(std::min<int64_t>((rows + kStartRows - 1) / kStartRows, 2 * cus()) + 1)), block(kStartThreads);
+    const dim3 grid((unsigned)(std::min<int64_t>((rows + kStartRows - 1) / kStartRows, (KF8 ? 8 : 2) * cus()) + 1)), block(kStartThreads);
     if (p.q_dtype == TQ4_BF16)
         launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p);
     else
         launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p);
 }
 // Few rows: many parts; many rows: two parts, most often, and several rows' loads at once.
-template <typename OutT> void launch_merge(const tq4::chunk::Args &p, int wr, hipStream_t st) {
+template <typename OutT> void launch_merge(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
-    const int per = wr == 8 ? 8 : 1;
-    const dim3 grid(p.groups, (32 * wr + kMergeHalves * per - 1) / (kMergeHalves * per)), block(kMergeThreads);
-    if (wr == 8)
+    const int rows = p.shape.rows, per = rows == 256 ? 8 : 1;
+    const dim3 grid(p.groups, (rows + kMergeHalves * per - 1) / (kMergeHalves * per)), block(kMergeThreads);
+    if (per == 8)
         launch(&chunk_merge_kernel<OutT, 8>, grid, block, st, p);
     else
         launch(&chunk_merge_kernel<OutT, 1>, grid, block, st, p);
@@ -169,7 +184,7 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     const int record = 16 * (key_bits + value_bits);  // SoA: bytes of codes
     p.slot_pos = a.kl == 0 ? Hk * record : a.slot_pos;
     p.slot_head = a.kl == 0 ? record : a.slot_head;
-    p.shape = tq4::chunk::Shape{32 * plan.wr, 64, Hq / Hk, Hk, causal != 0, std::min(window, 1 << 30), std::min(first_tokens, 1 << 30)};
+    p.shape = tq4::chunk::Shape{plan.rows, plan.tile, Hq / Hk, Hk, causal != 0, std::min(window, 1 << 30), std::min(first_tokens, 1 << 30)};
     p.longest = (int)std::min<int64_t>((int64_t)max_blocks_per_seq * block_size, (1 << 30));
     const bool fine = lse || out_dtype == TQ4_F16;
     if (a.key_fp8)
@@ -180,16 +195,16 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     if (rc)
         return rc;
     if (a.kl == 0)
-        fine ? launch_chunk<0, true>(a, p, plan.wr, st) : launch_chunk<0, false>(a, p, plan.wr, st);
+        fine ? launch_chunk<0, true>(a, p, plan.form, st) : launch_chunk<0, false>(a, p, plan.form, st);
     else
-        fine ? launch_chunk<1, true>(a, p, plan.wr, st) : launch_chunk<1, false>(a, p, plan.wr, st);
+        fine ? launch_chunk<1, true>(a, p, plan.form, st) : launch_chunk<1, false>(a, p, plan.form, st);
     rc = launch_status("chunk");
     if (rc)
         return rc;
     if (out_dtype == TQ4_BF16)
-        launch_merge<__bf16>(p, plan.wr, st);
+        launch_merge<__bf16>(p, st);
     else
-        launch_merge<_Float16>(p, plan.wr, st);
+        launch_merge<_Float16>(p, st);
     return launch_status("chunk merge");
 }
 
