@@ -57,7 +57,7 @@ struct Args {
 
 // ---- Queries and cuts ------------------------------------------------------------------------
 
-constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 32 * kStartWaves;
+constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 16 * kStartWaves;
 // The least work that a workgroup is given, in token tiles.
 constexpr double kLeast = 4.0;
 constexpr int kSnap = 2;
@@ -110,139 +110,120 @@ __device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
     }
 }
 
-// Query rows into operands: y = q @ rot_t, times the score scale, as f16 hi (and lo); rows that would pass f16's range are
-// scaled down and q_factor undoes it.  The rotation is a product with the rows in the columns, y^T = rot_t^T q^T, rot_t as f16
-// hi + lo and each row scaled by a power of two that puts its largest magnitude in [2^14, 2^15).  A workgroup stages
-// rot_t once and takes row tiles of 128, whose next rows are on their way; a lane has rows' dims in a row of eight (rot_t's
-// columns are dealt to the product's rows in that order).  FP8 keys: the row itself, scaled by the power of two that
-// puts its largest magnitude in [0.5, 1): exact.
-// Bound by the bytes it moves: 8192 x 32 rows 30 us (134 MB), where one tile a workgroup took 56.
+// Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two
+// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range are scaled down and q_factor
+// undoes it.  FP8 keys: the row itself, scaled by the power of two that puts its largest magnitude in [0.5, 1): exact.
+// 8192 x 32 rows: 53 us.  A form whose workgroups stage rot_t once and take one row tile after the other (32x32x16
+// products) took 39, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
+// clock through chunk_kernel (634 : 720 us, the same code).
 template <typename InT, bool KF8, bool LO>
 __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
     __shared__ __align__(16) _Float16 pt_hi[PT], pt_lo[PT];
-    if (blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.x == 0) {
         __shared__ double sums[kStartThreads];
         plan_cuts(a, sums);
         return;
     }
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
-    const int rows = a.tokens * a.num_q_heads, step = (gridDim.x - 1) * kStartRows;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, n = lane & 15, g = lane >> 4;
+    const int64_t rows = (int64_t)a.tokens * a.num_q_heads, r0 = ((int64_t)blockIdx.x - 1) * kStartRows + 16 * wave;
+    const int64_t ra = min(r0 + n, rows - 1);
+    const int64_t token = ra / a.num_q_heads;
+    const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (ra - token * a.num_q_heads) * kHeadDim;
     typedef InT in8 __attribute__((ext_vector_type(8)));
-    struct Rows {
-        in8 v[8];  // dims 16 k + 8 h ..
-    };
-    auto fetch = [&](Rows &q, int r0) __attribute__((always_inline)) {
-        const int r = min(r0 + c, rows - 1), token = r / a.num_q_heads;
-        const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (int64_t)(r - token * a.num_q_heads) * kHeadDim + 8 * h;
+    in8 qv[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            q.v[k] = *reinterpret_cast<const in8 *>(from + 16 * k);
-    };
-    auto row_max = [](float x) { return prefix::pair_max(x); };
-    int r0 = blockIdx.x * kStartRows + 32 * wave;
-    Rows q;
-    fetch(q, r0);
-    if constexpr (!KF8) {
+    for (int kb = 0; kb < 4; ++kb)
+        qv[kb] = *reinterpret_cast<const in8 *>(from + 32 * kb + 8 * g);
+    float amax = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            amax = fmaxf(amax, fabsf(to_float<InT>(qv[kb][j])));
+    amax = rot_row_max(amax);
+    const bool finite = amax > 0.f && amax < __builtin_inff();
+    if constexpr (KF8) {
+        const int e = finite ? -__builtin_amdgcn_frexp_expf(amax) : 0;
+        if (r0 + n >= rows)
+            return;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            half8 y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
+            *reinterpret_cast<half8 *>(a.q_hi + ra * kHeadDim + 32 * kb + 8 * g) = y;
+        }
+        if (g == 0)
+            a.q_factor[ra] = __builtin_ldexpf(a.score_scale_log2, -e);
+        return;
+    } else {
         constexpr int kIters = kHeadDim * (kHeadDim / 8) / kStartThreads;
 #pragma unroll
         for (int it = 0; it < kIters; ++it) {
-            const int i = threadIdx.x + it * kStartThreads, d = i % kHeadDim, kg = i / kHeadDim;
-            half8 hi, lo;
+            const int i = threadIdx.x + it * kStartThreads, c = i % kHeadDim, kg = i / kHeadDim;
+            half8 h, l;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float w = a.rot_t[(8 * kg + j) * kHeadDim + d];
-                hi[j] = (_Float16)w;
-                lo[j] = (_Float16)(w - (float)hi[j]);
+                const float w = a.rot_t[(8 * kg + j) * kHeadDim + c];
+                h[j] = (_Float16)w;
+                l[j] = (_Float16)(w - (float)h[j]);
             }
-            // dim 8 e + i in row 16 i + e (as V^T's)
-            const int row = 16 * (d & 7) + (d >> 3);
-            *reinterpret_cast<half8 *>(pt_hi + row * kRotPt + 8 * kg) = hi;
-            *reinterpret_cast<half8 *>(pt_lo + row * kRotPt + 8 * kg) = lo;
+            *reinterpret_cast<half8 *>(pt_hi + c * kRotPt + 8 * kg) = h;
+            *reinterpret_cast<half8 *>(pt_lo + c * kRotPt + 8 * kg) = l;
         }
         __syncthreads();
-    }
-    for (; r0 < rows; r0 += step) {
-        const Rows now = q;
-        if (r0 + step < rows)
-            fetch(q, r0 + step);
-        const int64_t row = r0 + c;
-        float amax = 0.f;
+        if (r0 >= rows)
+            return;
+        const int e = finite ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
+        half8 q[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                amax = fmaxf(amax, fabsf(to_float<InT>(now.v[k][j])));
-        amax = row_max(amax);
-        const bool finite = amax > 0.f && amax < __builtin_inff();
-        if constexpr (KF8) {
-            const int e = finite ? -__builtin_amdgcn_frexp_expf(amax) : 0;
-            if (row >= rows)
-                continue;
+                q[kb][j] = (_Float16)__builtin_ldexpf(to_float<InT>(qv[kb][j]), e);
+        // D: lane (n, g) has dims 16 cb + 4 g .. +3 of row n
+        floatx4 y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                half8 y;
+        for (int cb = 0; cb < 8; ++cb) {
+            y[cb] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    y[j] = (_Float16)__builtin_ldexpf(to_float<InT>(now.v[k][j]), e);
-                *reinterpret_cast<half8 *>(a.q_hi + row * kHeadDim + 16 * k + 8 * h) = y;
+            for (int kb = 0; kb < 4; ++kb) {
+                const int off = (16 * cb + n) * kRotPt + 32 * kb + 8 * g;
+                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_hi + off), q[kb], y[cb]);
+                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + off), q[kb], y[cb]);
             }
-            if (h == 0)
-                a.q_factor[row] = __builtin_ldexpf(a.score_scale_log2, -e);
-        } else {
-            const int e = finite ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
-            half8 x[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    x[k][j] = (_Float16)__builtin_ldexpf(to_float<InT>(now.v[k][j]), e);
-            // accumulator d, register 4 u + i: dim 8 (8 (u % 2) + 4 h + i) + 2 d + u / 2 of row c
-            floatx16 y[4];
-            float top = 0.f;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    y[d][k] = 0.f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int off = (32 * d + c) * kRotPt + 16 * k + 8 * h;
-                    y[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(pt_hi + off), x[k], y[d]);
-                    y[d] = prefix::mfma32(*reinterpret_cast<const half8 *>(pt_lo + off), x[k], y[d]);
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    y[d][k] = __builtin_ldexpf(y[d][k], -e) * a.score_scale_log2;
-                    top = fmaxf(top, fabsf(y[d][k]));
-                }
-            top = row_max(top);
-            const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-            if (row >= rows)
-                continue;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    half8 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float v = __builtin_ldexpf(y[j >> 1][8 * (j & 1) + 4 * u + i], f);
-                        asm("" : "+v"(v));  // (rounded once: hi and lo belong together)
-                        hi[j] = (_Float16)v;
-                        lo[j] = (_Float16)(v - (float)hi[j]);
-                    }
-                    const int64_t at = row * kHeadDim + 8 * (8 * u + 4 * h + i);
-                    *reinterpret_cast<half8 *>(a.q_hi + at) = hi;
-                    if constexpr (LO)
-                        *reinterpret_cast<half8 *>(a.q_lo + at) = lo;
-                }
-            if (h == 0)
-                a.q_factor[row] = __builtin_ldexpf(1.f, -f);
         }
+        float top = 0.f;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                y[cb][i] = __builtin_ldexpf(y[cb][i], -e) * a.score_scale_log2;
+                top = fmaxf(top, fabsf(y[cb][i]));
+            }
+        top = rot_row_max(top);
+        const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        if (r0 + n >= rows)
+            return;
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) {
+            half4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = __builtin_ldexpf(y[cb][i], f);
+                asm("" : "+v"(v));  // (rounded once: hi and lo belong together)
+                hi[i] = (_Float16)v;
+                lo[i] = (_Float16)(v - (float)hi[i]);
+            }
+            *reinterpret_cast<half4 *>(a.q_hi + ra * kHeadDim + 16 * cb + 4 * g) = hi;
+            if constexpr (LO)
+                *reinterpret_cast<half4 *>(a.q_lo + ra * kHeadDim + 16 * cb + 4 * g) = lo;
+        }
+        if (g == 0)
+            a.q_factor[ra] = __builtin_ldexpf(1.f, -f);
     }
 }
 
@@ -324,58 +305,62 @@ template <int LAYOUT, bool KF8, bool KB3, bool V3> struct Codes {
 struct Raw {
     uint4 a, b;  // codes; K: norm (FP8 keys: the codes' second half), V: scales and zeros
 };
-// The wave's 16 tokens: their records of the kv-head, and (SoA) its scalars.
+// The wave's 16 tokens: their records of the kv-head, and (SoA) its scalars, as buffers: a lane's offset in them is the
+// same in every tile, so that no address is worked out in vector registers.
 struct Place {
-    const uint8_t *data, *meta;
+    __amdgpu_buffer_rsrc_t data, meta;
 };
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const uint8_t *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, 0x7FFFFFFF, 0x00020000);
+}
+__device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t b, uint32_t at, int more) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)at, more, 0));
+}
+__device__ __forceinline__ uint4 load12(__amdgpu_buffer_rsrc_t b, uint32_t at, int more) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b96(b, (int)at, more, 0);
+    return uint4{(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], 0u};
+}
+__device__ __forceinline__ uint2 load8(__amdgpu_buffer_rsrc_t b, uint32_t at, int more) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(b, (int)at, more, 0));
+}
+__device__ __forceinline__ uint32_t load4(__amdgpu_buffer_rsrc_t b, uint32_t at, int more) {
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, (int)at, more, 0);
+}
+__device__ __forceinline__ uint32_t load2(__amdgpu_buffer_rsrc_t b, uint32_t at, int more) {
+    return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, (int)at, more, 0);
+}
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
 __device__ __forceinline__ Place place_of(const Args &a, int kvh, int blk, int within) {
     using C = Codes<LAYOUT, KF8, KB3, V3>;
     const uint8_t *b = a.cache + (uint64_t)(uint32_t)blk * (uint32_t)a.block_stride;
     const int bs = 1 << a.block_size_log2;
-    return Place{b + (uint32_t)(within * a.slot_pos + kvh * a.slot_head),
-                 LAYOUT == 0 ? b + (uint32_t)(bs * a.num_kv_heads * C::rec + 2 * (kvh * C::nf * bs + within)) : nullptr};
+    const uint8_t *data = b + (uint32_t)(within * a.slot_pos + kvh * a.slot_head);
+    const uint8_t *meta = LAYOUT == 0 ? b + (uint32_t)(bs * a.num_kv_heads * C::rec + 2 * (kvh * C::nf * bs + within)) : data;
+    return Place{buffer_at(data), buffer_at(meta)};
 }
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
 __device__ __forceinline__ void load_k(Raw &r, const Args &a, const Place &at, int lane) {
     using C = Codes<LAYOUT, KF8, KB3, V3>;
     const uint32_t token = (uint32_t)(lane >> 2) * (uint32_t)a.slot_pos, part = token + (lane & 3) * (C::kbytes / 4);
-    if constexpr (KB3) {
-        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(at.data + part);
-        r.a = uint4{w[0], w[1], w[2], 0u};
-    } else {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part);
-        r.a = uint4{w[0], w[1], w[2], w[3]};
-    }
-    if constexpr (KF8) {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part + 16);
-        r.b = uint4{w[0], w[1], w[2], w[3]};
-    } else if constexpr (LAYOUT == 0) {
-        r.b.x = *reinterpret_cast<const uint16_t *>(at.meta + 2u * (lane >> 2));
-    } else {
-        r.b.x = *reinterpret_cast<const uint16_t *>(at.data + token + C::kbytes);
-    }
+    r.a = KB3 ? load12(at.data, part, 0) : load16(at.data, part, 0);
+    if constexpr (KF8)
+        r.b = load16(at.data, part, 16);
+    else
+        r.b.x = LAYOUT == 0 ? load2(at.meta, 2u * (lane >> 2), 0) : load2(at.data, token, C::kbytes);
 }
 // (a: the lane's token's codes, 32 dims; b.xy or b.x: scales and zeros, see exchange)
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
 __device__ __forceinline__ void load_v(Raw &r, const Args &a, const Place &at, int lane) {
     using C = Codes<LAYOUT, KF8, KB3, V3>;
     const int row = lane >> 4, quad = (lane >> 2) & 3, j = lane & 3;
-    const uint32_t token = (uint32_t)(4 * quad + row) * (uint32_t)a.slot_pos + C::v0;
-    if constexpr (V3) {
-        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(at.data + token + 12 * j);
-        r.a = uint4{w[0], w[1], w[2], 0u};
-    } else {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + token + 16 * j);
-        r.a = uint4{w[0], w[1], w[2], w[3]};
-    }
+    const uint32_t token = (uint32_t)(4 * quad + row) * (uint32_t)a.slot_pos;
+    r.a = V3 ? load12(at.data, token + 12 * j, C::v0) : load16(at.data, token + 16 * j, C::v0);
     if constexpr (LAYOUT == 0) {  // even rows the four tokens' scales, odd rows their zeros
-        const uint8_t *m = at.meta + (uint32_t)((C::nf - 2) * 2 << a.block_size_log2);
-        const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(m + ((uint32_t)(row & 1) << (a.block_size_log2 + 1)) + 8u * quad);
-        r.b.x = s[0];
-        r.b.y = s[1];
+        const uint2 s = load8(at.meta, ((uint32_t)(row & 1) << (a.block_size_log2 + 1)) + 8u * quad, (C::nf - 2) * 2 << a.block_size_log2);
+        r.b.x = s.x;
+        r.b.y = s.y;
     } else {  // the token's own
-        r.b.x = *reinterpret_cast<const prefix::u32a2 *>(at.data + token + C::vbytes);
+        r.b.x = load4(at.data, token, C::v0 + C::vbytes);
     }
 }
 // Swaps x of the odd rows of 16 lanes with y of the even rows before them; of the upper two rows with the lower two.
@@ -491,6 +476,17 @@ template <int LAYOUT, bool KF8, bool KB3, bool FINE> struct KUnit {
     }
 };
 
+// Of pairs of f16: the larger magnitudes, as whole numbers (NaN and infinities above all others); of one, the larger.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t most_of(uint32_t x, uint32_t y) {
+    auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7FFF7FFFu); };
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(mag(x), mag(y)));
+}
+__device__ __forceinline__ uint32_t top_of(uint32_t x) {
+    const u16x2 v = __builtin_bit_cast(u16x2, x);
+    return v[0] > v[1] ? v[0] : v[1];
+}
+
 // A unit of V into LDS: begin() takes its scalars, write(m) dims 2 m and 2 m + 1 of it.
 template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
     half2v s01, s23, z01, z23;
@@ -509,10 +505,7 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
         }
         // magnitudes as whole numbers: scales of 2048 or zeros of 16384 and more might pass f16's range together
         // (FINE: scales of 128 and more times weights); NaN and infinities are above those
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7FFF7FFFu); };
-        const u16x2 ms = __builtin_elementwise_max(mag(s[0]), mag(s[1])), mz = __builtin_elementwise_max(mag(z[0]), mag(z[1]));
-        const uint32_t top_s = ms[0] > ms[1] ? ms[0] : ms[1], top_z = mz[0] > mz[1] ? mz[0] : mz[1];
+        const uint32_t top_s = top_of(most_of(s[0], s[1])), top_z = top_of(most_of(z[0], z[1]));
         const bool special = __any(top_s >= (FINE ? 0x5800u : 0x6800u) || top_z >= (FINE ? 0x7C00u : 0x7400u));
         float scale[4], zero[4];
         if (FINE || special)

@@ -85,8 +85,8 @@ template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq
 template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
     const int64_t rows = (int64_t)p.tokens * p.num_q_heads;
-    // (two workgroups' rotation matrices fit into a CU's LDS; the last workgroup makes the plan)
-    const dim3 grid((unsigned)(std::min<int64_t>((rows + kStartRows - 1) / kStartRows, (KF8 ? 8 : 2) * cus()) + 1)), block(kStartThreads);
+    // (the first workgroup makes the plan)
+    const dim3 grid((unsigned)((rows + kStartRows - 1) / kStartRows + 1)), block(kStartThreads);
     if (p.q_dtype == TQ4_BF16)
         launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p);
     else

@@ -31,33 +31,25 @@ __device__ __forceinline__ void few_load(FewRaw<LAYOUT, KF8> &r, const Args &a, 
     using C = Codes<LAYOUT, KF8, KB3, V3>;
     const int n = lane & 15, g = lane >> 4;
     const uint32_t token = (uint32_t)n * (uint32_t)a.slot_pos, part = token + g * (C::kbytes / 4);
-    if constexpr (KB3) {
-        const prefix::u32x3a2 w = *reinterpret_cast<const prefix::u32x3a2 *>(at.data + part);
-        r.k[half] = uint4{w[0], w[1], w[2], 0u};
-    } else {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part);
-        r.k[half] = uint4{w[0], w[1], w[2], w[3]};
-    }
-    if constexpr (KF8) {
-        const prefix::u32x4a2 w = *reinterpret_cast<const prefix::u32x4a2 *>(at.data + part + 16);
-        r.k2[half] = uint4{w[0], w[1], w[2], w[3]};
-    }
-    const uint32_t quad = (uint32_t)(4 * g) * (uint32_t)a.slot_pos + C::v0 + (V3 ? 3 : 4) * n;
+    r.k[half] = KB3 ? load12(at.data, part, 0) : load16(at.data, part, 0);
+    if constexpr (KF8)
+        r.k2[half] = load16(at.data, part, 16);
+    const uint32_t quad = (uint32_t)(4 * g) * (uint32_t)a.slot_pos + (V3 ? 3 : 4) * n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        r.v[4 * half + i] = *reinterpret_cast<const prefix::u32a1 *>(at.data + (uint32_t)(i * a.slot_pos) + quad);
+        r.v[4 * half + i] = load4(at.data, quad, i * a.slot_pos + C::v0);
     if constexpr (LAYOUT == 0) {
 #pragma unroll
         for (int f = 0; f < C::nf; ++f) {
-            const u32x2a8 s = *reinterpret_cast<const u32x2a8 *>(at.meta + ((uint32_t)(2 * f) << a.block_size_log2) + 8u * g);
+            const uint2 s = load8(at.meta, 8u * g, (2 * f) << a.block_size_log2);
             const int to = f + 3 - C::nf;
-            r.s[4 * to + 2 * half] = s[0];
-            r.s[4 * to + 2 * half + 1] = s[1];
+            r.s[4 * to + 2 * half] = s.x;
+            r.s[4 * to + 2 * half + 1] = s.y;
         }
     } else {
         if constexpr (!KF8)
-            r.s[half] = *reinterpret_cast<const uint16_t *>(at.data + token + C::kbytes);
-        r.s[2 + half] = *reinterpret_cast<const prefix::u32a2 *>(at.data + token + C::v0 + C::vbytes);
+            r.s[half] = load2(at.data, token, C::kbytes);
+        r.s[2 + half] = load4(at.data, token, C::v0 + C::vbytes);
     }
 }
 
@@ -293,6 +285,17 @@ void chunk_few_kernel(const Args a) {
                     }
                 }
             }
+            // scales of 128 and more, and what is not finite (of tokens past the sequence too, which then costs time only)
+            uint32_t top_s, top_z;
+            if constexpr (LAYOUT == 0) {
+                top_s = top_of(most_of(most_of(raw.s[4], raw.s[5]), most_of(raw.s[6], raw.s[7])));
+                top_z = top_of(most_of(most_of(raw.s[8], raw.s[9]), most_of(raw.s[10], raw.s[11])));
+            } else {
+                const uint32_t m = most_of(raw.s[2], raw.s[3]);
+                top_s = m & 0xFFFFu;
+                top_z = m >> 16;
+            }
+            const bool special = __any(top_s >= 0x5800u || top_z >= 0x7C00u);
             // (the codes are used up)
             load(i + 1);
             read_pages(i + 2);
@@ -303,14 +306,6 @@ void chunk_few_kernel(const Args a) {
                 for (int x = 0; x < 8; ++x)
                     if (t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= seq.len)
                         scale[x] = mid[x] = 0.f;
-            float top_scale = 0.f;
-            bool odd = false;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                top_scale = fmaxf(top_scale, fabsf(scale[x]));
-                odd |= !(fabsf(mid[x]) < __builtin_inff());
-            }
-            const bool special = __any(odd || !(top_scale < xdl::kLargeScale));
             const float most = special ? 1.f : 256.f;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
