@@ -62,28 +62,48 @@ constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows =
 constexpr double kLeast = 4.0;
 constexpr int kSnap = 2;
 
-// One workgroup: the work before each sequence, and from it every workgroup's place in the list.
-__device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
+// One workgroup: the work before each sequence, and from it every workgroup's place in the list.  (Batches of up to
+// kPlanned sequences are planned in LDS: 64 sequences 8 us in the workspace, 4 so.)
+constexpr int kPlanned = 1024;
+struct PlanLds {
+    double sums[kStartThreads], work[kPlanned + 1];
+    Seq seqs[kPlanned];
+};
+__device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
     const int tid = threadIdx.x, per = (a.batch + kStartThreads - 1) / kStartThreads;
     const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-    auto seq = [&](int b) { return seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest); };
+    const bool small = a.batch <= kPlanned;
+    double *work = small ? lds.work : a.work, *sums = lds.sums;
     double own = 0;
-    for (int b = b0; b < b1; ++b)
-        own += work_of(a.shape, seq(b));
-    sums[tid] = own;
-    __syncthreads();
-    for (int d = 1; d < kStartThreads; d <<= 1) {
-        const double before = tid >= d ? sums[tid - d] : 0.0;
-        __syncthreads();
-        sums[tid] += before;
-        __syncthreads();
-    }
-    double at = tid > 0 ? sums[tid - 1] : 0.0;
     for (int b = b0; b < b1; ++b) {
-        a.work[b] = at;
-        at += work_of(a.shape, seq(b));
+        const Seq q = seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest);
+        if (small)
+            lds.seqs[b] = q;
+        work[b] = work_of(a.shape, q);
+        own += work[b];
     }
-    const double total = sums[kStartThreads - 1];
+    auto seq = [&](int b) { return small ? lds.seqs[b] : seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest); };
+    // sums over the threads before this one
+    double at = own;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const double x = __shfl_up(at, d, kWave);
+        at += (tid & (kWave - 1)) >= d ? x : 0.0;
+    }
+    if ((tid & (kWave - 1)) == kWave - 1)
+        sums[tid / kWave] = at;
+    __syncthreads();
+    double total = 0;
+    for (int w = 0; w < kStartWaves; ++w) {
+        at += w < tid / kWave ? sums[w] : 0.0;
+        total += sums[w];
+    }
+    at -= own;
+    for (int b = b0; b < b1; ++b) {
+        const double x = work[b];
+        work[b] = at;
+        at += x;
+    }
     __syncthreads();
     const int used = max(1, (int)fmin((double)a.groups, total / kLeast));
     for (int w = tid; w <= a.groups; w += kStartThreads) {
@@ -93,15 +113,15 @@ __device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
             int lo = 0, hi = a.batch - 1;  // the last sequence with as little before it
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
-                if (a.work[mid] <= target)
+                if (work[mid] <= target)
                     lo = mid;
                 else
                     hi = mid - 1;
             }
-            Seq q = seq(lo);
+            const Seq q = seq(lo);
             c = Cut{lo, 0, 0, 0};
             if (q.n > 0 && w > 0)
-                c = cut_in(a.shape, q, lo, target - a.work[lo], kSnap);
+                c = cut_in(a.shape, q, lo, target - work[lo], kSnap);
             if (c.at == 0 && c.r == 0 && c.h == 0)
                 while (c.b < a.batch && seq(c.b).n == 0)
                     ++c.b;
@@ -119,10 +139,13 @@ __device__ __forceinline__ void plan_cuts(const Args &a, double *sums) {
 template <typename InT, bool KF8, bool LO>
 __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
-    __shared__ __align__(16) _Float16 pt_hi[PT], pt_lo[PT];
+    __shared__ __align__(16) union {
+        _Float16 pt[2][PT];
+        PlanLds plan;
+    } lds;
+    _Float16 *pt_hi = lds.pt[0], *pt_lo = lds.pt[1];
     if (blockIdx.x == 0) {
-        __shared__ double sums[kStartThreads];
-        plan_cuts(a, sums);
+        plan_cuts(a, lds.plan);
         return;
     }
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, n = lane & 15, g = lane >> 4;
@@ -487,6 +510,26 @@ __device__ __forceinline__ uint32_t top_of(uint32_t x) {
     return v[0] > v[1] ? v[0] : v[1];
 }
 
+// Dims 2 m and 2 m + 1 of two tokens' eight codes, less `less`, as f16 pairs: the code is put into the significand of 1024, or,
+// where it lies four bits up, of 64, whose last place there is a sixteenth; then that is taken off.
+template <bool V3>
+__device__ __forceinline__ void code_values(uint32_t a, uint32_t b, int m, float less, half2v &even, half2v &odd) {
+    if constexpr (V3) {
+        auto value = [&](int i) {
+            const uint32_t pair = ((a >> (3 * i)) & 7u) | (((b >> (3 * i)) & 7u) << 16);
+            return prefix::as_half2(pair | 0x64006400u) - prefix::splat((_Float16)(1024.f + less));
+        };
+        even = value(2 * m);
+        odd = value(2 * m + 1);
+    } else {
+        uint32_t low = 0x64006400u, high = 0x54005400u;
+        asm("" : "+v"(low), "+v"(high));
+        const uint32_t p = __builtin_amdgcn_perm(b, a, (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u);
+        even = prefix::as_half2((p & 0x000F000Fu) | low) - prefix::splat((_Float16)(1024.f + less));
+        odd = prefix::as_half2((p & 0x00F000F0u) | high) - prefix::splat((_Float16)(64.f + less));
+    }
+}
+
 // A unit of V into LDS: begin() takes its scalars, write(m) dims 2 m and 2 m + 1 of it.
 template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
     half2v s01, s23, z01, z23;
@@ -551,31 +594,21 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
             z23 = prefix::as_half2(z[1]);
         }
     }
-    // codes to f16: into the significand of 1024, then less 1024 (FINE: less 1024 and the middle code)
+    // codes to f16 (see code_values), FINE: less the middle code
     __device__ __forceinline__ void write(unsigned char *to, int m) {
-        const half2v k0 = prefix::splat((_Float16)(1024.f + (FINE ? kMiddle<V3> : 0.f)));
-        uint32_t magic = 0x64006400u;
-        asm("" : "+v"(magic));
-        auto put = [&](int i, uint32_t c01, uint32_t c23, uint32_t mask) {
-            half2v x = prefix::as_half2((c01 & mask) | magic) - k0, y = prefix::as_half2((c23 & mask) | magic) - k0;
+        auto put = [&](int i, half2v x, half2v y) {
             if constexpr (!FINE) {
                 x = __builtin_elementwise_fma(x, s01, z01);
                 y = __builtin_elementwise_fma(y, s23, z23);
             }
             *reinterpret_cast<uint2 *>(to + 16 * i * VROW) = uint2{prefix::as_u32(x), prefix::as_u32(y)};
         };
-        if constexpr (V3) {
-#pragma unroll
-            for (int i = 2 * m; i < 2 * m + 2; ++i) {
-                auto pair = [&](int t) { return ((v[t] >> (3 * i)) & 7u) | (((v[t + 1] >> (3 * i)) & 7u) << 16); };
-                put(i, pair(0), pair(2), 0xFFFFFFFFu);
-            }
-        } else {
-            const uint32_t sel = (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u;
-            const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel), p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
-            put(2 * m, p01, p23, 0x000F000Fu);
-            put(2 * m + 1, p01 >> 4, p23 >> 4, 0x000F000Fu);
-        }
+        constexpr float less = FINE ? kMiddle<V3> : 0.f;
+        half2v x0, x1, y0, y1;
+        code_values<V3>(v[0], v[1], m, less, x0, x1);
+        code_values<V3>(v[2], v[3], m, less, y0, y1);
+        put(2 * m, x0, y0);
+        put(2 * m + 1, x1, y1);
     }
 };
 

@@ -27,13 +27,19 @@ template <int LAYOUT, bool KF8> struct FewRaw {
     uint32_t s[LAYOUT == 0 ? 12 : 4];
 };
 template <int LAYOUT, bool KF8, bool KB3, bool V3>
-__device__ __forceinline__ void few_load(FewRaw<LAYOUT, KF8> &r, const Args &a, const Place &at, int half, int lane) {
+__device__ __forceinline__ void few_load_k(FewRaw<LAYOUT, KF8> &r, const Args &a, const Place &at, int half, int lane) {
     using C = Codes<LAYOUT, KF8, KB3, V3>;
     const int n = lane & 15, g = lane >> 4;
     const uint32_t token = (uint32_t)n * (uint32_t)a.slot_pos, part = token + g * (C::kbytes / 4);
     r.k[half] = KB3 ? load12(at.data, part, 0) : load16(at.data, part, 0);
     if constexpr (KF8)
         r.k2[half] = load16(at.data, part, 16);
+}
+template <int LAYOUT, bool KF8, bool KB3, bool V3>
+__device__ __forceinline__ void few_load_v(FewRaw<LAYOUT, KF8> &r, const Args &a, const Place &at, int half, int lane) {
+    using C = Codes<LAYOUT, KF8, KB3, V3>;
+    const int n = lane & 15, g = lane >> 4;
+    const uint32_t token = (uint32_t)n * (uint32_t)a.slot_pos;
     const uint32_t quad = (uint32_t)(4 * g) * (uint32_t)a.slot_pos + (V3 ? 3 : 4) * n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -102,17 +108,22 @@ void chunk_few_kernel(const Args a) {
             }
         };
         FewRaw<LAYOUT, KF8> raw;
-        auto load = [&](int i) __attribute__((always_inline)) {
+        auto load = [&](int i, auto k_too, auto v_too) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const Place p = place_of<LAYOUT, KF8, KB3, V3>(a, kvh, __builtin_amdgcn_readfirstlane(blk[k]),
                                                                (first_of(i) + 16 * k) & ((1 << a.block_size_log2) - 1));
-                few_load<LAYOUT, KF8, KB3, V3>(raw, a, p, k, lane);
+                if constexpr (k_too)
+                    few_load_k<LAYOUT, KF8, KB3, V3>(raw, a, p, k, lane);
+                if constexpr (v_too)
+                    few_load_v<LAYOUT, KF8, KB3, V3>(raw, a, p, k, lane);
             }
         };
+        const std::integral_constant<bool, true> yes;
+        const std::integral_constant<bool, false> no;
         if (n_tiles > 0) {
             read_pages(0);
-            load(0);
+            load(0, yes, yes);
             read_pages(1);
         }
         // the lane's rows
@@ -229,6 +240,7 @@ void chunk_few_kernel(const Args a) {
                         s[b][4 * k + x] = y[x];
                 }
             }
+            load(i + 1, yes, no);  // (its codes are used up: as early as may be)
             if constexpr (LAYOUT == 0) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -260,29 +272,17 @@ void chunk_few_kernel(const Args a) {
             // V's codes less the middle one: dim 8 n + d, the lane's eight tokens
             half8 v[8];
             {
-                const half2v k0 = prefix::splat((_Float16)(1024.f + kMiddle<V3>));
-                uint32_t magic = 0x64006400u;
-                asm("" : "+v"(magic));
-                auto value = [&](uint32_t codes) { return prefix::as_u32(prefix::as_half2(codes | magic) - k0); };
-                if constexpr (V3) {
 #pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        auto pair = [&](int t) { return ((raw.v[t] >> (3 * d)) & 7u) | (((raw.v[t + 1] >> (3 * d)) & 7u) << 16); };
-                        v[d] = xdl::as_half8(value(pair(0)), value(pair(2)), value(pair(4)), value(pair(6)));
-                    }
-                } else {
+                for (int m = 0; m < 4; ++m) {
+                    half2v even[4], odd[4];
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        const uint32_t sel = (uint32_t)m | 0x0C00u | ((uint32_t)(4 + m) << 16) | 0x0C000000u;
-                        uint32_t p[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-                            p[t] = __builtin_amdgcn_perm(raw.v[2 * t + 1], raw.v[2 * t], sel);
-                        v[2 * m] = xdl::as_half8(value(p[0] & 0x000F000Fu), value(p[1] & 0x000F000Fu), value(p[2] & 0x000F000Fu),
-                                                 value(p[3] & 0x000F000Fu));
-                        v[2 * m + 1] = xdl::as_half8(value((p[0] >> 4) & 0x000F000Fu), value((p[1] >> 4) & 0x000F000Fu),
-                                                     value((p[2] >> 4) & 0x000F000Fu), value((p[3] >> 4) & 0x000F000Fu));
-                    }
+                    for (int t = 0; t < 4; ++t)
+                        code_values<V3>(raw.v[2 * t], raw.v[2 * t + 1], m, kMiddle<V3>, even[t], odd[t]);
+                    auto pack = [](const half2v(&x)[4]) {
+                        return xdl::as_half8(prefix::as_u32(x[0]), prefix::as_u32(x[1]), prefix::as_u32(x[2]), prefix::as_u32(x[3]));
+                    };
+                    v[2 * m] = pack(even);
+                    v[2 * m + 1] = pack(odd);
                 }
             }
             // scales of 128 and more, and what is not finite (of tokens past the sequence too, which then costs time only)
@@ -296,8 +296,7 @@ void chunk_few_kernel(const Args a) {
                 top_z = m >> 16;
             }
             const bool special = __any(top_s >= 0x5800u || top_z >= 0x7C00u);
-            // (the codes are used up)
-            load(i + 1);
+            load(i + 1, no, yes);
             read_pages(i + 2);
             const bool masked = t0 + 32 > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
             // tokens past the sequence: their bytes may hold anything
@@ -380,7 +379,7 @@ void chunk_few_kernel(const Args a) {
             const int t0 = first_of(i);
             // (no row of the tile sees a token of the wave's)
             if (t0 >= limit_hi || (a.shape.window && t0 >= a.shape.first && t0 + 32 <= limit_lo - a.shape.window)) {
-                load(i + 1);
+                load(i + 1, yes, yes);
                 read_pages(i + 2);
             } else {
                 tile(i);
