@@ -877,16 +877,21 @@ def merge_states(out_a, lse_a, out_b, lse_b, *, out=None, lse=None):
     A result over no tokens (LSE -inf) counts as nothing, whatever its rows hold; two of them give zeros and -inf.
     ``out`` and ``lse`` are new tensors where none are given, and may be an input.
     """
-    _require(out_a.is_cuda and out_a.dtype in DTYPES and out_a.dim() >= 1 and out_a.size(-1) == HEAD_DIM,
-             f"out_a must be [..., {HEAD_DIM}]")
-    out = torch.empty_like(out_a, memory_format=torch.contiguous_format) if out is None else out
-    lse = torch.empty_like(lse_a, memory_format=torch.contiguous_format) if lse is None else lse
-    for t, name in ((out_a, "out_a"), (out_b, "out_b"), (out, "out")):
-        _check_tensor(t, name, out_a.dtype)
-        _require(t.shape == out_a.shape, "out_a, out_b and out must have one shape")
-    for t, name in ((lse_a, "lse_a"), (lse_b, "lse_b"), (lse, "lse")):
+    if not (out_a.is_cuda and out_a.dtype in DTYPES and out_a.dim() >= 1 and out_a.size(-1) == HEAD_DIM):
+        raise RuntimeError(f"out_a must be [..., {HEAD_DIM}] of fp32, bf16 or fp16, CUDA")
+    dtype, shape = out_a.dtype, out_a.shape
+    _check_tensor(out_a, "out_a", dtype)
+    _check_tensor(lse_a, "lse_a", torch.float32)
+    out = torch.empty_like(out_a) if out is None else out
+    lse = torch.empty_like(lse_a) if lse is None else lse
+    for t, name in ((out_b, "out_b"), (out, "out")):
+        _check_tensor(t, name, dtype)
+        _require(t.shape == shape, "out_a, out_b and out must have one shape")
+    rows = shape[:-1]
+    for t, name in ((lse_b, "lse_b"), (lse, "lse")):
         _check_tensor(t, name, torch.float32)
-        _require(t.shape == out_a.shape[:-1], "lse_a, lse_b and lse must be [...] of out_a [..., D]")
+    _require(lse_a.shape == rows and lse_b.shape == rows and lse.shape == rows,
+             "lse_a, lse_b and lse must be [...] of out_a [..., D]")
     _require(_same_device(out_a, out_b, out, lse_a, lse_b, lse), "all tensors must be on the same device")
     if lse.numel() == 0:
         return out, lse
