@@ -131,8 +131,9 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
 }
 
 // Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two
-// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range are scaled down and q_factor
-// undoes it.  FP8 keys: the row itself, scaled by the power of two that puts its largest magnitude in [0.5, 1): exact.
+// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range, or lie below 2^-8 near its
+// denormals, are scaled to its top and q_factor undoes it.  FP8 keys: the row itself, scaled by the power of two that
+// puts its largest magnitude in [0.5, 1): exact for dims down to 2^-13 of it, below that to 2^-25 of it.
 // 8192 x 32 rows: 53 us.  A form whose workgroups stage rot_t once and take one row tile after the other (32x32x16
 // products) took 39, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
 // clock through chunk_kernel (634 : 720 us, the same code).
@@ -227,7 +228,8 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
                 top = fmaxf(top, fabsf(y[cb][i]));
             }
         top = rot_row_max(top);
-        const int f = (top >= 32768.f && top < __builtin_inff()) ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        const bool small = top > 0.f && top < 0x1p-8f, large = top >= 32768.f && top < __builtin_inff();
+        const int f = small || large ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
         if (r0 + n >= rows)
             return;
         typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -830,8 +832,9 @@ void chunk_kernel(const Args a) {
             special = __builtin_amdgcn_readfirstlane(special);
             const bool masked = t0 + 32 * kAtOnce > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
             // The scores in log2 units, less the running maximum.  That one moves when the weights' sum passes `most`: a weight
-            // is then at most 2^13, in f16's range (FINE: times a scale of up to 128; with a larger one in the tile at most 1).
-            const float most = !FINE ? 8192.f : special ? 1.f : 256.f;
+            // is then at most 2^13, in f16's range (1024 where it may be multiplied by 1 / kShrink; FINE: 256 times a scale
+            // of up to 128, with a larger one in the tile 1).
+            const float most = FINE ? (special ? 1.f : 256.f) : special ? 1024.f : 8192.f;
             const bool fresh = __any(negm == __FLT_MAX__);  // rows that have seen nothing yet
             const float less = fresh ? 0.f : negm;
 #pragma unroll

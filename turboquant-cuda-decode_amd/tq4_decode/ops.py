@@ -784,7 +784,7 @@ def chunk_attention(query, rotation_t, kv_cache, block_table, seq_lens, query_st
     _require(D == HEAD_DIM, _QUERY_SHAPE)
     s0, s1, s2 = query.stride()
     _require(s2 == 1 and (s1 == D or Hq == 1), "query: heads must be contiguous")
-    stride = max(s0, Hq * D) if T <= 1 else s0
+    stride = Hq * D if T <= 1 else s0
     out_dtype = query.dtype if out_dtype is None else out_dtype
     _check_tensor(block_table, "block_table", torch.int32)
     _check_tensor(seq_lens, "seq_lens", torch.int32)
