@@ -117,6 +117,9 @@ int tq4_merge_states(const void *out_a, const float *lse_a, const void *out_b, c
         return fail(TQ4_E_UNSUPPORTED, "%s: head_dim %d unsupported (128)", what, D);
     if (!aligned(out_a, 16) || !aligned(out_b, 16) || !aligned(out, 16))
         return fail(TQ4_E_INVALID, "%s: out_a, out_b and out must be 16-byte aligned", what);
+    constexpr int64_t per = tq4::load::kThreads / 16 * tq4::load::kJoinRows;  // rows of a workgroup
+    if (rows > per * 0x7FFFFFFF)
+        return fail(TQ4_E_UNSUPPORTED, "%s: %lld rows are too many", what, (long long)rows);
     const int64_t bytes = rows * D * (dtype == TQ4_F32 ? 4 : 2);
     // in place is fine, partly is not
     const bool shifted = (out != out_a && overlap(out, bytes, out_a, bytes)) || (out != out_b && overlap(out, bytes, out_b, bytes)) ||
@@ -127,10 +130,7 @@ int tq4_merge_states(const void *out_a, const float *lse_a, const void *out_b, c
                        overlap(lse, 4 * rows, out_b, bytes);
     if (shifted || mixed)
         return fail(TQ4_E_INVALID, "%s: outputs may be one of the inputs, but not overlap them otherwise", what);
-    const int64_t per = tq4::load::kThreads / 16 * tq4::load::kJoinRows, groups = (rows + per - 1) / per;
-    if (groups > 0x7FFFFFFF)
-        return fail(TQ4_E_UNSUPPORTED, "%s: %lld rows are too many", what, (long long)rows);
-    const dim3 grid((unsigned)groups), block(tq4::load::kThreads);
+    const dim3 grid((unsigned)((rows + per - 1) / per)), block(tq4::load::kThreads);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     auto go = [&](auto zero) {
         using T = decltype(zero);

@@ -58,9 +58,6 @@ struct Args {
 // ---- Queries and cuts ------------------------------------------------------------------------
 
 constexpr int kStartWaves = 4, kStartThreads = kWave * kStartWaves, kStartRows = 16 * kStartWaves;
-// The least work that a workgroup is given, in token tiles.
-constexpr double kLeast = 4.0;
-constexpr int kSnap = 2;
 
 // One workgroup: the work before each sequence, and from it every workgroup's place in the list.  (Batches of up to
 // kPlanned sequences are planned in LDS: 64 sequences 8 us in the workspace, 4 so.)
@@ -105,29 +102,9 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
         at += x;
     }
     __syncthreads();
-    const int used = max(1, (int)fmin((double)a.groups, total / kLeast));
-    for (int w = tid; w <= a.groups; w += kStartThreads) {
-        Cut c{a.batch, 0, 0, 0};
-        if (w < used && total > 0) {
-            const double target = total * w / used;
-            int lo = 0, hi = a.batch - 1;  // the last sequence with as little before it
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (work[mid] <= target)
-                    lo = mid;
-                else
-                    hi = mid - 1;
-            }
-            const Seq q = seq(lo);
-            c = Cut{lo, 0, 0, 0};
-            if (q.n > 0 && w > 0)
-                c = cut_in(a.shape, q, lo, target - work[lo], kSnap);
-            if (c.at == 0 && c.r == 0 && c.h == 0)
-                while (c.b < a.batch && seq(c.b).n == 0)
-                    ++c.b;
-        }
-        a.cuts[w] = c;
-    }
+    const int used = groups_used(total, a.groups);
+    for (int w = tid; w <= a.groups; w += kStartThreads)
+        a.cuts[w] = cut_of(a.shape, seq, work, a.batch, total, used, w);
 }
 
 // Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two

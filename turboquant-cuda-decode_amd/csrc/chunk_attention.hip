@@ -1,5 +1,6 @@
 // Attention of several new tokens per sequence (tq4_chunk_attention, include/tq4_decode.h).
 #include <algorithm>
+#include <cmath>
 
 #include "abi.h"
 #include "chunk_few.h"
@@ -144,6 +145,8 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
         return fail(TQ4_E_UNSUPPORTED, "%s: block stride %lld above 2^31 - 1", what, (long long)cache_block_stride);
     if (!aligned(out, 16))
         return fail(TQ4_E_INVALID, "%s: out must be 16-byte aligned", what);
+    if (!(attn_scale < INFINITY))
+        return fail(TQ4_E_INVALID, "%s: attn_scale must be finite", what);
     if (window < 0 || first_tokens < 0 || (window > 0 && !causal))
         return fail(TQ4_E_INVALID, "%s: window (%d) and first_tokens (%d) must be at least 0, a window only with causal", what,
                     window, first_tokens);

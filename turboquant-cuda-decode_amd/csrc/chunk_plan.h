@@ -112,5 +112,36 @@ __device__ __forceinline__ Cut cut_in(const Shape &s, const Seq &q, int b, doubl
     return c;
 }
 
+// The least work that a workgroup is given, in token tiles: fewer workgroups than the grid's share a small call.
+constexpr double kLeast = 4.0;
+constexpr int kSnap = 2;
+__device__ __forceinline__ int groups_used(double total, int groups) {
+    const double n = total / kLeast;
+    return n < 1 ? 1 : n < groups ? (int)n : groups;
+}
+// Where workgroup w of `used` begins (w >= used: the end).  `seq(b)`: the sequences; work[b]: that of those before b.
+template <class SeqOf>
+__device__ __forceinline__ Cut cut_of(const Shape &s, SeqOf seq, const double *work, int batch, double total, int used, int w) {
+    if (w >= used || total <= 0)
+        return Cut{batch, 0, 0, 0};
+    const double target = total * w / used;
+    int lo = 0, hi = batch - 1;  // the last sequence with as little before it
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (work[mid] <= target)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const Seq q = seq(lo);
+    Cut c{lo, 0, 0, 0};
+    if (q.n > 0 && w > 0)
+        c = cut_in(s, q, lo, target - work[lo], kSnap);
+    if (c.at == 0 && c.r == 0 && c.h == 0)
+        while (c.b < batch && seq(c.b).n == 0)
+            ++c.b;
+    return c;
+}
+
 }  // namespace chunk
 }  // namespace tq4
