@@ -57,6 +57,10 @@ def attend(q, k, v, seen, sinks, scale, fine, rounded_keys):
                 var = RHO ** 2 * (MOST_FROM_MIDDLE ** 2 * p2.sum(-1, keepdims=True))
             else:     # V; the weight, whose sum is that of the rounded ones: an error of one moves the result by v - o
                 var = RHO ** 2 * (p2 @ seen_v ** 2 + spread(p2))
+                # or, for few rows, as `fine`: a lone token of value 0 has an exact v and v - o = 0, but its weight e times
+                # its scale s is rounded and meets the code's distance from the middle one, (v - middle) / s: off by
+                # RHO e |v - middle|, while the middle value and the sum have e itself
+                var = np.maximum(var, RHO ** 2 * MOST_FROM_MIDDLE ** 2 * p2.sum(-1, keepdims=True))
             if not fine and rounded_keys:
                 d2 = 2 * RHO ** 2 * ((qq ** 2) @ (k[:, h] ** 2).T) * scale ** 2
                 w = p2 * np.where(mask, d2, 0)

@@ -48,6 +48,8 @@ LENGTHS = [
     [(1, 1)], [(1, 333)], [(4, 337)], [(2, 2), (1, 64), (3, 65), (4, 63)], [(0, 10), (5, 17), (0, 0), (1, 4096)],
     [(8, 8), (7, 128), (1, 1000), (3, 129)], [(16, 700)], [(40, 40), (13, 500)], [(64, 64)], [(65, 190), (1, 30), (129, 129)],
     [(300, 300)], [(257, 1000), (90, 91)], [(700, 2000), (1, 5), (0, 7), (333, 333)],
+    # (more than 16 pairs of sequence and kv-head: row tiles of 64 and of 32 rows)
+    [(40, 200), (9, 64), (12, 12), (11, 333), (0, 5)] * 4, [(25, 130), (1, 900), (100, 101), (20, 64)] * 5,
 ]
 
 
@@ -62,7 +64,8 @@ def test_lengths(dev, pairs, hk, group):
 @pytest.mark.parametrize("preset", list(plain.PRESETS))
 @pytest.mark.parametrize("layout", ["soa", "aos", "aos_heads"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
-@pytest.mark.parametrize("pairs", [[(3, 130), (1, 77)], [(150, 333), (9, 200)], [(10, 100), (20, 20)]], ids=str)
+@pytest.mark.parametrize("pairs", [[(3, 130), (1, 77)], [(150, 333), (9, 200)], [(10, 100), (20, 20)],
+                                   [(10, 100), (20, 20), (11, 65)] * 4], ids=str)
 def test_presets(dev, preset, layout, dtype, pairs):
     b = Batch(7, pairs, 2, 4, bs=32, preset=preset, layout=layout, dtype=dtype)
     check(b, call(b, dev), "causal")
@@ -71,7 +74,7 @@ def test_presets(dev, preset, layout, dtype, pairs):
 
 
 @pytest.mark.parametrize("window,first", [(1, 0), (16, 0), (63, 1), (64, 64), (100, 5), (65, 130), (4096, 3), (1, 300)])
-@pytest.mark.parametrize("pairs", [[(1, 500), (3, 300)], [(20, 777)], [(200, 900), (130, 130)]], ids=str)
+@pytest.mark.parametrize("pairs", [[(1, 500), (3, 300)], [(20, 777)], [(200, 900), (130, 130)], [(20, 777), (9, 300)] * 5], ids=str)
 def test_windows(dev, window, first, pairs):
     b = Batch(11, pairs, 2, 4)
     check(b, call(b, dev, window=window, first=first), "window", window=window, first=first)

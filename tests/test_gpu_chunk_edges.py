@@ -14,8 +14,9 @@ from test_gpu_prefix_bits import scalars_of
 from tq4_decode import codebook, ops
 
 pytestmark = pytest.mark.gpu
-# few rows a sequence, 33 to 64, and more
-SIZES = pytest.mark.parametrize("pairs", [[(2, 333), (7, 90)], [(12, 300), (9, 130)], [(150, 420), (40, 77)]], ids=str)
+# row tiles of 32 rows, one and several a sequence; of 64 (more than 16 pairs of sequence and kv-head); of 256
+SIZES = pytest.mark.parametrize("pairs", [[(2, 333), (7, 90)], [(12, 300), (9, 130)], [(12, 300), (9, 130)] * 5,
+                                          [(150, 420), (40, 77)]], ids=str)
 
 
 def log_uniform(low, high):
@@ -75,7 +76,8 @@ def test_small_queries_of_large_keys(dev, pairs, lse):
     check(b, call(b, dev, lse=lse), "large queries", lse=lse)
 
 
-@pytest.mark.parametrize("pairs", [[(4, 333), (7, 90)], [(12, 300), (9, 130)], [(150, 420), (40, 77)]], ids=str)
+@pytest.mark.parametrize("pairs", [[(4, 333), (7, 90)], [(12, 300), (9, 130)], [(12, 300), (9, 130)] * 5,
+                                   [(150, 420), (40, 77)]], ids=str)
 @pytest.mark.parametrize("preset,layout", [("4bit", "soa"), ("4bit", "aos"), ("k8v4", "aos"), ("3bit", "soa")])
 @pytest.mark.parametrize("lse,window", [(False, 0), (True, 0), (False, 24), (True, 24)])
 def test_nans_that_a_row_does_not_see(dev, pairs, preset, layout, lse, window):

@@ -1077,19 +1077,33 @@ void chunk_kernel(const Args a) {
     }
 }
 
-// Joins the parts of a row tile that was cut: workgroup (w, i) rows of the one that workgroup w of chunk_kernel began and
-// did not end, PER of them per half wave.  Lane: dims 4 x .. +3 of its half's row.
-constexpr int kMergeThreads = 256, kMergeHalves = kMergeThreads / 32;
-template <typename OutT, int PER> __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(const Args a) {
-    const int w = blockIdx.x, x = threadIdx.x & 31, half = threadIdx.x >> 5;
+// Joins the parts of a row tile that was cut: workgroup (i, w) rows of the one that workgroup w of chunk_kernel began and
+// did not end, PER of them per half wave, four parts at a time.  Lane: dims 4 x .. +3 of its half's row.  Bound by the parts'
+// bytes: 8192 tokens of 32 heads 18.7 us (1, 4 and 8 rows per half wave: 21, 19.2, 23), 84 MB.  Consecutive workgroups
+// have the rows of one row tile: with w in their place the few row tiles of a lone sequence fell to one XCD (8 of them, 32 parts each:
+// 50 us, now 15).
+constexpr int kMergeThreads = 128, kMergeHalves = kMergeThreads / 32, kMergePer = 2;
+template <typename OutT> __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(const Args a) {
+    constexpr int PER = kMergePer;
+    const int w = blockIdx.y, x = threadIdx.x & 31, half = threadIdx.x >> 5;
     const Cut from = a.cuts[w], cut = a.cuts[w + 1];
     if (cut.b >= a.batch || cut.at == 0 || (same_tile(from, cut) && from.at > 0))
         return;
     const Seq seq = seq_of(a.starts, a.seq_lens, cut.b, a.tokens, a.longest);
-    const int rows = seq.n * a.shape.group, place0 = (blockIdx.y * kMergeHalves + half) * PER;
-    int parts = 2;  // part i: of workgroup w + i; the last is of the first whose own stretch ends in another row tile
-    while (same_tile(a.cuts[w + parts], cut))
-        ++parts;
+    const int rows = seq.n * a.shape.group, place0 = (blockIdx.x * kMergeHalves + half) * PER;
+    if (cut.r * a.shape.rows + (int)blockIdx.x * kMergeHalves * PER >= rows)
+        return;
+    // part i: of workgroup w + i; the last is of the first whose own stretch ends in another row tile (64 cuts at a time: one
+    // after the other 32 parts took 10 us)
+    int parts = 2;
+    for (;;) {
+        const uint64_t same = __ballot(same_tile(a.cuts[min(w + parts + (int)(threadIdx.x & 63), a.groups)], cut));
+        if (~same) {
+            parts += __builtin_ctzll(~same);
+            break;
+        }
+        parts += 64;
+    }
     auto slot = [&](int j) { return 2 * (w + j) + (j == 0 ? 1 : 0); };
     auto wrote = [&](int j) {  // (a workgroup without tiles wrote nothing)
         const Cut p = a.cuts[w + j], q = a.cuts[w + j + 1];
@@ -1124,7 +1138,7 @@ template <typename OutT, int PER> __global__ __launch_bounds__(kMergeThreads) vo
             acc[r] = float4{acc[r].x * scale, acc[r].y * scale, acc[r].z * scale, acc[r].w * scale};
             mx[r] = m_new;
         }
-        constexpr int AT_ONCE = PER >= 4 ? 1 : 4;  // parts
+        constexpr int AT_ONCE = 4;  // parts
         for (int j0 = 0; j0 < n; j0 += AT_ONCE) {
             float4 v[AT_ONCE][PER];
 #pragma unroll

@@ -9,21 +9,28 @@ using namespace tq4::abi;
 
 namespace {
 
-// How a call is spread over the device, by a sequence's query rows per kv-head (on average): workgroups on row tiles of
-// `rows` rows and token tiles of `tile`, `groups` of them at once.
+// How a call is spread over the device: workgroups on row tiles of `rows` rows and token tiles of `tile`, `groups` of
+// them at once.
 enum class Form { kMany, kSome, kFew };
 struct ChunkPlan {
     Form form;
     int rows, tile, groups;
 };
 int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
-ChunkPlan chunk_plan(int tokens, int batch, int group) {
-    const int64_t rows = (int64_t)tokens * group / batch;
-    if (rows > 64)
-        return {Form::kMany, 256, 64, cus()};
-    if (rows > 32)
+// By a sequence's query rows per kv-head (on average).  Every row tile reads and decodes the sequence again: one of 32, 64
+// and 256 rows takes 4 : 7 : 16 parts of a time (64 sequences of 4096 tokens, 8 kv-heads, per row tile 77, 135 and 310 us
+// in all), and the least sum is taken: 32, 48, 64, 96, 128 and 256 rows 102, 153, 172, 249, 328, 638 us in tiles of 32, 149, 142,
+// 144, 267, 273, 527 in tiles of 64, 304, 295, 298, 303, 310, 349 in tiles of 256.  Up to 16 (sequence, kv-head) pairs,
+// whose row tiles are all cut into many parts, those of 32 rows are ahead up to 128 rows (one sequence of 32768
+// tokens, 2 kv-heads, 48 and 128 rows: 48 and 55 us, 63 and 72, 64 and 72).
+ChunkPlan chunk_plan(int tokens, int batch, int Hq, int Hk) {
+    const int64_t rows = std::max<int64_t>((int64_t)tokens * (Hq / Hk) / batch, 1);
+    const int64_t few = 4 * ((rows + 31) / 32), some = 7 * ((rows + 63) / 64), many = 16 * ((rows + 255) / 256);
+    if ((few < some && few < many) || ((int64_t)batch * Hk <= 16 && rows <= 128))
+        return {Form::kFew, tq4::chunk::kFewRows, tq4::chunk::kFewTile, 2 * cus()};
+    if (some < many)
         return {Form::kSome, 64, 64, 2 * cus()};
-    return {Form::kFew, tq4::chunk::kFewRows, tq4::chunk::kFewTile, 2 * cus()};
+    return {Form::kMany, 256, 64, cus()};
 }
 
 struct Workspace {
@@ -31,7 +38,7 @@ struct Workspace {
 };
 Workspace workspace_of(int tokens, int batch, int Hq, int Hk) {
     const int64_t rows = (int64_t)tokens * Hq;
-    const ChunkPlan p = chunk_plan(tokens, batch, Hq / Hk);
+    const ChunkPlan p = chunk_plan(tokens, batch, Hq, Hk);
     auto up = [](int64_t x) { return (x + 63) / 64 * 64; };
     Workspace w{};
     w.q_lo = up(rows * tq4::kHeadDim / 2);
@@ -93,15 +100,10 @@ template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStr
     else
         launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p);
 }
-// Few rows: many parts; many rows: two parts, most often, and several rows' loads at once.
 template <typename OutT> void launch_merge(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
-    const int rows = p.shape.rows, per = rows == 256 ? 8 : 1;
-    const dim3 grid(p.groups, (rows + kMergeHalves * per - 1) / (kMergeHalves * per)), block(kMergeThreads);
-    if (per == 8)
-        launch(&chunk_merge_kernel<OutT, 8>, grid, block, st, p);
-    else
-        launch(&chunk_merge_kernel<OutT, 1>, grid, block, st, p);
+    constexpr int rows = kMergeHalves * kMergePer;
+    launch(&chunk_merge_kernel<OutT>, dim3((p.shape.rows + rows - 1) / rows, p.groups), dim3(kMergeThreads), st, p);
 }
 
 }  // namespace
@@ -154,7 +156,7 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     if (workspace_floats < ws.total || !aligned(workspace, 16))
         return fail(TQ4_E_INVALID, "%s: workspace of %lld floats, needs %lld, 16-byte aligned", what,
                     (long long)workspace_floats, (long long)ws.total);
-    const ChunkPlan plan = chunk_plan(tokens, B, Hq / Hk);
+    const ChunkPlan plan = chunk_plan(tokens, B, Hq, Hk);
     tq4::chunk::Args p{};
     p.query = query;
     p.rot_t = rot_t;
