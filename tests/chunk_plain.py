@@ -62,7 +62,10 @@ def attend(q, k, v, seen, sinks, scale, fine, rounded_keys):
                 # RHO e |v - middle|, while the middle value and the sum have e itself
                 var = np.maximum(var, RHO ** 2 * MOST_FROM_MIDDLE ** 2 * p2.sum(-1, keepdims=True))
             if not fine and rounded_keys:
-                d2 = 2 * RHO ** 2 * ((qq ** 2) @ (k[:, h] ** 2).T) * scale ** 2
+                # both factors, and the rotation's elements r[j][d], whose roundings move q[d] by RHO sqrt(sum_j q_j^2 r_jd^2): with
+                # r^2 about 1 / 128 everywhere, |q|^2 |k|^2 / 128 (a half more for where it is not)
+                k2 = k[:, h] ** 2
+                d2 = RHO ** 2 * (2 * (qq ** 2) @ k2.T + 1.5 / D * (qq ** 2).sum(-1)[:, None] * k2.sum(-1)[None]) * scale ** 2
                 w = p2 * np.where(mask, d2, 0)
                 var = var + spread(w)
                 dev_lse[:, h * g:(h + 1) * g] = np.sqrt(w.sum(-1)).reshape(n, g)

@@ -37,7 +37,7 @@ def test_values_past_f16(dev, pairs, preset, layout, lse):
     """Scales up to f16's largest beside small ones, and scores that pass the running maximum by much.
 
     Bar: every token's weight is off by at most 2^-11 (its rounding) and the scores' share (eight deviations of
-    rounding both factors; none with a log-sum-exp), and so is the sum of all, which counts twice; its value by 2^-11 (twice, for one
+    rounding both factors and the rotation; none with a log-sum-exp), and so is the sum of all, which counts twice; its value by 2^-11 (twice, for one
     that is stored a 32nd as large) and by 2^-10 of the middle codes' distance where its scale is part of the weight:
     8 codes of 15, so at most 16/15 of the largest |v| of the token."""
     b = Batch(21, pairs, 2, 4, preset=preset, layout=layout, query_scale=4.0, spoil=False,
@@ -57,7 +57,8 @@ def test_values_past_f16(dev, pairs, preset, layout, lse):
             s = np.where(seen, qq @ k.T * D ** -0.5, -np.inf)
             p = np.exp(s - s.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
-            dev_s = 0 if lse or preset == "k8v4" else RHO * np.sqrt(2 * ((qq ** 2) @ (k ** 2).T).max(-1)) * D ** -0.5
+            dev_s = 0 if lse or preset == "k8v4" else RHO * D ** -0.5 * np.sqrt(
+                (2 * (qq ** 2) @ (k ** 2).T + 1.5 / D * (qq ** 2).sum(-1)[:, None] * (k ** 2).sum(-1)).max(-1))
             size = p @ np.abs(v).max(-1)
             bar = (2.0 ** -8 * 1.01) * np.abs(p @ v) + ((2.0 ** -9 + 2 * 8 * dev_s + 2.0 ** -11) * size)[..., None] + 1e-4
             part = have[b.starts[i]:b.starts[i] + n, h * b.group:(h + 1) * b.group].reshape(-1, D)

@@ -16,8 +16,8 @@
 // that was cut go to the workspace, where chunk_merge_kernel joins them.
 //
 // Precision.  FINE (fp16 results, or a log-sum-exp): keys' codes and queries are f16 hi + lo, three products, V's codes
-// are exact and its scale is part of the weight, one f16.  Otherwise (bf16 results): codes, queries, V and weights
-// are one f16 each, a sixteenth of the result's own rounding.
+// are exact and its scale is part of the weight, one f16.  Otherwise (bf16 results): codes, queries (and the matrix that turns
+// them), V and weights are one f16 each, an eighth of the result's own rounding.
 #pragma once
 #include "chunk_plan.h"
 #include "prefix.h"
@@ -107,21 +107,21 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
         a.cuts[w] = cut_of(a.shape, seq, work, a.batch, total, used, w);
 }
 
-// Query rows into operands: y = q @ rot_t (f16 hi + lo products as rotate_mfma_kernel; a row scaled by a power of two
-// first), times the score scale, as f16 hi (and lo); rows that would pass f16's range, or lie below 2^-8 near its
+// Query rows into operands: y = q @ rot_t (a row scaled by a power of two first; rot_t as f16 hi + lo where LO keeps y as
+// pairs too, else rounded to f16, as much of an error as rounding y is), times the score scale, as f16 hi (and lo); rows that would pass f16's range, or lie below 2^-8 near its
 // denormals, are scaled to its top and q_factor undoes it.  FP8 keys: the row itself, scaled by the power of two that
 // puts its largest magnitude in [0.5, 1): exact for dims down to 2^-13 of it, below that to 2^-25 of it.
-// 8192 x 32 rows: 53 us.  A form whose workgroups stage rot_t once and take one row tile after the other (32x32x16
-// products) took 39, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
+// Bound by each workgroup's own rounding of rot_t: 8192 x 32 rows 39 us (with its low part 53), 134 MB in and out.  A form whose workgroups stage rot_t once and take one row tile after the other (32x32x16 products) took
+// 39 with the low part, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
 // clock through chunk_kernel (634 : 720 us, the same code).
 template <typename InT, bool KF8, bool LO>
 __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
     __shared__ __align__(16) union {
-        _Float16 pt[2][PT];
+        _Float16 pt[LO ? 2 : 1][PT];
         PlanLds plan;
     } lds;
-    _Float16 *pt_hi = lds.pt[0], *pt_lo = lds.pt[1];
+    _Float16 *pt_hi = lds.pt[0], *pt_lo = lds.pt[LO];
     if (blockIdx.x == 0) {
         plan_cuts(a, lds.plan);
         return;
@@ -169,10 +169,12 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
             for (int j = 0; j < 8; ++j) {
                 const float w = a.rot_t[(8 * kg + j) * kHeadDim + c];
                 h[j] = (_Float16)w;
-                l[j] = (_Float16)(w - (float)h[j]);
+                if constexpr (LO)
+                    l[j] = (_Float16)(w - (float)h[j]);
             }
             *reinterpret_cast<half8 *>(pt_hi + c * kRotPt + 8 * kg) = h;
-            *reinterpret_cast<half8 *>(pt_lo + c * kRotPt + 8 * kg) = l;
+            if constexpr (LO)
+                *reinterpret_cast<half8 *>(pt_lo + c * kRotPt + 8 * kg) = l;
         }
         __syncthreads();
         if (r0 >= rows)
@@ -193,7 +195,8 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
             for (int kb = 0; kb < 4; ++kb) {
                 const int off = (16 * cb + n) * kRotPt + 32 * kb + 8 * g;
                 y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_hi + off), q[kb], y[cb]);
-                y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + off), q[kb], y[cb]);
+                if constexpr (LO)
+                    y[cb] = xdl::mfma(*reinterpret_cast<const half8 *>(pt_lo + off), q[kb], y[cb]);
             }
         }
         float top = 0.f;
@@ -592,6 +595,16 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
 };
 
 // ---- The product -----------------------------------------------------------------------------
+
+// Bound by what a tile costs beside its products, and by the clock that both leave.  32 heads on 8 kv-heads: 8192 tokens on
+// themselves 640 us, 0.86 PFLOP/s of the visible products; 2048 behind 32768 1200 us, 0.94 (a bf16 product of 8192^3 reaches
+// 1.24).  A tile of 64 tokens takes a wave of 32 rows about 5060 cycles: its products 2050, softmax and decoding about 2490 of
+// vector work, and little of the one beside the other, since the four waves that decode V take longer than those
+// that decode K, which wait for them at the barrier.  FINE has three score products for one: 4 sequences of up to 1000 tokens, up to
+// 10000 before them, 3 bits, GQA 8: 720 us.
+// Tiles of 256 rows (WT = 1, eight waves) have two LDS buffers and decode a tile between the products of the one before it;
+// tiles of 64 rows (WT = 2) decode and multiply in turn, two workgroups a CU.  What did not pay: the next tile's
+// scores before the softmax of this one (registers spill), and the two halves of the waves a phase apart (the same time).
 
 __device__ __forceinline__ float *part_rows(const Args &a, int slot) { return a.parts + (int64_t)slot * a.shape.rows * kHeadDim; }
 __device__ __forceinline__ float *part_sums(const Args &a, int slot) {
