@@ -338,7 +338,8 @@ int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);
  * query: heads contiguous, tokens query_stride elements apart (whole 16-byte pieces); query and out are 16-bit
  * (TQ4_BF16, TQ4_F16), out [tokens, Hq, D] contiguous and 16-byte aligned.  lse [tokens, Hq] fp32 may be NULL: with it, and
  * for TQ4_F16 outputs, scores are products of f16 pairs and V's codes exact (weights times V's scale are rounded to f16);
- * else key codes, rotated queries, values and weights are rounded to f16 each, and outputs to bf16.
+ * else key codes, rot_t, rotated queries, values and weights are rounded to f16 each, and outputs to bf16.
+ * At most 2^30 query rows (tokens * Hq) and block strides below 2^31; attn_scale is finite.
  * workspace: at least tq4_chunk_workspace_floats(...) floats, 16-byte aligned, contents after the call unspecified;
  * two calls that may overlap need one each.  The grid depends on the shapes alone.  Cache, rot_t, centroids, sinks,
  * key_bits / value_bits, block sizes and errors as in tq4_window_decode.

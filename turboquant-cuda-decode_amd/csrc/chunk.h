@@ -10,7 +10,8 @@
 // maximum and sum are its own values, and the weights' registers are the B operand as they stand.
 //
 // Three launches.  chunk_start_kernel turns the queries into the keys' basis and rounds them to the products' operands;
-// one workgroup of it cuts the work (chunk_plan.h).  chunk_kernel: a workgroup of WR * WT waves takes its stretch of
+// its first workgroup cuts the work (chunk_plan.h), the next that of sequences with few rows, which have a product and a join
+// of their own (chunk_few.h).  chunk_kernel: a workgroup of WR * WT waves takes its stretch of
 // the list of row tiles of 32 WR rows; each wave has 32 rows and 1 / WT of the tokens of a tile of KT, which the
 // workgroup decodes once into LDS.  A row tile that one workgroup had whole is written as the result, the parts of one
 // that was cut go to the workspace, where chunk_merge_kernel joins them.
@@ -53,7 +54,15 @@ struct Args {
     int block_size_log2, slot_pos, slot_head;
     Shape shape;
     int longest;             // table_width blocks
+    int rows_least, rows_most;  // of a kv-head: sequences with fewer or more count as without new tokens
 };
+__device__ __forceinline__ Seq seq_at(const Args &a, int b) {
+    Seq q = seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest);
+    const int rows = q.n * a.shape.group;
+    if (rows < a.rows_least || rows > a.rows_most)
+        q.n = 0;
+    return q;
+}
 
 // ---- Queries and cuts ------------------------------------------------------------------------
 
@@ -73,13 +82,13 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
     double *work = small ? lds.work : a.work, *sums = lds.sums;
     double own = 0;
     for (int b = b0; b < b1; ++b) {
-        const Seq q = seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest);
+        const Seq q = seq_at(a, b);
         if (small)
             lds.seqs[b] = q;
         work[b] = work_of(a.shape, q);
         own += work[b];
     }
-    auto seq = [&](int b) { return small ? lds.seqs[b] : seq_of(a.starts, a.seq_lens, b, a.tokens, a.longest); };
+    auto seq = [&](int b) { return small ? lds.seqs[b] : seq_at(a, b); };
     // sums over the threads before this one
     double at = own;
 #pragma unroll
@@ -115,7 +124,7 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
 // 39 with the low part, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
 // clock through chunk_kernel (634 : 720 us, the same code).
 template <typename InT, bool KF8, bool LO>
-__global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a) {
+__global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a, const Args few, int plans) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
     __shared__ __align__(16) union {
         _Float16 pt[LO ? 2 : 1][PT];
@@ -126,8 +135,12 @@ __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a
         plan_cuts(a, lds.plan);
         return;
     }
+    if ((int)blockIdx.x < plans) {
+        plan_cuts(few, lds.plan);
+        return;
+    }
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, n = lane & 15, g = lane >> 4;
-    const int64_t rows = (int64_t)a.tokens * a.num_q_heads, r0 = ((int64_t)blockIdx.x - 1) * kStartRows + 16 * wave;
+    const int64_t rows = (int64_t)a.tokens * a.num_q_heads, r0 = ((int64_t)blockIdx.x - plans) * kStartRows + 16 * wave;
     const int64_t ra = min(r0 + n, rows - 1);
     const int64_t token = ra / a.num_q_heads;
     const InT *from = static_cast<const InT *>(a.query) + token * a.query_stride + (ra - token * a.num_q_heads) * kHeadDim;
@@ -649,7 +662,7 @@ void chunk_kernel(const Args a) {
     const int group = a.shape.group;
     xdl::lds_barrier();  // the table
     while (at.b < a.batch) {
-        const Seq seq = seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest);
+        const Seq seq = seq_at(a, at.b);
         const int rows = seq.n * group, kvh = at.h;
         const Visits vis = visits_of(a.shape, seq, at.r);
         const bool last = same_tile(at, end);
@@ -1084,7 +1097,7 @@ void chunk_kernel(const Args a) {
                 at.h = 0;
                 do
                     ++at.b;
-                while (at.b < a.batch && seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest).n == 0);
+                while (at.b < a.batch && seq_at(a, at.b).n == 0);
             }
         }
     }
@@ -1102,7 +1115,7 @@ template <typename OutT> __global__ __launch_bounds__(kMergeThreads) void chunk_
     const Cut from = a.cuts[w], cut = a.cuts[w + 1];
     if (cut.b >= a.batch || cut.at == 0 || (same_tile(from, cut) && from.at > 0))
         return;
-    const Seq seq = seq_of(a.starts, a.seq_lens, cut.b, a.tokens, a.longest);
+    const Seq seq = seq_at(a, cut.b);
     const int rows = seq.n * a.shape.group, place0 = (blockIdx.x * kMergeHalves + half) * PER;
     if (cut.r * a.shape.rows + (int)blockIdx.x * kMergeHalves * PER >= rows)
         return;

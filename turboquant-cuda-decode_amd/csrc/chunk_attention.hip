@@ -15,6 +15,7 @@ enum class Form { kMany, kSome, kFew };
 struct ChunkPlan {
     Form form;
     int rows, tile, groups;
+    int few;  // sequences with up to this many query rows take kFew in a product of their own (0: none do)
 };
 int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
 // By a sequence's query rows per kv-head (on average).  Every row tile reads and decodes the sequence again: one of 32, 64
@@ -23,18 +24,21 @@ int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
 // 144, 267, 273, 527 in tiles of 64, 304, 295, 298, 303, 310, 349 in tiles of 256.  Up to 16 (sequence, kv-head) pairs,
 // whose row tiles are all cut into many parts, those of 32 rows are ahead up to 128 rows (one sequence of 32768
 // tokens, 2 kv-heads, 48 and 128 rows: 48 and 55 us, 63 and 72, 64 and 72).
+// Batches whose average takes larger tiles may still have sequences with few rows (decoding beside a prompt's chunk), whose
+// every tile would cost as much as a full one: they have a product of their own (63 sequences of one token and one of
+// 2048, behind 4096: 455 us together, 262 so; a batch without such sequences pays 8 us for it).
 ChunkPlan chunk_plan(int tokens, int batch, int Hq, int Hk) {
     const int64_t rows = std::max<int64_t>((int64_t)tokens * (Hq / Hk) / batch, 1);
     const int64_t few = 4 * ((rows + 31) / 32), some = 7 * ((rows + 63) / 64), many = 16 * ((rows + 255) / 256);
     if ((few < some && few < many) || ((int64_t)batch * Hk <= 16 && rows <= 128))
-        return {Form::kFew, tq4::chunk::kFewRows, tq4::chunk::kFewTile, 2 * cus()};
+        return {Form::kFew, tq4::chunk::kFewRows, tq4::chunk::kFewTile, 2 * cus(), 0};
     if (some < many)
-        return {Form::kSome, 64, 64, 2 * cus()};
-    return {Form::kMany, 256, 64, cus()};
+        return {Form::kSome, 64, 64, 2 * cus(), batch > 1 ? 32 : 0};
+    return {Form::kMany, 256, 64, cus(), batch > 1 ? 96 : 0};
 }
 
 struct Workspace {
-    int64_t q_lo, factor, work, cuts, parts, total;  // offsets in floats
+    int64_t q_lo, factor, work, cuts, few_work, few_cuts, parts, total;  // offsets in floats
 };
 Workspace workspace_of(int tokens, int batch, int Hq, int Hk) {
     const int64_t rows = (int64_t)tokens * Hq;
@@ -45,7 +49,9 @@ Workspace workspace_of(int tokens, int batch, int Hq, int Hk) {
     w.factor = w.q_lo + up(rows * tq4::kHeadDim / 2);
     w.work = w.factor + up(rows);
     w.cuts = w.work + up(2 * ((int64_t)batch + 1));
-    w.parts = w.cuts + up(4 * ((int64_t)p.groups + 1));
+    w.few_work = w.cuts + up(4 * ((int64_t)p.groups + 1));
+    w.few_cuts = w.few_work + (p.few ? up(2 * ((int64_t)batch + 1)) : 0);
+    w.parts = w.few_cuts + (p.few ? up(4 * ((int64_t)2 * cus() + 1)) : 0);  // (no less than kFew's; one product after the other)
     w.total = w.parts + up((int64_t)2 * p.groups * p.rows * (tq4::kHeadDim + 1));
     return w;
 }
@@ -90,15 +96,14 @@ template <int LAYOUT, bool FINE> void launch_chunk(const Stage1Args &a, const tq
     else
         launch_few<LAYOUT, FINE>(a, p, st);
 }
-template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, hipStream_t st) {
+template <bool KF8, bool LO> void launch_start(const tq4::chunk::Args &p, const tq4::chunk::Args &few, int plans, hipStream_t st) {
     using namespace tq4::chunk;
     const int64_t rows = (int64_t)p.tokens * p.num_q_heads;
-    // (the first workgroup makes the plan)
-    const dim3 grid((unsigned)((rows + kStartRows - 1) / kStartRows + 1)), block(kStartThreads);
+    const dim3 grid((unsigned)((rows + kStartRows - 1) / kStartRows + plans)), block(kStartThreads);
     if (p.q_dtype == TQ4_BF16)
-        launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p);
+        launch(&chunk_start_kernel<__bf16, KF8, LO>, grid, block, st, p, few, plans);
     else
-        launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p);
+        launch(&chunk_start_kernel<_Float16, KF8, LO>, grid, block, st, p, few, plans);
 }
 template <typename OutT> void launch_merge(const tq4::chunk::Args &p, hipStream_t st) {
     using namespace tq4::chunk;
@@ -191,26 +196,37 @@ int tq4_chunk_attention(const void *query, int query_dtype, int64_t query_stride
     p.slot_head = a.kl == 0 ? record : a.slot_head;
     p.shape = tq4::chunk::Shape{plan.rows, plan.tile, Hq / Hk, Hk, causal != 0, std::min(window, 1 << 30), std::min(first_tokens, 1 << 30)};
     p.longest = (int)std::min<int64_t>((int64_t)max_blocks_per_seq * block_size, (1 << 30));
+    p.rows_most = 0x7FFFFFFF;
+    tq4::chunk::Args few = p;
+    if (plan.few) {
+        p.rows_least = plan.few + 1;
+        few.rows_most = plan.few;
+        few.shape.rows = tq4::chunk::kFewRows;
+        few.shape.tile = tq4::chunk::kFewTile;
+        few.groups = 2 * cus();
+        few.work = reinterpret_cast<double *>(workspace + ws.few_work);
+        few.cuts = reinterpret_cast<tq4::chunk::Cut *>(workspace + ws.few_cuts);
+    }
     const bool fine = lse || out_dtype == TQ4_F16;
+    const int plans = plan.few ? 2 : 1;
     if (a.key_fp8)
-        launch_start<true, false>(p, st);
+        launch_start<true, false>(p, few, plans, st);
     else
-        fine ? launch_start<false, true>(p, st) : launch_start<false, false>(p, st);
+        fine ? launch_start<false, true>(p, few, plans, st) : launch_start<false, false>(p, few, plans, st);
     rc = launch_status("chunk start");
-    if (rc)
-        return rc;
-    if (a.kl == 0)
-        fine ? launch_chunk<0, true>(a, p, plan.form, st) : launch_chunk<0, false>(a, p, plan.form, st);
-    else
-        fine ? launch_chunk<1, true>(a, p, plan.form, st) : launch_chunk<1, false>(a, p, plan.form, st);
-    rc = launch_status("chunk");
-    if (rc)
-        return rc;
-    if (out_dtype == TQ4_BF16)
-        launch_merge<__bf16>(p, st);
-    else
-        launch_merge<_Float16>(p, st);
-    return launch_status("chunk merge");
+    auto product = [&](const tq4::chunk::Args &p, Form form) {
+        if (a.kl == 0)
+            fine ? launch_chunk<0, true>(a, p, form, st) : launch_chunk<0, false>(a, p, form, st);
+        else
+            fine ? launch_chunk<1, true>(a, p, form, st) : launch_chunk<1, false>(a, p, form, st);
+        if (const int rc = launch_status("chunk"))
+            return rc;
+        out_dtype == TQ4_BF16 ? launch_merge<__bf16>(p, st) : launch_merge<_Float16>(p, st);
+        return launch_status("chunk merge");
+    };
+    if (!rc && plan.few)
+        rc = product(few, Form::kFew);
+    return rc ? rc : product(p, plan.form);
 }
 
 }  // extern "C"

@@ -88,7 +88,7 @@ void chunk_few_kernel(const Args a) {
     __syncthreads();
     const int group = a.shape.group;
     while (at.b < a.batch) {
-        const Seq seq = seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest);
+        const Seq seq = seq_at(a, at.b);
         const int rows = seq.n * group, kvh = at.h, row0 = at.r * a.shape.rows;
         const Visits vis = visits_of(a.shape, seq, at.r);
         const bool last = same_tile(at, end);
@@ -474,7 +474,7 @@ void chunk_few_kernel(const Args a) {
                 at.h = 0;
                 do
                     ++at.b;
-                while (at.b < a.batch && seq_of(a.starts, a.seq_lens, at.b, a.tokens, a.longest).n == 0);
+                while (at.b < a.batch && seq_at(a, at.b).n == 0);
             }
         }
     }

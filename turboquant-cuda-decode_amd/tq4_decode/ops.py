@@ -769,7 +769,7 @@ def chunk_attention(query, rotation_t, kv_cache, block_table, seq_lens, query_st
 
     ``query`` and the outputs are bf16 or fp16; heads are contiguous, tokens may be strided (a slice of a projection's
     output).  fp16 outputs and calls with ``return_lse`` take scores from f16 pairs and V's codes as they are, others
-    round keys, rotated queries, values and weights to f16.  ``workspace``: a ``ChunkWorkspace``, whose ``out`` and ``lse``
+    round keys, the rotation and rotated queries, values and weights to f16.  ``workspace``: a ``ChunkWorkspace``, whose ``out`` and ``lse``
     are returned.  Launches depend on shapes alone.  ``key_bits`` / ``value_bits``, ``sinks`` and block sizes as in
     ``window_decode``.
     """
