@@ -181,17 +181,22 @@ def test_starts_and_lengths_past_the_tensors(dev):
 
 
 @pytest.mark.parametrize("lse", [False, True])
-def test_replays_follow_lengths_and_starts(dev, lse):
-    kinds = [[(5, 200), (3, 64), (0, 9), (40, 400)], [(48, 48), (0, 0), (0, 0), (0, 0)], [(1, 1), (1, 300), (2, 2), (44, 333)],
-             [(12, 700), (12, 12), (12, 90), (12, 13)]]
-    batches = [Batch(40 + i, p, 2, 4, wide=44) for i, p in enumerate(kinds)]
+@pytest.mark.parametrize("tokens,kinds", [
+    (48, [[(5, 200), (3, 64), (0, 9), (40, 400)], [(48, 48), (0, 0), (0, 0), (0, 0)], [(1, 1), (1, 300), (2, 2), (44, 333)],
+          [(12, 700), (12, 12), (12, 90), (12, 13)]]),
+    # (sequences of up to 24 tokens have a product of their own: some, none, all, all but one)
+    (400, [[(24, 200), (3, 64), (0, 9), (373, 400)], [(100, 100), (100, 300), (25, 30), (175, 700)], [(24, 24), (1, 2), (20, 600), (5, 5)],
+           [(1, 700), (1, 1), (1, 333), (397, 397)]]),
+])
+def test_replays_follow_lengths_and_starts(dev, lse, tokens, kinds):
+    batches = [Batch(40 + i, p, 2, 4, wide=44, pad=(0, tokens - sum(n for n, _ in p))) for i, p in enumerate(kinds)]
     pool = max(b.cache.shape[0] for b in batches)
     first = batches[0]
     put = lambda x: torch.from_numpy(np.ascontiguousarray(x)).to(dev)  # noqa: E731
     cache = torch.zeros((pool,) + tuple(first.cache.shape[1:]), dtype=torch.uint8, device=dev)
-    query, table = torch.zeros(48, 8, D, dtype=torch.bfloat16, device=dev), put(first.table)
+    query, table = torch.zeros(tokens, 8, D, dtype=torch.bfloat16, device=dev), put(first.table)
     lens, starts, rot = put(first.lens), put(first.starts), put(first.rot)
-    ws = ops.ChunkWorkspace(48, 4, 8, 2, dev)
+    ws = ops.ChunkWorkspace(tokens, 4, 8, 2, dev)
     args = (query, rot, cache, table, lens, starts, put(codebook.centroids(D, 4).astype(np.float32)))
 
     def fill(b):
@@ -261,3 +266,14 @@ def test_blocks_past_4_gib(dev, layout, pairs):
     far = ops.cache_load(big, (at[slots // 16] * 16 + slots % 16).int().to(dev), put(b.rot),
                          put(codebook.centroids(D, 4).astype(np.float32)), layout="soa" if layout == "soa" else "aos")
     assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(small, far))
+
+
+@pytest.mark.parametrize("preset,layout", [("4bit", "soa"), ("3bit", "aos"), ("k8v4", "aos_heads")])
+@pytest.mark.parametrize("pairs", [
+    [(1, 300), (1, 77), (600, 900), (1, 1), (0, 20), (2, 500)] * 2,  # tiles of 256 rows and of 32
+    [(1, 300), (30, 90), (8, 8), (9, 200), (25, 25)] * 4,            # of 64 and of 32
+], ids=str)
+def test_single_tokens_beside_chunks(dev, preset, layout, pairs):
+    b = Batch(70, pairs, 4, 4, preset=preset, layout=layout)
+    for how in (dict(), dict(lse=True), dict(window=60, first=7), dict(sinks=True), dict(causal=False, lse=True)):
+        check(b, call(b, dev, **how), str(how), **how)
