@@ -334,7 +334,8 @@ int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);
  * these (itself included) and the first `first_tokens`.  Not causal (window 0): every new token sees all seq_lens[b]
  * tokens, as the context of a chunk whose own tokens are attended to elsewhere (tq4_merge_states joins the two).
  * A new token that sees nothing gets zeros and LSE -inf.  What starts and lengths name outside of query and
- * the table counts as not there; only the blocks of visible tokens are read.
+ * the table counts as not there; only blocks with a visible token are read, and the block-table entries of the others may
+ * hold anything.
  * query: heads contiguous, tokens query_stride elements apart (whole 16-byte pieces); query and out are 16-bit
  * (TQ4_BF16, TQ4_F16), out [tokens, Hq, D] contiguous and 16-byte aligned.  lse [tokens, Hq] fp32 may be NULL: with it, and
  * for TQ4_F16 outputs, scores are products of f16 pairs and V's codes exact (weights times V's scale are rounded to f16);

@@ -529,8 +529,8 @@ __device__ __forceinline__ void code_values(uint32_t a, uint32_t b, int m, float
 template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
     half2v s01, s23, z01, z23;
     uint32_t v[4];
-    // `valid`: tokens of the unit that the sequence has (4 or more: all; the others' bytes may hold anything, and count as
-    // zeros).  `quad`: of the tile.  (Of a wave, together.)
+    // `valid`: tokens of the unit that the sequence has and a row may see (4 or more: all; the others' bytes may hold anything,
+    // and count as zeros).  `quad`: of the tile.  (Of a wave, together.)
     template <class F> __device__ __forceinline__ void begin(const Raw &r, F &factors, int quad, bool cut, int valid) {
         uint32_t s[2], z[2];  // scales and zeros of tokens (0, 1) and (2, 3)
         exchange<LAYOUT, V3>(r, v, s, z);
@@ -665,6 +665,7 @@ void chunk_kernel(const Args a) {
         const Seq seq = seq_at(a, at.b);
         const int rows = seq.n * group, kvh = at.h;
         const Visits vis = visits_of(a.shape, seq, at.r);
+        const Seen seen = seen_of(a.shape, seq, at.r);
         const bool last = same_tile(at, end);
         const int tile0 = at.at, tile1 = last ? end.at : vis.count;
         if (last && tile0 >= tile1)
@@ -683,12 +684,13 @@ void chunk_kernel(const Args a) {
         int blk[U];
         // the first of the 16 tokens of the wave's units, in the tile
         auto group_of = [&](int k) __attribute__((always_inline)) { return 16 * (S::halves ? w % (WR * WT / 2) : w + k * WR * WT); };
-        // (no block past the sequence's last one is asked for; in that, any token is in bounds.  A vector load, though
+        // (no block past the sequence's last one is asked for, and none in front of the window; in the others, any token is in
+        // bounds.  A vector load, though
         // every lane's is the same: a scalar one in flight makes every wait for LDS a wait for it)
         auto read_pages = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                uint32_t at = (uint32_t)min(first_of(i) + group_of(k), seq.len - 1) >> a.block_size_log2;
+                uint32_t at = (uint32_t)read_at(seen, seq.len, first_of(i) + group_of(k)) >> a.block_size_log2;
                 asm("" : "+v"(at));
                 blk[k] = pages[at];
             }
@@ -723,9 +725,11 @@ void chunk_kernel(const Args a) {
             }
             if constexpr (v_too) {
                 const int quad = 4 * (u >> 6) + ((u >> 2) & 3), e = 4 * (u & 3) + ((u >> 4) & 3);
-                if (q == 0)
-                    vdec[x].begin(rv[x], factors[i % BUFS], quad, first_of(i) + KT > seq.len, seq.len - first_of(i) - 4 * quad);
-                else
+                if (q == 0) {
+                    const bool gone = hidden(seen, first_of(i) + group_of(x));
+                    vdec[x].begin(rv[x], factors[i % BUFS], quad, gone || first_of(i) + KT > seq.len,
+                                  gone ? 0 : seq.len - first_of(i) - 4 * quad);
+                } else
                     vdec[x].write(m + S::v + e * S::vrow + 16 * (2 * (quad >> 2) + (quad & 1)) + 8 * ((quad >> 1) & 1), q - 1);
             }
         };

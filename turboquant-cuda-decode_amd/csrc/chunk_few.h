@@ -91,6 +91,7 @@ void chunk_few_kernel(const Args a) {
         const Seq seq = seq_at(a, at.b);
         const int rows = seq.n * group, kvh = at.h, row0 = at.r * a.shape.rows;
         const Visits vis = visits_of(a.shape, seq, at.r);
+        const Seen seen = seen_of(a.shape, seq, at.r);
         const bool last = same_tile(at, end);
         const int tile0 = at.at, tile1 = last ? end.at : vis.count;
         if (last && tile0 >= tile1)
@@ -106,7 +107,7 @@ void chunk_few_kernel(const Args a) {
         auto read_pages = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                uint32_t p = (uint32_t)min(first_of(i) + 16 * k, seq.len - 1) >> a.block_size_log2;
+                uint32_t p = (uint32_t)read_at(seen, seq.len, first_of(i) + 16 * k) >> a.block_size_log2;
                 asm("" : "+v"(p));
                 blk[k] = pages[p];
             }
@@ -303,11 +304,12 @@ void chunk_few_kernel(const Args a) {
             load(i + 1, no, yes);
             read_pages(i + 2);
             const bool masked = t0 + 32 > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
-            // tokens past the sequence: their bytes may hold anything
-            if (t0 + 32 > seq.len)
+            // tokens past the sequence, and those whose block is not read: their bytes may hold anything
+            const bool gone[2] = {hidden(seen, t0), hidden(seen, t0 + 16)};
+            if (t0 + 32 > seq.len || gone[0] || gone[1])
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
-                    if (t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= seq.len)
+                    if (gone[x >> 2] || t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= seq.len)
                         scale[x] = mid[x] = 0.f;
             const float most = special ? 1.f : 256.f;
 #pragma unroll

@@ -51,6 +51,23 @@ __device__ __forceinline__ Visits visits_of(const Shape &s, const Seq &q, int r)
         return Visits{0, 0, tiles};
     return Visits{head, next - head, head + (tiles > next ? tiles - next : 0)};
 }
+// What a row tile sees: tokens before `first` and from `from` on, all before `end`.  Its token tiles may hold others in front of
+// the window, whose blocks may be anybody's by now: 16 tokens (they lie in one block) that no row sees are not read.
+struct Seen {
+    int first, from, end;
+};
+__device__ __forceinline__ Seen seen_of(const Shape &s, const Seq &q, int r) {
+    const int rows = q.n * s.group, first_row = r * s.rows;
+    const int last_row = first_row + s.rows < rows ? first_row + s.rows - 1 : rows - 1;
+    return Seen{s.first, s.window ? limit_of(s, q, first_row) - s.window : 0, limit_of(s, q, last_row)};
+}
+// Whether no row sees any of the 16 tokens from t on.
+__device__ __forceinline__ bool hidden(const Seen &s, int t) { return t >= s.first && t + 16 <= s.from; }
+// The token whose block is read for them: their own, the sequence's last one behind its end (whose block later rows see),
+// the row tile's last one for hidden ones.
+__device__ __forceinline__ int read_at(const Seen &s, int len, int t) {
+    return hidden(s, t) ? s.end - 1 : t < len - 1 ? t : len - 1;
+}
 // The work of a row tile in token tiles: about those it visits (a straight line through their number, so that sums
 // have a closed form) and kStart for the queries, the first loads and the results.
 constexpr double kStart = 3.0;
