@@ -18,7 +18,8 @@
 //
 // Precision.  FINE (fp16 results, or a log-sum-exp): keys' codes and queries are f16 hi + lo, three products, V's codes
 // are exact and its scale is part of the weight, one f16.  Otherwise (bf16 results): codes, queries (and the matrix that turns
-// them), V and weights are one f16 each, an eighth of the result's own rounding.
+// them), V and weights are rounded to one f16 each, every one of these an eighth of the result's own rounding.  Weights
+// keep that down to 2^-22 of a row's largest one (Headroom).
 #pragma once
 #include "chunk_plan.h"
 #include "prefix.h"
@@ -268,12 +269,13 @@ template <int WR, int WT, int KT, int BUFS, bool KF8, bool FINE> struct Form {
 };
 // What the softmax takes of a tile's tokens.  v: V's scale and its value at the middle code (FINE).  special: of each 16
 // tokens (those that one wave decodes at a time), whether their `fix` may differ from 1: the weight's factor where V is
-// stored smaller, NaN where V is not finite.
+// stored smaller, NaN where V is not finite.  top: the bits of their largest finite scale (FINE).
 template <int KT, bool KF8, bool FINE> struct alignas(16) Factors {
     float norm[KF8 ? 4 : KT];
     float2 v[FINE ? KT : 2];
     float fix[KT];
     uint32_t special[KT / 16];
+    uint32_t top[FINE ? KT / 16 : 4];
 };
 // The codes' table: pairs of centroids as f16, with their low parts (FINE), or with the sum of their squares (AoS slots,
 // which hold the raw norm).  It has LDS address 0, so that a lookup's address is the byte of codes, shifted.
@@ -541,10 +543,11 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
             z[0] &= m0;
             z[1] &= m1;
         }
-        // magnitudes as whole numbers: scales of 2048 or zeros of 16384 and more might pass f16's range together
-        // (FINE: scales of 128 and more times weights); NaN and infinities are above those
-        const uint32_t top_s = top_of(most_of(s[0], s[1])), top_z = top_of(most_of(z[0], z[1]));
-        const bool special = __any(top_s >= (FINE ? 0x5800u : 0x6800u) || top_z >= (FINE ? 0x7C00u : 0x7400u));
+        // magnitudes as whole numbers: scales of 2048 or zeros of 16384 and more might pass f16's range together; NaN and
+        // infinities are above those
+        uint32_t top_s = top_of(most_of(s[0], s[1]));
+        const uint32_t top_z = top_of(most_of(z[0], z[1]));
+        const bool special = __any(top_s >= (FINE ? 0x7C00u : 0x6800u) || top_z >= (FINE ? 0x7C00u : 0x7400u));
         float scale[4], zero[4];
         if (FINE || special)
 #pragma unroll
@@ -568,7 +571,10 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
                 }
             }
             *reinterpret_cast<float4 *>(factors.fix + 4 * quad) = float4{fix[0], fix[1], fix[2], fix[3]};
-            if constexpr (!FINE) {
+            if constexpr (FINE) {
+                const float top = fmaxf(fmaxf(fabsf(scale[0]), fabsf(scale[1])), fmaxf(fabsf(scale[2]), fabsf(scale[3])));
+                top_s = __builtin_bit_cast(uint16_t, (_Float16)top);
+            } else {
                 auto pair = [](float x, float y) { return prefix::as_u32(half2v{(_Float16)x, (_Float16)y}); };
                 s[0] = pair(scale[0], scale[1]);
                 s[1] = pair(scale[2], scale[3]);
@@ -578,6 +584,10 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
         }
         factors.special[quad >> 2] = special;
         if constexpr (FINE) {
+            // (the four quads of the wave's tokens: lanes 4 and 8 apart in each 16)
+            top_s = max(top_s, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top_s, 0x124, 0xF, 0xF, false));  // row_ror:4
+            top_s = max(top_s, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top_s, 0x128, 0xF, 0xF, false));  // row_ror:8
+            factors.top[quad >> 2] = top_s;
             float4 *to = reinterpret_cast<float4 *>(factors.v + 4 * quad);
             auto mid = [&](int i) { return fmaf(scale[i], kMiddle<V3>, zero[i]); };
             to[0] = float4{scale[0], mid(0), scale[1], mid(1)};
@@ -606,6 +616,21 @@ template <int LAYOUT, bool V3, bool FINE, int VROW> struct VUnit {
         put(2 * m + 1, x1, y1);
     }
 };
+
+// Where the softmax's running maximum lies.  A weight enters the products as one f16, so it is to use that range: with the
+// largest one at 1, weights below 2^-14 of it were denormals, and rows that one token dominates (13 nats above 32768 others, its
+// value small) off by 1 %.  A move puts the row's largest weight at 2^goal, and the next one waits until the weights of a
+// lane's tokens in a tile sum to more than `most`: so weights are at most that, and normal down to 2^(-14 - goal) of the
+// largest.  V's values as operands: weights themselves, 2^kGoal and 2^15 (where they may be multiplied by
+// 1 / kShrink, 2^10).  V's scale in the weight: products below 2^15, for scales below 2^e (the tile's largest one).
+constexpr float kGoal = 8.f, kMost = 0x1p15f, kMostShrunk = 0x1p10f;
+constexpr int kGoalBelow = 8;
+struct Headroom {
+    float goal, most;
+};
+__device__ __forceinline__ Headroom headroom_of(int e) {
+    return Headroom{(float)(15 - kGoalBelow - e), xdl::bitsf((uint32_t)(127 + 15 - e) << 23)};
+}
 
 // ---- The product -----------------------------------------------------------------------------
 
@@ -769,7 +794,7 @@ void chunk_kernel(const Args a) {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
                 acc[d][k] = 0.f;
-        float negm = __FLT_MAX__, l = 0.f, z = 0.f;  // -max in log2 units, this lane's shares of the sum and of V's middle values
+        float negm = __FLT_MAX__, l = 0.f, z = 0.f;  // goal - max in log2 units, this lane's shares of the sum and of V's middle values
 
         constexpr int kAtOnce = FINE ? 1 : S::sub;  // sub-tiles of 32 tokens at once
         constexpr int kEvery = 4;                   // products between two steps of decoding
@@ -838,10 +863,15 @@ void chunk_kernel(const Args a) {
                 special |= f.special[k];
             special = __builtin_amdgcn_readfirstlane(special);
             const bool masked = t0 + 32 * kAtOnce > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
-            // The scores in log2 units, less the running maximum.  That one moves when the weights' sum passes `most`: a weight
-            // is then at most 2^13, in f16's range (1024 where it may be multiplied by 1 / kShrink; FINE: 256 times a scale
-            // of up to 128, with a larger one in the tile 1).
-            const float most = FINE ? (special ? 1.f : 256.f) : special ? 1024.f : 8192.f;
+            Headroom room{kGoal, special ? kMostShrunk : kMost};
+            if constexpr (FINE) {  // (f16 with exponent bits x: below 2^(x - 14))
+                uint32_t top = f.top[0];
+#pragma unroll
+                for (int k = 1; k < KT / 16; ++k)
+                    top = max(top, f.top[k]);
+                room = headroom_of((__builtin_amdgcn_readfirstlane(top) >> 10) - 14);
+            }
+            // the scores in log2 units, less the running maximum
             const bool fresh = __any(negm == __FLT_MAX__);  // rows that have seen nothing yet
             const float less = fresh ? 0.f : negm;
 #pragma unroll
@@ -873,7 +903,7 @@ void chunk_kernel(const Args a) {
                 for (int k = 0; k < 16; ++k)
                     s[b][k] = fmaf(s[b][k], n[k], less);
             }
-            // the maximum moved by what the scores are above it (`up`: where they are; first: to the tile's own)
+            // the maximum moved by what the scores are above its goal (first: to the tile's own)
             auto move = [&](bool first) __attribute__((always_inline)) {
                 float mx = -INFINITY;
 #pragma unroll
@@ -882,7 +912,7 @@ void chunk_kernel(const Args a) {
                     for (int k = 0; k < 16; k += 2)
                         mx = prefix::max3(mx, s[b][k], s[b][k + 1]);
                 const float top = prefix::pair_max(mx), above = first ? top + negm : top;
-                const float negm_new = above > 0.f ? (first ? -top : negm - top) : negm;
+                const float negm_new = above > room.goal ? (first ? room.goal - top : negm + (room.goal - top)) : negm;
                 const float alpha = __builtin_amdgcn_exp2f(negm_new - negm), add = first ? negm_new : negm_new - negm;
                 negm = negm_new;
                 l *= alpha;
@@ -942,8 +972,7 @@ void chunk_kernel(const Args a) {
                         uint32_t pk[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const fp16x2 two = __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_exp2f(s[b][2 * k]),
-                                                                          __builtin_amdgcn_exp2f(s[b][2 * k + 1]));
+                            const fp16x2 two{(__fp16)__builtin_amdgcn_exp2f(s[b][2 * k]), (__fp16)__builtin_amdgcn_exp2f(s[b][2 * k + 1])};
                             sum = __builtin_amdgcn_fdot2(two, fp16x2{(__fp16)1.f, (__fp16)1.f}, sum, false);
                             pk[k] = __builtin_bit_cast(uint32_t, two);
                         }
@@ -953,7 +982,7 @@ void chunk_kernel(const Args a) {
                 }
             };
             weights();
-            if (__any(sum > most)) {
+            if (__any(sum > room.most)) {
                 move(false);
                 weights();
             }

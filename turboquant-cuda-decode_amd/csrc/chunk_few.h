@@ -290,17 +290,14 @@ void chunk_few_kernel(const Args a) {
                     v[2 * m + 1] = pack(odd);
                 }
             }
-            // scales of 128 and more, and what is not finite (of tokens past the sequence too, which then costs time only)
-            uint32_t top_s, top_z;
-            if constexpr (LAYOUT == 0) {
-                top_s = top_of(most_of(most_of(raw.s[4], raw.s[5]), most_of(raw.s[6], raw.s[7])));
-                top_z = top_of(most_of(most_of(raw.s[8], raw.s[9]), most_of(raw.s[10], raw.s[11])));
-            } else {
-                const uint32_t m = most_of(raw.s[2], raw.s[3]);
-                top_s = m & 0xFFFFu;
-                top_z = m >> 16;
-            }
-            const bool special = __any(top_s >= 0x5800u || top_z >= 0x7C00u);
+            // what is not finite (of tokens past the sequence too, which then costs time only)
+            uint32_t top_v;
+            if constexpr (LAYOUT == 0)
+                top_v = top_of(most_of(most_of(most_of(raw.s[4], raw.s[5]), most_of(raw.s[6], raw.s[7])),
+                                       most_of(most_of(raw.s[8], raw.s[9]), most_of(raw.s[10], raw.s[11]))));
+            else
+                top_v = top_of(most_of(raw.s[2], raw.s[3]));
+            const bool special = __any(top_v >= 0x7C00u);
             load(i + 1, no, yes);
             read_pages(i + 2);
             const bool masked = t0 + 32 > limit_lo || (a.shape.window && t0 < limit_hi - a.shape.window);
@@ -311,7 +308,19 @@ void chunk_few_kernel(const Args a) {
                 for (int x = 0; x < 8; ++x)
                     if (gone[x >> 2] || t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= seq.len)
                         scale[x] = mid[x] = 0.f;
-            const float most = special ? 1.f : 256.f;
+            // the largest scale of the wave's 32 tokens
+            float top_s = 0.f;
+            if (special) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    top_s = fmaxf(top_s, fabsf(scale[x]) < __builtin_inff() ? fabsf(scale[x]) : 0.f);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    top_s = fmaxf(top_s, fabsf(scale[x]));
+            }
+            top_s = xdl::max_xor16(xdl::max_xor32(top_s));
+            const Headroom room = headroom_of(__builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top_s)));
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 if (b >= blocks)
@@ -337,7 +346,7 @@ void chunk_few_kernel(const Args a) {
                     for (int x = 0; x < 8; x += 2)
                         mx = prefix::max3(mx, s[b][x], s[b][x + 1]);
                     const float top = xdl::max_xor16(xdl::max_xor32(mx)), above = first ? top + negm[b] : top;
-                    const float negm_new = above > 0.f ? (first ? -top : negm[b] - top) : negm[b];
+                    const float negm_new = above > room.goal ? (first ? room.goal - top : negm[b] + (room.goal - top)) : negm[b];
                     const float alpha = __builtin_amdgcn_exp2f(negm_new - negm[b]), add = first ? negm_new : negm_new - negm[b];
                     negm[b] = negm_new;
                     l[b] *= alpha;
@@ -370,7 +379,7 @@ void chunk_few_kernel(const Args a) {
                     }
                 };
                 weights();
-                if (__any(sum > most)) {
+                if (__any(sum > room.most)) {
                     move(false);
                     weights();
                 }
