@@ -829,7 +829,7 @@ def cache_load(kv_cache, slot_mapping, rotation_t, centroids, *, key_bits=4, val
 
     ``rotation_t`` is the writer's ``PiT``: keys come back in the basis that they were given in; None leaves them
     rotated (``q @ PiT`` attends to those).  ``centroids``: the 2^``key_bits`` of the codebook.  FP8 keys (``key_bits=8``) take neither.
-    A negative slot, or one past the cache, gives zeros.  Presets, layouts and block sizes as the writers'
+    A negative slot, or one past the cache, gives zeros; no slots at all, empty tensors.  Presets, layouts and block sizes as the writers'
     (``store``, ``store_preset``, ``store_fp8``, ``rope_store``).
     """
     fp8 = key_bits == 8
@@ -838,7 +838,7 @@ def cache_load(kv_cache, slot_mapping, rotation_t, centroids, *, key_bits=4, val
     slot = slot_bytes_fp8(HEAD_DIM) if fp8 else slot_bytes_preset(HEAD_DIM, key_bits, value_bits)
     bs, Hk, stride, lid = _cache_geometry(kv_cache, slot, layout, " (FP8 keys)" if fp8 else "")
     _check_tensor(slot_mapping, "slot_mapping", torch.int32)
-    _require(slot_mapping.dim() == 1 and slot_mapping.size(0) > 0, "slot_mapping must be [N], N > 0")
+    _require(slot_mapping.dim() == 1, "slot_mapping must be [N]")
     _require(dtype in DTYPES, "dtype must be float32, bfloat16 or float16")
     N = slot_mapping.size(0)
     shape = (N, Hk, HEAD_DIM)
@@ -860,6 +860,8 @@ def cache_load(kv_cache, slot_mapping, rotation_t, centroids, *, key_bits=4, val
             _require(tuple(rotation_t.shape) == (HEAD_DIM, HEAD_DIM), _ROTATION_SHAPE)
             tensors.append(rotation_t)
     _require(_same_device(*tensors), "all tensors must be on the same device")
+    if N == 0:
+        return key, value
     with _on_device(kv_cache.device):
         rc = _lib.load().tq4_cache_load(
             kv_cache.data_ptr(), slot_mapping.data_ptr(), None if fp8 or rotation_t is None else rotation_t.data_ptr(),
