@@ -333,7 +333,7 @@ int64_t tq4_prefix_workspace_floats(int B, int Hq, int Hk, int num_kv_splits);
  * are the last of those, and each sees itself and what lies before it; with window > 0 only the last `window` of
  * these (itself included) and the first `first_tokens`.  Not causal (window 0): every new token sees all seq_lens[b]
  * tokens, as the context of a chunk whose own tokens are attended to elsewhere (tq4_merge_states joins the two).
- * A new token that sees nothing gets zeros and LSE -inf.  What starts and lengths name outside of query and
+ * A new token that sees nothing gets zeros and LSE -inf (with sinks, the sink).  What starts and lengths name outside of query and
  * the table counts as not there; only blocks with a visible token are read, and the block-table entries of the others may
  * hold anything.
  * query: heads contiguous, tokens query_stride elements apart (whole 16-byte pieces); query and out are 16-bit

@@ -30,7 +30,6 @@ namespace chunk {
 using prefix::floatx16;
 using prefix::half2v;
 using xdl::half8;
-typedef uint32_t u32x2a8 __attribute__((ext_vector_type(2), aligned(8)));
 
 struct Args {
     const void *query;       // [tokens, heads, 128] of q_dtype
@@ -118,12 +117,14 @@ __device__ __forceinline__ void plan_cuts(const Args &a, PlanLds &lds) {
 }
 
 // Query rows into operands: y = q @ rot_t (a row scaled by a power of two first; rot_t as f16 hi + lo where LO keeps y as
-// pairs too, else rounded to f16, as much of an error as rounding y is), times the score scale, as f16 hi (and lo); rows that would pass f16's range, or lie below 2^-8 near its
-// denormals, are scaled to its top and q_factor undoes it.  FP8 keys: the row itself, scaled by the power of two that
-// puts its largest magnitude in [0.5, 1): exact for dims down to 2^-13 of it, below that to 2^-25 of it.
-// Bound by each workgroup's own rounding of rot_t: 8192 x 32 rows 39 us (with its low part 53), 134 MB in and out.  A form whose workgroups stage rot_t once and take one row tile after the other (32x32x16 products) took
-// 39 with the low part, but the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower
-// clock through chunk_kernel (634 : 720 us, the same code).
+// pairs too, else rounded to f16, as much of an error as rounding y is), times the score scale, as f16 hi (and lo); rows
+// that would pass f16's range, or lie below 2^-8 near its denormals, are scaled to its top and q_factor undoes it.  FP8
+// keys: the row itself, scaled by the power of two that puts its largest magnitude in [0.5, 1): exact for dims down to
+// 2^-13 of it, below that to 2^-25 of it.
+// Bound by each workgroup's own rounding of rot_t: 8192 x 32 rows 39 us (with its low part 53), 134 MB in and out.  A form
+// whose workgroups stage rot_t once and take one row tile after the other (32x32x16 products) took 39 with the low part, but
+// the whole call was slower by 70 of 710 us: behind its dense matrix phases the device kept a lower clock through
+// chunk_kernel (634 : 720 us, the same code).
 template <typename InT, bool KF8, bool LO>
 __global__ __launch_bounds__(kStartThreads) void chunk_start_kernel(const Args a, const Args few, int plans) {
     constexpr int PT = KF8 ? 8 : kHeadDim * kRotPt;
@@ -635,11 +636,11 @@ __device__ __forceinline__ Headroom headroom_of(int e) {
 // ---- The product -----------------------------------------------------------------------------
 
 // Bound by what a tile costs beside its products, and by the clock that both leave.  32 heads on 8 kv-heads: 8192 tokens on
-// themselves 640 us, 0.86 PFLOP/s of the visible products; 2048 behind 32768 1200 us, 0.94 (a bf16 product of 8192^3 reaches
+// themselves 655 us, 0.85 PFLOP/s of the visible products; 2048 behind 32768 1220 us, 0.93 (a bf16 product of 8192^3 reaches
 // 1.24).  A tile of 64 tokens takes a wave of 32 rows about 5060 cycles: its products 2050, softmax and decoding about 2490 of
 // vector work, and little of the one beside the other, since the four waves that decode V take longer than those
 // that decode K, which wait for them at the barrier.  FINE has three score products for one: 4 sequences of up to 1000 tokens, up to
-// 10000 before them, 3 bits, GQA 8: 720 us.
+// 10000 before them, 3 bits, GQA 8: 740 us.
 // Tiles of 256 rows (WT = 1, eight waves) have two LDS buffers and decode a tile between the products of the one before it;
 // tiles of 64 rows (WT = 2) decode and multiply in turn, two workgroups a CU.  What did not pay: the next tile's
 // scores before the softmax of this one (registers spill), and the two halves of the waves a phase apart (the same time).
@@ -710,8 +711,8 @@ void chunk_kernel(const Args a) {
         // the first of the 16 tokens of the wave's units, in the tile
         auto group_of = [&](int k) __attribute__((always_inline)) { return 16 * (S::halves ? w % (WR * WT / 2) : w + k * WR * WT); };
         // (no block past the sequence's last one is asked for, and none in front of the window; in the others, any token is in
-        // bounds.  A vector load, though
-        // every lane's is the same: a scalar one in flight makes every wait for LDS a wait for it)
+        // bounds.  A vector load, though every lane's is the same: a scalar one in flight makes every wait for LDS a wait
+        // for it)
         auto read_pages = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
@@ -723,7 +724,8 @@ void chunk_kernel(const Args a) {
         auto load = [&](int i, bool does_k, bool does_v) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const Place at = place_of<LAYOUT, KF8, KB3, V3>(a, kvh, __builtin_amdgcn_readfirstlane(blk[k]), (first_of(i) + group_of(k)) & ((1 << a.block_size_log2) - 1));
+                const int within = (first_of(i) + group_of(k)) & ((1 << a.block_size_log2) - 1);
+                const Place at = place_of<LAYOUT, KF8, KB3, V3>(a, kvh, __builtin_amdgcn_readfirstlane(blk[k]), within);
                 if (does_k)
                     load_k<LAYOUT, KF8, KB3, V3>(rk[k], a, at, lane);
                 if (does_v)

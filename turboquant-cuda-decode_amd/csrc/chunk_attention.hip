@@ -26,7 +26,9 @@ int cus() { return step_waves_held() / tq4::xdl::kStepWaves; }
 // tokens, 2 kv-heads, 48 and 128 rows: 48 and 55 us, 63 and 72, 64 and 72).
 // Batches whose average takes larger tiles may still have sequences with few rows (decoding beside a prompt's chunk), whose
 // every tile would cost as much as a full one: they have a product of their own (63 sequences of one token and one of
-// 2048, behind 4096: 455 us together, 262 so; a batch without such sequences pays 8 us for it).
+// 2048, behind 4096: 455 us together, 256 so; a batch without such sequences pays 8 us for it).  The average alone decides: where
+// it is small, a long chunk goes through kFew with the rest (256 single tokens and one of 1792, behind 4096: 583 us;
+// in two calls 279 and 156).
 ChunkPlan chunk_plan(int tokens, int batch, int Hq, int Hk) {
     const int64_t rows = std::max<int64_t>((int64_t)tokens * (Hq / Hk) / batch, 1);
     const int64_t few = 4 * ((rows + 31) / 32), some = 7 * ((rows + 63) / 64), many = 16 * ((rows + 255) / 256);

@@ -12,7 +12,7 @@
 // they stand, in the order of V's tokens.  The four waves of a workgroup take 32 of each 128 tokens and join in LDS.
 // Scores are one f16 product, or three of f16 pairs (FINE); V's scale is part of the weight, one f16.
 //
-// 64 sequences of 1 to 8 drafted tokens behind 512 to 8192 (32 heads on 8 kv-heads, 302 MB): 104 us, 2.9 TB/s of the copy's 5.1:
+// 64 sequences of 1 to 8 drafted tokens behind 512 to 8192 (32 heads on 8 kv-heads, 302 MB): 105 us, 2.9 TB/s of the copy's 5.1:
 // vector instructions in 58 % of the cycles, the rest the latency of records and lookups with two waves a SIMD.  The same
 // in tiles of 64 rows that a workgroup's waves share (chunk_kernel): 152.
 #pragma once

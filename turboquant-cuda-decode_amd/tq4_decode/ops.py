@@ -765,7 +765,8 @@ def chunk_attention(query, rotation_t, kv_cache, block_table, seq_lens, query_st
     put them there) and each sees itself and what lies before it; with ``window`` only the last ``window`` tokens
     (itself included) and the ``first_tokens`` first ones.  ``causal=False``: every new token sees all ``seq_lens[b]``
     tokens, as a context whose result ``merge_states`` joins with that of the chunk's own tokens.  A new token that sees
-    nothing gets zeros and LSE -inf.
+    nothing gets zeros and LSE -inf (with ``sinks``, the sink).  Only blocks with a visible token are read: the block-table entries
+    of the others may hold anything.
 
     ``query`` and the outputs are bf16 or fp16; heads are contiguous, tokens may be strided (a slice of a projection's
     output).  fp16 outputs and calls with ``return_lse`` take scores from f16 pairs and V's codes as they are, others
